@@ -80,15 +80,17 @@ def draw(rng):
         return dict(op=op, n_seq=n_seq, n_head_kv=n_head_kv, head_dim=head_dim, page_size=page, dtype=dtype,
                     max_len=_log_int(rng, 1, min(2048, (1 << 17) // n_seq)), chunk=chunk)
     n_seq = _log_int(rng, 1, 64)
-    most = (1 << 18) // n_seq if op == "attn" else (1 << 19) // n_seq
-    max_len = _log_int(rng, 1, min(131072, most))
+    if op == "select":  # enough blocks for a choice: at least 16, at most half of them taken
+        max_len = _log_int(rng, 16 * page, min(131072, max(16 * page, (1 << 19) // n_seq)))
+        if max_len > 16384 * page:
+            page = 16
+        blocks = (max_len + page - 1) // page
+        return dict(op=op, n_seq=n_seq, n_head=n_head, n_head_kv=n_head_kv, head_dim=head_dim, page_size=page,
+                    dtype=dtype, min_len=rng.choice([0, 1, max_len // 2, max_len]), max_len=max_len,
+                    k_blocks=_log_int(rng, 4, min(blocks // 2, 512)))
+    max_len = _log_int(rng, 1, min(131072, (1 << 18) // n_seq))
     min_len = rng.choice([0, 1, max_len // 2, max_len])
     blocks = (max_len + page - 1) // page
-    if op == "select":
-        if blocks > 16384:
-            page, blocks = 16, (max_len + 15) // 16
-        return dict(op=op, n_seq=n_seq, n_head=n_head, n_head_kv=n_head_kv, head_dim=head_dim, page_size=page,
-                    dtype=dtype, min_len=min_len, max_len=max_len, k_blocks=_log_int(rng, 1, min(blocks + 2, 512)))
     k_blocks = _log_int(rng, 1, min(blocks + 2, 512)) if rng.random() < 0.3 else 0
     return dict(op=op, n_seq=n_seq, n_head=n_head, n_head_kv=n_head_kv, head_dim=head_dim, page_size=page, dtype=dtype,
                 min_len=min_len, max_len=max_len, mask=rng.random() < 0.3, k_blocks=k_blocks)
@@ -229,7 +231,9 @@ def prepare(case, seed):
         m = torch.randn((n_seq, width), generator=gen, **dev)
         off = torch.rand((n_seq, width), generator=gen, **dev)
         m = m.masked_fill(off < 0.3, float("-inf")).masked_fill(off > 0.95, -65504.0)
-        m[n_seq // 2] = float("-inf")  # a row with nothing to attend to
+        longest = max(range(n_seq), key=lens.__getitem__)
+        m[(longest + 1) % n_seq] = float("-inf")  # a row with nothing to attend to
+        m[longest, 0] = 0.0
         s["mask_rows"] = m.to(torch.float16)
     s["sel"] = None
     if case["k_blocks"]:
