@@ -27,6 +27,7 @@ TYPE_F32 = 0
 TYPE_F16 = 1
 TYPE_Q4_0 = 2
 TYPE_Q8_0 = 8
+TYPE_BF16 = 30
 TYPE_A8W8 = 100  # this library's int8 layout for the reference's A8W8 scheme
 Q4_MODE_GGML = 0
 Q4_MODE_W4A16 = 1
@@ -77,6 +78,14 @@ P = C.c_void_p
 I64 = C.c_int64
 
 
+class _PagedKVStruct(C.Structure):
+    """b200_paged_kv of include/b200_paged.h."""
+
+    _fields_ = [("type", C.c_int), ("head_dim", C.c_int), ("n_head_kv", C.c_int), ("page_size", C.c_int),
+                ("n_pages", I64), ("k", P), ("v", P), ("k_page", I64), ("k_row", I64), ("k_head", I64),
+                ("v_page", I64), ("v_row", I64), ("v_head", I64), ("k_lo", P), ("k_hi", P)]
+
+
 def _declare(L):
     sig = {
         "b200_version": (C.c_char_p, []),
@@ -120,6 +129,21 @@ def _declare(L):
         "b200_swiglu_f32": (C.c_int, [P, P, P, I64, P]),
         "b200_add_f32": (C.c_int, [P, P, P, I64, P]),
         "b200_argmax_f32": (C.c_int, [P, I64, P, P]),
+        "b200_paged_plan": (
+            C.c_int,
+            [P, P, C.c_int, P, I64, C.c_int, C.c_int, P, I64, P, I64, P, P, P, P, P, P],
+        ),
+        "b200_paged_store": (C.c_int, [P, P, I64, P, I64, P, I64, P]),
+        "b200_paged_select_workspace_size": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+        "b200_paged_select": (
+            C.c_int,
+            [P, P, I64, C.c_int, C.c_int, P, I64, C.c_int, P, C.c_int, P, P, C.c_size_t, P],
+        ),
+        "b200_paged_attn_workspace_size": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
+        "b200_paged_attn": (
+            C.c_int,
+            [P, P, I64, C.c_int, C.c_int, P, I64, C.c_int, P, P, I64, P, C.c_int, C.c_float, P, P, C.c_size_t, P],
+        ),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -553,4 +577,277 @@ def kv_lengths_from_mask(mask_f16: np.ndarray) -> np.ndarray:
                                             out.ctypes.data_as(C.c_void_p)),
         "kv_lengths_from_mask",
     )
+    return out
+
+
+# ------------------------------------------------- paged key-value cache
+# Batched single-token decode over fixed-size pages (include/b200_paged.h):
+# one step is paged_plan (pages and slots for the step's tokens), then per
+# layer paged_store (the layer's K/V rows into their slots) and paged_attn,
+# for long contexts with paged_select before it.  Every call is asynchronous
+# on the current stream and may be captured into a CUDA graph; what varies
+# from step to step (lengths, tables, free pages) stays on the device.
+
+
+def _bad(what: str, msg: str):
+    raise B200Error(EINVAL, f"{what}: {msg}")
+
+
+class _on:
+    """The device's context current inside the block (a no-op when it is)."""
+
+    def __init__(self, device):
+        torch = _torch()
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *e):
+        if self.guard is not None:
+            self.guard.__exit__(*e)
+
+
+class PagedKV:
+    """One layer's cache: k and v [n_pages, page_size, n_head_kv, head_dim] of
+    float16 or bfloat16 on one CUDA device.  Any strides that are multiples of
+    16 bytes with a contiguous head dim work, so a [n_pages, n_head_kv,
+    page_size, head_dim] allocation is passed transposed.  k_lo and k_hi
+    (contiguous [n_pages, n_head_kv, head_dim] of the same type) are the pages'
+    key bounds, which paged_store keeps and paged_select reads; their initial
+    contents do not matter."""
+
+    def __init__(self, k, v, k_lo=None, k_hi=None):
+        torch = _torch()
+        if k.dim() != 4 or tuple(v.shape) != tuple(k.shape):
+            _bad("PagedKV", "k and v must be [n_pages, page_size, n_head_kv, head_dim]")
+        if k.dtype not in (torch.float16, torch.bfloat16):
+            raise B200Unsupported(EUNSUPPORTED, f"PagedKV of {k.dtype}")
+        if v.dtype != k.dtype or not k.is_cuda or v.device != k.device:
+            _bad("PagedKV", "k and v must have one type and be on one CUDA device")
+        self.n_pages, self.page_size, self.n_head_kv, self.head_dim = k.shape
+        if self.head_dim not in (64, 128, 256):
+            raise B200Unsupported(EUNSUPPORTED, f"PagedKV with head dim {self.head_dim}")
+        if k.numel() == 0 or self.n_pages * self.page_size >= 2**31 - 1:
+            _bad("PagedKV", "needs at least one slot and fewer than 2^31")
+        if k.stride(3) != 1 or v.stride(3) != 1:
+            _bad("PagedKV", "needs a contiguous head dim")
+        if (k_lo is None) != (k_hi is None):
+            _bad("PagedKV", "k_lo and k_hi go together")
+        for t in (k_lo, k_hi):
+            if t is not None and (t.dtype != k.dtype or t.device != k.device or not t.is_contiguous()
+                                  or tuple(t.shape) != (self.n_pages, self.n_head_kv, self.head_dim)):
+                _bad("PagedKV", "k_lo and k_hi must be contiguous [n_pages, n_head_kv, head_dim] of k's type and device")
+        strides = [s * 2 for t in (k, v) for s in t.stride()[:3]]
+        if any(s % 16 for s in strides) or any(t is not None and t.data_ptr() % 16 for t in (k, v, k_lo, k_hi)):
+            _bad("PagedKV", "strides and addresses must be multiples of 16 bytes")
+        self.k, self.v, self.k_lo, self.k_hi, self.device = k, v, k_lo, k_hi, k.device
+        self._c = _PagedKVStruct(TYPE_F16 if k.dtype == torch.float16 else TYPE_BF16, self.head_dim, self.n_head_kv,
+                                 self.page_size, self.n_pages, k.data_ptr(), v.data_ptr(), *strides,
+                                 None if k_lo is None else k_lo.data_ptr(), None if k_hi is None else k_hi.data_ptr())
+        self._ref = C.byref(self._c)
+
+
+class PagedPlan:
+    """Result of paged_plan."""
+
+    __slots__ = ("slots", "positions", "cu", "seq_lens", "n_free")
+
+    def __init__(self, slots, positions, cu, seq_lens, n_free):
+        self.slots, self.positions, self.cu, self.seq_lens, self.n_free = slots, positions, cu, seq_lens, n_free
+
+
+def _check_i32(what, device, **tensors):
+    torch = _torch()
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or t.device != device or (t.dim() == 1 and not t.is_contiguous()):
+            _bad(what, f"{name} must be a contiguous int32 tensor on {device}")
+
+
+def paged_plan(new_lens, seq_lens, block_table, free_pages, n_free, page_size: int, max_tokens: int,
+               seq_lens_out=None, n_free_out=None, slots=None, positions=None, cu=None) -> PagedPlan:
+    """Pages, lengths and slots of one step, on the device.
+
+    new_lens int32 [n_seq]: tokens each sequence appends (0: none, negative:
+    it ends and gives its pages back); seq_lens int32 [n_seq]: tokens it has;
+    block_table int32 [n_seq, max_blocks]: its pages, extended here;
+    free_pages int32 [n_pages] and n_free int32 [1]: the stack of free pages.
+    seq_lens and n_free are updated in place unless seq_lens_out / n_free_out
+    are given.  Returns slots int64 [max_tokens], positions int32 [max_tokens]
+    (-1: padding, or a token whose sequence was not served), cu int32
+    [n_seq + 1] (first row of each sequence) and the new seq_lens and n_free.
+    A sequence that the table, max_tokens or the free pages cannot take keeps
+    its length; the caller sees that from seq_lens."""
+    torch = _torch()
+    dev = seq_lens.device
+    if seq_lens.dim() != 1 or not seq_lens.is_cuda or new_lens.shape != seq_lens.shape or seq_lens.numel() == 0:
+        _bad("paged_plan", "seq_lens and new_lens must be [n_seq] on a CUDA device, n_seq >= 1")
+    n = seq_lens.numel()
+    if block_table.dim() != 2 or block_table.shape[0] != n or block_table.shape[1] == 0 or block_table.stride(1) != 1:
+        _bad("paged_plan", "block_table must be [n_seq, max_blocks] with contiguous rows")
+    if seq_lens_out is None:
+        seq_lens_out = seq_lens
+    if n_free_out is None:
+        n_free_out = n_free
+    if cu is None:
+        cu = torch.empty(n + 1, dtype=torch.int32, device=dev)
+    if slots is None:
+        slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+    if positions is None:
+        positions = torch.empty(max_tokens, dtype=torch.int32, device=dev)
+    _check_i32("paged_plan", dev, new_lens=new_lens, seq_lens=seq_lens, block_table=block_table,
+               free_pages=free_pages, n_free=n_free, seq_lens_out=seq_lens_out, n_free_out=n_free_out, cu=cu,
+               positions=positions)
+    if (free_pages.dim() != 1 or n_free.numel() != 1 or n_free_out.numel() != 1 or seq_lens_out.shape != seq_lens.shape
+            or cu.dim() != 1 or cu.numel() < n + 1 or positions.dim() != 1 or positions.numel() < max_tokens
+            or slots.dtype != torch.int64 or slots.device != dev or slots.dim() != 1 or not slots.is_contiguous()
+            or slots.numel() < max_tokens):
+        _bad("paged_plan", "free_pages [n_pages], n_free [1], cu [n_seq + 1] and slots, positions [max_tokens]")
+    with _on(dev):
+        rc = lib().b200_paged_plan(new_lens.data_ptr(), seq_lens.data_ptr(), n, block_table.data_ptr(),
+                                   block_table.stride(0), block_table.shape[1], page_size, free_pages.data_ptr(),
+                                   free_pages.numel(), n_free.data_ptr(), max_tokens, slots.data_ptr(),
+                                   positions.data_ptr(), cu.data_ptr(), seq_lens_out.data_ptr(),
+                                   n_free_out.data_ptr(), _stream(dev))
+    _check(rc, "paged_plan")
+    return PagedPlan(slots, positions, cu, seq_lens_out, n_free_out)
+
+
+def _rows_f32(what, name, t, row, dev):
+    """t as f32 rows of `row` contiguous values, 16-byte aligned (copied when
+    it is not); its row stride in floats."""
+    torch = _torch()
+    if t.dtype != torch.float32 or t.device != dev or t.dim() not in (2, 3) or t[0:1].numel() not in (0, row):
+        _bad(what, f"{name} must be f32 rows of {row} values on {dev}")
+    inner = t.stride(-1) == 1 and (t.dim() == 2 or t.stride(1) == t.shape[2] or t.shape[1] == 1)
+    if not inner or t.stride(0) % 4 or t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) < row):
+        t = t.contiguous() if not t.is_contiguous() else t.clone()
+    return t, t.stride(0)
+
+
+def paged_store(cache: PagedKV, k, v, slots):
+    """K and V rows of new tokens into the cache: k, v f32 [n_tokens,
+    n_head_kv, head_dim] (or [n_tokens, n_head_kv * head_dim], row strided),
+    slots int64 [n_tokens] from paged_plan (negative: skipped).  Rounds to the
+    cache type and, when the cache has key bounds, updates them."""
+    torch = _torch()
+    dev = cache.device
+    row = cache.n_head_kv * cache.head_dim
+    if (slots.dtype != torch.int64 or slots.device != dev or slots.dim() != 1 or not slots.is_contiguous()
+            or k.shape[0] != slots.numel() or v.shape[0] != slots.numel()):
+        _bad("paged_store", "slots must be a contiguous int64 [n_tokens] on the cache's device, one per row of k and v")
+    k, k_ld = _rows_f32("paged_store", "k", k, row, dev)
+    v, v_ld = _rows_f32("paged_store", "v", v, row, dev)
+    with _on(dev):
+        rc = lib().b200_paged_store(cache._ref, k.data_ptr(), k_ld, v.data_ptr(), v_ld, slots.data_ptr(),
+                                    slots.numel(), _stream(dev))
+    _check(rc, "paged_store")
+
+
+def _paged_batch(what, cache, q, block_table, seq_lens):
+    torch = _torch()
+    dev = cache.device
+    if q.dim() != 3 or q.dtype != torch.float32 or q.device != dev or q.shape[2] != cache.head_dim:
+        _bad(what, "q must be f32 [n_seq, n_head, head_dim] on the cache's device")
+    n_seq, n_head = q.shape[0], q.shape[1]
+    if n_head == 0 or n_head % cache.n_head_kv:
+        _bad(what, "n_head must be a multiple of the cache's n_head_kv")
+    _check_i32(what, dev, block_table=block_table, seq_lens=seq_lens)
+    if (block_table.dim() != 2 or block_table.shape[0] != n_seq or block_table.stride(1) != 1
+            or block_table.shape[1] == 0 or seq_lens.dim() != 1 or seq_lens.numel() != n_seq):
+        _bad(what, "block_table must be [n_seq, max_blocks] with contiguous rows and seq_lens [n_seq]")
+    return _rows_f32(what, "q", q, n_head * cache.head_dim, dev) + (n_seq, n_head)
+
+
+def _paged_workspace(what, workspace, size, dev, zeros):
+    torch = _torch()
+    if workspace is None:
+        return (torch.zeros if zeros else torch.empty)(size, dtype=torch.uint8, device=dev)
+    if workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
+        _bad(what, "workspace must be a contiguous uint8 tensor on the cache's device")
+    return workspace
+
+
+def paged_select(cache: PagedKV, q, block_table, seq_lens, n_sel: int, sel=None, workspace=None):
+    """The n_sel blocks of its sequence that each KV head should read for this
+    token: the newest block and those whose key bounds allow the largest q . k
+    (the largest over the KV head's query heads; ties: the lower block).
+
+    q f32 [n_seq, n_head, head_dim]; block_table int32 [n_seq, max_blocks];
+    seq_lens int32 [n_seq].  Returns int32 [n_seq, n_head_kv, n_sel]: block
+    numbers in ascending order, -1 past the sequence's last.  workspace: uint8
+    of paged_select_workspace_size bytes, allocated when not given."""
+    torch = _torch()
+    if cache.k_lo is None:
+        _bad("paged_select", "the cache has no key bounds")
+    dev = cache.device
+    q, q_stride, n_seq, n_head = _paged_batch("paged_select", cache, q, block_table, seq_lens)
+    shape = (n_seq, cache.n_head_kv, n_sel)
+    if sel is None:
+        if n_sel <= 0:
+            _bad("paged_select", "n_sel must be positive")
+        sel = torch.empty(shape, dtype=torch.int32, device=dev)
+    elif sel.dtype != torch.int32 or sel.device != dev or not sel.is_contiguous() or tuple(sel.shape) != shape:
+        _bad("paged_select", "sel must be a contiguous int32 [n_seq, n_head_kv, n_sel]")
+    if workspace is None:
+        size = paged_select_workspace_size(n_seq, cache.n_head_kv, block_table.shape[1])
+        workspace = _paged_workspace("paged_select", None, size, dev, zeros=False)
+    else:
+        _paged_workspace("paged_select", workspace, 0, dev, zeros=False)
+    with _on(dev):
+        rc = lib().b200_paged_select(cache._ref, q.data_ptr(), q_stride, n_seq, n_head, block_table.data_ptr(),
+                                     block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), n_sel,
+                                     sel.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream(dev))
+    _check(rc, "paged_select")
+    return sel
+
+
+def paged_select_workspace_size(n_seq: int, n_head_kv: int, max_blocks: int) -> int:
+    return int(lib().b200_paged_select_workspace_size(n_seq, n_head_kv, max_blocks))
+
+
+def paged_attn_workspace_size(head_dim: int, n_seq: int, n_head: int, n_head_kv: int) -> int:
+    return int(lib().b200_paged_attn_workspace_size(head_dim, n_seq, n_head, n_head_kv))
+
+
+def paged_attn(cache: PagedKV, q, block_table, seq_lens, scale: float, mask=None, sel=None, out=None, workspace=None):
+    """Attention of one new token per sequence over its cached tokens.
+
+    q f32 [n_seq, n_head, head_dim]; block_table int32 [n_seq, max_blocks];
+    seq_lens int32 [n_seq]; mask f16 [n_seq, >= max_blocks * page_size]
+    additive or None; sel int32 [n_seq, n_head_kv, n_sel] (paged_select) or
+    None for every block.  Returns f32 [n_seq, n_head, head_dim]; zeros where
+    nothing is attended to.  workspace: uint8 of paged_attn_workspace_size
+    bytes, zero-filled before its first use and not shared by calls that
+    overlap on the GPU; allocated and cleared for this call when not given."""
+    torch = _torch()
+    dev = cache.device
+    q, q_stride, n_seq, n_head = _paged_batch("paged_attn", cache, q, block_table, seq_lens)
+    width = block_table.shape[1] * cache.page_size
+    if mask is not None and (mask.dtype != torch.float16 or mask.device != dev or mask.dim() != 2
+                             or mask.shape[0] != n_seq or mask.shape[1] < width or mask.stride(1) != 1):
+        _bad("paged_attn", "mask must be f16 [n_seq, >= max_blocks * page_size] with contiguous rows")
+    if sel is not None and (sel.dtype != torch.int32 or sel.device != dev or not sel.is_contiguous()
+                            or sel.dim() != 3 or tuple(sel.shape[:2]) != (n_seq, cache.n_head_kv)
+                            or sel.shape[2] == 0):
+        _bad("paged_attn", "sel must be a contiguous int32 [n_seq, n_head_kv, n_sel]")
+    shape = (n_seq, n_head, cache.head_dim)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float32, device=dev)
+    elif out.dtype != torch.float32 or out.device != dev or not out.is_contiguous() or tuple(out.shape) != shape:
+        _bad("paged_attn", "out must be a contiguous f32 [n_seq, n_head, head_dim]")
+    if workspace is None:
+        size = paged_attn_workspace_size(cache.head_dim, n_seq, n_head, cache.n_head_kv)
+        workspace = _paged_workspace("paged_attn", None, size, dev, zeros=True)
+    else:
+        _paged_workspace("paged_attn", workspace, 0, dev, zeros=True)
+    with _on(dev):
+        rc = lib().b200_paged_attn(cache._ref, q.data_ptr(), q_stride, n_seq, n_head, block_table.data_ptr(),
+                                   block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
+                                   None if mask is None else mask.data_ptr(), 0 if mask is None else mask.stride(0),
+                                   None if sel is None else sel.data_ptr(), 0 if sel is None else sel.shape[2],
+                                   float(scale), out.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                                   _stream(dev))
+    _check(rc, "paged_attn")
     return out

@@ -1128,3 +1128,5 @@ extern "C" int b200_fa_decode_static_scratch(const float* q, const void* k, cons
     }
     return cuda_status(cudaGetLastError());
 }
+
+#include "paged_api.cuh"

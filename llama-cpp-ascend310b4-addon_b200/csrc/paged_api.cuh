@@ -1,0 +1,209 @@
+// paged_api.cuh -- the C ABI of include/b200_paged.h: argument checks and
+// launches.  Included by kernels.cu, whose helpers it uses.
+#pragma once
+
+#include "paged_attn.cuh"
+#include "paged_plan.cuh"
+#include "paged_select.cuh"
+#include "paged_store.cuh"
+
+namespace {
+
+int check_paged_kv(const b200_paged_kv* kv) {
+    if (!kv || !kv->k || !kv->v || kv->n_head_kv <= 0 || kv->page_size <= 0 || kv->n_pages <= 0 ||
+        kv->n_pages >= INT32_MAX / kv->page_size)
+        return B200_EINVAL;
+    if (kv->type != B200_TYPE_F16 && kv->type != B200_TYPE_BF16) return B200_EUNSUPPORTED;
+    if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256) return B200_EUNSUPPORTED;
+    const int64_t strides = kv->k_page | kv->k_row | kv->k_head | kv->v_page | kv->v_row | kv->v_head;
+    if (!aligned16(kv->k) || !aligned16(kv->v) || (strides & 15) || strides < 0) return B200_EINVAL;
+    if ((kv->k_lo == nullptr) != (kv->k_hi == nullptr) || !aligned16(kv->k_lo) || !aligned16(kv->k_hi))
+        return B200_EINVAL;
+    return B200_OK;
+}
+
+// What the queries, the block table and the lengths of a batch must satisfy.
+int check_paged_batch(const b200_paged_kv* kv, const float* q, int64_t q_stride, int n_seq, int n_head,
+                      const int32_t* block_table, int64_t table_stride, int max_blocks, const int32_t* seq_lens) {
+    if (!q || !block_table || !seq_lens || n_seq < 0 || n_seq > 65535 || n_head <= 0 || n_head % kv->n_head_kv ||
+        n_head > 65535)
+        return B200_EINVAL;
+    if (!aligned16(q) || (q_stride & 3) || (n_seq > 1 && q_stride < (int64_t)n_head * kv->head_dim)) return B200_EINVAL;
+    if (max_blocks <= 0 || (n_seq > 1 && table_stride < max_blocks) || max_blocks > INT32_MAX / kv->page_size)
+        return B200_EINVAL;
+    return B200_OK;
+}
+
+template <bool BF16>
+int launch_paged_store(const PagedStoreArgs& a, cudaStream_t st) {
+    const dim3 grid((unsigned)a.n_tokens, (unsigned)a.kv.n_head_kv);
+    switch (a.kv.head_dim) {
+        case 64: paged_store_kernel<BF16, 64><<<grid, kStoreThreads, 0, st>>>(a); break;
+        case 128: paged_store_kernel<BF16, 128><<<grid, kStoreThreads, 0, st>>>(a); break;
+        default: paged_store_kernel<BF16, 256><<<grid, kStoreThreads, 0, st>>>(a); break;
+    }
+    return cuda_status(cudaGetLastError());
+}
+
+template <bool BF16>
+int launch_paged_select(const PagedSelectArgs& a, int head_dim, cudaStream_t st) {
+    const int64_t items = (int64_t)a.n_seq * a.max_blocks * a.n_head_kv;
+    const unsigned grid = (unsigned)((items + kSelectThreads / 32 - 1) / (kSelectThreads / 32));
+    switch (head_dim) {
+        case 64: paged_score_kernel<BF16, 64><<<grid, kSelectThreads, 0, st>>>(a); break;
+        case 128: paged_score_kernel<BF16, 128><<<grid, kSelectThreads, 0, st>>>(a); break;
+        default: paged_score_kernel<BF16, 256><<<grid, kSelectThreads, 0, st>>>(a); break;
+    }
+    CR_(cuda_status(cudaGetLastError()));
+    paged_topk_kernel<<<(unsigned)(a.n_seq * a.n_head_kv), kSelectThreads, 0, st>>>(a);
+    return cuda_status(cudaGetLastError());
+}
+
+template <bool BF16>
+int launch_paged_attn(const PagedAttnArgs& a, cudaStream_t st) {
+    const int G = a.n_head / a.kv.n_head_kv;
+    const dim3 grid((unsigned)(a.kv.n_head_kv * ((G + kPaHeads - 1) / kPaHeads)), (unsigned)a.n_seq);
+    switch (a.kv.head_dim) {
+        case 64: paged_attn_kernel<BF16, 64><<<grid, kPaThreads, 0, st>>>(a); break;
+        case 128: paged_attn_kernel<BF16, 128><<<grid, kPaThreads, 0, st>>>(a); break;
+        default: paged_attn_kernel<BF16, 256><<<grid, kPaThreads, 0, st>>>(a); break;
+    }
+    return cuda_status(cudaGetLastError());
+}
+
+}  // namespace
+
+extern "C" {
+
+int b200_paged_plan(const int32_t* new_lens, const int32_t* seq_lens, int n_seq, int32_t* block_table,
+                    int64_t table_stride, int max_blocks, int page_size, int32_t* free_pages, int64_t n_pages,
+                    const int32_t* n_free, int64_t max_tokens, int64_t* slots, int32_t* positions, int32_t* cu,
+                    int32_t* seq_lens_out, int32_t* n_free_out, b200_stream_t stream) {
+    if (!new_lens || !seq_lens || !block_table || !free_pages || !n_free || !cu || !seq_lens_out || !n_free_out)
+        return B200_EINVAL;
+    if (n_seq <= 0 || max_blocks <= 0 || page_size <= 0 || n_pages <= 0 || max_tokens < 0 || max_tokens >= INT32_MAX ||
+        (max_tokens > 0 && (!slots || !positions)) || (n_seq > 1 && table_stride < max_blocks) ||
+        max_blocks > INT32_MAX / page_size || n_pages >= INT32_MAX / page_size)
+        return B200_EINVAL;
+    if (n_seq > B200_PAGED_PLAN_MAX_SEQS) return B200_EUNSUPPORTED;
+    PagedPlanArgs a;
+    a.new_lens = new_lens;
+    a.seq_lens = seq_lens;
+    a.table = block_table;
+    a.table_stride = table_stride;
+    a.free_pages = free_pages;
+    a.n_free = n_free;
+    a.slots = slots;
+    a.positions = positions;
+    a.cu = cu;
+    a.seq_lens_out = seq_lens_out;
+    a.n_free_out = n_free_out;
+    a.n_seq = n_seq;
+    a.max_blocks = max_blocks;
+    a.page_size = page_size;
+    a.n_pages = (int)n_pages;
+    a.max_tokens = (int)max_tokens;
+    const size_t smem = plan_smem_bytes(n_seq);
+    CR_(cuda_status(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)plan_smem_bytes(B200_PAGED_PLAN_MAX_SEQS))));
+    paged_plan_kernel<<<1, kPlanThreads, smem, (cudaStream_t)stream>>>(a);
+    return cuda_status(cudaGetLastError());
+}
+
+int b200_paged_store(const b200_paged_kv* kv, const float* k, int64_t k_ld, const float* v, int64_t v_ld,
+                     const int64_t* slots, int64_t n_tokens, b200_stream_t stream) {
+    CR_(check_paged_kv(kv));
+    if (n_tokens == 0) return B200_OK;
+    const int64_t row = (int64_t)kv->n_head_kv * kv->head_dim;
+    if (!k || !v || !slots || n_tokens < 0 || n_tokens > INT32_MAX || kv->n_head_kv > 65535 || !aligned16(k) ||
+        !aligned16(v) || (k_ld & 3) || (v_ld & 3) || (n_tokens > 1 && (k_ld < row || v_ld < row)))
+        return B200_EINVAL;
+    PagedStoreArgs a;
+    a.kv = *kv;
+    a.k = k;
+    a.v = v;
+    a.k_ld = k_ld;
+    a.v_ld = v_ld;
+    a.slots = slots;
+    a.n_tokens = n_tokens;
+    return kv->type == B200_TYPE_BF16 ? launch_paged_store<true>(a, (cudaStream_t)stream)
+                                      : launch_paged_store<false>(a, (cudaStream_t)stream);
+}
+
+size_t b200_paged_select_workspace_size(int n_seq, int n_head_kv, int max_blocks) {
+    if (n_seq < 0 || n_seq > 65535 || n_head_kv <= 0 || n_head_kv > 65535 || max_blocks <= 0 ||
+        max_blocks > B200_PAGED_SELECT_MAX_BLOCKS)
+        return 0;
+    return std::max((size_t)16, (size_t)n_seq * n_head_kv * max_blocks * sizeof(unsigned long long));
+}
+
+int b200_paged_select(const b200_paged_kv* kv, const float* q, int64_t q_stride, int n_seq, int n_head,
+                      const int32_t* block_table, int64_t table_stride, int max_blocks, const int32_t* seq_lens,
+                      int n_sel, int32_t* sel, void* workspace, size_t workspace_size, b200_stream_t stream) {
+    CR_(check_paged_kv(kv));
+    if (n_seq == 0) return B200_OK;
+    CR_(check_paged_batch(kv, q, q_stride, n_seq, n_head, block_table, table_stride, max_blocks, seq_lens));
+    if (!kv->k_lo || !sel || n_sel <= 0 || !workspace || !aligned16(workspace)) return B200_EINVAL;
+    if (max_blocks > B200_PAGED_SELECT_MAX_BLOCKS) return B200_EUNSUPPORTED;
+    if (workspace_size < b200_paged_select_workspace_size(n_seq, kv->n_head_kv, max_blocks)) return B200_EINVAL;
+    PagedSelectArgs a;
+    a.lo = static_cast<const uint16_t*>(kv->k_lo);
+    a.hi = static_cast<const uint16_t*>(kv->k_hi);
+    a.q = q;
+    a.q_stride = q_stride;
+    a.table = block_table;
+    a.table_stride = table_stride;
+    a.seq_lens = seq_lens;
+    a.sel = sel;
+    a.keys = static_cast<unsigned long long*>(workspace);
+    a.n_seq = n_seq;
+    a.n_head = n_head;
+    a.n_head_kv = kv->n_head_kv;
+    a.max_blocks = max_blocks;
+    a.page_size = kv->page_size;
+    a.n_pages = (int)kv->n_pages;
+    a.n_sel = n_sel;
+    return kv->type == B200_TYPE_BF16 ? launch_paged_select<true>(a, kv->head_dim, (cudaStream_t)stream)
+                                      : launch_paged_select<false>(a, kv->head_dim, (cudaStream_t)stream);
+}
+
+size_t b200_paged_attn_workspace_size(int head_dim, int n_seq, int n_head, int n_head_kv) {
+    if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || n_seq < 0 || n_seq > 65535 || n_head <= 0 ||
+        n_head > 65535 || n_head_kv <= 0 || n_head % n_head_kv)
+        return 0;
+    return 16;
+}
+
+int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, int n_seq, int n_head,
+                    const int32_t* block_table, int64_t table_stride, int max_blocks, const int32_t* seq_lens,
+                    const void* mask, int64_t mask_stride, const int32_t* sel, int n_sel, float scale, float* out,
+                    void* workspace, size_t workspace_size, b200_stream_t stream) {
+    CR_(check_paged_kv(kv));
+    if (n_seq == 0) return B200_OK;
+    CR_(check_paged_batch(kv, q, q_stride, n_seq, n_head, block_table, table_stride, max_blocks, seq_lens));
+    if (!out || !aligned16(out) || !workspace || !aligned16(workspace) || (sel && n_sel <= 0) ||
+        (reinterpret_cast<uintptr_t>(mask) & 1) ||
+        (mask && n_seq > 1 && mask_stride < (int64_t)max_blocks * kv->page_size) ||
+        workspace_size < b200_paged_attn_workspace_size(kv->head_dim, n_seq, n_head, kv->n_head_kv))
+        return B200_EINVAL;
+    PagedAttnArgs a;
+    a.kv = *kv;
+    a.q = q;
+    a.q_stride = q_stride;
+    a.table = block_table;
+    a.table_stride = table_stride;
+    a.seq_lens = seq_lens;
+    a.mask = static_cast<const uint16_t*>(mask);
+    a.mask_stride = mask_stride;
+    a.sel = sel;
+    a.out = out;
+    a.scale = scale;
+    a.n_seq = n_seq;
+    a.n_head = n_head;
+    a.n_sel = n_sel;
+    a.max_blocks = max_blocks;
+    return kv->type == B200_TYPE_BF16 ? launch_paged_attn<true>(a, (cudaStream_t)stream)
+                                      : launch_paged_attn<false>(a, (cudaStream_t)stream);
+}
+
+}  // extern "C"
