@@ -59,17 +59,44 @@ int launch_paged_select(const PagedSelectArgs& a, int head_dim, cudaStream_t st)
     return cuda_status(cudaGetLastError());
 }
 
-template <bool BF16>
-int launch_paged_attn(const PagedAttnArgs& a, cudaStream_t st) {
-    const int G = a.n_head / a.kv.n_head_kv;
-    const dim3 grid((unsigned)(a.kv.n_head_kv * ((G + kPaHeads - 1) / kPaHeads)), (unsigned)a.n_seq);
-    switch (a.kv.head_dim) {
-        case 64: paged_attn_kernel<BF16, 64><<<grid, kPaThreads, 0, st>>>(a); break;
-        case 128: paged_attn_kernel<BF16, 128><<<grid, kPaThreads, 0, st>>>(a); break;
-        default: paged_attn_kernel<BF16, 256><<<grid, kPaThreads, 0, st>>>(a); break;
-    }
+bool g_paged_attn_attr[kMaxDevices][2][3];
+
+// Opts an instantiation into its shared memory, once per device.
+template <bool BF16, int D>
+int set_paged_attn_attr() {
+    const int dev = current_device();
+    if (dev < 0 || dev >= kMaxDevices) return B200_EINVAL;
+    bool& done = g_paged_attn_attr[dev][BF16][D == 64 ? 0 : D == 128 ? 1 : 2];
+    std::lock_guard<std::mutex> lk(g_attr_mu);
+    if (done) return B200_OK;
+    CR_(cuda_status(cudaFuncSetAttribute(paged_attn_kernel<BF16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         pa_smem<D>())));
+    done = true;
+    return B200_OK;
+}
+
+template <bool BF16, int D>
+int launch_paged_attn_d(const PagedAttnArgs& a, cudaStream_t st) {
+    CR_((set_paged_attn_attr<BF16, D>()));
+    // the lengths are on the device: at most this many units
+    const int64_t width = (int64_t)(a.sel ? a.n_sel : a.max_blocks) * a.kv.page_size;
+    const int64_t units = (int64_t)a.n_seq * a.kv.n_head_kv * a.chunks * ((width + kPaTok - 1) / kPaTok);
+    const int64_t grid = std::min<int64_t>(kPaCtas, (units + pa_warps(D) - 1) / pa_warps(D));
+    paged_attn_kernel<BF16, D><<<(unsigned)grid, 32 * pa_warps(D), pa_smem<D>(), st>>>(a);
     return cuda_status(cudaGetLastError());
 }
+
+template <bool BF16>
+int launch_paged_attn(const PagedAttnArgs& a, cudaStream_t st) {
+    switch (a.kv.head_dim) {
+        case 64: return launch_paged_attn_d<BF16, 64>(a, st);
+        case 128: return launch_paged_attn_d<BF16, 128>(a, st);
+        default: return launch_paged_attn_d<BF16, 256>(a, st);
+    }
+}
+
+int paged_chunks(int n_head, int n_head_kv) { return (n_head / n_head_kv + kPaHeads - 1) / kPaHeads; }
+size_t paged_pieces_bytes(int head_dim) { return align256((size_t)kPaCtas * 2 * pa_piece(head_dim) * sizeof(float)); }
 
 }  // namespace
 
@@ -171,7 +198,8 @@ size_t b200_paged_attn_workspace_size(int head_dim, int n_seq, int n_head, int n
     if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || n_seq < 0 || n_seq > 65535 || n_head <= 0 ||
         n_head > 65535 || n_head_kv <= 0 || n_head % n_head_kv)
         return 0;
-    return 16;
+    return paged_pieces_bytes(head_dim) +
+           align256((size_t)n_seq * n_head_kv * paged_chunks(n_head, n_head_kv) * sizeof(unsigned int));
 }
 
 int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, int n_seq, int n_head,
@@ -184,6 +212,8 @@ int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, i
     if (!out || !aligned16(out) || !workspace || !aligned16(workspace) || (sel && n_sel <= 0) ||
         (reinterpret_cast<uintptr_t>(mask) & 1) ||
         (mask && n_seq > 1 && mask_stride < (int64_t)max_blocks * kv->page_size) ||
+        (sel && n_sel > INT32_MAX / kv->page_size) ||
+        (int64_t)n_seq * kv->n_head_kv * paged_chunks(n_head, kv->n_head_kv) > INT32_MAX ||
         workspace_size < b200_paged_attn_workspace_size(kv->head_dim, n_seq, n_head, kv->n_head_kv))
         return B200_EINVAL;
     PagedAttnArgs a;
@@ -197,6 +227,9 @@ int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, i
     a.mask_stride = mask_stride;
     a.sel = sel;
     a.out = out;
+    a.chunks = paged_chunks(n_head, kv->n_head_kv);
+    a.pieces = static_cast<float*>(workspace);
+    a.tickets = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(workspace) + paged_pieces_bytes(kv->head_dim));
     a.scale = scale;
     a.n_seq = n_seq;
     a.n_head = n_head;
