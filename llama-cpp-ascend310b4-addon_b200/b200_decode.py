@@ -593,20 +593,19 @@ def _bad(what: str, msg: str):
     raise B200Error(EINVAL, f"{what}: {msg}")
 
 
-class _on:
-    """The device's context current inside the block (a no-op when it is)."""
-
-    def __init__(self, device):
-        torch = _torch()
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+def _launch(what: str, device, fn, *args):
+    """fn(*args, stream) on the device's current stream, the device current.
+    A call costs the host about as much as a small kernel takes, so this asks
+    for the bare stream handle (torch.cuda.current_stream builds an object)."""
+    torch = _torch()
+    i = device.index
+    if torch.cuda.current_device() == i:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc != OK:
+        _check(rc, what)
 
 
 class PagedKV:
@@ -658,11 +657,15 @@ class PagedPlan:
         self.slots, self.positions, self.cu, self.seq_lens, self.n_free = slots, positions, cu, seq_lens, n_free
 
 
-def _check_i32(what, device, **tensors):
+def _check_i32(what, device, names, *tensors):
     torch = _torch()
-    for name, t in tensors.items():
+    for name, t in zip(names, tensors):
         if t.dtype != torch.int32 or t.device != device or (t.dim() == 1 and not t.is_contiguous()):
             _bad(what, f"{name} must be a contiguous int32 tensor on {device}")
+
+
+_PLAN_I32 = ("new_lens", "seq_lens", "block_table", "free_pages", "n_free", "seq_lens_out", "n_free_out", "cu",
+             "positions")
 
 
 def paged_plan(new_lens, seq_lens, block_table, free_pages, n_free, page_size: int, max_tokens: int,
@@ -691,26 +694,22 @@ def paged_plan(new_lens, seq_lens, block_table, free_pages, n_free, page_size: i
     if n_free_out is None:
         n_free_out = n_free
     if cu is None:
-        cu = torch.empty(n + 1, dtype=torch.int32, device=dev)
+        cu = seq_lens.new_empty(n + 1)
     if slots is None:
         slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
     if positions is None:
-        positions = torch.empty(max_tokens, dtype=torch.int32, device=dev)
-    _check_i32("paged_plan", dev, new_lens=new_lens, seq_lens=seq_lens, block_table=block_table,
-               free_pages=free_pages, n_free=n_free, seq_lens_out=seq_lens_out, n_free_out=n_free_out, cu=cu,
-               positions=positions)
+        positions = seq_lens.new_empty(max_tokens)
+    _check_i32("paged_plan", dev, _PLAN_I32, new_lens, seq_lens, block_table, free_pages, n_free, seq_lens_out,
+               n_free_out, cu, positions)
     if (free_pages.dim() != 1 or n_free.numel() != 1 or n_free_out.numel() != 1 or seq_lens_out.shape != seq_lens.shape
             or cu.dim() != 1 or cu.numel() < n + 1 or positions.dim() != 1 or positions.numel() < max_tokens
             or slots.dtype != torch.int64 or slots.device != dev or slots.dim() != 1 or not slots.is_contiguous()
             or slots.numel() < max_tokens):
         _bad("paged_plan", "free_pages [n_pages], n_free [1], cu [n_seq + 1] and slots, positions [max_tokens]")
-    with _on(dev):
-        rc = lib().b200_paged_plan(new_lens.data_ptr(), seq_lens.data_ptr(), n, block_table.data_ptr(),
-                                   block_table.stride(0), block_table.shape[1], page_size, free_pages.data_ptr(),
-                                   free_pages.numel(), n_free.data_ptr(), max_tokens, slots.data_ptr(),
-                                   positions.data_ptr(), cu.data_ptr(), seq_lens_out.data_ptr(),
-                                   n_free_out.data_ptr(), _stream(dev))
-    _check(rc, "paged_plan")
+    _launch("paged_plan", dev, lib().b200_paged_plan, new_lens.data_ptr(), seq_lens.data_ptr(), n,
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], page_size, free_pages.data_ptr(),
+            free_pages.numel(), n_free.data_ptr(), max_tokens, slots.data_ptr(), positions.data_ptr(), cu.data_ptr(),
+            seq_lens_out.data_ptr(), n_free_out.data_ptr())
     return PagedPlan(slots, positions, cu, seq_lens_out, n_free_out)
 
 
@@ -718,12 +717,16 @@ def _rows_f32(what, name, t, row, dev):
     """t as f32 rows of `row` contiguous values, 16-byte aligned (copied when
     it is not); its row stride in floats."""
     torch = _torch()
-    if t.dtype != torch.float32 or t.device != dev or t.dim() not in (2, 3) or t[0:1].numel() not in (0, row):
+    shape, stride = t.shape, t.stride()
+    width = shape[1] if len(shape) == 2 else shape[1] * shape[2] if len(shape) == 3 else -1
+    if t.dtype != torch.float32 or t.device != dev or width != row:
         _bad(what, f"{name} must be f32 rows of {row} values on {dev}")
-    inner = t.stride(-1) == 1 and (t.dim() == 2 or t.stride(1) == t.shape[2] or t.shape[1] == 1)
-    if not inner or t.stride(0) % 4 or t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) < row):
-        t = t.contiguous() if not t.is_contiguous() else t.clone()
-    return t, t.stride(0)
+    ld = stride[0]
+    if (stride[-1] != 1 or (len(shape) == 3 and stride[1] != shape[2] and shape[1] != 1) or ld % 4
+            or t.data_ptr() % 16 or (shape[0] > 1 and ld < row)):
+        t = t.clone(memory_format=torch.contiguous_format)
+        ld = row
+    return t, ld
 
 
 def paged_store(cache: PagedKV, k, v, slots):
@@ -739,25 +742,26 @@ def paged_store(cache: PagedKV, k, v, slots):
         _bad("paged_store", "slots must be a contiguous int64 [n_tokens] on the cache's device, one per row of k and v")
     k, k_ld = _rows_f32("paged_store", "k", k, row, dev)
     v, v_ld = _rows_f32("paged_store", "v", v, row, dev)
-    with _on(dev):
-        rc = lib().b200_paged_store(cache._ref, k.data_ptr(), k_ld, v.data_ptr(), v_ld, slots.data_ptr(),
-                                    slots.numel(), _stream(dev))
-    _check(rc, "paged_store")
+    _launch("paged_store", dev, lib().b200_paged_store, cache._ref, k.data_ptr(), k_ld, v.data_ptr(), v_ld,
+            slots.data_ptr(), slots.numel())
 
 
 def _paged_batch(what, cache, q, block_table, seq_lens):
     torch = _torch()
-    dev = cache.device
-    if q.dim() != 3 or q.dtype != torch.float32 or q.device != dev or q.shape[2] != cache.head_dim:
+    dev, shape = cache.device, q.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim:
         _bad(what, "q must be f32 [n_seq, n_head, head_dim] on the cache's device")
-    n_seq, n_head = q.shape[0], q.shape[1]
+    n_seq, n_head = shape[0], shape[1]
     if n_head == 0 or n_head % cache.n_head_kv:
         _bad(what, "n_head must be a multiple of the cache's n_head_kv")
-    _check_i32(what, dev, block_table=block_table, seq_lens=seq_lens)
-    if (block_table.dim() != 2 or block_table.shape[0] != n_seq or block_table.stride(1) != 1
-            or block_table.shape[1] == 0 or seq_lens.dim() != 1 or seq_lens.numel() != n_seq):
-        _bad(what, "block_table must be [n_seq, max_blocks] with contiguous rows and seq_lens [n_seq]")
-    return _rows_f32(what, "q", q, n_head * cache.head_dim, dev) + (n_seq, n_head)
+    ts, i32 = block_table.shape, torch.int32
+    if (block_table.dtype != i32 or block_table.device != dev or len(ts) != 2 or ts[0] != n_seq or ts[1] == 0
+            or block_table.stride(1) != 1 or seq_lens.dtype != i32 or seq_lens.device != dev
+            or seq_lens.shape != shape[:1] or not seq_lens.is_contiguous()):
+        _bad(what, "block_table must be int32 [n_seq, max_blocks] with contiguous rows and seq_lens int32 [n_seq], "
+                   "on the cache's device")
+    q, ld = _rows_f32(what, "q", q, n_head * cache.head_dim, dev)
+    return q, ld, n_seq, n_head
 
 
 def _paged_workspace(what, workspace, size, dev, zeros):
@@ -787,7 +791,7 @@ def paged_select(cache: PagedKV, q, block_table, seq_lens, n_sel: int, sel=None,
     if sel is None:
         if n_sel <= 0:
             _bad("paged_select", "n_sel must be positive")
-        sel = torch.empty(shape, dtype=torch.int32, device=dev)
+        sel = seq_lens.new_empty(shape)
     elif sel.dtype != torch.int32 or sel.device != dev or not sel.is_contiguous() or tuple(sel.shape) != shape:
         _bad("paged_select", "sel must be a contiguous int32 [n_seq, n_head_kv, n_sel]")
     if workspace is None:
@@ -795,11 +799,9 @@ def paged_select(cache: PagedKV, q, block_table, seq_lens, n_sel: int, sel=None,
         workspace = _paged_workspace("paged_select", None, size, dev, zeros=False)
     else:
         _paged_workspace("paged_select", workspace, 0, dev, zeros=False)
-    with _on(dev):
-        rc = lib().b200_paged_select(cache._ref, q.data_ptr(), q_stride, n_seq, n_head, block_table.data_ptr(),
-                                     block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), n_sel,
-                                     sel.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream(dev))
-    _check(rc, "paged_select")
+    _launch("paged_select", dev, lib().b200_paged_select, cache._ref, q.data_ptr(), q_stride, n_seq, n_head,
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), n_sel,
+            sel.data_ptr(), workspace.data_ptr(), workspace.numel())
     return sel
 
 
@@ -834,7 +836,7 @@ def paged_attn(cache: PagedKV, q, block_table, seq_lens, scale: float, mask=None
         _bad("paged_attn", "sel must be a contiguous int32 [n_seq, n_head_kv, n_sel]")
     shape = (n_seq, n_head, cache.head_dim)
     if out is None:
-        out = torch.empty(shape, dtype=torch.float32, device=dev)
+        out = q.new_empty(shape)
     elif out.dtype != torch.float32 or out.device != dev or not out.is_contiguous() or tuple(out.shape) != shape:
         _bad("paged_attn", "out must be a contiguous f32 [n_seq, n_head, head_dim]")
     if workspace is None:
@@ -842,12 +844,9 @@ def paged_attn(cache: PagedKV, q, block_table, seq_lens, scale: float, mask=None
         workspace = _paged_workspace("paged_attn", None, size, dev, zeros=True)
     else:
         _paged_workspace("paged_attn", workspace, 0, dev, zeros=True)
-    with _on(dev):
-        rc = lib().b200_paged_attn(cache._ref, q.data_ptr(), q_stride, n_seq, n_head, block_table.data_ptr(),
-                                   block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
-                                   None if mask is None else mask.data_ptr(), 0 if mask is None else mask.stride(0),
-                                   None if sel is None else sel.data_ptr(), 0 if sel is None else sel.shape[2],
-                                   float(scale), out.data_ptr(), workspace.data_ptr(), workspace.numel(),
-                                   _stream(dev))
-    _check(rc, "paged_attn")
+    _launch("paged_attn", dev, lib().b200_paged_attn, cache._ref, q.data_ptr(), q_stride, n_seq, n_head,
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
+            None if mask is None else mask.data_ptr(), 0 if mask is None else mask.stride(0),
+            None if sel is None else sel.data_ptr(), 0 if sel is None else sel.shape[2], scale, out.data_ptr(),
+            workspace.data_ptr(), workspace.numel())
     return out
