@@ -213,9 +213,11 @@ int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, i
         (reinterpret_cast<uintptr_t>(mask) & 1) ||
         (mask && n_seq > 1 && mask_stride < (int64_t)max_blocks * kv->page_size) ||
         (sel && n_sel > INT32_MAX / kv->page_size) ||
-        (int64_t)n_seq * kv->n_head_kv * paged_chunks(n_head, kv->n_head_kv) > INT32_MAX ||
         workspace_size < b200_paged_attn_workspace_size(kv->head_dim, n_seq, n_head, kv->n_head_kv))
         return B200_EINVAL;
+    const int64_t width = (int64_t)(sel ? n_sel : max_blocks) * kv->page_size;
+    const int64_t segments = (int64_t)n_seq * kv->n_head_kv * paged_chunks(n_head, kv->n_head_kv);
+    if (segments * ((width + kPaTok - 1) / kPaTok) > INT32_MAX) return B200_EUNSUPPORTED;  // units are counted in int
     PagedAttnArgs a;
     a.kv = *kv;
     a.q = q;

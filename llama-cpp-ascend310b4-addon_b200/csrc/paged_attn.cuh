@@ -53,12 +53,13 @@ B200_HD constexpr int pa_tile(int D) { return kPaTok * D * 2; }
 // Bookkeeping beside the ring and the pieces in shared memory.
 template <int W, int S>
 struct PaShared {
-    long long part[W], base[W];   // prefix-sum partials; first unit of the sequence a warp starts in
-    long long from[2 * W];        // first unit of a piece's segment
-    int seq[W];                   // the sequence a warp starts in
-    int seg[2 * W], nu[2 * W];    // a piece's segment (-1: no piece) and its units
+    int part[W], base[W];       // prefix-sum partials; first unit of the sequence a warp starts in
+    int seq[W];                 // the sequence a warp starts in
+    int from[2 * W];            // first unit of a piece's segment
+    int seg[2 * W], nu[2 * W];  // a piece's segment (-1: no piece) and its units
     unsigned valid[W][S], live[W][S];  // positions of a stage that exist; that the mask leaves in
     float mask[W][S][kPaTok];
+    float joint[3][kPaHeads];   // a joined segment's maxima, sums, mask reference
     int last;
 };
 template <int D>
@@ -169,25 +170,59 @@ __device__ __forceinline__ float pa_rel(float m, float mk, float mk_all) {
     return m == -INFINITY ? -INFINITY : m + (mk - mk_all) * 1.44269504f;
 }
 
-// Joins n pieces (piece(i) -> address, in shared memory or, written by other
-// CTAs, in global memory) for element e of the 8 x D outputs: the
-// unnormalised value, and the references and sum of its head.
-template <int D, bool GLOBAL, class F>
-__device__ __forceinline__ float pa_join(int n, int e, F piece, float& m, float& l, float& mk) {
-    const int at_m = kPaHeads * D + e / D, at_l = at_m + kPaHeads, at_mk = kPaHeads * D + 2 * kPaHeads;
+// Joins n pieces of a segment (piece(i) -> address, in shared memory or,
+// written by other CTAs, in global memory): put(e, v) receives the
+// unnormalised values of outputs e .. e + 3, with the references and sums of
+// the 8 heads in `joint`.  wgt: n x 8 floats of shared memory.  A warp per
+// head finds the pieces' weights, a lane per piece; the values are then summed
+// four columns a thread, in order of the pieces, eight loads in flight.
+template <int D, int T, bool GLOBAL, class F, class G>
+__device__ __forceinline__ void pa_join(int n, F piece, float* wgt, float (&joint)[3][kPaHeads], G put) {
+    constexpr int W = T / 32, AT_M = kPaHeads * D, AT_L = AT_M + kPaHeads, AT_MK = AT_L + kPaHeads;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     auto ld = [](const float* p) { return GLOBAL ? __ldcg(p) : *p; };
-    mk = -INFINITY, m = -INFINITY, l = 0.f;
-    for (int i = 0; i < n; ++i) mk = fmaxf(mk, ld(piece(i) + at_mk));
-    for (int i = 0; i < n; ++i) m = fmaxf(m, pa_rel(ld(piece(i) + at_m), ld(piece(i) + at_mk), mk));
-    float o = 0.f;
-    if (m == -INFINITY) return o;
-    for (int i = 0; i < n; ++i) {
-        const float* p = piece(i);
-        const float w = pa_exp2(pa_rel(ld(p + at_m), ld(p + at_mk), mk) - m);
-        l += w * ld(p + at_l);
-        o += w * ld(p + e);
+    for (int j = warp; j < kPaHeads; j += W) {
+        float mk = -INFINITY;
+        for (int k = lane; k < n; k += 32) mk = fmaxf(mk, ld(piece(k) + AT_MK));
+        mk = warp_max(mk);
+        float m = -INFINITY;
+        for (int k = lane; k < n; k += 32) m = fmaxf(m, pa_rel(ld(piece(k) + AT_M + j), ld(piece(k) + AT_MK), mk));
+        m = warp_max(m);
+        float l = 0.f;
+        for (int k = lane; k < n; k += 32) {
+            const float r = pa_rel(ld(piece(k) + AT_M + j), ld(piece(k) + AT_MK), mk);
+            const float w = r == -INFINITY ? 0.f : pa_exp2(r - m);
+            wgt[k * kPaHeads + j] = w;
+            l += w * ld(piece(k) + AT_L + j);
+        }
+        l = warp_sum(l);
+        if (lane == 0) joint[0][j] = m, joint[1][j] = l, joint[2][j] = mk;
     }
-    return o;
+    __syncthreads();
+    for (int e = 4 * (int)threadIdx.x; e < kPaHeads * D; e += 4 * T) {
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        int k = 0;
+        for (; k + 8 <= n; k += 8) {
+            float4 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float4* p = reinterpret_cast<const float4*>(piece(k + i) + e);
+                v[i] = GLOBAL ? __ldcg(p) : *p;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float w = wgt[(k + i) * kPaHeads + e / D];
+                o.x += w * v[i].x, o.y += w * v[i].y, o.z += w * v[i].z, o.w += w * v[i].w;
+            }
+        }
+        for (; k < n; ++k) {
+            const float4* p = reinterpret_cast<const float4*>(piece(k) + e);
+            const float4 v = GLOBAL ? __ldcg(p) : *p;
+            const float w = wgt[k * kPaHeads + e / D];
+            o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
+        }
+        put(e, o);
+    }
 }
 
 template <bool BF16, int D>
@@ -208,37 +243,38 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
     // ---- the lengths' prefix sums: this CTA's range and its warps' starts ----
     const int per = (a.n_seq + T - 1) / T;
     const int s_lo = min(a.n_seq, tid * per), s_hi = min(a.n_seq, s_lo + per);
-    long long mine = 0;
+    int mine = 0;
     for (int s = s_lo; s < s_hi; ++s) {
         const int len = a.seq_lens[s];
         if (blockIdx.x == 0 && (len < 0 || len > a.max_blocks * ps)) record_status(B200_DEVSTATUS_BOUNDS);
         mine += pa_units(a, pa_len(a, s));
     }
-    long long incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+        const int x = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += x;
     }
     if (lane == 31) sh.part[warp] = incl;
     if (tid < 2 * W) sh.seg[tid] = -1;
     __syncthreads();
-    long long total = 0;
+    int total = 0;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
         if (w < warp) incl += sh.part[w];
         total += sh.part[w];
     }
     total *= hh_n;
-    const long long per_cta = max((total + gridDim.x - 1) / gridDim.x, (long long)W);
-    const long long cb = min(total, per_cta * blockIdx.x), ce = min(total, cb + per_cta);
+    const int per_cta = max((int)((total + gridDim.x - 1u) / gridDim.x), W);
+    const int cb = (int)min((unsigned)total, (unsigned)per_cta * blockIdx.x);
+    const int ce = (int)min((unsigned)total, (unsigned)cb + (unsigned)per_cta);
     {
-        long long at = (incl - mine) * hh_n;
+        int at = (incl - mine) * hh_n;
         for (int s = s_lo; s < s_hi; ++s) {
-            const long long end = at + (long long)pa_units(a, pa_len(a, s)) * hh_n;
+            const int end = at + pa_units(a, pa_len(a, s)) * hh_n;
             if (end > cb && at < ce)
                 for (int w = 0; w < W; ++w) {
-                    const long long b = cb + (ce - cb) * w / W;
+                    const int b = cb + (ce - cb) * w / W;
                     if (b >= at && b < end) sh.seq[w] = s, sh.base[w] = at;
                 }
             at = end;
@@ -255,18 +291,18 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
     float* const heads = reinterpret_cast<float*>(pa_sm + W * S * 2 * TILE);
     float* const head_piece = heads + warp * PIECE;  // a segment begun by an earlier warp
     float* const tail_piece = reinterpret_cast<float*>(pa_sm + warp * (S * 2 * TILE));  // one left to a later warp
-    const long long fb = cb + (ce - cb) * warp / W, fe = cb + (ce - cb) * (warp + 1) / W;
+    const int fb = cb + (ce - cb) * warp / W, fe = cb + (ce - cb) * (warp + 1) / W;
 
     if (fb < fe) {
         PaCursor in, cur;
         in.s = sh.seq[warp];
         in.len = pa_len(a, in.s);
         in.nu = pa_units(a, in.len);
-        in.hh = (int)((fb - sh.base[warp]) / in.nu);
-        in.u = (int)((fb - sh.base[warp]) % in.nu);
+        in.hh = (fb - sh.base[warp]) / in.nu;
+        in.u = (fb - sh.base[warp]) - in.hh * in.nu;
         cur = in;
-        long long seg_from = fb - in.u;  // first unit of the current segment
-        long long to_issue = fe - fb, to_do = to_issue;
+        int seg_from = fb - in.u;  // first unit of the current segment
+        int to_issue = fe - fb, to_do = to_issue;
 
         // ---- producer: this lane looks after token lane & 15 of a unit ----
         const int q16 = kPaTok / ps, r16 = kPaTok % ps;
@@ -364,43 +400,42 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
         // ---- consumer: this thread holds head g, positions 2 t4, 2 t4 + 1 (+ 8) ----
         uint32_t qf[KT][4], q3[BF16 ? KT : 1][2];
         float o[2 * KT][2], m = -INFINITY, l = 0.f, mk = -INFINITY, f = 0.f;
-        bool begin = true;
+        auto load_q = [&]() {
+            const int chunk = cur.hh % a.chunks, head = cur.hh / a.chunks;
+            const int j = chunk * kPaHeads + g;
+            const float* qr = a.q + cur.s * a.q_stride + (int64_t)(head * G + (j < G ? j : 0)) * D + 2 * t4;
+            float2 x[2 * KT];
+            float amax = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2 * KT; ++i) {
+                x[i] = *reinterpret_cast<const float2*>(qr + 8 * i);
+                if (j >= G) x[i] = make_float2(0.f, 0.f);
+                amax = fmaxf(amax, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+            }
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            // q 2^-ex has its largest entry in [1, 2)
+            const int ex = min(max((int)(__float_as_uint(amax) >> 23) - 127, -120), 120);
+            const float up = __uint_as_float((unsigned)(127 - ex) << 23);
+            f = a.scale * 1.44269504f * __uint_as_float((unsigned)(127 + ex) << 23);
+#pragma unroll
+            for (int i = 0; i < 2 * KT; ++i) {
+                x[i].x *= up, x[i].y *= up;
+                qf[i >> 1][2 * (i & 1)] = pa_split<BF16>(x[i].x, x[i].y);
+                qf[i >> 1][2 * (i & 1) + 1] = pa_split<BF16>(x[i].x, x[i].y);
+                if (BF16) q3[i >> 1][i & 1] = pa_split<BF16>(x[i].x, x[i].y);
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * KT; ++i) o[i][0] = o[i][1] = 0.f;
+            m = -INFINITY, l = 0.f, mk = a.mask != nullptr ? -INFINITY : 0.f;
+        };
+        load_q();
         int stage = 0;
         const int mi = lane >> 3, ri = lane & 7;
         for (; to_do > 0; --to_do) {
             pa_wait<S - 2>();
             __syncwarp();
             issue(stage == 0 ? S - 1 : stage - 1);
-            if (begin) {
-                const int chunk = cur.hh % a.chunks, head = cur.hh / a.chunks;
-                const int j = chunk * kPaHeads + g;
-                const float* qr = a.q + cur.s * a.q_stride + (int64_t)(head * G + (j < G ? j : 0)) * D + 2 * t4;
-                float2 x[2 * KT];
-                float amax = 0.f;
-#pragma unroll
-                for (int i = 0; i < 2 * KT; ++i) {
-                    x[i] = *reinterpret_cast<const float2*>(qr + 8 * i);
-                    if (j >= G) x[i] = make_float2(0.f, 0.f);
-                    amax = fmaxf(amax, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
-                }
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                // q 2^-ex has its largest entry in [1, 2)
-                const int ex = min(max((int)(__float_as_uint(amax) >> 23) - 127, -120), 120);
-                const float up = __uint_as_float((unsigned)(127 - ex) << 23);
-                f = a.scale * 1.44269504f * __uint_as_float((unsigned)(127 + ex) << 23);
-#pragma unroll
-                for (int i = 0; i < 2 * KT; ++i) {
-                    x[i].x *= up, x[i].y *= up;
-                    qf[i >> 1][2 * (i & 1)] = pa_split<BF16>(x[i].x, x[i].y);
-                    qf[i >> 1][2 * (i & 1) + 1] = pa_split<BF16>(x[i].x, x[i].y);
-                    if (BF16) q3[i >> 1][i & 1] = pa_split<BF16>(x[i].x, x[i].y);
-                }
-#pragma unroll
-                for (int i = 0; i < 2 * KT; ++i) o[i][0] = o[i][1] = 0.f;
-                m = -INFINITY, l = 0.f, mk = a.mask != nullptr ? -INFINITY : 0.f;
-                begin = false;
-            }
             const unsigned valid = sh.valid[warp][stage];
             const unsigned live = a.mask != nullptr ? sh.live[warp][stage] : valid;
             const uint32_t kst = ring + stage * (2 * TILE), vst = kst + TILE;
@@ -521,10 +556,12 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                         sh.nu[2 * warp + tail] = cur.nu;
                     }
                 }
-                begin = true;
             }
-            if (seg_end) seg_from += cur.nu;
-            if (to_do > 1 && !pa_advance(a, cur, hh_n)) break;
+            if (to_do > 1) {
+                if (seg_end) seg_from += cur.nu;
+                if (!pa_advance(a, cur, hh_n)) break;
+                if (seg_end) load_q();
+            }
         }
         pa_wait<0>();
     }
@@ -534,6 +571,9 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
     auto piece_at = [&](int i) -> float* {
         return (i & 1) ? reinterpret_cast<float*>(pa_sm + (i >> 1) * (S * 2 * TILE)) : heads + (i >> 1) * PIECE;
     };
+    // weights of the pieces being joined: in warp 0's ring, behind its tail piece
+    float* const wgt = reinterpret_cast<float*>(pa_sm + align256(PIECE * 4));
+    static_assert(kPaCtas * kPaHeads * 4 + PIECE * 4 + 256 <= S * 2 * TILE, "weights beside the tail piece");
     for (int i = 0; i < 2 * W;) {
         const int seg = sh.seg[i];
         if (seg < 0) {
@@ -543,44 +583,39 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
         int list[2 * W], n = 0;
         for (; i < 2 * W && (sh.seg[i] == seg || sh.seg[i] < 0); ++i)
             if (sh.seg[i] == seg) list[n++] = i;
-        const long long from = sh.from[list[0]], end = from + sh.nu[list[0]];
+        const int from = sh.from[list[0]], end = from + sh.nu[list[0]];
         const bool whole = from >= cb && end <= ce;
         const int s = seg / hh_n, hh = seg % hh_n, head = hh / a.chunks, j0 = (hh % a.chunks) * kPaHeads;
         float* out = a.out + ((int64_t)s * a.n_head + head * G + j0) * D;
         float* mine_g = a.pieces + (int64_t)(2 * blockIdx.x + (from >= cb ? 1 : 0)) * PIECE;
-        for (int e = tid; e < kPaHeads * D; e += T) {
-            float m, l, mk;
-            const float o = pa_join<D, false>(n, e, [&](int k) { return piece_at(list[k]); }, m, l, mk);
-            if (whole) {
-                if (j0 + e / D < G) out[e] = l > 0.f ? o / l : 0.f;
-            } else {
-                __stcg(mine_g + e, o);
-                if (e % D == 0) {
-                    __stcg(mine_g + kPaHeads * D + e / D, m);
-                    __stcg(mine_g + kPaHeads * D + kPaHeads + e / D, l);
-                    if (e == 0) __stcg(mine_g + kPaHeads * D + 2 * kPaHeads, mk);
-                }
-            }
-        }
-        if (whole) continue;
-        const int c0 = (int)(from / per_cta), c1 = (int)((end - 1) / per_cta);
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) sh.last = atomicAdd(a.tickets + seg, 1u) == (unsigned)(c1 - c0);
-        __syncthreads();
-        if (sh.last) {
+        auto finish = [&](int e, float4 o) {
+            const float l = sh.joint[1][e / D], inv = l > 0.f ? 1.f / l : 0.f;
+            if (j0 + e / D < G)
+                *reinterpret_cast<float4*>(out + e) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        };
+        pa_join<D, T, false>(n, [&](int k) -> const float* { return piece_at(list[k]); }, wgt, sh.joint,
+                             [&](int e, float4 o) {
+                                 if (whole) finish(e, o);
+                                 else __stcg(reinterpret_cast<float4*>(mine_g + e), o);
+                             });
+        if (!whole) {
+            if (tid < 2 * kPaHeads) __stcg(mine_g + kPaHeads * D + tid, sh.joint[tid / kPaHeads][tid % kPaHeads]);
+            if (tid == 0) __stcg(mine_g + kPaHeads * D + 2 * kPaHeads, sh.joint[2][0]);
+            const int c0 = from / per_cta, c1 = (end - 1) / per_cta;
             __threadfence();
-            for (int e = tid; e < kPaHeads * D; e += T) {
-                float m, l, mk;
-                const float o = pa_join<D, true>(
-                    c1 - c0 + 1, e,
+            __syncthreads();
+            if (tid == 0) sh.last = atomicAdd(a.tickets + seg, 1u) == (unsigned)(c1 - c0);
+            __syncthreads();
+            if (sh.last) {
+                __threadfence();
+                pa_join<D, T, true>(
+                    c1 - c0 + 1,
                     [&](int k) -> const float* { return a.pieces + (int64_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * PIECE; },
-                    m, l, mk);
-                if (j0 + e / D < G) out[e] = l > 0.f ? o / l : 0.f;
+                    wgt, sh.joint, finish);
+                if (tid == 0) a.tickets[seg] = 0u;
             }
-            if (tid == 0) a.tickets[seg] = 0u;
         }
-        __syncthreads();
+        __syncthreads();  // wgt and joint are free again
     }
 }
 
