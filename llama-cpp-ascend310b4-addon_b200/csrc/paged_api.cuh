@@ -199,7 +199,7 @@ size_t b200_paged_attn_workspace_size(int head_dim, int n_seq, int n_head, int n
         n_head > 65535 || n_head_kv <= 0 || n_head % n_head_kv)
         return 0;
     return paged_pieces_bytes(head_dim) +
-           align256((size_t)n_seq * n_head_kv * paged_chunks(n_head, n_head_kv) * sizeof(unsigned int));
+           align256((size_t)n_seq * n_head_kv * paged_chunks(n_head, n_head_kv) * kPaHeads * sizeof(unsigned int));
 }
 
 int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, int n_seq, int n_head,

@@ -53,14 +53,14 @@ B200_HD constexpr int pa_tile(int D) { return kPaTok * D * 2; }
 // Bookkeeping beside the ring and the pieces in shared memory.
 template <int W, int S>
 struct PaShared {
-    int part[W], base[W];       // prefix-sum partials; first unit of the sequence a warp starts in
-    int seq[W];                 // the sequence a warp starts in
-    int from[2 * W];            // first unit of a piece's segment
-    int seg[2 * W], nu[2 * W];  // a piece's segment (-1: no piece) and its units
+    int part[W];                // prefix-sum partials
+    int seq[W], base[W];        // the sequence a warp starts in and that one's first unit
+    // pieces of a warp, [0] of a segment begun by an earlier warp, [1] of one left
+    // to a later warp: segment (-1: none), its first unit and length, its first
+    // row of the output and rows
+    int seg[2][W], from[2][W], nu[2][W], row[2][W], rows[2][W];
     unsigned valid[W][S], live[W][S];  // positions of a stage that exist; that the mask leaves in
     float mask[W][S][kPaTok];
-    float joint[3][kPaHeads];   // a joined segment's maxima, sums, mask reference
-    int last;
 };
 template <int D>
 constexpr int pa_smem() {
@@ -80,7 +80,7 @@ struct PagedAttnArgs {
     const int32_t* sel;
     float* out;
     float* pieces;          // [kPaCtas][2][pa_piece]
-    unsigned int* tickets;  // [n_seq * n_head_kv * chunks], zero between calls
+    unsigned int* tickets;  // [n_seq * n_head_kv * chunks][8], zero between calls
     float scale;
     int n_seq, n_head, n_sel, max_blocks, chunks;
 };
@@ -136,9 +136,9 @@ __device__ __forceinline__ uint32_t pa_split(float& x, float& y) {
     return w;
 }
 
-// Where a warp is in its range: unit u of nu of the segment (s, hh).
+// Where a warp is in its range: unit u of nu of the segment (s, head, chunk).
 struct PaCursor {
-    int s, hh, u, nu, len;
+    int s, head, chunk, u, nu, len;
 };
 
 __device__ __forceinline__ int pa_len(const PagedAttnArgs& a, int s) {
@@ -151,11 +151,13 @@ __device__ __forceinline__ int pa_units(const PagedAttnArgs& a, int len) {
     return (int)(((unsigned)len + kPaTok - 1) / kPaTok);
 }
 // To the next unit; false past the last sequence.
-__device__ __forceinline__ bool pa_advance(const PagedAttnArgs& a, PaCursor& c, int hh_n) {
+__device__ __forceinline__ bool pa_advance(const PagedAttnArgs& a, PaCursor& c) {
     if (++c.u < c.nu) return true;
     c.u = 0;
-    if (++c.hh < hh_n) return true;
-    c.hh = 0;
+    if (++c.chunk < a.chunks) return true;
+    c.chunk = 0;
+    if (++c.head < a.kv.n_head_kv) return true;
+    c.head = 0;
     do {
         if (++c.s >= a.n_seq) return false;
         c.len = pa_len(a, c.s);
@@ -170,60 +172,62 @@ __device__ __forceinline__ float pa_rel(float m, float mk, float mk_all) {
     return m == -INFINITY ? -INFINITY : m + (mk - mk_all) * 1.44269504f;
 }
 
-// Joins n pieces of a segment (piece(i) -> address, in shared memory or,
-// written by other CTAs, in global memory): put(e, v) receives the
-// unnormalised values of outputs e .. e + 3, with the references and sums of
-// the 8 heads in `joint`.  wgt: n x 8 floats of shared memory.  A warp per
-// head finds the pieces' weights, a lane per piece; the values are then summed
-// four columns a thread, in order of the pieces, eight loads in flight.
-template <int D, int T, bool GLOBAL, class F, class G>
-__device__ __forceinline__ void pa_join(int n, F piece, float* wgt, float (&joint)[3][kPaHeads], G put) {
-    constexpr int W = T / 32, AT_M = kPaHeads * D, AT_L = AT_M + kPaHeads, AT_MK = AT_L + kPaHeads;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto ld = [](const float* p) { return GLOBAL ? __ldcg(p) : *p; };
-    for (int j = warp; j < kPaHeads; j += W) {
-        float mk = -INFINITY;
-        for (int k = lane; k < n; k += 32) mk = fmaxf(mk, ld(piece(k) + AT_MK));
-        mk = warp_max(mk);
-        float m = -INFINITY;
-        for (int k = lane; k < n; k += 32) m = fmaxf(m, pa_rel(ld(piece(k) + AT_M + j), ld(piece(k) + AT_MK), mk));
-        m = warp_max(m);
-        float l = 0.f;
-        for (int k = lane; k < n; k += 32) {
-            const float r = pa_rel(ld(piece(k) + AT_M + j), ld(piece(k) + AT_MK), mk);
-            const float w = r == -INFINITY ? 0.f : pa_exp2(r - m);
-            wgt[k * kPaHeads + j] = w;
-            l += w * ld(piece(k) + AT_L + j);
-        }
-        l = warp_sum(l);
-        if (lane == 0) joint[0][j] = m, joint[1][j] = l, joint[2][j] = mk;
-    }
-    __syncthreads();
-    for (int e = 4 * (int)threadIdx.x; e < kPaHeads * D; e += 4 * T) {
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        int k = 0;
-        for (; k + 8 <= n; k += 8) {
-            float4 v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float4* p = reinterpret_cast<const float4*>(piece(k + i) + e);
-                v[i] = GLOBAL ? __ldcg(p) : *p;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float w = wgt[(k + i) * kPaHeads + e / D];
-                o.x += w * v[i].x, o.y += w * v[i].y, o.z += w * v[i].z, o.w += w * v[i].w;
-            }
-        }
-        for (; k < n; ++k) {
-            const float4* p = reinterpret_cast<const float4*>(piece(k) + e);
-            const float4 v = GLOBAL ? __ldcg(p) : *p;
-            const float w = wgt[k * kPaHeads + e / D];
-            o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
-        }
-        put(e, o);
-    }
+__device__ __forceinline__ float pa_warp_max(float v) {
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
 }
+__device__ __forceinline__ float4 pa_lds4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+// One head of a segment being joined by one warp: the unnormalised values of
+// columns 4 (lane + 32 i) .. + 3 (D = 64: lanes 16-31 idle), their maximum,
+// sum and mask reference.
+template <int D>
+struct PaJoint {
+    static constexpr int NV = (D + 127) / 128;
+    float4 v[NV];
+    float m = -INFINITY, l = 0.f, mk = -INFINITY;
+
+    // Adds n <= 32 pieces in order: lane k brings piece k's maximum, sum and
+    // mask reference; its row of values is in shared memory at row + k * stride
+    // (piece `odd` at odd_row).
+    __device__ __forceinline__ void add(int n, float pm, float pl, float pk, bool masked, uint32_t row,
+                                        uint32_t stride, int odd, uint32_t odd_row) {
+        const int lane = threadIdx.x & 31;
+        const float nk = masked ? fmaxf(mk, pa_warp_max(pk)) : 0.f;
+        if (masked) pm = pa_rel(pm, pk, nk), m = pa_rel(m, mk, nk);
+        mk = nk;
+        const float nm = fmaxf(m, pa_warp_max(pm));
+        const float old = m == -INFINITY ? 0.f : pa_exp2(m - nm);
+        const float w = pm == -INFINITY ? 0.f : pa_exp2(pm - nm);
+        m = nm;
+        l = l * old + warp_sum(w * pl);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i].x *= old, v[i].y *= old, v[i].z *= old, v[i].w *= old;
+        const uint32_t col = 16 * (lane % (D / 4 < 32 ? D / 4 : 32));
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+            const float wk = __shfl_sync(0xffffffffu, w, k);
+            const uint32_t at = (k == odd ? odd_row : row + k * stride) + col;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const float4 x = pa_lds4(at + 512 * i);
+                v[i].x += wk * x.x, v[i].y += wk * x.y, v[i].z += wk * x.z, v[i].w += wk * x.w;
+            }
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+};
 
 template <bool BF16, int D>
 __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAttnArgs a) {
@@ -232,6 +236,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
     constexpr int LPR = D / 8;             // 16-byte lanes per row
     constexpr int RPI = 32 / LPR;          // rows per copy instruction
     constexpr int TILE = pa_tile(D), RB = 2 * D, PIECE = pa_piece(D);
+    constexpr bool EARLY_Q = D <= 128;     // queries fetched before a unit is issued; D = 256 lacks the registers
     extern __shared__ __align__(128) uint8_t pa_sm[];
     PaShared<W, S>& sh = *reinterpret_cast<PaShared<W, S>*>(pa_sm + W * (S * 2 * TILE + PIECE * 4));
 
@@ -240,10 +245,12 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
     const int ps = a.kv.page_size, G = a.n_head / a.kv.n_head_kv;
     const int hh_n = a.kv.n_head_kv * a.chunks;
 
-    // ---- the lengths' prefix sums: this CTA's range and its warps' starts ----
-    const int per = (a.n_seq + T - 1) / T;
-    const int s_lo = min(a.n_seq, tid * per), s_hi = min(a.n_seq, s_lo + per);
-    int mine = 0;
+    // ---- this CTA's range of the units, and where in it this warp starts ----
+    if (tid < W) sh.seg[0][tid] = -1, sh.seg[1][tid] = -1;
+    int total, mine, before, seq0 = 0, base0 = 0;  // units: of all, of this thread's sequences, of those before
+    const int per = a.n_seq <= 32 ? 1 : (a.n_seq + T - 1) / T;
+    const int s_lo = min(a.n_seq, (a.n_seq <= 32 ? lane : tid) * per), s_hi = min(a.n_seq, s_lo + per);
+    mine = 0;
     for (int s = s_lo; s < s_hi; ++s) {
         const int len = a.seq_lens[s];
         if (blockIdx.x == 0 && (len < 0 || len > a.max_blocks * ps)) record_status(B200_DEVSTATUS_BOUNDS);
@@ -255,29 +262,38 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
         const int x = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += x;
     }
-    if (lane == 31) sh.part[warp] = incl;
-    if (tid < 2 * W) sh.seg[tid] = -1;
-    __syncthreads();
-    int total = 0;
+    if (a.n_seq <= 32) {  // every warp knows all lengths
+        total = __shfl_sync(0xffffffffu, incl, 31);
+    } else {
+        if (lane == 31) sh.part[warp] = incl;
+        __syncthreads();
+        total = 0;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-        if (w < warp) incl += sh.part[w];
-        total += sh.part[w];
+        for (int w = 0; w < W; ++w) {
+            if (w < warp) incl += sh.part[w];
+            total += sh.part[w];
+        }
     }
+    before = (incl - mine) * hh_n;
     total *= hh_n;
     const int per_cta = max((int)((total + gridDim.x - 1u) / gridDim.x), W);
     const int cb = (int)min((unsigned)total, (unsigned)per_cta * blockIdx.x);
     const int ce = (int)min((unsigned)total, (unsigned)cb + (unsigned)per_cta);
-    {
-        int at = (incl - mine) * hh_n;
+    const int per_warp = (ce - cb + W - 1) / W;
+    const int fb = min(ce, cb + per_warp * warp), fe = min(ce, fb + per_warp);
+    if (a.n_seq <= 32) {
+        const unsigned at = __ballot_sync(0xffffffffu, fb >= before && fb < before + mine * hh_n);
+        seq0 = at ? __ffs(at) - 1 : 0;
+        base0 = __shfl_sync(0xffffffffu, before, seq0);
+    } else {
         for (int s = s_lo; s < s_hi; ++s) {
-            const int end = at + pa_units(a, pa_len(a, s)) * hh_n;
-            if (end > cb && at < ce)
+            const int end = before + pa_units(a, pa_len(a, s)) * hh_n;
+            if (end > cb && before < ce)
                 for (int w = 0; w < W; ++w) {
-                    const int b = cb + (ce - cb) * w / W;
-                    if (b >= at && b < end) sh.seq[w] = s, sh.base[w] = at;
+                    const int b = cb + per_warp * w;
+                    if (b >= before && b < end) sh.seq[w] = s, sh.base[w] = before;
                 }
-            at = end;
+            before = end;
         }
     }
     // sequences without a unit
@@ -286,23 +302,37 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
             for (int e = tid; e < a.n_head * D; e += T) a.out[(int64_t)s * a.n_head * D + e] = 0.f;
     __syncthreads();
     if (cb >= ce) return;
+    if (a.n_seq > 32) seq0 = sh.seq[warp], base0 = sh.base[warp];
 
     const uint32_t ring = smem_u32(pa_sm) + warp * (S * 2 * TILE);
-    float* const heads = reinterpret_cast<float*>(pa_sm + W * S * 2 * TILE);
-    float* const head_piece = heads + warp * PIECE;  // a segment begun by an earlier warp
-    float* const tail_piece = reinterpret_cast<float*>(pa_sm + warp * (S * 2 * TILE));  // one left to a later warp
-    const int fb = cb + (ce - cb) * warp / W, fe = cb + (ce - cb) * (warp + 1) / W;
+    // Pieces: of a segment begun by an earlier warp, of one left to a later warp
+    // (that one in the ring, which is free by then).
+    auto head_piece = [&](int w) -> float* {
+        return reinterpret_cast<float*>(pa_sm + W * S * 2 * TILE + w * PIECE * 4);
+    };
+    auto tail_piece = [&](int w) -> float* { return reinterpret_cast<float*>(pa_sm + w * (S * 2 * TILE)); };
 
     if (fb < fe) {
         PaCursor in, cur;
-        in.s = sh.seq[warp];
+        in.s = seq0;
         in.len = pa_len(a, in.s);
         in.nu = pa_units(a, in.len);
-        in.hh = (fb - sh.base[warp]) / in.nu;
-        in.u = (fb - sh.base[warp]) - in.hh * in.nu;
+        const int hh0 = (fb - base0) / in.nu;
+        in.u = (fb - base0) - hh0 * in.nu;
+        in.head = hh0 / a.chunks;
+        in.chunk = hh0 - in.head * a.chunks;
         cur = in;
         int seg_from = fb - in.u;  // first unit of the current segment
         int to_issue = fe - fb, to_do = to_issue;
+
+        // the first segment's queries, on their way while the page table is read
+        float2 qx[2 * KT];
+        auto fetch_q = [&]() {
+            const int j = cur.chunk * kPaHeads + g;
+            const float* qr = a.q + cur.s * a.q_stride + (int64_t)(cur.head * G + (j < G ? j : 0)) * D + 2 * t4;
+#pragma unroll
+            for (int i = 0; i < 2 * KT; ++i) qx[i] = *reinterpret_cast<const float2*>(qr + 8 * i);
+        };
 
         // ---- producer: this lane looks after token lane & 15 of a unit ----
         const int q16 = kPaTok / ps, r16 = kPaTok % ps;
@@ -312,20 +342,26 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
         float mask_pending = 0.f;
         int mask_stage = -1;
         unsigned valid_pending = 0;
-        auto entry = [&](int e, int& page, int& blk) {
-            blk = e, page = -1;
+        // entries e and e + 32 of the block list (only_second: the second alone);
+        // the loads of both go out before either is looked at
+        auto window = [&](int e, bool only_second) {
             const int nb = (int)(((unsigned)in.len + (unsigned)ps - 1u) / (unsigned)ps);
+            int x0 = e, x1 = e + 32;
             if (a.sel != nullptr) {
-                const int64_t hk = (int64_t)in.s * a.kv.n_head_kv + in.hh / a.chunks;
-                blk = e < a.n_sel ? a.sel[hk * a.n_sel + e] : -1;
+                const int32_t* list = a.sel + ((int64_t)in.s * a.kv.n_head_kv + in.head) * a.n_sel;
+                x0 = !only_second && e < a.n_sel ? list[e] : -1;
+                x1 = e + 32 < a.n_sel ? list[e + 32] : -1;
             }
-            if (blk >= 0 && blk < nb) {
-                page = a.table[in.s * a.table_stride + blk];
-                if ((unsigned)page >= (unsigned)a.kv.n_pages) {
-                    record_status(B200_DEVSTATUS_BOUNDS);
-                    page = -1;
-                }
-            }
+            const int32_t* row_of = a.table + in.s * a.table_stride;
+            const bool on0 = !only_second && (unsigned)x0 < (unsigned)nb, on1 = (unsigned)x1 < (unsigned)nb;
+            int y0 = -1, y1 = -1;
+            if (on0) y0 = row_of[x0];
+            if (on1) y1 = row_of[x1];
+            const bool bad0 = on0 && (unsigned)y0 >= (unsigned)a.kv.n_pages;
+            const bool bad1 = on1 && (unsigned)y1 >= (unsigned)a.kv.n_pages;
+            if (bad0 || bad1) record_status(B200_DEVSTATUS_BOUNDS);
+            if (!only_second) p0 = bad0 ? -1 : y0, b0 = x0;
+            p1 = bad1 ? -1 : y1, b1 = x1;
         };
         auto flush_mask = [&]() {
             if (mask_stage >= 0) {
@@ -343,8 +379,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                     bi = (int)(vt / (unsigned)ps);
                     row = (int)(vt % (unsigned)ps);
                     w0 = (int)((unsigned)in.u * kPaTok / (unsigned)ps);
-                    entry(w0 + lane, p0, b0);
-                    entry(w0 + 32 + lane, p1, b1);
+                    window(w0 + lane, false);
                     fresh = false;
                 } else {
                     bi += q16;
@@ -353,7 +388,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                     if (__shfl_sync(0xffffffffu, bi, 0) >= w0 + 32) {
                         w0 += 32;
                         p0 = p1, b0 = b1;
-                        entry(w0 + 32 + lane, p1, b1);
+                        window(w0 + lane, true);
                     }
                 }
                 const int x = bi - w0;  // 0 .. 47
@@ -366,9 +401,8 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                 }
                 const bool ok = page >= 0 && row < in.len - blk * ps;
                 const unsigned valid = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-                const int head = in.hh / a.chunks;
-                const long long ko = ok ? page * a.kv.k_page + row * a.kv.k_row + head * a.kv.k_head : 0;
-                const long long vo = ok ? page * a.kv.v_page + row * a.kv.v_row + head * a.kv.v_head : 0;
+                const long long ko = ok ? page * a.kv.k_page + row * a.kv.k_row + in.head * a.kv.k_head : 0;
+                const long long vo = ok ? page * a.kv.v_page + row * a.kv.v_row + in.head * a.kv.v_head : 0;
                 if (lane == 0) sh.valid[warp][stage] = valid;
                 if (a.mask != nullptr) {
                     mask_pending = ok ? h2f(a.mask[in.s * a.mask_stride + (int64_t)blk * ps + row]) : -INFINITY;
@@ -388,29 +422,21 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                     pa_cp16(d + TILE, vp + vr, on);
                 }
                 --to_issue;
-                const int s_was = in.s, hh_was = in.hh;
-                if (to_issue > 0 && !pa_advance(a, in, hh_n)) to_issue = 0;
-                fresh = in.s != s_was || in.hh != hh_was;
+                if (to_issue > 0 && !pa_advance(a, in)) to_issue = 0;
+                fresh = in.u == 0;
             }
             pa_commit();
         };
-#pragma unroll
-        for (int st = 0; st < S - 1; ++st) issue(st);
-
         // ---- consumer: this thread holds head g, positions 2 t4, 2 t4 + 1 (+ 8) ----
         uint32_t qf[KT][4], q3[BF16 ? KT : 1][2];
         float o[2 * KT][2], m = -INFINITY, l = 0.f, mk = -INFINITY, f = 0.f;
-        auto load_q = [&]() {
-            const int chunk = cur.hh % a.chunks, head = cur.hh / a.chunks;
-            const int j = chunk * kPaHeads + g;
-            const float* qr = a.q + cur.s * a.q_stride + (int64_t)(head * G + (j < G ? j : 0)) * D + 2 * t4;
-            float2 x[2 * KT];
+        auto take_q = [&]() {
+            const bool mine_q = cur.chunk * kPaHeads + g < G;
             float amax = 0.f;
 #pragma unroll
             for (int i = 0; i < 2 * KT; ++i) {
-                x[i] = *reinterpret_cast<const float2*>(qr + 8 * i);
-                if (j >= G) x[i] = make_float2(0.f, 0.f);
-                amax = fmaxf(amax, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+                if (!mine_q) qx[i] = make_float2(0.f, 0.f);
+                amax = fmaxf(amax, fmaxf(fabsf(qx[i].x), fabsf(qx[i].y)));
             }
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
@@ -420,22 +446,35 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
             f = a.scale * 1.44269504f * __uint_as_float((unsigned)(127 + ex) << 23);
 #pragma unroll
             for (int i = 0; i < 2 * KT; ++i) {
-                x[i].x *= up, x[i].y *= up;
-                qf[i >> 1][2 * (i & 1)] = pa_split<BF16>(x[i].x, x[i].y);
-                qf[i >> 1][2 * (i & 1) + 1] = pa_split<BF16>(x[i].x, x[i].y);
-                if (BF16) q3[i >> 1][i & 1] = pa_split<BF16>(x[i].x, x[i].y);
+                float x = qx[i].x * up, y = qx[i].y * up;
+                qf[i >> 1][2 * (i & 1)] = pa_split<BF16>(x, y);
+                qf[i >> 1][2 * (i & 1) + 1] = pa_split<BF16>(x, y);
+                if (BF16) q3[i >> 1][i & 1] = pa_split<BF16>(x, y);
             }
 #pragma unroll
             for (int i = 0; i < 2 * KT; ++i) o[i][0] = o[i][1] = 0.f;
             m = -INFINITY, l = 0.f, mk = a.mask != nullptr ? -INFINITY : 0.f;
         };
-        load_q();
-        int stage = 0;
+        // The loop runs S - 1 units ahead with the copies: its first S - 1 turns
+        // only issue.
+        bool new_q = true;
+        int stage = 0, ahead = 0;
         const int mi = lane >> 3, ri = lane & 7;
-        for (; to_do > 0; --to_do) {
-            pa_wait<S - 2>();
-            __syncwarp();
-            issue(stage == 0 ? S - 1 : stage - 1);
+#pragma unroll 1
+        for (int turn = 1 - S; to_do > 0; ++turn) {
+            if (EARLY_Q && new_q && (turn == 1 - S || turn > 0)) fetch_q();
+            if (turn >= 0) {
+                pa_wait<S - 2>();
+                __syncwarp();
+            }
+            issue(ahead);
+            ahead = ahead + 1 == S ? 0 : ahead + 1;
+            if (turn < 0) continue;
+            if (new_q) {
+                if (!EARLY_Q) fetch_q();
+                take_q();
+                new_q = false;
+            }
             const unsigned valid = sh.valid[warp][stage];
             const unsigned live = a.mask != nullptr ? sh.live[warp][stage] : valid;
             const uint32_t kst = ring + stage * (2 * TILE), vst = kst + TILE;
@@ -529,93 +568,155 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                 l += __shfl_xor_sync(0xffffffffu, l, 1);
                 l += __shfl_xor_sync(0xffffffffu, l, 2);
                 if (seg_end && seg_from >= fb) {  // the whole segment
-                    const int chunk = cur.hh % a.chunks, head = cur.hh / a.chunks;
-                    const int j = chunk * kPaHeads + g;
+                    const int j = cur.chunk * kPaHeads + g;
                     const float inv = l > 0.f ? 1.f / l : 0.f;
                     if (j < G) {
-                        float* dst = a.out + ((int64_t)cur.s * a.n_head + head * G + j) * D + 2 * t4;
+                        float* dst = a.out + ((int64_t)cur.s * a.n_head + cur.head * G + j) * D + 2 * t4;
 #pragma unroll
                         for (int i = 0; i < 2 * KT; ++i)
                             *reinterpret_cast<float2*>(dst + 8 * i) = make_float2(o[i][0] * inv, o[i][1] * inv);
                     }
                 } else {
-                    const bool tail = !seg_end;
-                    if (tail) {  // the last piece of this warp: its ring is free
+                    if (!seg_end) {  // the last piece of this warp: its ring is free
                         pa_wait<0>();
                         __syncwarp();
                     }
-                    float* p = tail ? tail_piece : head_piece;
+                    float* p = seg_end ? head_piece(warp) : tail_piece(warp);
 #pragma unroll
                     for (int i = 0; i < 2 * KT; ++i)
                         *reinterpret_cast<float2*>(p + g * D + 8 * i + 2 * t4) = make_float2(o[i][0], o[i][1]);
                     if (t4 == 0) p[kPaHeads * D + g] = m, p[kPaHeads * D + kPaHeads + g] = l;
                     if (lane == 0) {
                         p[kPaHeads * D + 2 * kPaHeads] = mk;
-                        sh.seg[2 * warp + tail] = cur.s * hh_n + cur.hh;
-                        sh.from[2 * warp + tail] = seg_from;
-                        sh.nu[2 * warp + tail] = cur.nu;
+                        const int x = seg_end ? 0 : 1;
+                        sh.seg[x][warp] = (cur.s * a.kv.n_head_kv + cur.head) * a.chunks + cur.chunk;
+                        sh.from[x][warp] = seg_from;
+                        sh.nu[x][warp] = cur.nu;
+                        sh.row[x][warp] = cur.s * a.n_head + cur.head * G + cur.chunk * kPaHeads;
+                        sh.rows[x][warp] = min(kPaHeads, G - cur.chunk * kPaHeads);
                     }
                 }
             }
-            if (to_do > 1) {
+            if (--to_do > 0) {
                 if (seg_end) seg_from += cur.nu;
-                if (!pa_advance(a, cur, hh_n)) break;
-                if (seg_end) load_q();
+                if (!pa_advance(a, cur)) break;
+                new_q = seg_end;
             }
         }
         pa_wait<0>();
     }
     __syncthreads();
 
-    // ---- join the pieces of cut segments ----
-    auto piece_at = [&](int i) -> float* {
-        return (i & 1) ? reinterpret_cast<float*>(pa_sm + (i >> 1) * (S * 2 * TILE)) : heads + (i >> 1) * PIECE;
+    // ---- join the pieces of cut segments: a warp per head ----
+    // A segment's pieces lie in consecutive warps: tail pieces, and the last one
+    // a head piece where the segment ends inside this CTA.  Masks over warps:
+    const int tl = lane < W ? sh.seg[1][lane] : -1, hd = lane < W ? sh.seg[0][lane] : -1;
+    int prev = __shfl_up_sync(0xffffffffu, tl, 1);
+    if (lane == 0) prev = -1;
+    const unsigned goes_on = __ballot_sync(0xffffffffu, tl >= 0 && tl == prev);  // tail of the same segment as before
+    const unsigned starts = __ballot_sync(0xffffffffu, tl >= 0 && tl != prev);
+    const unsigned ends = __ballot_sync(0xffffffffu, hd >= 0 && hd == prev);     // head of the tail before
+    const unsigned alone = __ballot_sync(0xffffffffu, hd >= 0 && hd != prev);
+    constexpr int AT_M = kPaHeads * D, AT_L = AT_M + kPaHeads, AT_MK = AT_L + kPaHeads, NV = PaJoint<D>::NV;
+    const bool masked = a.mask != nullptr, has_col = 4 * lane < D;
+    auto put_out = [&](int row, const PaJoint<D>& t) {
+        const float inv = t.l > 0.f ? 1.f / t.l : 0.f;
+        float4* out = reinterpret_cast<float4*>(a.out + (int64_t)row * D) + lane;
+        if (has_col)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                out[32 * i] = make_float4(t.v[i].x * inv, t.v[i].y * inv, t.v[i].z * inv, t.v[i].w * inv);
     };
-    // weights of the pieces being joined: in warp 0's ring, behind its tail piece
-    float* const wgt = reinterpret_cast<float*>(pa_sm + align256(PIECE * 4));
-    static_assert(kPaCtas * kPaHeads * 4 + PIECE * 4 + 256 <= S * 2 * TILE, "weights beside the tail piece");
-    for (int i = 0; i < 2 * W;) {
-        const int seg = sh.seg[i];
-        if (seg < 0) {
-            ++i;
-            continue;
-        }
-        int list[2 * W], n = 0;
-        for (; i < 2 * W && (sh.seg[i] == seg || sh.seg[i] < 0); ++i)
-            if (sh.seg[i] == seg) list[n++] = i;
-        const int from = sh.from[list[0]], end = from + sh.nu[list[0]];
+    int open0 = -1, open1 = -1;  // segments cut by the CTA's borders: where to find them in sh (2 * warp + slot)
+#pragma unroll 1
+    for (unsigned todo = starts | alone << 16; todo != 0; todo &= todo - 1) {
+        const int bit = __ffs(todo) - 1, w0 = bit & 15, slot = bit >= 16 ? 0 : 1;
+        const int run = slot == 0 ? 0 : __ffs(~(goes_on >> (w0 + 1))) - 1;  // further tail pieces
+        const bool closed = slot == 0 || ((ends >> (w0 + run + 1)) & 1);
+        const int n = slot == 0 ? 1 : 1 + run + (closed ? 1 : 0);
+        const int from = sh.from[slot][w0], end = from + sh.nu[slot][w0], rows = sh.rows[slot][w0];
         const bool whole = from >= cb && end <= ce;
-        const int s = seg / hh_n, hh = seg % hh_n, head = hh / a.chunks, j0 = (hh % a.chunks) * kPaHeads;
-        float* out = a.out + ((int64_t)s * a.n_head + head * G + j0) * D;
-        float* mine_g = a.pieces + (int64_t)(2 * blockIdx.x + (from >= cb ? 1 : 0)) * PIECE;
-        auto finish = [&](int e, float4 o) {
-            const float l = sh.joint[1][e / D], inv = l > 0.f ? 1.f / l : 0.f;
-            if (j0 + e / D < G)
-                *reinterpret_cast<float4*>(out + e) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-        };
-        pa_join<D, T, false>(n, [&](int k) -> const float* { return piece_at(list[k]); }, wgt, sh.joint,
-                             [&](int e, float4 o) {
-                                 if (whole) finish(e, o);
-                                 else __stcg(reinterpret_cast<float4*>(mine_g + e), o);
-                             });
         if (!whole) {
-            if (tid < 2 * kPaHeads) __stcg(mine_g + kPaHeads * D + tid, sh.joint[tid / kPaHeads][tid % kPaHeads]);
-            if (tid == 0) __stcg(mine_g + kPaHeads * D + 2 * kPaHeads, sh.joint[2][0]);
-            const int c0 = from / per_cta, c1 = (end - 1) / per_cta;
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) sh.last = atomicAdd(a.tickets + seg, 1u) == (unsigned)(c1 - c0);
-            __syncthreads();
-            if (sh.last) {
-                __threadfence();
-                pa_join<D, T, true>(
-                    c1 - c0 + 1,
-                    [&](int k) -> const float* { return a.pieces + (int64_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * PIECE; },
-                    wgt, sh.joint, finish);
-                if (tid == 0) a.tickets[seg] = 0u;
+            if (open0 < 0) open0 = 2 * w0 + slot;
+            else open1 = 2 * w0 + slot;
+        }
+#pragma unroll 1
+        for (int j = warp; j < rows; j += W) {
+            PaJoint<D> t;
+            t.clear();
+            float pm = -INFINITY, pl = 0.f, pk = -INFINITY;
+            if (lane < n) {
+                const float* p = closed && lane == n - 1 ? head_piece(w0 + lane) : tail_piece(w0 + lane);
+                pm = p[AT_M + j], pl = p[AT_L + j], pk = p[AT_MK];
+            }
+            t.add(n, pm, pl, pk, masked, smem_u32(tail_piece(w0) + j * D), S * 2 * TILE, closed ? n - 1 : -1,
+                  smem_u32(head_piece(w0 + n - 1) + j * D));
+            if (whole) {
+                put_out(sh.row[slot][w0] + j, t);
+            } else {
+                float* p = a.pieces + (int64_t)(2 * blockIdx.x + (from >= cb ? 1 : 0)) * PIECE;
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (has_col) __stcg(reinterpret_cast<float4*>(p + j * D + 4 * lane + 128 * i), t.v[i]);
+                if (lane == 0) {
+                    __stcg(p + AT_M + j, t.m);
+                    __stcg(p + AT_L + j, t.l);
+                    __stcg(p + AT_MK, t.mk);
+                }
             }
         }
-        __syncthreads();  // wgt and joint are free again
+    }
+    if (open0 < 0) return;
+    // The CTA whose ticket completes a head's segment joins that head.  Lane i
+    // draws the tickets of this warp's i-th head.
+    __threadfence();
+    __syncwarp();
+    unsigned got0 = 0, got1 = 0;
+    const int my_j = warp + lane * W;
+    if (my_j < sh.rows[open0 & 1][open0 >> 1])
+        got0 = atomicAdd(a.tickets + (int64_t)sh.seg[open0 & 1][open0 >> 1] * kPaHeads + my_j, 1u);
+    if (open1 >= 0 && my_j < sh.rows[open1 & 1][open1 >> 1])
+        got1 = atomicAdd(a.tickets + (int64_t)sh.seg[open1 & 1][open1 >> 1] * kPaHeads + my_j, 1u);
+    __threadfence();
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+        const int at = i ? open1 : open0;
+        if (at < 0) break;
+        const int from = sh.from[at & 1][at >> 1], rows = sh.rows[at & 1][at >> 1];
+        const int c0 = from / per_cta, n = (from + sh.nu[at & 1][at >> 1] - 1) / per_cta - c0 + 1;
+        // piece k: slot 1 of CTA c0, where the segment starts, then slot 0 of the next CTAs
+        auto piece = [&](int k) -> const float* { return a.pieces + (int64_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * PIECE; };
+#pragma unroll 1
+        for (int j = warp, x = 0; j < rows; j += W, ++x) {
+            if (__shfl_sync(0xffffffffu, i ? got1 : got0, x) != (unsigned)(n - 1)) continue;
+            // 32 pieces at a time into this warp's ring, behind its tail piece
+            // (which other warps may still be reading)
+            const uint32_t buf = smem_u32(tail_piece(warp)) + (uint32_t)align256(PIECE * 4);
+            static_assert(32 * D * 4 + PIECE * 4 + 256 <= S * 2 * TILE, "32 rows of a head in a warp's ring");
+            PaJoint<D> t;
+            t.clear();
+#pragma unroll 1
+            for (int c = 0; c < n; c += 32) {
+                const int here = min(32, n - c);
+                float pm = -INFINITY, pl = 0.f, pk = -INFINITY;
+#pragma unroll 4
+                for (int k = 0; k < here; ++k)
+#pragma unroll
+                    for (int y = 0; y < NV; ++y)
+                        if (has_col) pa_cp16(buf + k * (4 * D) + 16 * lane + 512 * y, piece(c + k) + j * D + 4 * lane + 128 * y, true);
+                pa_commit();
+                if (lane < here) {
+                    const float* p = piece(c + lane);
+                    pm = __ldcg(p + AT_M + j), pl = __ldcg(p + AT_L + j), pk = __ldcg(p + AT_MK);
+                }
+                pa_wait<0>();
+                __syncwarp();
+                t.add(here, pm, pl, pk, masked, buf, 4 * D, -1, 0u);
+                __syncwarp();
+            }
+            put_out(sh.row[at & 1][at >> 1] + j, t);
+            if (lane == 0) a.tickets[(int64_t)sh.seg[at & 1][at >> 1] * kPaHeads + j] = 0u;
+        }
     }
 }
 
