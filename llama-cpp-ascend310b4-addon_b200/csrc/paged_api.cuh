@@ -6,6 +6,7 @@
 #include "paged_plan.cuh"
 #include "paged_select.cuh"
 #include "paged_store.cuh"
+#include "paged_work.cuh"
 
 namespace {
 
@@ -45,18 +46,46 @@ int launch_paged_store(const PagedStoreArgs& a, cudaStream_t st) {
     return cuda_status(cudaGetLastError());
 }
 
+bool g_paged_select_attr[kMaxDevices][2][3];
+
+template <bool BF16, int D>
+int launch_paged_select_d(const PagedSelectArgs& a, cudaStream_t st) {
+    const int dev = current_device();
+    if (dev < 0 || dev >= kMaxDevices) return B200_EINVAL;
+    {
+        bool& done = g_paged_select_attr[dev][BF16][D == 64 ? 0 : D == 128 ? 1 : 2];
+        std::lock_guard<std::mutex> lk(g_attr_mu);
+        if (!done) {
+            CR_(cuda_status(cudaFuncSetAttribute(paged_score_kernel<BF16, D>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, score_smem<D>())));
+            CR_(cuda_status(cudaFuncSetAttribute(paged_topk_kernel<BF16, D>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 kTopkKeys * (int)sizeof(float))));
+            done = true;
+        }
+    }
+    const int64_t units = (int64_t)a.n_seq * a.n_head_kv * paged_units(a.max_blocks);
+    const int64_t grid = std::min<int64_t>(kPaCtas, (units + pa_warps(D) - 1) / pa_warps(D));
+    paged_score_kernel<BF16, D><<<(unsigned)grid, 32 * pa_warps(D), score_smem<D>(), st>>>(a);
+    CR_(cuda_status(cudaGetLastError()));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.n_seq * a.n_head_kv), 1, 1);
+    cfg.blockDim = dim3(kTopkThreads, 1, 1);
+    cfg.dynamicSmemBytes = std::min(a.max_blocks, kTopkKeys) * sizeof(float);
+    cfg.stream = st;
+    cudaLaunchAttribute at = pdl_attr();
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, paged_topk_kernel<BF16, D>, a));
+}
+
 template <bool BF16>
 int launch_paged_select(const PagedSelectArgs& a, int head_dim, cudaStream_t st) {
-    const int64_t items = (int64_t)a.n_seq * a.max_blocks * a.n_head_kv;
-    const unsigned grid = (unsigned)((items + kSelectThreads / 32 - 1) / (kSelectThreads / 32));
     switch (head_dim) {
-        case 64: paged_score_kernel<BF16, 64><<<grid, kSelectThreads, 0, st>>>(a); break;
-        case 128: paged_score_kernel<BF16, 128><<<grid, kSelectThreads, 0, st>>>(a); break;
-        default: paged_score_kernel<BF16, 256><<<grid, kSelectThreads, 0, st>>>(a); break;
+        case 64: return launch_paged_select_d<BF16, 64>(a, st);
+        case 128: return launch_paged_select_d<BF16, 128>(a, st);
+        default: return launch_paged_select_d<BF16, 256>(a, st);
     }
-    CR_(cuda_status(cudaGetLastError()));
-    paged_topk_kernel<<<(unsigned)(a.n_seq * a.n_head_kv), kSelectThreads, 0, st>>>(a);
-    return cuda_status(cudaGetLastError());
 }
 
 bool g_paged_attn_attr[kMaxDevices][2][3];
@@ -161,7 +190,10 @@ size_t b200_paged_select_workspace_size(int n_seq, int n_head_kv, int max_blocks
     if (n_seq < 0 || n_seq > 65535 || n_head_kv <= 0 || n_head_kv > 65535 || max_blocks <= 0 ||
         max_blocks > B200_PAGED_SELECT_MAX_BLOCKS)
         return 0;
-    return std::max((size_t)16, (size_t)n_seq * n_head_kv * max_blocks * sizeof(unsigned long long));
+    const size_t rows = (size_t)n_seq * n_head_kv;
+    return std::max((size_t)256, align256(rows * max_blocks * sizeof(unsigned long long)) +
+                                     align256(rows * max_blocks * sizeof(float)) +
+                                     align256(rows * paged_units(max_blocks) * sizeof(unsigned int)));
 }
 
 int b200_paged_select(const b200_paged_kv* kv, const float* q, int64_t q_stride, int n_seq, int n_head,
@@ -172,6 +204,7 @@ int b200_paged_select(const b200_paged_kv* kv, const float* q, int64_t q_stride,
     CR_(check_paged_batch(kv, q, q_stride, n_seq, n_head, block_table, table_stride, max_blocks, seq_lens));
     if (!kv->k_lo || !sel || n_sel <= 0 || !workspace || !aligned16(workspace)) return B200_EINVAL;
     if (max_blocks > B200_PAGED_SELECT_MAX_BLOCKS) return B200_EUNSUPPORTED;
+    if ((int64_t)n_seq * kv->n_head_kv * paged_units(max_blocks) > INT32_MAX) return B200_EUNSUPPORTED;
     if (workspace_size < b200_paged_select_workspace_size(n_seq, kv->n_head_kv, max_blocks)) return B200_EINVAL;
     PagedSelectArgs a;
     a.lo = static_cast<const uint16_t*>(kv->k_lo);
@@ -182,7 +215,13 @@ int b200_paged_select(const b200_paged_kv* kv, const float* q, int64_t q_stride,
     a.table_stride = table_stride;
     a.seq_lens = seq_lens;
     a.sel = sel;
-    a.keys = static_cast<unsigned long long*>(workspace);
+    const size_t rows = (size_t)n_seq * kv->n_head_kv;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    a.exact = reinterpret_cast<unsigned long long*>(ws);
+    ws += align256(rows * max_blocks * sizeof(unsigned long long));
+    a.approx = reinterpret_cast<float*>(ws);
+    ws += align256(rows * max_blocks * sizeof(float));
+    a.unit_max = reinterpret_cast<unsigned int*>(ws);
     a.n_seq = n_seq;
     a.n_head = n_head;
     a.n_head_kv = kv->n_head_kv;

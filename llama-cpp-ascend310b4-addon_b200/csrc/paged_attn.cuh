@@ -35,13 +35,11 @@
 #include "../../include/b200_paged.h"
 #include "args.h"
 #include "common.cuh"
-#include "paged_select.cuh"
+#include "paged_work.cuh"
 
 namespace b200 {
 
 constexpr int kPaHeads = 8;   // query heads of one KV head handled together
-constexpr int kPaTok = 16;    // positions per unit
-constexpr int kPaCtas = 148;  // CTAs of a full grid: one per SM
 
 // Warps per CTA and ring stages per warp: 192 KB of ring in every case.
 B200_HD constexpr int pa_warps(int D) { return D == 64 ? 12 : D == 128 ? 8 : 4; }
@@ -53,8 +51,7 @@ B200_HD constexpr int pa_tile(int D) { return kPaTok * D * 2; }
 // Bookkeeping beside the ring and the pieces in shared memory.
 template <int W, int S>
 struct PaShared {
-    int part[W];                // prefix-sum partials
-    int seq[W], base[W];        // the sequence a warp starts in and that one's first unit
+    PaRangeShared<W> range;
     // pieces of a warp, [0] of a segment begun by an earlier warp, [1] of one left
     // to a later warp: segment (-1: none), its first unit and length, its first
     // row of the output and rows
@@ -84,57 +81,6 @@ struct PagedAttnArgs {
     float scale;
     int n_seq, n_head, n_sel, max_blocks, chunks;
 };
-
-__device__ __forceinline__ void pa_cp16(uint32_t dst, const void* src, bool on) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void pa_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void pa_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void pa_ldsm(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-__device__ __forceinline__ void pa_ldsm_t(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-template <bool BF16>
-__device__ __forceinline__ void pa_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                       uint32_t b1) {
-    if (BF16)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-            "{%0,%1,%2,%3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-            "{%0,%1,%2,%3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float pa_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// High 16-bit part of two values packed in a word; x, y become the remainders.
-template <bool BF16>
-__device__ __forceinline__ uint32_t pa_split(float& x, float& y) {
-    const uint32_t w = pack16<BF16>(x, y);
-    const float2 f = unpack16<BF16>(w);
-    x -= f.x;
-    y -= f.y;
-    return w;
-}
 
 // Where a warp is in its range: unit u of nu of the segment (s, head, chunk).
 struct PaCursor {
@@ -172,11 +118,6 @@ __device__ __forceinline__ float pa_rel(float m, float mk, float mk_all) {
     return m == -INFINITY ? -INFINITY : m + (mk - mk_all) * 1.44269504f;
 }
 
-__device__ __forceinline__ float pa_warp_max(float v) {
-    float r;
-    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-    return r;
-}
 __device__ __forceinline__ float4 pa_lds4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -245,64 +186,17 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
     const int ps = a.kv.page_size, G = a.n_head / a.kv.n_head_kv;
     const int hh_n = a.kv.n_head_kv * a.chunks;
 
-    // ---- this CTA's range of the units, and where in it this warp starts ----
     if (tid < W) sh.seg[0][tid] = -1, sh.seg[1][tid] = -1;
-    int total, mine, before, seq0 = 0, base0 = 0;  // units: of all, of this thread's sequences, of those before
-    const int per = a.n_seq <= 32 ? 1 : (a.n_seq + T - 1) / T;
-    const int s_lo = min(a.n_seq, (a.n_seq <= 32 ? lane : tid) * per), s_hi = min(a.n_seq, s_lo + per);
-    mine = 0;
-    for (int s = s_lo; s < s_hi; ++s) {
-        const int len = a.seq_lens[s];
-        if (blockIdx.x == 0 && (len < 0 || len > a.max_blocks * ps)) record_status(B200_DEVSTATUS_BOUNDS);
-        mine += pa_units(a, pa_len(a, s));
-    }
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += x;
-    }
-    if (a.n_seq <= 32) {  // every warp knows all lengths
-        total = __shfl_sync(0xffffffffu, incl, 31);
-    } else {
-        if (lane == 31) sh.part[warp] = incl;
-        __syncthreads();
-        total = 0;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            if (w < warp) incl += sh.part[w];
-            total += sh.part[w];
-        }
-    }
-    before = (incl - mine) * hh_n;
-    total *= hh_n;
-    const int per_cta = max((int)((total + gridDim.x - 1u) / gridDim.x), W);
-    const int cb = (int)min((unsigned)total, (unsigned)per_cta * blockIdx.x);
-    const int ce = (int)min((unsigned)total, (unsigned)cb + (unsigned)per_cta);
-    const int per_warp = (ce - cb + W - 1) / W;
-    const int fb = min(ce, cb + per_warp * warp), fe = min(ce, fb + per_warp);
-    if (a.n_seq <= 32) {
-        const unsigned at = __ballot_sync(0xffffffffu, fb >= before && fb < before + mine * hh_n);
-        seq0 = at ? __ffs(at) - 1 : 0;
-        base0 = __shfl_sync(0xffffffffu, before, seq0);
-    } else {
-        for (int s = s_lo; s < s_hi; ++s) {
-            const int end = before + pa_units(a, pa_len(a, s)) * hh_n;
-            if (end > cb && before < ce)
-                for (int w = 0; w < W; ++w) {
-                    const int b = cb + per_warp * w;
-                    if (b >= before && b < end) sh.seq[w] = s, sh.base[w] = before;
-                }
-            before = end;
-        }
-    }
+    if (blockIdx.x == 0)
+        for (int s = tid; s < a.n_seq; s += T)
+            if (a.seq_lens[s] < 0 || a.seq_lens[s] > a.max_blocks * ps) record_status(B200_DEVSTATUS_BOUNDS);
+    const PaRange<W> range(sh.range, a.n_seq, hh_n, [&](int s) { return pa_units(a, pa_len(a, s)); });
+    const int cb = range.cb, ce = range.ce, per_cta = range.per_cta, fb = range.fb, fe = range.fe;
     // sequences without a unit
     for (int s = blockIdx.x; s < a.n_seq; s += gridDim.x)
         if (pa_len(a, s) == 0)
             for (int e = tid; e < a.n_head * D; e += T) a.out[(int64_t)s * a.n_head * D + e] = 0.f;
-    __syncthreads();
     if (cb >= ce) return;
-    if (a.n_seq > 32) seq0 = sh.seq[warp], base0 = sh.base[warp];
 
     const uint32_t ring = smem_u32(pa_sm) + warp * (S * 2 * TILE);
     // Pieces: of a segment begun by an earlier warp, of one left to a later warp
@@ -314,11 +208,11 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
 
     if (fb < fe) {
         PaCursor in, cur;
-        in.s = seq0;
+        in.s = range.seq0;
         in.len = pa_len(a, in.s);
         in.nu = pa_units(a, in.len);
-        const int hh0 = (fb - base0) / in.nu;
-        in.u = (fb - base0) - hh0 * in.nu;
+        const int hh0 = (fb - range.base0) / in.nu;
+        in.u = (fb - range.base0) - hh0 * in.nu;
         in.head = hh0 / a.chunks;
         in.chunk = hh0 - in.head * a.chunks;
         cur = in;
