@@ -58,9 +58,6 @@ int launch_paged_select_d(const PagedSelectArgs& a, cudaStream_t st) {
         if (!done) {
             CR_(cuda_status(cudaFuncSetAttribute(paged_score_kernel<BF16, D>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, score_smem<D>())));
-            CR_(cuda_status(cudaFuncSetAttribute(paged_topk_kernel<BF16, D>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 kTopkKeys * (int)sizeof(float))));
             done = true;
         }
     }
@@ -71,7 +68,6 @@ int launch_paged_select_d(const PagedSelectArgs& a, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.n_seq * a.n_head_kv), 1, 1);
     cfg.blockDim = dim3(kTopkThreads, 1, 1);
-    cfg.dynamicSmemBytes = std::min(a.max_blocks, kTopkKeys) * sizeof(float);
     cfg.stream = st;
     cudaLaunchAttribute at = pdl_attr();
     cfg.attrs = &at;
@@ -192,7 +188,7 @@ size_t b200_paged_select_workspace_size(int n_seq, int n_head_kv, int max_blocks
         return 0;
     const size_t rows = (size_t)n_seq * n_head_kv;
     return std::max((size_t)256, align256(rows * max_blocks * sizeof(unsigned long long)) +
-                                     align256(rows * max_blocks * sizeof(float)) +
+                                     align256(rows * max_blocks * sizeof(float)) + align256(rows * sizeof(float2)) +
                                      align256(rows * paged_units(max_blocks) * sizeof(unsigned int)));
 }
 
@@ -221,6 +217,8 @@ int b200_paged_select(const b200_paged_kv* kv, const float* q, int64_t q_stride,
     ws += align256(rows * max_blocks * sizeof(unsigned long long));
     a.approx = reinterpret_cast<float*>(ws);
     ws += align256(rows * max_blocks * sizeof(float));
+    a.group = reinterpret_cast<float2*>(ws);
+    ws += align256(rows * sizeof(float2));
     a.unit_max = reinterpret_cast<unsigned int*>(ws);
     a.n_seq = n_seq;
     a.n_head = n_head;

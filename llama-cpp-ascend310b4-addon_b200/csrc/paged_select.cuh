@@ -37,20 +37,12 @@ struct PagedSelectArgs {
     int32_t* sel;
     unsigned long long* exact;  // [n_seq][n_head_kv][max_blocks] ordered 64-bit scores, where needed
     float* approx;              // [n_seq][n_head_kv][max_blocks] scores of q 2^-ex
+    float2* group;              // [n_seq][n_head_kv] 2^-ex and max_j sum |q_jd| 2^-ex
     unsigned int* unit_max;     // [n_seq][n_head_kv][ceil(max_blocks / 16)] largest |bound|, as 16-bit patterns
     int n_seq, n_head, n_head_kv, max_blocks, page_size, n_pages, n_sel;
 };
 
 B200_HD constexpr int paged_units(int blocks) { return (blocks + kPaTok - 1) / kPaTok; }
-
-// Exponent of the largest |q| of a KV head's query heads (n contiguous values,
-// a multiple of 32), clamped as in the attention kernel; one warp.
-__device__ __forceinline__ int group_exponent(const float* q, int n) {
-    float m = 0.f;
-    for (int i = threadIdx.x & 31; i < n; i += 32) m = fmaxf(m, fabsf(q[i]));
-    m = pa_warp_max(m);
-    return min(max((int)(__float_as_uint(m) >> 23) - 127, -120), 120);
-}
 
 template <int W, int S>
 struct ScoreShared {
@@ -155,20 +147,47 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_score_kernel(PagedS
         issue(ahead);
         ahead = ahead + 1 == S ? 0 : ahead + 1;
         if (turn < 0) continue;
-        const float* qg = a.q + cur.s * a.q_stride + (int64_t)cur.head * G * D;
-        if (new_q) up = __uint_as_float((unsigned)(127 - group_exponent(qg, G * D)) << 23);
+        const int64_t sh_ = (int64_t)cur.s * H + cur.head;
+        const float* qg = a.q + cur.s * a.q_stride + (int64_t)cur.head * G * D + 2 * t4;
+        // this thread's values of head j0 + g; rows past the group repeat its last head
+        auto fetch_q = [&](int j0, float2 (&x)[2 * KT]) {
+            const float* qr = qg + min(j0 + g, G - 1) * D;
+#pragma unroll
+            for (int i = 0; i < 2 * KT; ++i) x[i] = *reinterpret_cast<const float2*>(qr + 8 * i);
+        };
+        if (new_q) {  // one power of two for the whole group: the scores are compared across its heads
+            float big = 0.f, sum = 0.f;
+#pragma unroll 1
+            for (int j0 = 0; j0 < G; j0 += kPaHeads) {
+                float2 x[2 * KT];
+                fetch_q(j0, x);
+                float one = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2 * KT; ++i) {
+                    big = fmaxf(big, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+                    one += fabsf(x[i].x) + fabsf(x[i].y);
+                }
+                one += __shfl_xor_sync(0xffffffffu, one, 1);
+                one += __shfl_xor_sync(0xffffffffu, one, 2);
+                sum = one > sum || one != one ? one : sum;  // NaN stays
+            }
+            big = pa_warp_max(big);
+            asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(sum) : "f"(sum));
+            const int ex = min(max((int)(__float_as_uint(big) >> 23) - 127, -120), 120);
+            up = __uint_as_float((unsigned)(127 - ex) << 23);
+            if (lane == 0 && cur.u == 0) a.group[sh_] = make_float2(up, sum * up);
+        }
         const uint32_t hst = ring + stage * (2 * TILE), lst = hst + TILE;
         float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         unsigned top = 0;
 #pragma unroll 1
         for (int j0 = 0; j0 < G; j0 += kPaHeads) {
             if (new_q || G > kPaHeads) {
-                const int j = min(j0 + g, G - 1);  // rows past the group repeat its last head
-                const float* qr = qg + j * D + 2 * t4;
+                float2 v[2 * KT];
+                fetch_q(j0, v);
 #pragma unroll
                 for (int i = 0; i < 2 * KT; ++i) {
-                    const float2 v = *reinterpret_cast<const float2*>(qr + 8 * i);
-                    float x = v.x * up, y = v.y * up;
+                    float x = v[i].x * up, y = v[i].y * up;
                     plus[i >> 1][i & 1] = (x > 0.f ? 0xffffu : 0u) | (y > 0.f ? 0xffff0000u : 0u);
                     qf[i >> 1][2 * (i & 1)] = pa_split<BF16>(x, y);
                     qf[i >> 1][2 * (i & 1) + 1] = pa_split<BF16>(x, y);
@@ -204,7 +223,6 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_score_kernel(PagedS
 #pragma unroll
             for (int i = 0; i < 4; ++i) best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], o));
         top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
-        const int64_t sh_ = (int64_t)cur.s * H + cur.head;
         if (lane < 4) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -236,55 +254,76 @@ __device__ __forceinline__ float from_order_key(unsigned k) {
     return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k);
 }
 
-// One warp: the 64-bit score of block b, every lane.
+// One warp: the 64-bit score of block b for query head j of KV head h, every
+// lane.
 template <bool BF16, int D>
-__device__ __forceinline__ unsigned long long exact_score(const PagedSelectArgs& a, int s, int h, int b) {
+__device__ __forceinline__ double exact_score(const PagedSelectArgs& a, int s, int h, int j, int page) {
     constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31, G = a.n_head / a.n_head_kv;
-    const int page = a.table[s * a.table_stride + b];
-    if ((unsigned)page >= (unsigned)a.n_pages) return 0ull;
+    const int lane = threadIdx.x & 31;
     const int64_t at = ((int64_t)page * a.n_head_kv + h) * D + lane * E;
-    float lo[E], hi[E];
+    const float* q = a.q + s * a.q_stride + (int64_t)(h * (a.n_head / a.n_head_kv) + j) * D + lane * E;
+    double x = 0.0;
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
-        const float2 l = unpack16<BF16>(*reinterpret_cast<const uint32_t*>(a.lo + at + e));
-        const float2 u = unpack16<BF16>(*reinterpret_cast<const uint32_t*>(a.hi + at + e));
-        lo[e] = l.x, lo[e + 1] = l.y, hi[e] = u.x, hi[e + 1] = u.y;
+        const float2 lo = unpack16<BF16>(*reinterpret_cast<const uint32_t*>(a.lo + at + e));
+        const float2 hi = unpack16<BF16>(*reinterpret_cast<const uint32_t*>(a.hi + at + e));
+        const float2 v = *reinterpret_cast<const float2*>(q + e);
+        x += fmax((double)v.x * lo.x, (double)v.x * hi.x);
+        x += fmax((double)v.y * lo.y, (double)v.y * hi.y);
     }
-    double best = -INFINITY;
-    bool nan = false;
-    for (int j = 0; j < G; ++j) {
-        const float* q = a.q + s * a.q_stride + (int64_t)(h * G + j) * D + lane * E;
-        double x = 0.0;
 #pragma unroll
-        for (int e = 0; e < E; ++e) x += fmax((double)q[e] * lo[e], (double)q[e] * hi[e]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        nan |= x != x;
-        best = fmax(best, x);
-    }
-    return nan ? 0ull : order_key(best);
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
 }
 
-constexpr int kTopkThreads = 512;
-constexpr int kTopkKeys = 24576;  // scores kept in shared memory
-constexpr int kTopkBand = 256;    // undecided blocks ranked in shared memory
+constexpr int kTopkThreads = 1024;
+constexpr int kTopkKeys = 8;      // consecutive scores a thread holds
+constexpr int kTopkBins = 2048;
+constexpr int kTopkList = 256;    // scores of one bin, or undecided blocks, ranked in shared memory
 
-// One CTA per (sequence, KV head).
+// Exclusive prefix of v over the CTA's threads, and the total; part: 32 ints.
+__device__ __forceinline__ int block_prefix(int v, int* part, int& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += x;
+    }
+    __syncthreads();  // the previous call's readers are done with part
+    if (lane == 31) part[warp] = incl;
+    __syncthreads();
+    const int mine = lane < (int)blockDim.x / 32 ? part[lane] : 0;
+    total = __reduce_add_sync(0xffffffffu, mine);
+    return incl - v + __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
+}
+
+// One CTA per (sequence, KV head).  A thread holds 8 consecutive scores (more
+// than 8192 blocks: tile by tile, read again in every pass).
+//   1. tau by a histogram of 2048 equal bins between the smallest and largest
+//      score (x -> bin is monotone, so the bins are in order), then by rank in
+//      the one bin that holds it; by bisection of the bits where that bin is
+//      crowded, as with many equal scores.
+//   2. the undecided blocks in 64 bits, one warp per block and query head, and
+//      their ranks; by bisection where there are more than 256.
+//   3. the chosen blocks in order, one prefix sum per tile.
 template <bool BF16, int D>
 __global__ void __launch_bounds__(kTopkThreads) paged_topk_kernel(PagedSelectArgs a) {
-    constexpr int T = kTopkThreads, W = T / 32;
-    extern __shared__ __align__(16) float topk_keys[];
+    constexpr int T = kTopkThreads, E = kTopkKeys, W = T / 32, L = kTopkList;
+    __shared__ int hist[kTopkBins];
     __shared__ int count[64];
-    __shared__ int band[kTopkBand], chosen[kTopkBand];
-    __shared__ unsigned long long band_key[kTopkBand];
-    __shared__ int n_band, s_ties;
-    __shared__ unsigned s_max;
-    __shared__ float s_sum[W];
-    __shared__ int wsum[2][W];
+    __shared__ float list[L];
+    __shared__ int band[L], band_nan[L], chosen[L];
+    __shared__ unsigned long long band_key[L];
+    __shared__ int part[32];
+    __shared__ int n_list, n_band, n_in, s_bin, s_rank;
+    __shared__ unsigned s_top, s_low, s_high, s_tau;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int sh_ = blockIdx.x, s = sh_ / a.n_head_kv, h = sh_ - s * a.n_head_kv;
     const int G = a.n_head / a.n_head_kv;
+    for (int i = tid; i < kTopkBins; i += T) hist[i] = 0;
+    if (tid < 64) count[tid] = 0;
+    if (tid == 0) n_list = n_band = n_in = 0, s_top = s_high = 0, s_low = 0xffffffffu;
     griddep_wait();  // the scores
     const int len = a.seq_lens[s];
     const int nb = paged_blocks(len, a.max_blocks, a.page_size);
@@ -300,181 +339,213 @@ __global__ void __launch_bounds__(kTopkThreads) paged_topk_kernel(PagedSelectArg
         return;
     }
     const float* score = a.approx + (int64_t)sh_ * a.max_blocks;
-    if (m <= kTopkKeys) {
-        for (int i = tid; i < m; i += T) topk_keys[i] = score[i];
-        score = topk_keys;
+    float x[E];
+    int tile = -1;
+    const int tiles = (m + T * E - 1) / (T * E);
+    auto each = [&](auto f) {  // f(i, score) over this thread's scores
+        for (int t = 0; t < tiles; ++t) {
+            if (t != tile) {
+                tile = t;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int i = (t * T + tid) * E + e;
+                    x[e] = i < m ? score[i] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int i = (t * T + tid) * E + e;
+                if (i < m) f(i, x[e]);
+            }
+        }
+    };
+    {
+        unsigned top = 0, low = 0xffffffffu, high = 0;
+        const int nu = paged_units(nb);
+        for (int i = tid; i < nu; i += T) top = max(top, a.unit_max[(int64_t)sh_ * paged_units(a.max_blocks) + i]);
+        each([&](int, float v) {
+            const unsigned k = order_key(v);
+            high = max(high, k);
+            if (v != -INFINITY) low = min(low, k);
+        });
+        top = __reduce_max_sync(0xffffffffu, top);
+        low = __reduce_min_sync(0xffffffffu, low);
+        high = __reduce_max_sync(0xffffffffu, high);
+        __syncthreads();  // the counters are cleared
+        if (lane == 0) {
+            atomicMax(&s_top, top);
+            atomicMin(&s_low, low);
+            atomicMax(&s_high, high);
+        }
     }
-    if (tid < 64) count[tid] = 0;
-    if (tid == 0) n_band = 0, s_ties = 0, s_max = 0;
+    const float2 group = a.group[sh_];
+    __syncthreads();
     // eps, with S = max_j sum |q'_jd| * max |bound| and q' = q 2^-ex, whose
     // largest entry is in [1, 2): the parts of q' leave out at most 2^-23 each, in
     // all D 2^-23 S; D / 8 instructions (bf16: D / 4) each truncate 17 terms
     // below 2^-24 S, in all 17 D 2^-27 S (bf16: twice that).  D 2^-21 S (bf16:
     // twice that) covers both, 1e-30 what underflows.
-    const float* qg = a.q + s * a.q_stride + (int64_t)h * G * D;
-    const float up = __uint_as_float((unsigned)(127 - group_exponent(qg, G * D)) << 23);
-    float qs = 0.f;
-    for (int j = warp; j < G; j += W) {
-        float x = 0.f;
-        for (int d = lane; d < D; d += 32) x += fabsf(qg[j * D + d] * up);
-        x = warp_sum(x);
-        qs = x > qs || x != x ? x : qs;  // NaN stays
-    }
-    __syncthreads();
-    if (lane == 0) s_sum[warp] = qs;
-    {
-        const int nu = paged_units(nb);
-        unsigned top = 0;
-        for (int i = tid; i < nu; i += T) top = max(top, a.unit_max[(int64_t)sh_ * paged_units(a.max_blocks) + i]);
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) atomicMax(&s_max, top);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < W; ++w) qs = s_sum[w] > qs || s_sum[w] != s_sum[w] ? s_sum[w] : qs;
-    const float biggest = BF16 ? __uint_as_float(s_max << 16) : h2f((uint16_t)s_max);
-    const float eps = qs * biggest * ((BF16 ? 2.f : 1.f) * D * 4.76837158e-7f) * 1.001f + 1e-30f;
-
-    // tau: the need-th largest score, bit by bit from the top; with exactly
-    // `need` scores at or above the trial it is the smallest of those
-    unsigned tau_key = 0;
-    bool sure = eps < 1e30f;  // false: bounds or queries that are not finite, nothing is decided by the scores
+    const float biggest = BF16 ? __uint_as_float(s_top << 16) : h2f((uint16_t)s_top);
+    const float eps = group.y * biggest * ((BF16 ? 2.f : 1.f) * D * 4.76837158e-7f) * 1.001f + 1e-30f;
+    const bool sure = eps < 1e30f;  // not: bounds or queries that are not finite, nothing is decided by the scores
+    float tau = 0.f;
     if (sure) {
-        int bit = 31;
-        for (; bit >= 0; --bit) {
-            const unsigned trial = tau_key | 1u << bit;
-            int c = 0;
-            for (int i = tid; i < m; i += T) c += order_key(score[i]) >= trial;
-            c = __reduce_add_sync(0xffffffffu, c);
-            if (lane == 0 && c) atomicAdd(&count[bit], c);
+        const float low = from_order_key(s_low), high = from_order_key(s_high);
+        const float per_bin = high > low ? (kTopkBins - 1) / (high - low) : 0.f;  // (0 where high - low overflows)
+        auto bin = [&](float v) {
+            return v == -INFINITY ? 0 : min(kTopkBins - 1, max(0, (int)((v - low) * per_bin)));
+        };
+        each([&](int, float v) { atomicAdd(&hist[bin(v)], 1); });
+        __syncthreads();
+        // from the top bin down: the one where the need-th score is
+        static_assert(kTopkBins == 2 * T, "two bins a thread");
+        const int b0 = kTopkBins - 1 - 2 * tid, h0 = hist[b0], h1 = hist[b0 - 1];
+        int total;
+        const int above = block_prefix(h0 + h1, part, total);
+        if (above < need && need <= above + h0) s_bin = b0, s_rank = need - above;
+        else if (above + h0 < need && need <= above + h0 + h1) s_bin = b0 - 1, s_rank = need - above - h0;
+        __syncthreads();
+        const int where = s_bin, rank = s_rank;  // the rank-th largest of this bin
+        if (hist[where] <= L) {
+            each([&](int, float v) {
+                if (bin(v) == where) list[atomicAdd(&n_list, 1)] = v;
+            });
             __syncthreads();
-            c = count[bit];
-            if (c >= need) tau_key = trial;
-            if (c == need) break;
-        }
-        if (bit >= 0) {
-            unsigned low = 0xffffffffu;
-            for (int i = tid; i < m; i += T) {
-                const unsigned k = order_key(score[i]);
-                if (k >= tau_key) low = min(low, k);
+            const int n = n_list;
+            for (int k = tid; k < n; k += T) {
+                int more = 0, same = 0;
+                for (int y = 0; y < n; ++y) more += list[y] > list[k], same += list[y] == list[k];
+                if (more < rank && rank <= more + same) s_tau = order_key(list[k]);  // equal scores, equal keys
             }
-            low = __reduce_min_sync(0xffffffffu, low);
-            if (tid == 0) s_max = 0xffffffffu;
-            __syncthreads();
-            if (lane == 0) atomicMin(&s_max, low);
-            __syncthreads();
-            tau_key = s_max;
+        } else {
+            unsigned key = 0;
+            for (int bit = 31; bit >= 0; --bit) {
+                const unsigned trial = key | 1u << bit;
+                int c = 0;
+                each([&](int, float v) { c += bin(v) == where && order_key(v) >= trial; });
+                c = __reduce_add_sync(0xffffffffu, c);
+                if (lane == 0 && c) atomicAdd(&count[bit], c);
+                __syncthreads();
+                if (count[bit] >= rank) key = trial;
+            }
+            if (tid == 0) s_tau = key;
         }
+        __syncthreads();
+        tau = from_order_key(s_tau);
     }
-    const float tau = sure ? from_order_key(tau_key) : 0.f;
-    const float above = sure ? tau + 2.01f * eps : INFINITY, below = sure ? tau - 2.01f * eps : -INFINITY;
-    // in: score > above; undecided: [below, above]
-    auto undecided = [&](float x) { return !sure || (x >= below && x <= above); };
-    int n_in = 0;
-    for (int i = tid; i < m; i += T) {
-        const float x = score[i];
-        if (undecided(x)) {
-            const int k = atomicAdd(&n_band, 1);
-            if (k < kTopkBand) band[k] = i;
-        } else if (x > above) {
-            ++n_in;
-        }
+    // chosen: score > over; undecided: [under, over]
+    const float over = sure ? tau + 2.01f * eps : INFINITY, under = sure ? tau - 2.01f * eps : -INFINITY;
+    auto undecided = [&](float v) { return !sure || (v >= under && v <= over); };
+    {
+        int c = 0;
+        each([&](int i, float v) {
+            if (undecided(v)) {
+                const int k = atomicAdd(&n_band, 1);
+                if (k < L) band[k] = i;
+            } else if (v > over) {
+                ++c;
+            }
+        });
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (lane == 0 && c) atomicAdd(&n_in, c);
     }
-    n_in = __reduce_add_sync(0xffffffffu, n_in);
-    if (lane == 0 && n_in) atomicAdd(&count[32], n_in);
     __syncthreads();
-    const int nbnd = n_band, left = need - count[32];  // `left` of the nbnd undecided blocks
-    const bool small = nbnd <= kTopkBand;
-    unsigned long long cut = 0;  // large bands: the smallest 64-bit key chosen, `ties` of its equals
+    const int nbnd = n_band, left = need - n_in;  // `left` of the nbnd undecided blocks
+    const bool all_in = left == nbnd, small = nbnd <= L;
+    unsigned long long* exact = a.exact + (int64_t)sh_ * a.max_blocks;
+    unsigned long long cut = 0;  // many undecided: the smallest 64-bit key chosen, and `ties` of its equals
     int ties = 0;
-    if (left == nbnd) {
-        // all of them
-    } else if (small) {
-        for (int k = warp; k < nbnd; k += W) {
-            const unsigned long long key = exact_score<BF16, D>(a, s, h, band[k]);
-            if (lane == 0) band_key[k] = key;
+    if (!all_in && small) {
+        for (int k = tid; k < nbnd; k += T) band_key[k] = 0, band_nan[k] = 0;
+        __syncthreads();
+        for (int y = warp; y < nbnd * G; y += W) {
+            const int k = y / G, page = a.table[s * a.table_stride + band[k]];
+            if ((unsigned)page >= (unsigned)a.n_pages) continue;  // stays below everything
+            const double v = exact_score<BF16, D>(a, s, h, y - k * G, page);
+            if (lane == 0) {
+                if (v != v) band_nan[k] = 1;
+                else atomicMax(&band_key[k], order_key(v));
+            }
         }
         __syncthreads();
         for (int k = tid; k < nbnd; k += T) {
+            const unsigned long long mine = band_nan[k] ? 0 : band_key[k];
             int rank = 0;
-            for (int x = 0; x < nbnd; ++x)
-                rank += band_key[x] > band_key[k] || (band_key[x] == band_key[k] && band[x] < band[k]);
+            for (int y = 0; y < nbnd; ++y) {
+                const unsigned long long other = band_nan[y] ? 0 : band_key[y];
+                rank += other > mine || (other == mine && band[y] < band[k]);
+            }
             chosen[k] = rank < left;
         }
         __syncthreads();
-    } else {
-        unsigned long long* exact = a.exact + (int64_t)sh_ * a.max_blocks;
+    } else if (!all_in) {
         for (int i = warp; i < m; i += W) {
             if (!undecided(score[i])) continue;
-            const unsigned long long key = exact_score<BF16, D>(a, s, h, i);
+            const int page = a.table[s * a.table_stride + i];
+            unsigned long long key = 0;
+            if ((unsigned)page < (unsigned)a.n_pages) {
+                bool nan = false;
+                for (int j = 0; j < G; ++j) {
+                    const double v = exact_score<BF16, D>(a, s, h, j, page);
+                    nan |= v != v;
+                    if (v == v) key = max(key, order_key(v));
+                }
+                if (nan) key = 0;
+            }
             if (lane == 0) exact[i] = key;
         }
         __syncthreads();
         if (tid < 64) count[tid] = 0;
+        if (tid == 0) n_list = 0;
         __syncthreads();
         for (int bit = 63; bit >= 0; --bit) {
             const unsigned long long trial = cut | 1ull << bit;
             int c = 0;
-            for (int i = tid; i < m; i += T) c += undecided(score[i]) && exact[i] >= trial;
+            each([&](int i, float v) { c += undecided(v) && exact[i] >= trial; });
             c = __reduce_add_sync(0xffffffffu, c);
             if (lane == 0 && c) atomicAdd(&count[bit], c);
             __syncthreads();
             if (count[bit] >= left) cut = trial;
         }
         int c = 0;
-        for (int i = tid; i < m; i += T) c += undecided(score[i]) && exact[i] > cut;
+        each([&](int i, float v) { c += undecided(v) && exact[i] > cut; });
         c = __reduce_add_sync(0xffffffffu, c);
-        if (lane == 0 && c) atomicAdd(&s_ties, c);
+        if (lane == 0 && c) atomicAdd(&n_list, c);
         __syncthreads();
-        ties = left - s_ties;
+        ties = left - n_list;
     }
 
     // the chosen blocks in ascending order
     int done = 0, tied = 0;
-    for (int base = 0; base < m; base += T) {
-        const int i = base + tid;
-        bool take = false, tie = false;
-        if (i < m) {
-            const float x = score[i];
-            if (undecided(x)) {
-                if (left == nbnd) {
-                    take = true;
-                } else if (small) {
-                    for (int k = 0; k < nbnd; ++k)
-                        if (band[k] == i) take = chosen[k];
-                } else {
-                    const unsigned long long key = a.exact[(int64_t)sh_ * a.max_blocks + i];
-                    take = key > cut;
-                    tie = key == cut;
-                }
-            } else {
-                take = x > above;
-            }
-        }
-        if (!small && left != nbnd) {  // equals of the cut: the first `ties` of them
-            const unsigned tm = __ballot_sync(0xffffffffu, tie);
-            if (lane == 0) wsum[0][warp] = __popc(tm);
-            __syncthreads();
-            int at = tied + __popc(tm & ((1u << lane) - 1u)), all = 0;
-            for (int w = 0; w < W; ++w) {
-                if (w < warp) at += wsum[0][w];
-                all += wsum[0][w];
-            }
-            take |= tie && at < ties;
-            tied += all;
-        }
-        const unsigned km = __ballot_sync(0xffffffffu, take);
-        if (lane == 0) wsum[1][warp] = __popc(km);
-        __syncthreads();
-        int at = done + __popc(km & ((1u << lane) - 1u)), all = 0;
+    for (int t = 0; t < tiles; ++t) {
+        unsigned take = 0, tie = 0;  // bit e: this thread's e-th score of the tile
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            if (w < warp) at += wsum[1][w];
-            all += wsum[1][w];
+        for (int e = 0; e < E; ++e) {
+            const int i = (t * T + tid) * E + e;
+            if (i >= m) break;
+            const float v = tiles == 1 ? x[e] : score[i];
+            if (!undecided(v)) {
+                take |= (v > over ? 1u : 0u) << e;
+            } else if (all_in) {
+                take |= 1u << e;
+            } else if (small) {
+                for (int k = 0; k < nbnd; ++k)
+                    if (band[k] == i && chosen[k]) take |= 1u << e;
+            } else {
+                take |= (exact[i] > cut ? 1u : 0u) << e;
+                tie |= (exact[i] == cut ? 1u : 0u) << e;
+            }
         }
-        if (take) out[at] = i;
-        done += all;
-        __syncthreads();
+        int total;
+        if (!all_in && !small) {  // of the cut's equals the first `ties`
+            int at = tied + block_prefix(__popc(tie), part, total);
+            for (; tie != 0; tie &= tie - 1)
+                if (at++ < ties) take |= tie & (0u - tie);
+            tied += total;
+        }
+        int at = done + block_prefix(__popc(take), part, total);
+        for (; take != 0; take &= take - 1) out[at++] = (t * T + tid) * E + __ffs(take) - 1;
+        done += total;
     }
     if (tid == 0) out[need] = m;
 }

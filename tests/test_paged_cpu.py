@@ -91,13 +91,13 @@ BAD_BATCH = [dict(q=None), dict(q=PTR + 4), dict(q_stride=510), dict(q_stride=50
              dict(n_seq=65536), dict(n_head=0), dict(n_head=3), dict(n_head=-2), dict(block_table=None),
              dict(table_stride=3), dict(max_blocks=0), dict(seq_lens=None),
              dict(max_blocks=1 << 28, table_stride=1 << 28)]
-SELECT = dict(n_sel=2, sel=PTR, workspace=PTR, workspace_size=768, stream=None)
+SELECT = dict(n_sel=2, sel=PTR, workspace=PTR, workspace_size=1024, stream=None)
 ATTN = dict(mask=None, mask_stride=0, sel=None, n_sel=0, scale=1.0, out=PTR, workspace=PTR, workspace_size=1 << 30,
             stream=None)
 
 
 @pytest.mark.parametrize("over", BAD_BATCH + [dict(n_sel=0), dict(n_sel=-1), dict(sel=None), dict(workspace=None),
-                                              dict(workspace=PTR + 8), dict(workspace_size=767)])
+                                              dict(workspace=PTR + 8), dict(workspace_size=1023)])
 def test_select_refuses(over):
     kv = kv_struct()
     a = {**BATCH, **SELECT, **over}
@@ -134,8 +134,8 @@ def test_empty_batches_are_nothing_to_do():
 
 def test_workspace_sizes():
     bw = B()
-    assert bw.paged_select_workspace_size(2, 2, 4) == 768  # three arrays of at most 256 bytes
-    assert bw.paged_select_workspace_size(16, 8, 2048) == 16 * 8 * (2048 * 12 + 128 * 4)
+    assert bw.paged_select_workspace_size(2, 2, 4) == 1024  # four arrays of at most 256 bytes
+    assert bw.paged_select_workspace_size(16, 8, 2048) == 16 * 8 * (2048 * 12 + 128 * 4 + 8)
     assert bw.paged_select_workspace_size(-1, 2, 5) == bw.paged_select_workspace_size(3, 0, 5) == 0
     assert bw.paged_select_workspace_size(3, 2, 0) == bw.paged_select_workspace_size(1, 1, (1 << 20) + 1) == 0
     for bad in [(96, 2, 4, 2), (128, -1, 4, 2), (128, 2, 0, 2), (128, 2, 4, 0), (128, 2, 5, 2)]:
