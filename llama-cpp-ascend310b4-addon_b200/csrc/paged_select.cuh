@@ -10,7 +10,7 @@
 // second finds the need-th largest of those, tau.  The exact need-th largest
 // score is within eps of tau, so a block above tau + 2 eps is chosen and one
 // below tau - 2 eps is not, whatever the rounding; the blocks in between
-// (three or so of 2048) are scored again in 64 bits and ranked.
+// (mostly the one at tau) are scored again in 64 bits and ranked.
 //
 // max(q lo, q hi) summed over d is  q+ . hi + q- . lo  with q+ = max(q, 0),
 // q- = min(q, 0): two matrix products per block, with the operands of the
@@ -194,7 +194,9 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_score_kernel(PagedS
                     if (BF16) q3[i >> 1][i & 1] = pa_split<BF16>(x, y);
                 }
             }
-            float sc[2][4] = {};
+            // each instruction from zero, added up outside the tensor core, which
+            // truncates: the bound on the sum is what keeps the undecided few
+            float sc[4] = {};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {  // q+ with hi, then q- with lo
 #pragma unroll
@@ -207,14 +209,17 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_score_kernel(PagedS
                     const uint32_t m0 = half ? ~plus[kt][0] : plus[kt][0], m1 = half ? ~plus[kt][1] : plus[kt][1];
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
-                        pa_mma<BF16>(sc[n], qf[kt][0] & m0, qf[kt][1] & m0, qf[kt][2] & m1, qf[kt][3] & m1, b[2 * n],
+                        float d[4] = {};
+                        pa_mma<BF16>(d, qf[kt][0] & m0, qf[kt][1] & m0, qf[kt][2] & m1, qf[kt][3] & m1, b[2 * n],
                                      b[2 * n + 1]);
-                        if (BF16) pa_mma<BF16>(sc[n], q3[kt][0] & m0, 0u, q3[kt][1] & m1, 0u, b[2 * n], b[2 * n + 1]);
+                        if (BF16) pa_mma<BF16>(d, q3[kt][0] & m0, 0u, q3[kt][1] & m1, 0u, b[2 * n], b[2 * n + 1]);
+                        sc[2 * n] += d[0] + d[2];
+                        sc[2 * n + 1] += d[1] + d[3];
                     }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) best[i] = fmaxf(best[i], sc[i >> 1][i & 1] + sc[i >> 1][2 + (i & 1)]);
+            for (int i = 0; i < 4; ++i) best[i] = fmaxf(best[i], sc[i]);
         }
         const unsigned valid = sh.valid[warp][stage];
         // the largest over the heads, which are 8 lanes; then lanes 0-3 hold the unit
@@ -277,7 +282,7 @@ __device__ __forceinline__ double exact_score(const PagedSelectArgs& a, int s, i
 }
 
 constexpr int kTopkThreads = 1024;
-constexpr int kTopkKeys = 8;      // consecutive scores a thread holds
+constexpr int kTopkKeys = 8;      // consecutive scores a thread holds, at most
 constexpr int kTopkBins = 2048;
 constexpr int kTopkList = 256;    // scores of one bin, or undecided blocks, ranked in shared memory
 
@@ -298,8 +303,8 @@ __device__ __forceinline__ int block_prefix(int v, int* part, int& total) {
     return incl - v + __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
 }
 
-// One CTA per (sequence, KV head).  A thread holds 8 consecutive scores (more
-// than 8192 blocks: tile by tile, read again in every pass).
+// One CTA per (sequence, KV head).  A thread holds up to 8 consecutive scores
+// (more than 8192 blocks: tile by tile, read again in every pass).
 //   1. tau by a histogram of 2048 equal bins between the smallest and largest
 //      score (x -> bin is monotone, so the bins are in order), then by rank in
 //      the one bin that holds it; by bisection of the bits where that bin is
@@ -324,8 +329,8 @@ __global__ void __launch_bounds__(kTopkThreads) paged_topk_kernel(PagedSelectArg
     for (int i = tid; i < kTopkBins; i += T) hist[i] = 0;
     if (tid < 64) count[tid] = 0;
     if (tid == 0) n_list = n_band = n_in = 0, s_top = s_high = 0, s_low = 0xffffffffu;
-    griddep_wait();  // the scores
     const int len = a.seq_lens[s];
+    griddep_wait();  // the scores
     const int nb = paged_blocks(len, a.max_blocks, a.page_size);
     if (tid == 0 && h == 0 && (len < 0 || len > (int64_t)a.max_blocks * a.page_size)) record_status(B200_DEVSTATUS_BOUNDS);
     int32_t* out = a.sel + (int64_t)sh_ * a.n_sel;
@@ -341,21 +346,21 @@ __global__ void __launch_bounds__(kTopkThreads) paged_topk_kernel(PagedSelectArg
     const float* score = a.approx + (int64_t)sh_ * a.max_blocks;
     float x[E];
     int tile = -1;
-    const int tiles = (m + T * E - 1) / (T * E);
+    const int per = min(E, (m + T - 1) / T), tiles = (m + T * per - 1) / (T * per);
     auto each = [&](auto f) {  // f(i, score) over this thread's scores
         for (int t = 0; t < tiles; ++t) {
             if (t != tile) {
                 tile = t;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const int i = (t * T + tid) * E + e;
-                    x[e] = i < m ? score[i] : -INFINITY;
+                    const int i = (t * T + tid) * per + e;
+                    x[e] = e < per && i < m ? score[i] : -INFINITY;
                 }
             }
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const int i = (t * T + tid) * E + e;
-                if (i < m) f(i, x[e]);
+                const int i = (t * T + tid) * per + e;
+                if (e < per && i < m) f(i, x[e]);
             }
         }
     };
@@ -380,13 +385,14 @@ __global__ void __launch_bounds__(kTopkThreads) paged_topk_kernel(PagedSelectArg
     }
     const float2 group = a.group[sh_];
     __syncthreads();
-    // eps, with S = max_j sum |q'_jd| * max |bound| and q' = q 2^-ex, whose
-    // largest entry is in [1, 2): the parts of q' leave out at most 2^-23 each, in
-    // all D 2^-23 S; D / 8 instructions (bf16: D / 4) each truncate 17 terms
-    // below 2^-24 S, in all 17 D 2^-27 S (bf16: twice that).  D 2^-21 S (bf16:
-    // twice that) covers both, 1e-30 what underflows.
+    // eps, with q' = q 2^-ex, whose largest entry is in [1, 2), M = max |bound| and
+    // S = M max_j sum |q'_jd|: the parts of q' leave out at most 2^-23 of each
+    // entry, in all D 2^-23 M; an instruction (bf16: two) truncates 16 products
+    // (33 terms) below 2^-24 of the largest, in all 33 2^-24 S; adding its high
+    // and low halves and the D / 8 instructions rounds D / 8 + 1 times by 2^-24 S
+    // at most.  1e-30 covers what underflows.
     const float biggest = BF16 ? __uint_as_float(s_top << 16) : h2f((uint16_t)s_top);
-    const float eps = group.y * biggest * ((BF16 ? 2.f : 1.f) * D * 4.76837158e-7f) * 1.001f + 1e-30f;
+    const float eps = biggest * (D * 0x1p-23f + group.y * (36 + D / 8) * 0x1p-24f) * 1.01f + 1e-30f;
     const bool sure = eps < 1e30f;  // not: bounds or queries that are not finite, nothing is decided by the scores
     float tau = 0.f;
     if (sure) {
@@ -521,8 +527,8 @@ __global__ void __launch_bounds__(kTopkThreads) paged_topk_kernel(PagedSelectArg
         unsigned take = 0, tie = 0;  // bit e: this thread's e-th score of the tile
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int i = (t * T + tid) * E + e;
-            if (i >= m) break;
+            const int i = (t * T + tid) * per + e;
+            if (e >= per || i >= m) break;
             const float v = tiles == 1 ? x[e] : score[i];
             if (!undecided(v)) {
                 take |= (v > over ? 1u : 0u) << e;
@@ -544,7 +550,7 @@ __global__ void __launch_bounds__(kTopkThreads) paged_topk_kernel(PagedSelectArg
             tied += total;
         }
         int at = done + block_prefix(__popc(take), part, total);
-        for (; take != 0; take &= take - 1) out[at++] = (t * T + tid) * E + __ffs(take) - 1;
+        for (; take != 0; take &= take - 1) out[at++] = (t * T + tid) * per + __ffs(take) - 1;
         done += total;
     }
     if (tid == 0) out[need] = m;
