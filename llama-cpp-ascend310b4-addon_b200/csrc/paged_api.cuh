@@ -35,13 +35,49 @@ int check_paged_batch(const b200_paged_kv* kv, const float* q, int64_t q_stride,
     return B200_OK;
 }
 
+bool g_paged_plan_attr[kMaxDevices];
+
+int launch_paged_plan(const PagedPlanArgs& a, cudaStream_t st) {
+    const int dev = current_device();
+    if (dev < 0 || dev >= kMaxDevices) return B200_EINVAL;
+    {
+        std::lock_guard<std::mutex> lk(g_attr_mu);
+        if (!g_paged_plan_attr[dev]) {
+            CR_(cuda_status(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)plan_smem_bytes(B200_PAGED_PLAN_MAX_SEQS))));
+            g_paged_plan_attr[dev] = true;
+        }
+    }
+    // one cluster: every CTA scans the sequences, and each takes its share of
+    // the token rows
+    const int rows = std::max(a.max_tokens, a.n_seq);
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3((unsigned)std::min(kPlanThreads, (rows + 63) / 64 * 64), 1, 1);
+    cfg.gridDim = dim3((unsigned)std::min(kPlanCtas, (a.max_tokens + 2 * kPlanThreads - 1) / (2 * kPlanThreads) + 1), 1, 1);
+    cfg.dynamicSmemBytes = plan_smem_bytes(a.n_seq);
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = cfg.gridDim.x;
+    at.val.clusterDim.y = 1;
+    at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, paged_plan_kernel, a));
+}
+
 template <bool BF16>
 int launch_paged_store(const PagedStoreArgs& a, cudaStream_t st) {
-    const dim3 grid((unsigned)a.n_tokens, (unsigned)a.kv.n_head_kv);
+    // about four CTAs' worth of tiles for every place a CTA of this size has on
+    // the GPU: decode steps, whose tokens are runs of their own, get one each,
+    // prompts few that find no run
+    const int64_t want = (a.n_tokens * a.kv.n_head_kv + 4735) / 4736;
+    const int tile = (int)std::max<int64_t>(1, std::min<int64_t>(want, std::min(kStoreTile, a.kv.page_size)));
+    const dim3 grid((unsigned)((a.n_tokens + tile - 1) / tile), (unsigned)a.kv.n_head_kv);
     switch (a.kv.head_dim) {
-        case 64: paged_store_kernel<BF16, 64><<<grid, kStoreThreads, 0, st>>>(a); break;
-        case 128: paged_store_kernel<BF16, 128><<<grid, kStoreThreads, 0, st>>>(a); break;
-        default: paged_store_kernel<BF16, 256><<<grid, kStoreThreads, 0, st>>>(a); break;
+        case 64: paged_store_kernel<BF16, 64><<<grid, kStoreThreads, 0, st>>>(a, tile); break;
+        case 128: paged_store_kernel<BF16, 128><<<grid, kStoreThreads, 0, st>>>(a, tile); break;
+        default: paged_store_kernel<BF16, 256><<<grid, kStoreThreads, 0, st>>>(a, tile); break;
     }
     return cuda_status(cudaGetLastError());
 }
@@ -155,11 +191,7 @@ int b200_paged_plan(const int32_t* new_lens, const int32_t* seq_lens, int n_seq,
     a.page_size = page_size;
     a.n_pages = (int)n_pages;
     a.max_tokens = (int)max_tokens;
-    const size_t smem = plan_smem_bytes(n_seq);
-    CR_(cuda_status(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)plan_smem_bytes(B200_PAGED_PLAN_MAX_SEQS))));
-    paged_plan_kernel<<<1, kPlanThreads, smem, (cudaStream_t)stream>>>(a);
-    return cuda_status(cudaGetLastError());
+    return launch_paged_plan(a, (cudaStream_t)stream);
 }
 
 int b200_paged_store(const b200_paged_kv* kv, const float* k, int64_t k_ld, const float* v, int64_t v_ld,

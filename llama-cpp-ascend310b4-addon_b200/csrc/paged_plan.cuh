@@ -4,8 +4,12 @@
 // pages needed, pages given back): a token's sequence, a new page's block and
 // a popped stack entry are then found by binary search in shared memory, so
 // the writes are spread over threads by output element, however uneven the
-// sequences are.
+// sequences are.  The call is bound by latency (a few hundred KB at most): one
+// cluster of up to 8 CTAs, each with the sums of all sequences, so nothing but
+// one barrier separates reading the lengths from replacing them in place.
 #pragma once
+
+#include <cooperative_groups.h>
 
 #include "args.h"
 #include "common.cuh"
@@ -28,6 +32,7 @@ struct PagedPlanArgs {
 };
 
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanCtas = 8;
 
 B200_HD inline size_t plan_smem_bytes(int n_seq) { return (size_t)(4 * n_seq + 3) * sizeof(int); }
 
@@ -75,7 +80,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
     const int cap = (int)min((long long)a.max_blocks * ps, (long long)INT32_MAX);
     int n0 = a.n_free[0];
     if (n0 < 0 || n0 > a.n_pages) {
-        if (tid == 0) record_status(B200_DEVSTATUS_BOUNDS);
+        if (tid == 0 && blockIdx.x == 0) record_status(B200_DEVSTATUS_BOUNDS);
         n0 = n0 < 0 ? 0 : a.n_pages;
     }
     if (tid == 0) s_got = 0, s_cu[0] = 0, s_need[0] = 0, s_back[0] = 0;
@@ -122,7 +127,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
     __syncthreads();
     long long top = n0 + back_sum;
     if (top > a.n_pages) {  // more pages given back than exist: the surplus is dropped
-        if (tid == 0) record_status(B200_DEVSTATUS_BOUNDS);
+        if (tid == 0 && blockIdx.x == 0) record_status(B200_DEVSTATUS_BOUNDS);
         top = a.n_pages;
     }
     const int pool = (int)top, n_back = pool - n0;
@@ -142,7 +147,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
     };
     auto blocks_of = [&](int tokens) { return (int)(((unsigned)tokens + (unsigned)ps - 1u) / (unsigned)ps); };
 
-    for (int t = tid; t < a.max_tokens; t += blockDim.x) {
+    const int at = blockIdx.x * blockDim.x + tid, step = gridDim.x * blockDim.x;
+    for (int t = at; t < a.max_tokens; t += step) {
         int64_t slot = -1;
         int pos = -1;
         if (t < s_cu[n]) {
@@ -164,16 +170,18 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
         a.slots[t] = slot;
         a.positions[t] = pos;
     }
-    for (int r = tid; r < got; r += blockDim.x) {
+    for (int r = at; r < got; r += step) {
         const int i = find_segment(s_need, n, r);
         a.table[i * a.table_stride + blocks_of(s_old[i]) + (r - s_need[i])] = popped(r);
     }
-    for (int r = tid; r < n_back; r += blockDim.x) {
+    for (int r = at; r < n_back; r += step) {
         const int page = given_back(r);
         if ((unsigned)page >= (unsigned)a.n_pages) record_status(B200_DEVSTATUS_BOUNDS);
         a.free_pages[n0 + r] = page;
     }
-    for (int i = tid; i < n; i += blockDim.x) {
+    // every CTA has read the lengths and the page count
+    cooperative_groups::this_cluster().sync();
+    for (int i = at; i < n; i += step) {
         const int old = s_old[i];
         int len = old >= 0 ? old : ~old;
         if (a.new_lens[i] < 0) len = 0;
@@ -181,7 +189,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
         a.seq_lens_out[i] = len;
         a.cu[i] = s_cu[i];
     }
-    if (tid == 0) {
+    if (at == 0) {
         a.cu[n] = s_cu[n];
         a.n_free_out[0] = pool - got;
     }

@@ -35,80 +35,108 @@ struct PagedStoreArgs {
     int64_t n_tokens;
 };
 
-constexpr int kStoreThreads = 128;
+constexpr int kStoreThreads = 256;
+constexpr int kStoreTile = 32;  // tokens whose runs one CTA looks for, at most
+constexpr int kStoreRows = 4;   // rows a thread has in flight
 
-// CTA (t, head): active where token t opens a run of tokens of one page; it
-// stores the run's rows of that head.
+// CTA (tile of `tile` tokens, head): the runs of tokens of one page that begin
+// in its tile, wherever they end.  D / 8 lanes take a row of the head, 16 bytes
+// of the page each, and the CTA's groups of lanes every kStoreThreads / (D / 8)-th
+// row; a page's bounds are theirs alone, so they meet in shared memory once per
+// run, without atomics.  Bound by memory: 12 bytes per element.
 template <bool BF16, int D>
-__global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(PagedStoreArgs a) {
-    constexpr int LPR = D / 8;                  // lanes per row, 8 values each
-    constexpr int RPP = kStoreThreads / LPR;    // rows per pass
-    __shared__ float s_lo[RPP][D], s_hi[RPP][D];
-    __shared__ int s_first;
+__global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(PagedStoreArgs a, int tile) {
+    constexpr int LPR = D / 8;                // lanes per row, 8 values each
+    constexpr int RPP = kStoreThreads / LPR;  // rows per pass
+    constexpr int W = kStoreThreads / 32;
+    __shared__ float s_lo[W][D], s_hi[W][D];
     const int64_t n_slots = a.kv.n_pages * a.kv.page_size;
-    const int ps = a.kv.page_size, head = blockIdx.y, tid = threadIdx.x;
+    const int ps = a.kv.page_size, head = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
     const int g = tid / LPR, d = (tid % LPR) * 8;
-    auto page_of = [&](int64_t t) -> int {
-        if (t < 0 || t >= a.n_tokens) return -1;
-        const int64_t s = a.slots[t];
-        return s >= 0 && s < n_slots ? (int)((unsigned)s / (unsigned)ps) : -1;
-    };
-    const int64_t t0 = blockIdx.x;
-    const int page = page_of(t0);
-    if (page < 0) {
-        if (tid == 0 && a.slots[t0] >= n_slots) record_status(B200_DEVSTATUS_BOUNDS);
-        return;
+    auto slot_of = [&](int64_t t) -> int64_t { return t >= 0 && t < a.n_tokens ? a.slots[t] : -1; };
+    auto page_of = [&](int64_t s) -> int { return s >= 0 && s < n_slots ? (int)((unsigned)s / (unsigned)ps) : -1; };
+    const int64_t first = (int64_t)blockIdx.x * tile;
+    unsigned starts;
+    {
+        const int64_t s = lane < tile ? slot_of(first + lane) : -1;
+        if (s >= n_slots) record_status(B200_DEVSTATUS_BOUNDS);
+        const int page = page_of(s), before = page_of(slot_of(first + lane - 1));
+        starts = __ballot_sync(0xffffffffu, page >= 0 && page != before);
     }
-    if (page_of(t0 - 1) == page) return;
-    if (tid == 0) s_first = 0;
-    float lo[8], hi[8];
+    for (; starts != 0; starts &= starts - 1) {
+        const int64_t t0 = first + __ffs(starts) - 1;
+        const int page = page_of(slot_of(t0));
+        float lo[8], hi[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) lo[e] = INFINITY, hi[e] = -INFINITY;
-    bool first = false;
-    for (int j = g; j < ps; j += RPP) {
-        const int64_t t = t0 + j;
-        if (page_of(t) != page) break;
-        const int row = (int)(a.slots[t] - (int64_t)page * ps);
-        first |= row == 0;
-        const float4* src = reinterpret_cast<const float4*>(a.k + t * a.k_ld + head * D + d);
-        const float4 x = src[0], y = src[1];
-        const float4* vs = reinterpret_cast<const float4*>(a.v + t * a.v_ld + head * D + d);
-        const float4 vx = vs[0], vy = vs[1];
-        const uint4 w = make_uint4(pack16<BF16>(x.x, x.y), pack16<BF16>(x.z, x.w), pack16<BF16>(y.x, y.y),
-                                   pack16<BF16>(y.z, y.w));
-        const uint4 u = make_uint4(pack16<BF16>(vx.x, vx.y), pack16<BF16>(vx.z, vx.w), pack16<BF16>(vy.x, vy.y),
-                                   pack16<BF16>(vy.z, vy.w));
-        uint8_t* kd = static_cast<uint8_t*>(a.kv.k) + page * a.kv.k_page + row * a.kv.k_row + head * a.kv.k_head;
-        uint8_t* vd = static_cast<uint8_t*>(a.kv.v) + page * a.kv.v_page + row * a.kv.v_row + head * a.kv.v_head;
-        *reinterpret_cast<uint4*>(kd + 2 * d) = w;
-        *reinterpret_cast<uint4*>(vd + 2 * d) = u;
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        for (int e = 0; e < 8; ++e) lo[e] = INFINITY, hi[e] = -INFINITY;
+        bool opens = false;  // row 0 of the page is among the rows
+        const float* ks = a.k + head * D + d;
+        const float* vs = a.v + head * D + d;
+        uint8_t* kd = static_cast<uint8_t*>(a.kv.k) + page * a.kv.k_page + head * a.kv.k_head + 2 * d;
+        uint8_t* vd = static_cast<uint8_t*>(a.kv.v) + page * a.kv.v_page + head * a.kv.v_head + 2 * d;
+        for (int j = g; j < ps; j += RPP * kStoreRows) {
+            int row[kStoreRows];  // -1: not of this run
+            float4 x[kStoreRows][2], y[kStoreRows][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = unpack16<BF16>(ws[e]);
-            lo[2 * e] = fminf(lo[2 * e], f.x), hi[2 * e] = fmaxf(hi[2 * e], f.x);
-            lo[2 * e + 1] = fminf(lo[2 * e + 1], f.y), hi[2 * e + 1] = fmaxf(hi[2 * e + 1], f.y);
+            for (int r = 0; r < kStoreRows; ++r) {
+                const int64_t s = j + r * RPP < ps ? slot_of(t0 + j + r * RPP) : -1;
+                row[r] = page_of(s) == page ? (int)(s - (int64_t)page * ps) : -1;
+            }
+#pragma unroll
+            for (int r = 0; r < kStoreRows; ++r)
+                if (row[r] >= 0) {
+                    const int64_t t = t0 + j + r * RPP;
+                    const float4* kp = reinterpret_cast<const float4*>(ks + t * a.k_ld);
+                    const float4* vp = reinterpret_cast<const float4*>(vs + t * a.v_ld);
+                    x[r][0] = __ldcs(kp), x[r][1] = __ldcs(kp + 1), y[r][0] = __ldcs(vp), y[r][1] = __ldcs(vp + 1);
+                }
+#pragma unroll
+            for (int r = 0; r < kStoreRows; ++r) {
+                if (row[r] < 0) continue;
+                opens |= row[r] == 0;
+                const uint4 w = make_uint4(pack16<BF16>(x[r][0].x, x[r][0].y), pack16<BF16>(x[r][0].z, x[r][0].w),
+                                           pack16<BF16>(x[r][1].x, x[r][1].y), pack16<BF16>(x[r][1].z, x[r][1].w));
+                const uint4 u = make_uint4(pack16<BF16>(y[r][0].x, y[r][0].y), pack16<BF16>(y[r][0].z, y[r][0].w),
+                                           pack16<BF16>(y[r][1].x, y[r][1].y), pack16<BF16>(y[r][1].z, y[r][1].w));
+                *reinterpret_cast<uint4*>(kd + row[r] * a.kv.k_row) = w;
+                *reinterpret_cast<uint4*>(vd + row[r] * a.kv.v_row) = u;
+                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = unpack16<BF16>(ws[e]);
+                    lo[2 * e] = fminf(lo[2 * e], f.x), hi[2 * e] = fmaxf(hi[2 * e], f.x);
+                    lo[2 * e + 1] = fminf(lo[2 * e + 1], f.y), hi[2 * e + 1] = fmaxf(hi[2 * e + 1], f.y);
+                }
+            }
+            if (row[kStoreRows - 1] < 0) break;  // the run is consecutive: it ends before this row
         }
-    }
-    if (a.kv.k_lo == nullptr) return;
+        if (a.kv.k_lo == nullptr) continue;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s_lo[g][d + e] = lo[e], s_hi[g][d + e] = hi[e];
-    __syncthreads();
-    if (first) s_first = 1;
-    __syncthreads();
-    for (int c = 2 * tid; c < D; c += 2 * kStoreThreads) {
-        float2 l = make_float2(INFINITY, INFINITY), h = make_float2(-INFINITY, -INFINITY);
-        uint32_t* pl = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.kv.k_lo) +
-                                                   ((int64_t)page * a.kv.n_head_kv + head) * D + c);
-        uint32_t* ph = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.kv.k_hi) +
-                                                   ((int64_t)page * a.kv.n_head_kv + head) * D + c);
-        if (!s_first) l = unpack16<BF16>(*pl), h = unpack16<BF16>(*ph);
-        for (int r = 0; r < RPP; ++r) {
-            l.x = fminf(l.x, s_lo[r][c]), l.y = fminf(l.y, s_lo[r][c + 1]);
-            h.x = fmaxf(h.x, s_hi[r][c]), h.y = fmaxf(h.y, s_hi[r][c + 1]);
+        for (int o = LPR; o < 32; o <<= 1)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                lo[e] = fminf(lo[e], __shfl_xor_sync(0xffffffffu, lo[e], o));
+                hi[e] = fmaxf(hi[e], __shfl_xor_sync(0xffffffffu, hi[e], o));
+            }
+        if (lane < LPR)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s_lo[tid >> 5][d + e] = lo[e], s_hi[tid >> 5][d + e] = hi[e];
+        const bool fresh = __syncthreads_or(opens);
+        for (int c = 2 * tid; c < D; c += 2 * kStoreThreads) {
+            float2 l = make_float2(INFINITY, INFINITY), h = make_float2(-INFINITY, -INFINITY);
+            const int64_t at = ((int64_t)page * a.kv.n_head_kv + head) * D + c;
+            uint32_t* pl = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.kv.k_lo) + at);
+            uint32_t* ph = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.kv.k_hi) + at);
+            if (!fresh) l = unpack16<BF16>(*pl), h = unpack16<BF16>(*ph);
+#pragma unroll
+            for (int r = 0; r < W; ++r) {
+                l.x = fminf(l.x, s_lo[r][c]), l.y = fminf(l.y, s_lo[r][c + 1]);
+                h.x = fmaxf(h.x, s_hi[r][c]), h.y = fmaxf(h.y, s_hi[r][c + 1]);
+            }
+            *pl = pack16<BF16>(l.x, l.y);
+            *ph = pack16<BF16>(h.x, h.y);
         }
-        *pl = pack16<BF16>(l.x, l.y);
-        *ph = pack16<BF16>(h.x, h.y);
+        __syncthreads();  // the next run's rows may replace s_lo, s_hi
     }
 }
 
