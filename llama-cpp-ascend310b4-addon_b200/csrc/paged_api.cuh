@@ -68,10 +68,10 @@ int launch_paged_plan(const PagedPlanArgs& a, cudaStream_t st) {
 
 template <bool BF16>
 int launch_paged_store(const PagedStoreArgs& a, cudaStream_t st) {
-    // about four CTAs' worth of tiles for every place a CTA of this size has on
-    // the GPU: decode steps, whose tokens are runs of their own, get one each,
-    // prompts few that find no run
-    const int64_t want = (a.n_tokens * a.kv.n_head_kv + 4735) / 4736;
+    // two tiles for every place a CTA of this size has on the GPU: decode steps,
+    // whose tokens are runs of their own, get one CTA each, prompts few that
+    // find no run
+    const int64_t want = (a.n_tokens * a.kv.n_head_kv + 2367) / 2368;
     const int tile = (int)std::max<int64_t>(1, std::min<int64_t>(want, std::min(kStoreTile, a.kv.page_size)));
     const dim3 grid((unsigned)((a.n_tokens + tile - 1) / tile), (unsigned)a.kv.n_head_kv);
     switch (a.kv.head_dim) {

@@ -44,6 +44,18 @@ struct PagedSelectArgs {
 
 B200_HD constexpr int paged_units(int blocks) { return (blocks + kPaTok - 1) / kPaTok; }
 
+// Larger of two pairs of 16-bit values; NaN where either is NaN.
+template <bool BF16>
+__device__ __forceinline__ uint32_t max16_nan(uint32_t x, uint32_t y) {
+    if (BF16) {
+        const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&x),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&y));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+    const __half2 r = __hmax2_nan(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 template <int W, int S>
 struct ScoreShared {
     PaRangeShared<W> range;
@@ -205,7 +217,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_score_kernel(PagedS
                     const int r = 8 * (mi >> 1) + ri, c = 2 * kt + (mi & 1);
                     pa_ldsm(b, (half ? lst : hst) + r * RB + ((c ^ ri) << 4));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) top = __vmaxu2(top, b[i] & 0x7fff7fffu);
+                    for (int i = 0; i < 4; ++i) top = max16_nan<BF16>(top, b[i] & 0x7fff7fffu);
                     const uint32_t m0 = half ? ~plus[kt][0] : plus[kt][0], m1 = half ? ~plus[kt][1] : plus[kt][1];
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {

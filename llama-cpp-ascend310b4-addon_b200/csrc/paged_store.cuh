@@ -37,7 +37,7 @@ struct PagedStoreArgs {
 
 constexpr int kStoreThreads = 256;
 constexpr int kStoreTile = 32;  // tokens whose runs one CTA looks for, at most
-constexpr int kStoreRows = 4;   // rows a thread has in flight
+constexpr int kStoreRows = 2;   // rows a thread has in flight
 
 // CTA (tile of `tile` tokens, head): the runs of tokens of one page that begin
 // in its tile, wherever they end.  D / 8 lanes take a row of the head, 16 bytes
@@ -45,7 +45,7 @@ constexpr int kStoreRows = 4;   // rows a thread has in flight
 // row; a page's bounds are theirs alone, so they meet in shared memory once per
 // run, without atomics.  Bound by memory: 12 bytes per element.
 template <bool BF16, int D>
-__global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(PagedStoreArgs a, int tile) {
+__global__ void __launch_bounds__(kStoreThreads, 4) paged_store_kernel(PagedStoreArgs a, int tile) {
     constexpr int LPR = D / 8;                // lanes per row, 8 values each
     constexpr int RPP = kStoreThreads / LPR;  // rows per pass
     constexpr int W = kStoreThreads / 32;
@@ -72,6 +72,14 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(PagedStoreAr
         bool opens = false;  // row 0 of the page is among the rows
         const float* ks = a.k + head * D + d;
         const float* vs = a.v + head * D + d;
+        // the page's bounds so far, on their way while the rows are read
+        static_assert(D <= 2 * kStoreThreads, "a thread keeps two channels");
+        const int64_t bounds_at = (((int64_t)page * a.kv.n_head_kv + head) * D + 2 * tid) / 2;
+        uint32_t* pl = static_cast<uint32_t*>(a.kv.k_lo) + bounds_at;
+        uint32_t* ph = static_cast<uint32_t*>(a.kv.k_hi) + bounds_at;
+        const bool keeps = a.kv.k_lo != nullptr && 2 * tid < D;
+        uint32_t old_lo = 0, old_hi = 0;
+        if (keeps) old_lo = *pl, old_hi = *ph;
         uint8_t* kd = static_cast<uint8_t*>(a.kv.k) + page * a.kv.k_page + head * a.kv.k_head + 2 * d;
         uint8_t* vd = static_cast<uint8_t*>(a.kv.v) + page * a.kv.v_page + head * a.kv.v_head + 2 * d;
         for (int j = g; j < ps; j += RPP * kStoreRows) {
@@ -122,12 +130,10 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(PagedStoreAr
 #pragma unroll
             for (int e = 0; e < 8; ++e) s_lo[tid >> 5][d + e] = lo[e], s_hi[tid >> 5][d + e] = hi[e];
         const bool fresh = __syncthreads_or(opens);
-        for (int c = 2 * tid; c < D; c += 2 * kStoreThreads) {
+        if (keeps) {
+            const int c = 2 * tid;
             float2 l = make_float2(INFINITY, INFINITY), h = make_float2(-INFINITY, -INFINITY);
-            const int64_t at = ((int64_t)page * a.kv.n_head_kv + head) * D + c;
-            uint32_t* pl = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.kv.k_lo) + at);
-            uint32_t* ph = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.kv.k_hi) + at);
-            if (!fresh) l = unpack16<BF16>(*pl), h = unpack16<BF16>(*ph);
+            if (!fresh) l = unpack16<BF16>(old_lo), h = unpack16<BF16>(old_hi);
 #pragma unroll
             for (int r = 0; r < W; ++r) {
                 l.x = fminf(l.x, s_lo[r][c]), l.y = fminf(l.y, s_lo[r][c + 1]);
