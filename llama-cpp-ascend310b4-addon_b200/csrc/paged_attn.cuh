@@ -447,8 +447,8 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                     pa_ldsm_t(b, vst + r * RB + ((c ^ ri) << 4));
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
-                        float d[4] = {};
-                        pa_mma<BF16>(d, wa[0], wa[1], wa[2], wa[3], b[2 * n], b[2 * n + 1]);
+                        float d[4];
+                        pa_mma0<BF16>(d, wa[0], wa[1], wa[2], wa[3], b[2 * n], b[2 * n + 1]);
                         if (BF16) pa_mma<BF16>(d, w3[0], 0u, w3[1], 0u, b[2 * n], b[2 * n + 1]);
                         o[2 * kt + n][0] = fmaf(o[2 * kt + n][0], corr, d[0] + d[2]);
                         o[2 * kt + n][1] = fmaf(o[2 * kt + n][1], corr, d[1] + d[3]);

@@ -44,15 +44,16 @@ struct PagedSelectArgs {
 
 B200_HD constexpr int paged_units(int blocks) { return (blocks + kPaTok - 1) / kPaTok; }
 
-// Larger of two pairs of 16-bit values; NaN where either is NaN.
+// Larger magnitudes of two pairs of 16-bit values; NaN where either is NaN.
 template <bool BF16>
-__device__ __forceinline__ uint32_t max16_nan(uint32_t x, uint32_t y) {
+__device__ __forceinline__ uint32_t max16_abs(uint32_t x, uint32_t y) {
     if (BF16) {
         const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&x),
-                                             *reinterpret_cast<const __nv_bfloat162*>(&y));
+                                             __habs2(*reinterpret_cast<const __nv_bfloat162*>(&y)));
         return *reinterpret_cast<const uint32_t*>(&r);
     }
-    const __half2 r = __hmax2_nan(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+    const __half2 r =
+        __hmax2_nan(*reinterpret_cast<const __half2*>(&x), __habs2(*reinterpret_cast<const __half2*>(&y)));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
@@ -206,28 +207,32 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_score_kernel(PagedS
                     if (BF16) q3[i >> 1][i & 1] = pa_split<BF16>(x, y);
                 }
             }
-            // each instruction from zero, added up outside the tensor core, which
-            // truncates: the bound on the sum is what keeps the undecided few
+            // two k steps at a time from zero, added up outside the tensor core,
+            // which truncates: the bound on the sum is what keeps the undecided few
             float sc[4] = {};
 #pragma unroll
             for (int half = 0; half < 2; ++half) {  // q+ with hi, then q- with lo
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    uint32_t b[4];
-                    const int r = 8 * (mi >> 1) + ri, c = 2 * kt + (mi & 1);
-                    pa_ldsm(b, (half ? lst : hst) + r * RB + ((c ^ ri) << 4));
+                for (int kt = 0; kt < KT; kt += 2) {
+                    float d[2][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) top = max16_nan<BF16>(top, b[i] & 0x7fff7fffu);
-                    const uint32_t m0 = half ? ~plus[kt][0] : plus[kt][0], m1 = half ? ~plus[kt][1] : plus[kt][1];
+                    for (int y = kt; y < kt + 2; ++y) {
+                        uint32_t b[4];
+                        const int r = 8 * (mi >> 1) + ri, c = 2 * y + (mi & 1);
+                        pa_ldsm(b, (half ? lst : hst) + r * RB + ((c ^ ri) << 4));
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        float d[4] = {};
-                        pa_mma<BF16>(d, qf[kt][0] & m0, qf[kt][1] & m0, qf[kt][2] & m1, qf[kt][3] & m1, b[2 * n],
-                                     b[2 * n + 1]);
-                        if (BF16) pa_mma<BF16>(d, q3[kt][0] & m0, 0u, q3[kt][1] & m1, 0u, b[2 * n], b[2 * n + 1]);
-                        sc[2 * n] += d[0] + d[2];
-                        sc[2 * n + 1] += d[1] + d[3];
+                        for (int i = 0; i < 4; ++i) top = max16_abs<BF16>(top, b[i]);
+                        const uint32_t m0 = half ? ~plus[y][0] : plus[y][0], m1 = half ? ~plus[y][1] : plus[y][1];
+                        const uint32_t a0 = qf[y][0] & m0, a1 = qf[y][1] & m0, a2 = qf[y][2] & m1, a3 = qf[y][3] & m1;
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            if (y == kt) pa_mma0<BF16>(d[n], a0, a1, a2, a3, b[2 * n], b[2 * n + 1]);
+                            else pa_mma<BF16>(d[n], a0, a1, a2, a3, b[2 * n], b[2 * n + 1]);
+                            if (BF16) pa_mma<BF16>(d[n], q3[y][0] & m0, 0u, q3[y][1] & m1, 0u, b[2 * n], b[2 * n + 1]);
+                        }
                     }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[i] += d[i >> 1][i & 1] + d[i >> 1][2 + (i & 1)];
                 }
             }
 #pragma unroll
@@ -399,12 +404,12 @@ __global__ void __launch_bounds__(kTopkThreads) paged_topk_kernel(PagedSelectArg
     __syncthreads();
     // eps, with q' = q 2^-ex, whose largest entry is in [1, 2), M = max |bound| and
     // S = M max_j sum |q'_jd|: the parts of q' leave out at most 2^-23 of each
-    // entry, in all D 2^-23 M; an instruction (bf16: two) truncates 16 products
-    // (33 terms) below 2^-24 of the largest, in all 33 2^-24 S; adding its high
-    // and low halves and the D / 8 instructions rounds D / 8 + 1 times by 2^-24 S
-    // at most.  1e-30 covers what underflows.
+    // entry, in all D 2^-23 M; a chain of two instructions (bf16: four) truncates
+    // its 33 (67) terms below 2^-24 of the largest, in all 67 2^-24 S; adding high
+    // and low halves and the D / 16 chains rounds D / 16 + 1 times by 2^-24 S at
+    // most.  1e-30 covers what underflows.
     const float biggest = BF16 ? __uint_as_float(s_top << 16) : h2f((uint16_t)s_top);
-    const float eps = biggest * (D * 0x1p-23f + group.y * (36 + D / 8) * 0x1p-24f) * 1.01f + 1e-30f;
+    const float eps = biggest * (D * 0x1p-23f + group.y * (70 + D / 16) * 0x1p-24f) * 1.01f + 1e-30f;
     const bool sure = eps < 1e30f;  // not: bounds or queries that are not finite, nothing is decided by the scores
     float tau = 0.f;
     if (sure) {
