@@ -230,6 +230,9 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
 
         // ---- producer: this lane looks after token lane & 15 of a unit ----
         const int q16 = kPaTok / ps, r16 = kPaTok % ps;
+        const bool aligned = ps % kPaTok == 0;  // a unit lies in one page
+        const uint32_t lc = lane % LPR, lr = lane / LPR;  // this lane's 16 bytes of a row, its row of a copy
+        const long long lane_k = lr * a.kv.k_row + 16 * lc, lane_v = lr * a.kv.v_row + 16 * lc;
         int bi = 0, row = 0, w0 = 0;     // its block (list entry) and row; first entry of the page window
         int p0 = -1, p1 = -1, b0 = -1, b1 = -1;  // pages and blocks of entries w0 + lane, w0 + 32 + lane
         bool fresh = true;
@@ -279,41 +282,52 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                     bi += q16;
                     row += r16;
                     if (row >= ps) row -= ps, ++bi;
-                    if (__shfl_sync(0xffffffffu, bi, 0) >= w0 + 32) {
+                    if ((aligned ? bi : __shfl_sync(0xffffffffu, bi, 0)) >= w0 + 32) {
                         w0 += 32;
                         p0 = p1, b0 = b1;
                         window(w0 + lane, true);
                     }
                 }
-                const int x = bi - w0;  // 0 .. 47
-                const int pa = __shfl_sync(0xffffffffu, p0, x & 31), pb = __shfl_sync(0xffffffffu, p1, x & 31);
-                const int page = x < 32 ? pa : pb;
-                int blk = bi;
-                if (a.sel != nullptr) {
-                    const int ba = __shfl_sync(0xffffffffu, b0, x & 31), bb = __shfl_sync(0xffffffffu, b1, x & 31);
-                    blk = x < 32 ? ba : bb;
+                const int x = bi - w0;  // 0 .. 31, 46 where a unit spans pages
+                int page = __shfl_sync(0xffffffffu, p0, x & 31), blk = bi;
+                if (a.sel != nullptr) blk = __shfl_sync(0xffffffffu, b0, x & 31);
+                if (!aligned) {
+                    const int pb = __shfl_sync(0xffffffffu, p1, x & 31);
+                    const int bb = __shfl_sync(0xffffffffu, b1, x & 31);
+                    if (x >= 32) page = pb, blk = a.sel != nullptr ? bb : bi;
                 }
                 const bool ok = page >= 0 && row < in.len - blk * ps;
                 const unsigned valid = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-                const long long ko = ok ? page * a.kv.k_page + row * a.kv.k_row + in.head * a.kv.k_head : 0;
-                const long long vo = ok ? page * a.kv.v_page + row * a.kv.v_row + in.head * a.kv.v_head : 0;
                 if (lane == 0) sh.valid[warp][stage] = valid;
                 if (a.mask != nullptr) {
                     mask_pending = ok ? h2f(a.mask[in.s * a.mask_stride + (int64_t)blk * ps + row]) : -INFINITY;
                     mask_stage = stage;
                     valid_pending = valid;
                 }
-                const uint32_t kst = ring + stage * (2 * TILE), c = lane % LPR;
-                const uint8_t* kp = static_cast<const uint8_t*>(a.kv.k) + 16 * c;
-                const uint8_t* vp = static_cast<const uint8_t*>(a.kv.v) + 16 * c;
+                const uint32_t kst = ring + stage * (2 * TILE) + lr * RB;
+                const uint8_t *kb = static_cast<const uint8_t*>(a.kv.k), *vb = static_cast<const uint8_t*>(a.kv.v);
+                if (aligned && valid == 0xffffu) {  // 16 rows of one page: a base and steps
+                    const int row0 = row - (lane & 15);
+                    kb += page * a.kv.k_page + row0 * a.kv.k_row + in.head * a.kv.k_head + lane_k;
+                    vb += page * a.kv.v_page + row0 * a.kv.v_row + in.head * a.kv.v_head + lane_v;
 #pragma unroll
-                for (int i = 0; i < kPaTok / RPI; ++i) {
-                    const int r = i * RPI + lane / LPR;
-                    const long long kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
-                    const uint32_t d = kst + r * RB + ((c ^ (r & 7)) << 4);
-                    const bool on = (valid >> r) & 1;
-                    pa_cp16(d, kp + kr, on);
-                    pa_cp16(d + TILE, vp + vr, on);
+                    for (int i = 0; i < kPaTok / RPI; ++i) {
+                        const uint32_t d = kst + i * RPI * RB + ((lc ^ ((i * RPI + lr) & 7)) << 4);
+                        pa_cp16(d, kb + i * RPI * a.kv.k_row);
+                        pa_cp16(d + TILE, vb + i * RPI * a.kv.v_row);
+                    }
+                } else {  // row by row from the lane that looks after it; zeros for those that do not exist
+                    const long long ko = ok ? page * a.kv.k_page + row * a.kv.k_row + in.head * a.kv.k_head : 0;
+                    const long long vo = ok ? page * a.kv.v_page + row * a.kv.v_row + in.head * a.kv.v_head : 0;
+#pragma unroll
+                    for (int i = 0; i < kPaTok / RPI; ++i) {
+                        const int r = i * RPI + lr;
+                        const long long kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+                        const uint32_t d = kst + i * RPI * RB + ((lc ^ (r & 7)) << 4);
+                        const bool on = (valid >> r) & 1;
+                        pa_cp16(d, kb + kr + 16 * lc, on);
+                        pa_cp16(d + TILE, vb + vr + 16 * lc, on);
+                    }
                 }
                 --to_issue;
                 if (to_issue > 0 && !pa_advance(a, in)) to_issue = 0;
@@ -323,7 +337,25 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
         };
         // ---- consumer: this thread holds head g, positions 2 t4, 2 t4 + 1 (+ 8) ----
         uint32_t qf[KT][4], q3[BF16 ? KT : 1][2];
-        float o[2 * KT][2], m = -INFINITY, l = 0.f, mk = -INFINITY, f = 0.f;
+        // Outputs: acc is what the tensor core adds up itself (high and low parts of
+        // w apart), emptied into o every FLUSH units: it truncates, and 4 of its
+        // additions stay below the rounding of one f32.  m is the weights'
+        // reference: it follows the running maximum only when that has grown by
+        // 2^3, which w has room for (w <= 2^15 in f16), so o is rarely rescaled.
+        constexpr int FLUSH = D <= 128 ? 4 : 1;  // (D = 256 lacks the registers)
+        float o[2 * KT][2], acc[D <= 128 ? 2 * KT : 1][4];
+        float m = -INFINITY, l = 0.f, mk = -INFINITY, f = 0.f;
+        int pending = 0;  // units in acc
+        auto flush = [&]() {
+            if (FLUSH == 1) return;
+#pragma unroll
+            for (int i = 0; i < (FLUSH > 1 ? 2 * KT : 0); ++i) {
+                o[i][0] += acc[i][0] + acc[i][2];
+                o[i][1] += acc[i][1] + acc[i][3];
+                acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+            }
+            pending = 0;
+        };
         auto take_q = [&]() {
             const bool mine_q = cur.chunk * kPaHeads + g < G;
             float amax = 0.f;
@@ -347,6 +379,9 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
             }
 #pragma unroll
             for (int i = 0; i < 2 * KT; ++i) o[i][0] = o[i][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < (FLUSH > 1 ? 2 * KT : 0); ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+            pending = 0;
             m = -INFINITY, l = 0.f, mk = a.mask != nullptr ? -INFINITY : 0.f;
         };
         // The loop runs S - 1 units ahead with the copies: its first S - 1 turns
@@ -383,7 +418,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                     __syncwarp();
                 }
                 // S = q K^T: 8 heads (high parts, low parts) x 16 positions
-                float sc[2][4] = {};
+                float sc[2][4];
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
                     uint32_t b[4];  // positions 0-7: dims 0-7, 8-15; positions 8-15: the same
@@ -391,7 +426,8 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                     pa_ldsm(b, kst + r * RB + ((c ^ ri) << 4));
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
-                        pa_mma<BF16>(sc[n], qf[kt][0], qf[kt][1], qf[kt][2], qf[kt][3], b[2 * n], b[2 * n + 1]);
+                        if (kt == 0) pa_mma0<BF16>(sc[n], qf[kt][0], qf[kt][1], qf[kt][2], qf[kt][3], b[2 * n], b[2 * n + 1]);
+                        else pa_mma<BF16>(sc[n], qf[kt][0], qf[kt][1], qf[kt][2], qf[kt][3], b[2 * n], b[2 * n + 1]);
                         if (BF16) pa_mma<BF16>(sc[n], q3[kt][0], 0u, q3[kt][1], 0u, b[2 * n], b[2 * n + 1]);
                     }
                 }
@@ -415,24 +451,31 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                     for (int i = 0; i < 4; ++i) bias[i] = (bias[i] - mk) * 1.44269504f;
                 }
                 float top = -INFINITY;
-                bool on[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    on[i] = (live >> (8 * (i >> 1) + 2 * t4 + (i & 1))) & 1;
-                    if (on[i]) top = fmaxf(top, fmaf(x[i], f, bias[i]));
-                }
+                for (int i = 0; i < 4; ++i)
+                    if (live == 0xffffu || (live >> (8 * (i >> 1) + 2 * t4 + (i & 1))) & 1)
+                        top = fmaxf(top, fmaf(x[i], f, bias[i]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float mn = fmaxf(m, top);
-                const float corr = pa_exp2(m - mn);  // 0 at the first unit: m is -inf, mn is not
-                m = mn;
-                float w[4], sum = 0.f;
+                const bool grown = top > m + 3.f;  // (at the first unit m is -inf)
+                if (__any_sync(0xffffffffu, grown)) {
+                    flush();
+                    const float mn = grown ? top : m;
+                    const float corr = m == -INFINITY ? 0.f : pa_exp2(m - mn);
+                    l *= corr;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    w[i] = on[i] ? pa_exp2(fmaf(x[i], f, bias[i] - mn)) * 4096.f : 0.f;
-                    sum += w[i];
+                    for (int i = 0; i < 2 * KT; ++i) o[i][0] *= corr, o[i][1] *= corr;
+                    m = mn;
                 }
-                l = l * corr + sum;
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = pa_exp2(fmaf(x[i], f, bias[i] - m)) * 4096.f;
+                if (live != 0xffffu) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!((live >> (8 * (i >> 1) + 2 * t4 + (i & 1))) & 1)) w[i] = 0.f;
+                }
+                l += (w[0] + w[1]) + (w[2] + w[3]);
                 // O += w V: the pieces of w as they stand are the A operand
                 uint32_t wa[4], w3[2];
                 wa[0] = pa_split<BF16>(w[0], w[1]);
@@ -447,18 +490,26 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                     pa_ldsm_t(b, vst + r * RB + ((c ^ ri) << 4));
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
-                        float d[4];
-                        pa_mma0<BF16>(d, wa[0], wa[1], wa[2], wa[3], b[2 * n], b[2 * n + 1]);
-                        if (BF16) pa_mma<BF16>(d, w3[0], 0u, w3[1], 0u, b[2 * n], b[2 * n + 1]);
-                        o[2 * kt + n][0] = fmaf(o[2 * kt + n][0], corr, d[0] + d[2]);
-                        o[2 * kt + n][1] = fmaf(o[2 * kt + n][1], corr, d[1] + d[3]);
+                        if (FLUSH > 1) {
+                            float(&d)[4] = acc[(2 * kt + n) % (sizeof(acc) / sizeof(acc[0]))];
+                            pa_mma<BF16>(d, wa[0], wa[1], wa[2], wa[3], b[2 * n], b[2 * n + 1]);
+                            if (BF16) pa_mma<BF16>(d, w3[0], 0u, w3[1], 0u, b[2 * n], b[2 * n + 1]);
+                        } else {
+                            float d[4];
+                            pa_mma0<BF16>(d, wa[0], wa[1], wa[2], wa[3], b[2 * n], b[2 * n + 1]);
+                            if (BF16) pa_mma<BF16>(d, w3[0], 0u, w3[1], 0u, b[2 * n], b[2 * n + 1]);
+                            o[2 * kt + n][0] += d[0] + d[2];
+                            o[2 * kt + n][1] += d[1] + d[3];
+                        }
                     }
                 }
+                if (FLUSH > 1 && ++pending == FLUSH) flush();
             }
             stage = stage + 1 == S ? 0 : stage + 1;
 
             const bool seg_end = cur.u + 1 == cur.nu;
             if (seg_end || to_do == 1) {
+                if (pending) flush();
                 l += __shfl_xor_sync(0xffffffffu, l, 1);
                 l += __shfl_xor_sync(0xffffffffu, l, 2);
                 if (seg_end && seg_from >= fb) {  // the whole segment
