@@ -120,31 +120,32 @@ int launch_paged_select(const PagedSelectArgs& a, int head_dim, cudaStream_t st)
     }
 }
 
-bool g_paged_attn_attr[kMaxDevices][2][3];
+bool g_paged_attn_attr[kMaxDevices][2][3][2];
 
-// Opts an instantiation into its shared memory, once per device.
-template <bool BF16, int D>
-int set_paged_attn_attr() {
+template <bool BF16, int D, bool MASK>
+int launch_paged_attn_dm(const PagedAttnArgs& a, cudaStream_t st) {
     const int dev = current_device();
     if (dev < 0 || dev >= kMaxDevices) return B200_EINVAL;
-    bool& done = g_paged_attn_attr[dev][BF16][D == 64 ? 0 : D == 128 ? 1 : 2];
-    std::lock_guard<std::mutex> lk(g_attr_mu);
-    if (done) return B200_OK;
-    CR_(cuda_status(cudaFuncSetAttribute(paged_attn_kernel<BF16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         pa_smem<D>())));
-    done = true;
-    return B200_OK;
-}
-
-template <bool BF16, int D>
-int launch_paged_attn_d(const PagedAttnArgs& a, cudaStream_t st) {
-    CR_((set_paged_attn_attr<BF16, D>()));
+    {
+        bool& done = g_paged_attn_attr[dev][BF16][D == 64 ? 0 : D == 128 ? 1 : 2][MASK];
+        std::lock_guard<std::mutex> lk(g_attr_mu);
+        if (!done) {
+            CR_(cuda_status(cudaFuncSetAttribute(paged_attn_kernel<BF16, D, MASK>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, pa_smem<D>())));
+            done = true;
+        }
+    }
     // the lengths are on the device: at most this many units
     const int64_t width = (int64_t)(a.sel ? a.n_sel : a.max_blocks) * a.kv.page_size;
     const int64_t units = (int64_t)a.n_seq * a.kv.n_head_kv * a.chunks * ((width + kPaTok - 1) / kPaTok);
     const int64_t grid = std::min<int64_t>(kPaCtas, (units + pa_warps(D) - 1) / pa_warps(D));
-    paged_attn_kernel<BF16, D><<<(unsigned)grid, 32 * pa_warps(D), pa_smem<D>(), st>>>(a);
+    paged_attn_kernel<BF16, D, MASK><<<(unsigned)grid, 32 * pa_warps(D), pa_smem<D>(), st>>>(a);
     return cuda_status(cudaGetLastError());
+}
+
+template <bool BF16, int D>
+int launch_paged_attn_d(const PagedAttnArgs& a, cudaStream_t st) {
+    return a.mask ? launch_paged_attn_dm<BF16, D, true>(a, st) : launch_paged_attn_dm<BF16, D, false>(a, st);
 }
 
 template <bool BF16>
@@ -306,6 +307,7 @@ int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, i
     a.n_head = n_head;
     a.n_sel = n_sel;
     a.max_blocks = max_blocks;
+    a.near_rows = std::max(kv->k_row, kv->v_row) < ((int64_t)1 << 31) / kPaTok;
     return kv->type == B200_TYPE_BF16 ? launch_paged_attn<true>(a, (cudaStream_t)stream)
                                       : launch_paged_attn<false>(a, (cudaStream_t)stream);
 }

@@ -32,6 +32,8 @@
 // outside the tensor core, which truncates its own.
 #pragma once
 
+#include <utility>
+
 #include "../../include/b200_paged.h"
 #include "args.h"
 #include "common.cuh"
@@ -80,7 +82,14 @@ struct PagedAttnArgs {
     unsigned int* tickets;  // [n_seq * n_head_kv * chunks][8], zero between calls
     float scale;
     int n_seq, n_head, n_sel, max_blocks, chunks;
+    int near_rows;          // 16 rows of a page span less than 2^31 bytes
 };
+
+// f(integral_constant<I>) for I of the sequence.
+template <size_t... I, class F>
+__device__ __forceinline__ void copy_rows(std::index_sequence<I...>, F f) {
+    (f(std::integral_constant<int, (int)I>{}), ...);
+}
 
 // Where a warp is in its range: unit u of nu of the segment (s, head, chunk).
 struct PaCursor {
@@ -170,7 +179,7 @@ struct PaJoint {
     }
 };
 
-template <bool BF16, int D>
+template <bool BF16, int D, bool MASK>
 __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAttnArgs a) {
     constexpr int W = pa_warps(D), S = pa_stages(D), T = 32 * W;
     constexpr int KT = D / 16;             // k steps of q . k, pairs of output tiles
@@ -232,7 +241,14 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
         const int q16 = kPaTok / ps, r16 = kPaTok % ps;
         const bool aligned = ps % kPaTok == 0;  // a unit lies in one page
         const uint32_t lc = lane % LPR, lr = lane / LPR;  // this lane's 16 bytes of a row, its row of a copy
-        const long long lane_k = lr * a.kv.k_row + 16 * lc, lane_v = lr * a.kv.v_row + 16 * lc;
+        // (a unit of one page: 16 rows at 32-bit steps from its first)
+        const bool near_rows = aligned && a.near_rows;
+        constexpr int SW = 8 / RPI;  // the swizzle repeats after 8 rows
+        uint32_t dst_of[SW];
+#pragma unroll
+        for (int i = 0; i < SW; ++i) dst_of[i] = ring + lr * RB + ((lc ^ ((i * RPI + lr) & 7)) << 4);
+        const uint32_t k_step = (uint32_t)(RPI * a.kv.k_row), v_step = (uint32_t)(RPI * a.kv.v_row);
+        const uint32_t k_lane = (uint32_t)(lr * a.kv.k_row) + 16 * lc, v_lane = (uint32_t)(lr * a.kv.v_row) + 16 * lc;
         int bi = 0, row = 0, w0 = 0;     // its block (list entry) and row; first entry of the page window
         int p0 = -1, p1 = -1, b0 = -1, b1 = -1;  // pages and blocks of entries w0 + lane, w0 + 32 + lane
         bool fresh = true;
@@ -269,7 +285,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
             }
         };
         auto issue = [&](int stage) {
-            if (a.mask != nullptr) flush_mask();
+            if (MASK) flush_mask();
             if (to_issue > 0) {
                 if (fresh) {
                     const unsigned vt = (unsigned)in.u * kPaTok + (lane & 15);
@@ -299,31 +315,30 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                 const bool ok = page >= 0 && row < in.len - blk * ps;
                 const unsigned valid = __ballot_sync(0xffffffffu, ok) & 0xffffu;
                 if (lane == 0) sh.valid[warp][stage] = valid;
-                if (a.mask != nullptr) {
+                if (MASK) {
                     mask_pending = ok ? h2f(a.mask[in.s * a.mask_stride + (int64_t)blk * ps + row]) : -INFINITY;
                     mask_stage = stage;
                     valid_pending = valid;
                 }
-                const uint32_t kst = ring + stage * (2 * TILE) + lr * RB;
                 const uint8_t *kb = static_cast<const uint8_t*>(a.kv.k), *vb = static_cast<const uint8_t*>(a.kv.v);
-                if (aligned && valid == 0xffffu) {  // 16 rows of one page: a base and steps
+                const uint32_t at = stage * (2 * TILE);
+                if (near_rows && valid == 0xffffu) {  // 16 rows of one page: a base and steps
                     const int row0 = row - (lane & 15);
-                    kb += page * a.kv.k_page + row0 * a.kv.k_row + in.head * a.kv.k_head + lane_k;
-                    vb += page * a.kv.v_page + row0 * a.kv.v_row + in.head * a.kv.v_head + lane_v;
-#pragma unroll
-                    for (int i = 0; i < kPaTok / RPI; ++i) {
-                        const uint32_t d = kst + i * RPI * RB + ((lc ^ ((i * RPI + lr) & 7)) << 4);
-                        pa_cp16(d, kb + i * RPI * a.kv.k_row);
-                        pa_cp16(d + TILE, vb + i * RPI * a.kv.v_row);
-                    }
+                    kb += page * a.kv.k_page + row0 * a.kv.k_row + in.head * a.kv.k_head;
+                    vb += page * a.kv.v_page + row0 * a.kv.v_row + in.head * a.kv.v_head;
+                    copy_rows(std::make_index_sequence<kPaTok / RPI>{}, [&](auto ic) {
+                        constexpr int I = decltype(ic)::value, OFF = I / SW * (SW * RPI * RB) + I % SW * (RPI * RB);
+                        pa_cp16_at<OFF>(dst_of[I % SW] + at, kb + (k_lane + I * k_step));
+                        pa_cp16_at<OFF + TILE>(dst_of[I % SW] + at, vb + (v_lane + I * v_step));
+                    });
                 } else {  // row by row from the lane that looks after it; zeros for those that do not exist
                     const long long ko = ok ? page * a.kv.k_page + row * a.kv.k_row + in.head * a.kv.k_head : 0;
                     const long long vo = ok ? page * a.kv.v_page + row * a.kv.v_row + in.head * a.kv.v_head : 0;
 #pragma unroll
                     for (int i = 0; i < kPaTok / RPI; ++i) {
                         const int r = i * RPI + lr;
+                        const uint32_t d = dst_of[i % SW] + at + i * RPI * RB;
                         const long long kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
-                        const uint32_t d = kst + i * RPI * RB + ((lc ^ (r & 7)) << 4);
                         const bool on = (valid >> r) & 1;
                         pa_cp16(d, kb + kr + 16 * lc, on);
                         pa_cp16(d + TILE, vb + vr + 16 * lc, on);
@@ -382,7 +397,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
 #pragma unroll
             for (int i = 0; i < (FLUSH > 1 ? 2 * KT : 0); ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
             pending = 0;
-            m = -INFINITY, l = 0.f, mk = a.mask != nullptr ? -INFINITY : 0.f;
+            m = -INFINITY, l = 0.f, mk = MASK ? -INFINITY : 0.f;
         };
         // The loop runs S - 1 units ahead with the copies: its first S - 1 turns
         // only issue.
@@ -405,7 +420,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                 new_q = false;
             }
             const unsigned valid = sh.valid[warp][stage];
-            const unsigned live = a.mask != nullptr ? sh.live[warp][stage] : valid;
+            const unsigned live = MASK ? sh.live[warp][stage] : valid;
             const uint32_t kst = ring + stage * (2 * TILE), vst = kst + TILE;
             if (live) {
                 if (live != valid) {  // masked positions: their values may be anything
@@ -434,7 +449,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                 float x[4], bias[4] = {};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[i] = sc[i >> 1][i & 1] + sc[i >> 1][2 + (i & 1)];
-                if (a.mask != nullptr) {
+                if (MASK) {
                     float top = -INFINITY;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -563,7 +578,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
     const unsigned ends = __ballot_sync(0xffffffffu, hd >= 0 && hd == prev);     // head of the tail before
     const unsigned alone = __ballot_sync(0xffffffffu, hd >= 0 && hd != prev);
     constexpr int AT_M = kPaHeads * D, AT_L = AT_M + kPaHeads, AT_MK = AT_L + kPaHeads, NV = PaJoint<D>::NV;
-    const bool masked = a.mask != nullptr, has_col = 4 * lane < D;
+    const bool masked = MASK, has_col = 4 * lane < D;
     auto put_out = [&](int row, const PaJoint<D>& t) {
         const float inv = t.l > 0.f ? 1.f / t.l : 0.f;
         float4* out = reinterpret_cast<float4*>(a.out + (int64_t)row * D) + lane;

@@ -20,8 +20,10 @@ __device__ __forceinline__ int paged_blocks(int len, int max_blocks, int page_si
 __device__ __forceinline__ void pa_cp16(uint32_t dst, const void* src, bool on) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void pa_cp16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// 16 bytes to dst + OFF.
+template <int OFF>
+__device__ __forceinline__ void pa_cp16_at(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0 + %2], [%1], 16;" ::"r"(dst), "l"(src), "n"(OFF) : "memory");
 }
 __device__ __forceinline__ void pa_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
