@@ -87,7 +87,7 @@ struct PagedAttnArgs {
 
 // f(integral_constant<I>) for I of the sequence.
 template <size_t... I, class F>
-__device__ __forceinline__ void copy_rows(std::index_sequence<I...>, F f) {
+__device__ __forceinline__ void unrolled(std::index_sequence<I...>, F f) {
     (f(std::integral_constant<int, (int)I>{}), ...);
 }
 
@@ -324,12 +324,14 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                 const uint32_t at = stage * (2 * TILE);
                 if (near_rows && valid == 0xffffu) {  // 16 rows of one page: a base and steps
                     const int row0 = row - (lane & 15);
-                    kb += page * a.kv.k_page + row0 * a.kv.k_row + in.head * a.kv.k_head;
-                    vb += page * a.kv.v_page + row0 * a.kv.v_row + in.head * a.kv.v_head;
-                    copy_rows(std::make_index_sequence<kPaTok / RPI>{}, [&](auto ic) {
+                    kb += page * a.kv.k_page + row0 * a.kv.k_row + in.head * a.kv.k_head + k_lane;
+                    vb += page * a.kv.v_page + row0 * a.kv.v_row + in.head * a.kv.v_head + v_lane;
+                    unrolled(std::make_index_sequence<kPaTok / RPI>{}, [&](auto ic) {
                         constexpr int I = decltype(ic)::value, OFF = I / SW * (SW * RPI * RB) + I % SW * (RPI * RB);
-                        pa_cp16_at<OFF>(dst_of[I % SW] + at, kb + (k_lane + I * k_step));
-                        pa_cp16_at<OFF + TILE>(dst_of[I % SW] + at, vb + (v_lane + I * v_step));
+                        pa_cp16_at<OFF>(dst_of[I % SW] + at, kb);
+                        pa_cp16_at<OFF + TILE>(dst_of[I % SW] + at, vb);
+                        kb += k_step;
+                        vb += v_step;
                     });
                 } else {  // row by row from the lane that looks after it; zeros for those that do not exist
                     const long long ko = ok ? page * a.kv.k_page + row * a.kv.k_row + in.head * a.kv.k_head : 0;
@@ -403,7 +405,16 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
         // only issue.
         bool new_q = true;
         int stage = 0, ahead = 0;
+        // this lane's ldmatrix rows: 16 dims of a k step are 32 bytes, which the
+        // swizzle moves within 128; K: positions 0-7 dims 0-7, 8-15, positions
+        // 8-15 the same; V: dims 0-7 positions 0-7, 8-15, the next 8 dims the same
         const int mi = lane >> 3, ri = lane & 7;
+        uint32_t k_at[4], v_at[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            k_at[i] = ring + (8 * (mi >> 1) + ri) * RB + (((2 * i + (mi & 1)) ^ ri) << 4);
+            v_at[i] = ring + TILE + (8 * (mi & 1) + ri) * RB + (((2 * i + (mi >> 1)) ^ ri) << 4);
+        }
 #pragma unroll 1
         for (int turn = 1 - S; to_do > 0; ++turn) {
             if (EARLY_Q && new_q && (turn == 1 - S || turn > 0)) fetch_q();
@@ -421,31 +432,30 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
             }
             const unsigned valid = sh.valid[warp][stage];
             const unsigned live = MASK ? sh.live[warp][stage] : valid;
-            const uint32_t kst = ring + stage * (2 * TILE), vst = kst + TILE;
+            const uint32_t st = stage * (2 * TILE);
             if (live) {
                 if (live != valid) {  // masked positions: their values may be anything
                     for (int r = 0; r < kPaTok; ++r)
                         if (((valid & ~live) >> r) & 1)
                             for (int c = lane; c < RB / 16; c += 32)
-                                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vst + r * RB + 16 * c),
+                                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + st + TILE + r * RB + 16 * c),
                                              "r"(0u)
                                              : "memory");
                     __syncwarp();
                 }
                 // S = q K^T: 8 heads (high parts, low parts) x 16 positions
                 float sc[2][4];
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    uint32_t b[4];  // positions 0-7: dims 0-7, 8-15; positions 8-15: the same
-                    const int r = 8 * (mi >> 1) + ri, c = 2 * kt + (mi & 1);
-                    pa_ldsm(b, kst + r * RB + ((c ^ ri) << 4));
+                unrolled(std::make_index_sequence<KT>{}, [&](auto ic) {
+                    constexpr int kt = decltype(ic)::value;
+                    uint32_t b[4];
+                    pa_ldsm_at<kt / 4 * 128>(b, k_at[kt % 4] + st);
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
                         if (kt == 0) pa_mma0<BF16>(sc[n], qf[kt][0], qf[kt][1], qf[kt][2], qf[kt][3], b[2 * n], b[2 * n + 1]);
                         else pa_mma<BF16>(sc[n], qf[kt][0], qf[kt][1], qf[kt][2], qf[kt][3], b[2 * n], b[2 * n + 1]);
-                        if (BF16) pa_mma<BF16>(sc[n], q3[kt][0], 0u, q3[kt][1], 0u, b[2 * n], b[2 * n + 1]);
+                        if (BF16) pa_mma<BF16>(sc[n], q3[BF16 ? kt : 0][0], 0u, q3[BF16 ? kt : 0][1], 0u, b[2 * n], b[2 * n + 1]);
                     }
-                }
+                });
                 float x[4], bias[4] = {};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[i] = sc[i >> 1][i & 1] + sc[i >> 1][2 + (i & 1)];
@@ -465,11 +475,16 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
 #pragma unroll
                     for (int i = 0; i < 4; ++i) bias[i] = (bias[i] - mk) * 1.44269504f;
                 }
-                float top = -INFINITY;
+                float top;
+                if (live == 0xffffu) {
+                    top = fmaxf(fmaxf(fmaf(x[0], f, bias[0]), fmaf(x[1], f, bias[1])),
+                                fmaxf(fmaf(x[2], f, bias[2]), fmaf(x[3], f, bias[3])));
+                } else {
+                    top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (live == 0xffffu || (live >> (8 * (i >> 1) + 2 * t4 + (i & 1))) & 1)
-                        top = fmaxf(top, fmaf(x[i], f, bias[i]));
+                    for (int i = 0; i < 4; ++i)
+                        if ((live >> (8 * (i >> 1) + 2 * t4 + (i & 1))) & 1) top = fmaxf(top, fmaf(x[i], f, bias[i]));
+                }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const bool grown = top > m + 3.f;  // (at the first unit m is -inf)
@@ -498,11 +513,10 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                 wa[2] = pa_split<BF16>(w[2], w[3]);
                 wa[3] = pa_split<BF16>(w[2], w[3]);
                 if (BF16) w3[0] = pa_split<BF16>(w[0], w[1]), w3[1] = pa_split<BF16>(w[2], w[3]);
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    uint32_t b[4];  // dims 16 kt .. + 7: positions 0-7, 8-15; the next 8 dims
-                    const int r = 8 * (mi & 1) + ri, c = 2 * kt + (mi >> 1);
-                    pa_ldsm_t(b, vst + r * RB + ((c ^ ri) << 4));
+                unrolled(std::make_index_sequence<KT>{}, [&](auto ic) {
+                    constexpr int kt = decltype(ic)::value;
+                    uint32_t b[4];
+                    pa_ldsm_t_at<kt / 4 * 128>(b, v_at[kt % 4] + st);
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
                         if (FLUSH > 1) {
@@ -517,7 +531,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                             o[2 * kt + n][1] += d[1] + d[3];
                         }
                     }
-                }
+                });
                 if (FLUSH > 1 && ++pending == FLUSH) flush();
             }
             stage = stage + 1 == S ? 0 : stage + 1;

@@ -36,10 +36,19 @@ __device__ __forceinline__ void pa_ldsm(uint32_t (&r)[4], uint32_t addr) {
                  : "r"(addr)
                  : "memory");
 }
-__device__ __forceinline__ void pa_ldsm_t(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+// The same at addr + OFF, and transposed.
+template <int OFF>
+__device__ __forceinline__ void pa_ldsm_at(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4 + %5];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
+                 : "r"(addr), "n"(OFF)
+                 : "memory");
+}
+template <int OFF>
+__device__ __forceinline__ void pa_ldsm_t_at(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4 + %5];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr), "n"(OFF)
                  : "memory");
 }
 template <bool BF16>
