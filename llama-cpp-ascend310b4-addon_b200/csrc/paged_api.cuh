@@ -17,7 +17,7 @@ int check_paged_kv(const b200_paged_kv* kv) {
     if (kv->type != B200_TYPE_F16 && kv->type != B200_TYPE_BF16) return B200_EUNSUPPORTED;
     if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256) return B200_EUNSUPPORTED;
     const int64_t strides = kv->k_page | kv->k_row | kv->k_head | kv->v_page | kv->v_row | kv->v_head;
-    if (!aligned16(kv->k) || !aligned16(kv->v) || (strides & 15) || strides < 0) return B200_EINVAL;
+    if (!aligned16(kv->k) || !aligned16(kv->v) || (strides & 15) || strides < 0 || strides >> 36) return B200_EINVAL;
     if ((kv->k_lo == nullptr) != (kv->k_hi == nullptr) || !aligned16(kv->k_lo) || !aligned16(kv->k_hi))
         return B200_EINVAL;
     return B200_OK;

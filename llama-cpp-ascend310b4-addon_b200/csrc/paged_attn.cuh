@@ -105,9 +105,8 @@ __device__ __forceinline__ int pa_units(const PagedAttnArgs& a, int len) {
     if (a.sel != nullptr && len > 0) len = a.n_sel * a.kv.page_size;
     return (int)(((unsigned)len + kPaTok - 1) / kPaTok);
 }
-// To the next unit; false past the last sequence.
-__device__ __forceinline__ bool pa_advance(const PagedAttnArgs& a, PaCursor& c) {
-    if (++c.u < c.nu) return true;
+// To the first unit of the next segment; false past the last sequence.
+__device__ __forceinline__ bool pa_next(const PagedAttnArgs& a, PaCursor& c) {
     c.u = 0;
     if (++c.chunk < a.chunks) return true;
     c.chunk = 0;
@@ -121,8 +120,7 @@ __device__ __forceinline__ bool pa_advance(const PagedAttnArgs& a, PaCursor& c) 
     return true;
 }
 
-// Weight of a piece with maximum m and mask reference mk against the joint
-// references.
+// Maximum m of a piece with mask reference mk, against the reference mk_all.
 __device__ __forceinline__ float pa_rel(float m, float mk, float mk_all) {
     return m == -INFINITY ? -INFINITY : m + (mk - mk_all) * 1.44269504f;
 }
@@ -134,6 +132,15 @@ __device__ __forceinline__ float4 pa_lds4(uint32_t addr) {
                  : "r"(addr)
                  : "memory");
     return v;
+}
+
+// p + I * step in one instruction.
+template <int I>
+__device__ __forceinline__ const uint8_t* pa_step(const uint8_t* p, uint32_t step) {
+    if (I == 0) return p;
+    uint64_t r;
+    asm("mad.wide.u32 %0, %1, %2, %3;" : "=l"(r) : "r"(step), "n"(I), "l"(p));
+    return reinterpret_cast<const uint8_t*>(r);
 }
 
 // One head of a segment being joined by one warp: the unnormalised values of
@@ -247,11 +254,15 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
         uint32_t dst_of[SW];
 #pragma unroll
         for (int i = 0; i < SW; ++i) dst_of[i] = ring + lr * RB + ((lc ^ ((i * RPI + lr) & 7)) << 4);
+        const uint32_t kp16 = (uint32_t)(a.kv.k_page >> 4), kr16 = (uint32_t)(a.kv.k_row >> 4);
+        const uint32_t vp16 = (uint32_t)(a.kv.v_page >> 4), vr16 = (uint32_t)(a.kv.v_row >> 4);
         const uint32_t k_step = (uint32_t)(RPI * a.kv.k_row), v_step = (uint32_t)(RPI * a.kv.v_row);
         const uint32_t k_lane = (uint32_t)(lr * a.kv.k_row) + 16 * lc, v_lane = (uint32_t)(lr * a.kv.v_row) + 16 * lc;
         int bi = 0, row = 0, w0 = 0;     // its block (list entry) and row; first entry of the page window
         int p0 = -1, p1 = -1, b0 = -1, b1 = -1;  // pages and blocks of entries w0 + lane, w0 + 32 + lane
+        int run = 0;                     // units to go in this segment and this window
         bool fresh = true;
+        const uint8_t *k_head = nullptr, *v_head = nullptr;
         float mask_pending = 0.f;
         int mask_stage = -1;
         unsigned valid_pending = 0;
@@ -284,25 +295,36 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                 mask_stage = -1;
             }
         };
+        // another segment, or the next 32 entries of this one's list
+        auto refill = [&]() {
+            if (in.u == in.nu) fresh = pa_next(a, in);
+            const unsigned vt = (unsigned)in.u * kPaTok + (lane & 15);
+            bi = (int)(vt / (unsigned)ps);
+            row = (int)(vt - (unsigned)bi * (unsigned)ps);
+            if (fresh) {
+                w0 = (int)((unsigned)in.u * kPaTok / (unsigned)ps);
+                window(w0 + lane, false);
+                k_head = static_cast<const uint8_t*>(a.kv.k) + in.head * a.kv.k_head;
+                v_head = static_cast<const uint8_t*>(a.kv.v) + in.head * a.kv.v_head;
+                fresh = false;
+            } else {
+                w0 += 32;
+                p0 = p1, b0 = b1;
+                window(w0 + lane, true);
+            }
+            // units that begin before entry w0 + 32
+            const long long here = ((long long)(w0 + 32) * ps - (long long)in.u * kPaTok + kPaTok - 1) / kPaTok;
+            run = (int)min((long long)(in.nu - in.u), here);
+        };
         auto issue = [&](int stage) {
             if (MASK) flush_mask();
             if (to_issue > 0) {
-                if (fresh) {
-                    const unsigned vt = (unsigned)in.u * kPaTok + (lane & 15);
-                    bi = (int)(vt / (unsigned)ps);
-                    row = (int)(vt % (unsigned)ps);
-                    w0 = (int)((unsigned)in.u * kPaTok / (unsigned)ps);
-                    window(w0 + lane, false);
-                    fresh = false;
+                if (run == 0) {
+                    refill();
                 } else {
                     bi += q16;
                     row += r16;
                     if (row >= ps) row -= ps, ++bi;
-                    if ((aligned ? bi : __shfl_sync(0xffffffffu, bi, 0)) >= w0 + 32) {
-                        w0 += 32;
-                        p0 = p1, b0 = b1;
-                        window(w0 + lane, true);
-                    }
                 }
                 const int x = bi - w0;  // 0 .. 31, 46 where a unit spans pages
                 int page = __shfl_sync(0xffffffffu, p0, x & 31), blk = bi;
@@ -320,35 +342,32 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                     mask_stage = stage;
                     valid_pending = valid;
                 }
-                const uint8_t *kb = static_cast<const uint8_t*>(a.kv.k), *vb = static_cast<const uint8_t*>(a.kv.v);
                 const uint32_t at = stage * (2 * TILE);
                 if (near_rows && valid == 0xffffu) {  // 16 rows of one page: a base and steps
-                    const int row0 = row - (lane & 15);
-                    kb += page * a.kv.k_page + row0 * a.kv.k_row + in.head * a.kv.k_head + k_lane;
-                    vb += page * a.kv.v_page + row0 * a.kv.v_row + in.head * a.kv.v_head + v_lane;
+                    const uint32_t row0 = row - (lane & 15);
+                    const uint8_t* kb = k_head + k_lane + (((uint64_t)(uint32_t)page * kp16 + (uint64_t)row0 * kr16) << 4);
+                    const uint8_t* vb = v_head + v_lane + (((uint64_t)(uint32_t)page * vp16 + (uint64_t)row0 * vr16) << 4);
                     unrolled(std::make_index_sequence<kPaTok / RPI>{}, [&](auto ic) {
                         constexpr int I = decltype(ic)::value, OFF = I / SW * (SW * RPI * RB) + I % SW * (RPI * RB);
-                        pa_cp16_at<OFF>(dst_of[I % SW] + at, kb);
-                        pa_cp16_at<OFF + TILE>(dst_of[I % SW] + at, vb);
-                        kb += k_step;
-                        vb += v_step;
+                        pa_cp16_at<OFF>(dst_of[I % SW] + at, pa_step<I>(kb, k_step));
+                        pa_cp16_at<OFF + TILE>(dst_of[I % SW] + at, pa_step<I>(vb, v_step));
                     });
                 } else {  // row by row from the lane that looks after it; zeros for those that do not exist
-                    const long long ko = ok ? page * a.kv.k_page + row * a.kv.k_row + in.head * a.kv.k_head : 0;
-                    const long long vo = ok ? page * a.kv.v_page + row * a.kv.v_row + in.head * a.kv.v_head : 0;
+                    const long long ko = ok ? page * a.kv.k_page + row * a.kv.k_row : 0;
+                    const long long vo = ok ? page * a.kv.v_page + row * a.kv.v_row : 0;
 #pragma unroll
                     for (int i = 0; i < kPaTok / RPI; ++i) {
                         const int r = i * RPI + lr;
                         const uint32_t d = dst_of[i % SW] + at + i * RPI * RB;
                         const long long kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
                         const bool on = (valid >> r) & 1;
-                        pa_cp16(d, kb + kr + 16 * lc, on);
-                        pa_cp16(d + TILE, vb + vr + 16 * lc, on);
+                        pa_cp16(d, k_head + kr + 16 * lc, on);
+                        pa_cp16(d + TILE, v_head + vr + 16 * lc, on);
                     }
                 }
                 --to_issue;
-                if (to_issue > 0 && !pa_advance(a, in)) to_issue = 0;
-                fresh = in.u == 0;
+                --run;
+                ++in.u;
             }
             pa_commit();
         };
@@ -403,8 +422,9 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
         };
         // The loop runs S - 1 units ahead with the copies: its first S - 1 turns
         // only issue.
-        bool new_q = true;
-        int stage = 0, ahead = 0;
+        int stage = 0, ahead = 0, lead = S - 1;
+        int part = min(cur.nu - cur.u, to_do), turns = part;  // units of this segment in this range, and to go
+        bool special = true, fetch = true;  // the first turns, or a new segment: queries to fetch
         // this lane's ldmatrix rows: 16 dims of a k step are 32 bytes, which the
         // swizzle moves within 128; K: positions 0-7 dims 0-7, 8-15, positions
         // 8-15 the same; V: dims 0-7 positions 0-7, 8-15, the next 8 dims the same
@@ -416,19 +436,23 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
             v_at[i] = ring + TILE + (8 * (mi & 1) + ri) * RB + (((2 * i + (mi >> 1)) ^ ri) << 4);
         }
 #pragma unroll 1
-        for (int turn = 1 - S; to_do > 0; ++turn) {
-            if (EARLY_Q && new_q && (turn == 1 - S || turn > 0)) fetch_q();
-            if (turn >= 0) {
-                pa_wait<S - 2>();
-                __syncwarp();
+        for (;;) {
+            if (special && EARLY_Q && fetch) {
+                fetch_q();
+                fetch = false;
             }
+            pa_wait<S - 2>();
+            __syncwarp();
             issue(ahead);
             ahead = ahead + 1 == S ? 0 : ahead + 1;
-            if (turn < 0) continue;
-            if (new_q) {
+            if (special) {
+                if (lead > 0) {
+                    --lead;
+                    continue;
+                }
                 if (!EARLY_Q) fetch_q();
                 take_q();
-                new_q = false;
+                special = false;
             }
             const unsigned valid = sh.valid[warp][stage];
             const unsigned live = MASK ? sh.live[warp][stage] : valid;
@@ -536,9 +560,9 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
             }
             stage = stage + 1 == S ? 0 : stage + 1;
 
-            const bool seg_end = cur.u + 1 == cur.nu;
-            if (seg_end || to_do == 1) {
-                if (pending) flush();
+            if (--turns == 0) {
+                const bool seg_end = cur.u + part == cur.nu;
+                flush();
                 l += __shfl_xor_sync(0xffffffffu, l, 1);
                 l += __shfl_xor_sync(0xffffffffu, l, 2);
                 if (seg_end && seg_from >= fb) {  // the whole segment
@@ -570,11 +594,12 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                         sh.rows[x][warp] = min(kPaHeads, G - cur.chunk * kPaHeads);
                     }
                 }
-            }
-            if (--to_do > 0) {
-                if (seg_end) seg_from += cur.nu;
-                if (!pa_advance(a, cur)) break;
-                new_q = seg_end;
+                to_do -= part;
+                if (to_do == 0) break;
+                seg_from += cur.nu;  // the range goes on, so the segment has ended
+                if (!pa_next(a, cur)) break;
+                part = turns = min(cur.nu, to_do);
+                special = fetch = true;
             }
         }
         pa_wait<0>();

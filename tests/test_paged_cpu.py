@@ -49,7 +49,7 @@ def test_plan_refuses_more_sequences_than_it_scans():
 BAD_KV = [dict(k=None), dict(v=None), dict(n_head_kv=0), dict(page_size=0), dict(n_pages=0), dict(k=PTR + 8),
           dict(v=PTR + 2), dict(k_page=8), dict(k_row=520), dict(k_head=2), dict(v_page=-16), dict(v_row=264),
           dict(v_head=8), dict(k_lo=None), dict(k_hi=None), dict(k_lo=PTR + 8), dict(k_hi=PTR + 4),
-          dict(page_size=1 << 20, n_pages=1 << 12)]
+          dict(page_size=1 << 20, n_pages=1 << 12), dict(k_page=1 << 36), dict(v_row=1 << 40)]
 UNSUPPORTED_KV = [dict(type=0), dict(type=2), dict(type=99), dict(head_dim=96), dict(head_dim=512), dict(head_dim=0)]
 
 
