@@ -599,12 +599,12 @@ def _launch(what: str, device, fn, *args):
     for the bare stream handle (torch.cuda.current_stream builds an object)."""
     torch = _torch()
     i = device.index
-    if torch.cuda.current_device() == i:
+    if torch._C._cuda_getDevice() == i:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(i):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
-    if rc != OK:
+    if rc:
         _check(rc, what)
 
 
@@ -657,17 +657,6 @@ class PagedPlan:
         self.slots, self.positions, self.cu, self.seq_lens, self.n_free = slots, positions, cu, seq_lens, n_free
 
 
-def _check_i32(what, device, names, *tensors):
-    torch = _torch()
-    for name, t in zip(names, tensors):
-        if t.dtype != torch.int32 or t.device != device or (t.dim() == 1 and not t.is_contiguous()):
-            _bad(what, f"{name} must be a contiguous int32 tensor on {device}")
-
-
-_PLAN_I32 = ("new_lens", "seq_lens", "block_table", "free_pages", "n_free", "seq_lens_out", "n_free_out", "cu",
-             "positions")
-
-
 def paged_plan(new_lens, seq_lens, block_table, free_pages, n_free, page_size: int, max_tokens: int,
                seq_lens_out=None, n_free_out=None, slots=None, positions=None, cu=None) -> PagedPlan:
     """Pages, lengths and slots of one step, on the device.
@@ -683,31 +672,45 @@ def paged_plan(new_lens, seq_lens, block_table, free_pages, n_free, page_size: i
     A sequence that the table, max_tokens or the free pages cannot take keeps
     its length; the caller sees that from seq_lens."""
     torch = _torch()
-    dev = seq_lens.device
-    if seq_lens.dim() != 1 or not seq_lens.is_cuda or new_lens.shape != seq_lens.shape or seq_lens.numel() == 0:
+    dev, i32, shape, table = seq_lens.device, torch.int32, seq_lens.shape, block_table.shape
+    if len(shape) != 1 or dev.type != "cuda" or new_lens.shape != shape or shape[0] == 0:
         _bad("paged_plan", "seq_lens and new_lens must be [n_seq] on a CUDA device, n_seq >= 1")
-    n = seq_lens.numel()
-    if block_table.dim() != 2 or block_table.shape[0] != n or block_table.shape[1] == 0 or block_table.stride(1) != 1:
+    n = shape[0]
+    if len(table) != 2 or table[0] != n or table[1] == 0 or block_table.stride(1) != 1:
         _bad("paged_plan", "block_table must be [n_seq, max_blocks] with contiguous rows")
+    if max_tokens < 0:
+        _bad("paged_plan", "max_tokens must not be negative")
     if seq_lens_out is None:
         seq_lens_out = seq_lens
+    elif seq_lens_out.shape != shape or seq_lens_out.dtype != i32 or seq_lens_out.device != dev \
+            or not seq_lens_out.is_contiguous():
+        _bad("paged_plan", "seq_lens_out must be a contiguous int32 [n_seq] on seq_lens' device")
     if n_free_out is None:
         n_free_out = n_free
+    elif n_free_out.numel() != 1 or n_free_out.dtype != i32 or n_free_out.device != dev:
+        _bad("paged_plan", "n_free_out must be an int32 [1] on seq_lens' device")
+    if (seq_lens.dtype != i32 or new_lens.dtype != i32 or block_table.dtype != i32 or free_pages.dtype != i32
+            or n_free.dtype != i32 or new_lens.device != dev or block_table.device != dev or free_pages.device != dev
+            or n_free.device != dev or n_free.numel() != 1 or free_pages.dim() != 1 or not free_pages.is_contiguous()
+            or not seq_lens.is_contiguous() or not new_lens.is_contiguous()):
+        _bad("paged_plan", "new_lens [n_seq], seq_lens [n_seq], block_table, free_pages [n_pages] and n_free [1] must be "
+                           "contiguous int32 tensors on one device")
     if cu is None:
         cu = seq_lens.new_empty(n + 1)
+    elif cu.dtype != i32 or cu.device != dev or cu.dim() != 1 or cu.numel() < n + 1 or not cu.is_contiguous():
+        _bad("paged_plan", "cu must be a contiguous int32 [n_seq + 1] on seq_lens' device")
     if slots is None:
         slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+    elif slots.dtype != torch.int64 or slots.device != dev or slots.dim() != 1 or slots.numel() < max_tokens \
+            or not slots.is_contiguous():
+        _bad("paged_plan", "slots must be a contiguous int64 [max_tokens] on seq_lens' device")
     if positions is None:
         positions = seq_lens.new_empty(max_tokens)
-    _check_i32("paged_plan", dev, _PLAN_I32, new_lens, seq_lens, block_table, free_pages, n_free, seq_lens_out,
-               n_free_out, cu, positions)
-    if (free_pages.dim() != 1 or n_free.numel() != 1 or n_free_out.numel() != 1 or seq_lens_out.shape != seq_lens.shape
-            or cu.dim() != 1 or cu.numel() < n + 1 or positions.dim() != 1 or positions.numel() < max_tokens
-            or slots.dtype != torch.int64 or slots.device != dev or slots.dim() != 1 or not slots.is_contiguous()
-            or slots.numel() < max_tokens):
-        _bad("paged_plan", "free_pages [n_pages], n_free [1], cu [n_seq + 1] and slots, positions [max_tokens]")
+    elif positions.dtype != i32 or positions.device != dev or positions.dim() != 1 or positions.numel() < max_tokens \
+            or not positions.is_contiguous():
+        _bad("paged_plan", "positions must be a contiguous int32 [max_tokens] on seq_lens' device")
     _launch("paged_plan", dev, lib().b200_paged_plan, new_lens.data_ptr(), seq_lens.data_ptr(), n,
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], page_size, free_pages.data_ptr(),
+            block_table.data_ptr(), block_table.stride(0), table[1], page_size, free_pages.data_ptr(),
             free_pages.numel(), n_free.data_ptr(), max_tokens, slots.data_ptr(), positions.data_ptr(), cu.data_ptr(),
             seq_lens_out.data_ptr(), n_free_out.data_ptr())
     return PagedPlan(slots, positions, cu, seq_lens_out, n_free_out)
@@ -764,13 +767,9 @@ def _paged_batch(what, cache, q, block_table, seq_lens):
     return q, ld, n_seq, n_head
 
 
-def _paged_workspace(what, workspace, size, dev, zeros):
-    torch = _torch()
-    if workspace is None:
-        return (torch.zeros if zeros else torch.empty)(size, dtype=torch.uint8, device=dev)
-    if workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
+def _check_workspace(what, workspace, dev):
+    if workspace.dtype != _torch().uint8 or workspace.device != dev or not workspace.is_contiguous():
         _bad(what, "workspace must be a contiguous uint8 tensor on the cache's device")
-    return workspace
 
 
 def paged_select(cache: PagedKV, q, block_table, seq_lens, n_sel: int, sel=None, workspace=None):
@@ -796,9 +795,9 @@ def paged_select(cache: PagedKV, q, block_table, seq_lens, n_sel: int, sel=None,
         _bad("paged_select", "sel must be a contiguous int32 [n_seq, n_head_kv, n_sel]")
     if workspace is None:
         size = paged_select_workspace_size(n_seq, cache.n_head_kv, block_table.shape[1])
-        workspace = _paged_workspace("paged_select", None, size, dev, zeros=False)
+        workspace = torch.empty(size, dtype=torch.uint8, device=dev)
     else:
-        _paged_workspace("paged_select", workspace, 0, dev, zeros=False)
+        _check_workspace("paged_select", workspace, dev)
     _launch("paged_select", dev, lib().b200_paged_select, cache._ref, q.data_ptr(), q_stride, n_seq, n_head,
             block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), n_sel,
             sel.data_ptr(), workspace.data_ptr(), workspace.numel())
@@ -826,27 +825,31 @@ def paged_attn(cache: PagedKV, q, block_table, seq_lens, scale: float, mask=None
     torch = _torch()
     dev = cache.device
     q, q_stride, n_seq, n_head = _paged_batch("paged_attn", cache, q, block_table, seq_lens)
-    width = block_table.shape[1] * cache.page_size
-    if mask is not None and (mask.dtype != torch.float16 or mask.device != dev or mask.dim() != 2
-                             or mask.shape[0] != n_seq or mask.shape[1] < width or mask.stride(1) != 1):
-        _bad("paged_attn", "mask must be f16 [n_seq, >= max_blocks * page_size] with contiguous rows")
-    if sel is not None and (sel.dtype != torch.int32 or sel.device != dev or not sel.is_contiguous()
-                            or sel.dim() != 3 or tuple(sel.shape[:2]) != (n_seq, cache.n_head_kv)
-                            or sel.shape[2] == 0):
-        _bad("paged_attn", "sel must be a contiguous int32 [n_seq, n_head_kv, n_sel]")
-    shape = (n_seq, n_head, cache.head_dim)
+    if mask is None:
+        mask_ptr, mask_stride = None, 0
+    else:
+        if (mask.dtype != torch.float16 or mask.device != dev or mask.dim() != 2 or mask.shape[0] != n_seq
+                or mask.shape[1] < block_table.shape[1] * cache.page_size or mask.stride(1) != 1):
+            _bad("paged_attn", "mask must be f16 [n_seq, >= max_blocks * page_size] with contiguous rows")
+        mask_ptr, mask_stride = mask.data_ptr(), mask.stride(0)
+    if sel is None:
+        sel_ptr, n_sel = None, 0
+    else:
+        s = sel.shape
+        if (sel.dtype != torch.int32 or sel.device != dev or not sel.is_contiguous() or len(s) != 3 or s[0] != n_seq
+                or s[1] != cache.n_head_kv or s[2] == 0):
+            _bad("paged_attn", "sel must be a contiguous int32 [n_seq, n_head_kv, n_sel]")
+        sel_ptr, n_sel = sel.data_ptr(), s[2]
     if out is None:
-        out = q.new_empty(shape)
-    elif out.dtype != torch.float32 or out.device != dev or not out.is_contiguous() or tuple(out.shape) != shape:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.dtype != torch.float32 or out.device != dev or not out.is_contiguous() or out.shape != q.shape:
         _bad("paged_attn", "out must be a contiguous f32 [n_seq, n_head, head_dim]")
     if workspace is None:
         size = paged_attn_workspace_size(cache.head_dim, n_seq, n_head, cache.n_head_kv)
-        workspace = _paged_workspace("paged_attn", None, size, dev, zeros=True)
+        workspace = torch.zeros(size, dtype=torch.uint8, device=dev)
     else:
-        _paged_workspace("paged_attn", workspace, 0, dev, zeros=True)
+        _check_workspace("paged_attn", workspace, dev)
     _launch("paged_attn", dev, lib().b200_paged_attn, cache._ref, q.data_ptr(), q_stride, n_seq, n_head,
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
-            None if mask is None else mask.data_ptr(), 0 if mask is None else mask.stride(0),
-            None if sel is None else sel.data_ptr(), 0 if sel is None else sel.shape[2], scale, out.data_ptr(),
-            workspace.data_ptr(), workspace.numel())
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), mask_ptr,
+            mask_stride, sel_ptr, n_sel, scale, out.data_ptr(), workspace.data_ptr(), workspace.numel())
     return out
