@@ -45,7 +45,7 @@ extern "C" {
 /* One layer's cache.  Element (page, row, head, d) of K is at byte
  * page * k_page + row * k_row + head * k_head + d * 2 of k, V likewise: any
  * order of rows and heads inside a page works.  k, v and every stride are
- * multiples of 16 bytes, the strides below 2^36. */
+ * multiples of 16 bytes; K and V span less than 64 GiB each. */
 typedef struct {
     int type;      /* B200_TYPE_F16 or B200_TYPE_BF16 */
     int head_dim;  /* 64, 128 or 256 */

@@ -17,7 +17,13 @@ int check_paged_kv(const b200_paged_kv* kv) {
     if (kv->type != B200_TYPE_F16 && kv->type != B200_TYPE_BF16) return B200_EUNSUPPORTED;
     if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256) return B200_EUNSUPPORTED;
     const int64_t strides = kv->k_page | kv->k_row | kv->k_head | kv->v_page | kv->v_row | kv->v_head;
-    if (!aligned16(kv->k) || !aligned16(kv->v) || (strides & 15) || strides < 0 || strides >> 36) return B200_EINVAL;
+    if (!aligned16(kv->k) || !aligned16(kv->v) || (strides & 15) || strides < 0) return B200_EINVAL;
+    // the last byte of K and of V: offsets are counted in 16-byte steps in 32 bits
+    const int64_t span = (int64_t)1 << 36;
+    if ((strides >> 36) || kv->n_pages > span / std::max<int64_t>(1, std::max(kv->k_page, kv->v_page)) ||
+        (kv->n_pages - 1) * kv->k_page + (kv->page_size - 1) * kv->k_row + (kv->n_head_kv - 1) * kv->k_head >= span ||
+        (kv->n_pages - 1) * kv->v_page + (kv->page_size - 1) * kv->v_row + (kv->n_head_kv - 1) * kv->v_head >= span)
+        return B200_EUNSUPPORTED;
     if ((kv->k_lo == nullptr) != (kv->k_hi == nullptr) || !aligned16(kv->k_lo) || !aligned16(kv->k_hi))
         return B200_EINVAL;
     return B200_OK;
@@ -120,45 +126,53 @@ int launch_paged_select(const PagedSelectArgs& a, int head_dim, cudaStream_t st)
     }
 }
 
-bool g_paged_attn_attr[kMaxDevices][2][3][2];
+bool g_paged_attn_attr[kMaxDevices][2][3][2][2];
 
-template <bool BF16, int D, bool MASK>
+template <bool BF16, int D, int NC, bool MASK>
 int launch_paged_attn_dm(const PagedAttnArgs& a, cudaStream_t st) {
     const int dev = current_device();
     if (dev < 0 || dev >= kMaxDevices) return B200_EINVAL;
     {
-        bool& done = g_paged_attn_attr[dev][BF16][D == 64 ? 0 : D == 128 ? 1 : 2][MASK];
+        bool& done = g_paged_attn_attr[dev][BF16][D == 64 ? 0 : D == 128 ? 1 : 2][NC - 1][MASK];
         std::lock_guard<std::mutex> lk(g_attr_mu);
         if (!done) {
-            CR_(cuda_status(cudaFuncSetAttribute(paged_attn_kernel<BF16, D, MASK>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, pa_smem<D>())));
+            CR_(cuda_status(cudaFuncSetAttribute(paged_attn_kernel<BF16, D, NC, MASK>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, pa_smem<D, NC>())));
             done = true;
         }
     }
     // the lengths are on the device: at most this many units
     const int64_t width = (int64_t)(a.sel ? a.n_sel : a.max_blocks) * a.kv.page_size;
     const int64_t units = (int64_t)a.n_seq * a.kv.n_head_kv * a.chunks * ((width + kPaTok - 1) / kPaTok);
-    const int64_t grid = std::min<int64_t>(kPaCtas, (units + pa_warps(D) - 1) / pa_warps(D));
-    paged_attn_kernel<BF16, D, MASK><<<(unsigned)grid, 32 * pa_warps(D), pa_smem<D>(), st>>>(a);
+    const int64_t grid = std::min<int64_t>(kPaCtas, (units + pa_warps(D, NC) - 1) / pa_warps(D, NC));
+    paged_attn_kernel<BF16, D, NC, MASK><<<(unsigned)grid, 32 * pa_warps(D, NC), pa_smem<D, NC>(), st>>>(a);
     return cuda_status(cudaGetLastError());
 }
 
-template <bool BF16, int D>
+template <bool BF16, int D, int NC>
 int launch_paged_attn_d(const PagedAttnArgs& a, cudaStream_t st) {
-    return a.mask ? launch_paged_attn_dm<BF16, D, true>(a, st) : launch_paged_attn_dm<BF16, D, false>(a, st);
+    return a.mask ? launch_paged_attn_dm<BF16, D, NC, true>(a, st) : launch_paged_attn_dm<BF16, D, NC, false>(a, st);
 }
 
 template <bool BF16>
 int launch_paged_attn(const PagedAttnArgs& a, cudaStream_t st) {
+    const bool two = pa_groups(a.kv.head_dim, a.n_head / a.kv.n_head_kv) == 2;
     switch (a.kv.head_dim) {
-        case 64: return launch_paged_attn_d<BF16, 64>(a, st);
-        case 128: return launch_paged_attn_d<BF16, 128>(a, st);
-        default: return launch_paged_attn_d<BF16, 256>(a, st);
+        case 64: return two ? launch_paged_attn_d<BF16, 64, 2>(a, st) : launch_paged_attn_d<BF16, 64, 1>(a, st);
+        case 128: return two ? launch_paged_attn_d<BF16, 128, 2>(a, st) : launch_paged_attn_d<BF16, 128, 1>(a, st);
+        default: return launch_paged_attn_d<BF16, 256, 1>(a, st);
     }
 }
 
-int paged_chunks(int n_head, int n_head_kv) { return (n_head / n_head_kv + kPaHeads - 1) / kPaHeads; }
-size_t paged_pieces_bytes(int head_dim) { return align256((size_t)kPaCtas * 2 * pa_piece(head_dim) * sizeof(float)); }
+// Passes over a KV head's query heads, and heads of one.
+int paged_heads(int head_dim, int n_head, int n_head_kv) { return kPaHeads * pa_groups(head_dim, n_head / n_head_kv); }
+int paged_chunks(int head_dim, int n_head, int n_head_kv) {
+    const int heads = paged_heads(head_dim, n_head, n_head_kv);
+    return (n_head / n_head_kv + heads - 1) / heads;
+}
+size_t paged_pieces_bytes(int head_dim, int n_head, int n_head_kv) {
+    return align256((size_t)kPaCtas * 2 * pa_piece(head_dim, pa_groups(head_dim, n_head / n_head_kv)) * sizeof(float));
+}
 
 }  // namespace
 
@@ -268,8 +282,9 @@ size_t b200_paged_attn_workspace_size(int head_dim, int n_seq, int n_head, int n
     if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || n_seq < 0 || n_seq > 65535 || n_head <= 0 ||
         n_head > 65535 || n_head_kv <= 0 || n_head % n_head_kv)
         return 0;
-    return paged_pieces_bytes(head_dim) +
-           align256((size_t)n_seq * n_head_kv * paged_chunks(n_head, n_head_kv) * kPaHeads * sizeof(unsigned int));
+    return paged_pieces_bytes(head_dim, n_head, n_head_kv) +
+           align256((size_t)n_seq * n_head_kv * paged_chunks(head_dim, n_head, n_head_kv) *
+                    paged_heads(head_dim, n_head, n_head_kv) * sizeof(unsigned int));
 }
 
 int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, int n_seq, int n_head,
@@ -286,7 +301,7 @@ int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, i
         workspace_size < b200_paged_attn_workspace_size(kv->head_dim, n_seq, n_head, kv->n_head_kv))
         return B200_EINVAL;
     const int64_t width = (int64_t)(sel ? n_sel : max_blocks) * kv->page_size;
-    const int64_t segments = (int64_t)n_seq * kv->n_head_kv * paged_chunks(n_head, kv->n_head_kv);
+    const int64_t segments = (int64_t)n_seq * kv->n_head_kv * paged_chunks(kv->head_dim, n_head, kv->n_head_kv);
     if (segments * ((width + kPaTok - 1) / kPaTok) > INT32_MAX) return B200_EUNSUPPORTED;  // units are counted in int
     PagedAttnArgs a;
     a.kv = *kv;
@@ -299,14 +314,15 @@ int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, i
     a.mask_stride = mask_stride;
     a.sel = sel;
     a.out = out;
-    a.chunks = paged_chunks(n_head, kv->n_head_kv);
+    a.chunks = paged_chunks(kv->head_dim, n_head, kv->n_head_kv);
     a.pieces = static_cast<float*>(workspace);
-    a.tickets = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(workspace) + paged_pieces_bytes(kv->head_dim));
+    a.tickets = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(workspace) + paged_pieces_bytes(kv->head_dim, n_head, kv->n_head_kv));
     a.scale = scale;
     a.n_seq = n_seq;
     a.n_head = n_head;
     a.n_sel = n_sel;
     a.max_blocks = max_blocks;
+    a.same_rows = kv->k_page == kv->v_page && kv->k_row == kv->v_row;
     a.near_rows = std::max(kv->k_row, kv->v_row) < ((int64_t)1 << 31) / kPaTok;
     return kv->type == B200_TYPE_BF16 ? launch_paged_attn<true>(a, (cudaStream_t)stream)
                                       : launch_paged_attn<false>(a, (cudaStream_t)stream);

@@ -43,11 +43,17 @@ namespace b200 {
 
 constexpr int kPaHeads = 8;   // query heads of one KV head handled together
 
-// Warps per CTA and ring stages per warp: 192 KB of ring in every case.
-B200_HD constexpr int pa_warps(int D) { return D == 64 ? 12 : D == 128 ? 8 : 4; }
-B200_HD constexpr int pa_stages(int D) { return D == 64 ? 4 : 3; }
-// Floats of one piece: o [8][D], m [8], l [8], mask reference.
-B200_HD constexpr int pa_piece(int D) { return kPaHeads * D + 2 * kPaHeads + 4; }
+// Groups of 8 query heads a pass takes (NC): one up to 8 query heads per KV
+// head, else two, so that 9 to 16 read the cache once (head dim 256 lacks the
+// registers).
+B200_HD constexpr int pa_groups(int D, int G) { return G > kPaHeads && D < 256 ? 2 : 1; }
+// Warps per CTA and ring stages per warp: up to 192 KB of ring.
+B200_HD constexpr int pa_warps(int D, int NC = 1) {
+    return NC == 2 ? (D == 64 ? 8 : 6) : D == 64 ? 12 : D == 128 ? 8 : 4;
+}
+B200_HD constexpr int pa_stages(int D, int NC = 1) { return NC == 2 ? (D == 64 ? 5 : 3) : D == 64 ? 4 : 3; }
+// Floats of one piece: o [8 NC][D], m [8 NC], l [8 NC], mask reference.
+B200_HD constexpr int pa_piece(int D, int NC = 1) { return kPaHeads * NC * (D + 2) + 4; }
 B200_HD constexpr int pa_tile(int D) { return kPaTok * D * 2; }
 
 // Bookkeeping beside the ring and the pieces in shared memory.
@@ -61,10 +67,10 @@ struct PaShared {
     unsigned valid[W][S], live[W][S];  // positions of a stage that exist; that the mask leaves in
     float mask[W][S][kPaTok];
 };
-template <int D>
+template <int D, int NC>
 constexpr int pa_smem() {
-    return pa_warps(D) * (pa_stages(D) * 2 * pa_tile(D) + pa_piece(D) * 4) +
-           (int)sizeof(PaShared<pa_warps(D), pa_stages(D)>);
+    return pa_warps(D, NC) * (pa_stages(D, NC) * 2 * pa_tile(D) + pa_piece(D, NC) * 4) +
+           (int)sizeof(PaShared<pa_warps(D, NC), pa_stages(D, NC)>);
 }
 
 struct PagedAttnArgs {
@@ -79,10 +85,11 @@ struct PagedAttnArgs {
     const int32_t* sel;
     float* out;
     float* pieces;          // [kPaCtas][2][pa_piece]
-    unsigned int* tickets;  // [n_seq * n_head_kv * chunks][8], zero between calls
+    unsigned int* tickets;  // [n_seq * n_head_kv * chunks][8 NC], zero between calls
     float scale;
     int n_seq, n_head, n_sel, max_blocks, chunks;
     int near_rows;          // 16 rows of a page span less than 2^31 bytes
+    int same_rows;          // K and V have the same page and row strides
 };
 
 // f(integral_constant<I>) for I of the sequence.
@@ -186,14 +193,15 @@ struct PaJoint {
     }
 };
 
-template <bool BF16, int D, bool MASK>
-__global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAttnArgs a) {
-    constexpr int W = pa_warps(D), S = pa_stages(D), T = 32 * W;
+template <bool BF16, int D, int NC, bool MASK>
+__global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(PagedAttnArgs a) {
+    constexpr int W = pa_warps(D, NC), S = pa_stages(D, NC), T = 32 * W;
+    constexpr int NH = kPaHeads * NC;      // query heads of a pass
     constexpr int KT = D / 16;             // k steps of q . k, pairs of output tiles
     constexpr int LPR = D / 8;             // 16-byte lanes per row
     constexpr int RPI = 32 / LPR;          // rows per copy instruction
-    constexpr int TILE = pa_tile(D), RB = 2 * D, PIECE = pa_piece(D);
-    constexpr bool EARLY_Q = D <= 128;     // queries fetched before a unit is issued; D = 256 lacks the registers
+    constexpr int TILE = pa_tile(D), RB = 2 * D, PIECE = pa_piece(D, NC);
+    constexpr bool EARLY_Q = NC == 1 && D <= 128;  // queries fetched before a unit is issued, if registers allow
     extern __shared__ __align__(128) uint8_t pa_sm[];
     PaShared<W, S>& sh = *reinterpret_cast<PaShared<W, S>*>(pa_sm + W * (S * 2 * TILE + PIECE * 4));
 
@@ -236,19 +244,24 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
         int to_issue = fe - fb, to_do = to_issue;
 
         // the first segment's queries, on their way while the page table is read
-        float2 qx[2 * KT];
+        float2 qx[NC][2 * KT];
         auto fetch_q = [&]() {
-            const int j = cur.chunk * kPaHeads + g;
-            const float* qr = a.q + cur.s * a.q_stride + (int64_t)(cur.head * G + (j < G ? j : 0)) * D + 2 * t4;
 #pragma unroll
-            for (int i = 0; i < 2 * KT; ++i) qx[i] = *reinterpret_cast<const float2*>(qr + 8 * i);
+            for (int c = 0; c < NC; ++c) {
+                const int j = cur.chunk * NH + kPaHeads * c + g;
+                const float* qr = a.q + cur.s * a.q_stride + (int64_t)(cur.head * G + (j < G ? j : 0)) * D + 2 * t4;
+#pragma unroll
+                for (int i = 0; i < 2 * KT; ++i) qx[c][i] = *reinterpret_cast<const float2*>(qr + 8 * i);
+            }
         };
 
         // ---- producer: this lane looks after token lane & 15 of a unit ----
         const int q16 = kPaTok / ps, r16 = kPaTok % ps;
         const bool aligned = ps % kPaTok == 0;  // a unit lies in one page
         const uint32_t lc = lane % LPR, lr = lane / LPR;  // this lane's 16 bytes of a row, its row of a copy
-        // (a unit of one page: 16 rows at 32-bit steps from its first)
+        // Offsets of pages and rows in 16-byte steps, in 32 bits: K and V span less
+        // than 64 GiB each.  A unit of one page is copied at fixed steps from its
+        // first row (near_rows), any other row by row.
         const bool near_rows = aligned && a.near_rows;
         constexpr int SW = 8 / RPI;  // the swizzle repeats after 8 rows
         uint32_t dst_of[SW];
@@ -263,7 +276,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
         int run = 0;                     // units to go in this segment and this window
         bool fresh = true;
         const uint8_t *k_head = nullptr, *v_head = nullptr;
-        float mask_pending = 0.f;
+        uint16_t mask_pending = 0;  // as loaded: converting it here would wait for it
         int mask_stage = -1;
         unsigned valid_pending = 0;
         // entries e and e + 32 of the block list (only_second: the second alone);
@@ -289,8 +302,9 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
         };
         auto flush_mask = [&]() {
             if (mask_stage >= 0) {
-                const unsigned live = __ballot_sync(0xffffffffu, mask_pending != -INFINITY) & valid_pending;
-                if (lane < kPaTok) sh.mask[warp][mask_stage][lane] = mask_pending;
+                const float v = (valid_pending >> (lane & 15)) & 1 ? h2f(mask_pending) : -INFINITY;
+                const unsigned live = __ballot_sync(0xffffffffu, v != -INFINITY) & 0xffffu;
+                if (lane < kPaTok) sh.mask[warp][mask_stage][lane] = v;
                 if (lane == 0) sh.live[warp][mask_stage] = live;
                 mask_stage = -1;
             }
@@ -338,31 +352,31 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                 const unsigned valid = __ballot_sync(0xffffffffu, ok) & 0xffffu;
                 if (lane == 0) sh.valid[warp][stage] = valid;
                 if (MASK) {
-                    mask_pending = ok ? h2f(a.mask[in.s * a.mask_stride + (int64_t)blk * ps + row]) : -INFINITY;
+                    if (ok) mask_pending = a.mask[in.s * a.mask_stride + (int64_t)blk * ps + row];
                     mask_stage = stage;
                     valid_pending = valid;
                 }
                 const uint32_t at = stage * (2 * TILE);
                 if (near_rows && valid == 0xffffu) {  // 16 rows of one page: a base and steps
                     const uint32_t row0 = row - (lane & 15);
-                    const uint8_t* kb = k_head + k_lane + (((uint64_t)(uint32_t)page * kp16 + (uint64_t)row0 * kr16) << 4);
-                    const uint8_t* vb = v_head + v_lane + (((uint64_t)(uint32_t)page * vp16 + (uint64_t)row0 * vr16) << 4);
+                    const uint8_t* kb = pa_step<16>(k_head + k_lane, page * kp16 + row0 * kr16);
+                    const uint8_t* vb = pa_step<16>(v_head + v_lane, page * vp16 + row0 * vr16);
                     unrolled(std::make_index_sequence<kPaTok / RPI>{}, [&](auto ic) {
                         constexpr int I = decltype(ic)::value, OFF = I / SW * (SW * RPI * RB) + I % SW * (RPI * RB);
                         pa_cp16_at<OFF>(dst_of[I % SW] + at, pa_step<I>(kb, k_step));
                         pa_cp16_at<OFF + TILE>(dst_of[I % SW] + at, pa_step<I>(vb, v_step));
                     });
                 } else {  // row by row from the lane that looks after it; zeros for those that do not exist
-                    const long long ko = ok ? page * a.kv.k_page + row * a.kv.k_row : 0;
-                    const long long vo = ok ? page * a.kv.v_page + row * a.kv.v_row : 0;
+                    const uint32_t ko = ok ? page * kp16 + row * kr16 : 0u, vo = ok ? page * vp16 + row * vr16 : 0u;
 #pragma unroll
                     for (int i = 0; i < kPaTok / RPI; ++i) {
                         const int r = i * RPI + lr;
                         const uint32_t d = dst_of[i % SW] + at + i * RPI * RB;
-                        const long long kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+                        const uint32_t kr = __shfl_sync(0xffffffffu, ko, r);
+                        const uint32_t vr = a.same_rows ? kr : __shfl_sync(0xffffffffu, vo, r);
                         const bool on = (valid >> r) & 1;
-                        pa_cp16(d, k_head + kr + 16 * lc, on);
-                        pa_cp16(d + TILE, v_head + vr + 16 * lc, on);
+                        pa_cp16(d, pa_step<16>(k_head, kr + lc), on);
+                        pa_cp16(d + TILE, pa_step<16>(v_head, vr + lc), on);
                     }
                 }
                 --to_issue;
@@ -372,53 +386,61 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
             pa_commit();
         };
         // ---- consumer: this thread holds head g, positions 2 t4, 2 t4 + 1 (+ 8) ----
-        uint32_t qf[KT][4], q3[BF16 ? KT : 1][2];
+        uint32_t qf[NC][KT][4], q3[NC][BF16 ? KT : 1][2];
         // Outputs: acc is what the tensor core adds up itself (high and low parts of
         // w apart), emptied into o every FLUSH units: it truncates, and 4 of its
         // additions stay below the rounding of one f32.  m is the weights'
         // reference: it follows the running maximum only when that has grown by
         // 2^3, which w has room for (w <= 2^15 in f16), so o is rarely rescaled.
-        constexpr int FLUSH = D <= 128 ? 4 : 1;  // (D = 256 lacks the registers)
-        float o[2 * KT][2], acc[D <= 128 ? 2 * KT : 1][4];
-        float m = -INFINITY, l = 0.f, mk = -INFINITY, f = 0.f;
+        constexpr int FLUSH = D * NC <= 128 ? 4 : 1;  // (the others lack the registers)
+        float o[NC][2 * KT][2], acc[NC][FLUSH > 1 ? 2 * KT : 1][4];
+        float m[NC], l[NC], f[NC], mk = -INFINITY;
         int pending = 0;  // units in acc
         auto flush = [&]() {
             if (FLUSH == 1) return;
 #pragma unroll
-            for (int i = 0; i < (FLUSH > 1 ? 2 * KT : 0); ++i) {
-                o[i][0] += acc[i][0] + acc[i][2];
-                o[i][1] += acc[i][1] + acc[i][3];
-                acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-            }
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < (FLUSH > 1 ? 2 * KT : 0); ++i) {
+                    float(&d)[4] = acc[c][i];
+                    o[c][i][0] += d[0] + d[2];
+                    o[c][i][1] += d[1] + d[3];
+                    d[0] = d[1] = d[2] = d[3] = 0.f;
+                }
             pending = 0;
         };
         auto take_q = [&]() {
-            const bool mine_q = cur.chunk * kPaHeads + g < G;
-            float amax = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2 * KT; ++i) {
-                if (!mine_q) qx[i] = make_float2(0.f, 0.f);
-                amax = fmaxf(amax, fmaxf(fabsf(qx[i].x), fabsf(qx[i].y)));
+            for (int c = 0; c < NC; ++c) {
+                const bool mine_q = cur.chunk * NH + kPaHeads * c + g < G;
+                float amax = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2 * KT; ++i) {
+                    if (!mine_q) qx[c][i] = make_float2(0.f, 0.f);
+                    amax = fmaxf(amax, fmaxf(fabsf(qx[c][i].x), fabsf(qx[c][i].y)));
+                }
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                // q 2^-ex has its largest entry in [1, 2)
+                const int ex = min(max((int)(__float_as_uint(amax) >> 23) - 127, -120), 120);
+                const float up = __uint_as_float((unsigned)(127 - ex) << 23);
+                f[c] = a.scale * 1.44269504f * __uint_as_float((unsigned)(127 + ex) << 23);
+#pragma unroll
+                for (int i = 0; i < 2 * KT; ++i) {
+                    float x = qx[c][i].x * up, y = qx[c][i].y * up;
+                    qf[c][i >> 1][2 * (i & 1)] = pa_split<BF16>(x, y);
+                    qf[c][i >> 1][2 * (i & 1) + 1] = pa_split<BF16>(x, y);
+                    if (BF16) q3[c][i >> 1][i & 1] = pa_split<BF16>(x, y);
+                }
+#pragma unroll
+                for (int i = 0; i < 2 * KT; ++i) o[c][i][0] = o[c][i][1] = 0.f;
+#pragma unroll
+                for (int i = 0; i < (FLUSH > 1 ? 2 * KT : 0); ++i)
+                    acc[c][i][0] = acc[c][i][1] = acc[c][i][2] = acc[c][i][3] = 0.f;
+                m[c] = -INFINITY, l[c] = 0.f;
             }
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            // q 2^-ex has its largest entry in [1, 2)
-            const int ex = min(max((int)(__float_as_uint(amax) >> 23) - 127, -120), 120);
-            const float up = __uint_as_float((unsigned)(127 - ex) << 23);
-            f = a.scale * 1.44269504f * __uint_as_float((unsigned)(127 + ex) << 23);
-#pragma unroll
-            for (int i = 0; i < 2 * KT; ++i) {
-                float x = qx[i].x * up, y = qx[i].y * up;
-                qf[i >> 1][2 * (i & 1)] = pa_split<BF16>(x, y);
-                qf[i >> 1][2 * (i & 1) + 1] = pa_split<BF16>(x, y);
-                if (BF16) q3[i >> 1][i & 1] = pa_split<BF16>(x, y);
-            }
-#pragma unroll
-            for (int i = 0; i < 2 * KT; ++i) o[i][0] = o[i][1] = 0.f;
-#pragma unroll
-            for (int i = 0; i < (FLUSH > 1 ? 2 * KT : 0); ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
             pending = 0;
-            m = -INFINITY, l = 0.f, mk = MASK ? -INFINITY : 0.f;
+            mk = MASK ? -INFINITY : 0.f;
         };
         // The loop runs S - 1 units ahead with the copies: its first S - 1 turns
         // only issue.
@@ -459,30 +481,32 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
             const uint32_t st = stage * (2 * TILE);
             if (live) {
                 if (live != valid) {  // masked positions: their values may be anything
-                    for (int r = 0; r < kPaTok; ++r)
-                        if (((valid & ~live) >> r) & 1)
-                            for (int c = lane; c < RB / 16; c += 32)
-                                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + st + TILE + r * RB + 16 * c),
-                                             "r"(0u)
-                                             : "memory");
+#pragma unroll
+                    for (int i = 0; i < kPaTok / RPI; ++i)
+                        if (((valid & ~live) >> (i * RPI + lr)) & 1)
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
+                                             ring + st + TILE + (i * RPI + lr) * RB + 16 * lc),
+                                         "r"(0u)
+                                         : "memory");
                     __syncwarp();
                 }
                 // S = q K^T: 8 heads (high parts, low parts) x 16 positions
-                float sc[2][4];
+                float sc[NC][2][4];
                 unrolled(std::make_index_sequence<KT>{}, [&](auto ic) {
-                    constexpr int kt = decltype(ic)::value;
+                    constexpr int kt = decltype(ic)::value, k3 = BF16 ? kt : 0;
                     uint32_t b[4];
                     pa_ldsm_at<kt / 4 * 128>(b, k_at[kt % 4] + st);
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        if (kt == 0) pa_mma0<BF16>(sc[n], qf[kt][0], qf[kt][1], qf[kt][2], qf[kt][3], b[2 * n], b[2 * n + 1]);
-                        else pa_mma<BF16>(sc[n], qf[kt][0], qf[kt][1], qf[kt][2], qf[kt][3], b[2 * n], b[2 * n + 1]);
-                        if (BF16) pa_mma<BF16>(sc[n], q3[BF16 ? kt : 0][0], 0u, q3[BF16 ? kt : 0][1], 0u, b[2 * n], b[2 * n + 1]);
-                    }
-                });
-                float x[4], bias[4] = {};
+                    for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = sc[i >> 1][i & 1] + sc[i >> 1][2 + (i & 1)];
+                        for (int n = 0; n < 2; ++n) {
+                            const uint32_t(&q)[4] = qf[c][kt];
+                            if (kt == 0) pa_mma0<BF16>(sc[c][n], q[0], q[1], q[2], q[3], b[2 * n], b[2 * n + 1]);
+                            else pa_mma<BF16>(sc[c][n], q[0], q[1], q[2], q[3], b[2 * n], b[2 * n + 1]);
+                            if (BF16) pa_mma<BF16>(sc[c][n], q3[c][k3][0], 0u, q3[c][k3][1], 0u, b[2 * n], b[2 * n + 1]);
+                        }
+                });
+                float bias[4] = {};
                 if (MASK) {
                     float top = -INFINITY;
 #pragma unroll
@@ -493,68 +517,84 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     if (top > mk) {
-                        m = pa_rel(m, mk, top);
+#pragma unroll
+                        for (int c = 0; c < NC; ++c) m[c] = pa_rel(m[c], mk, top);
                         mk = top;
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) bias[i] = (bias[i] - mk) * 1.44269504f;
                 }
-                float top;
-                if (live == 0xffffu) {
-                    top = fmaxf(fmaxf(fmaf(x[0], f, bias[0]), fmaf(x[1], f, bias[1])),
-                                fmaxf(fmaf(x[2], f, bias[2]), fmaf(x[3], f, bias[3])));
-                } else {
-                    top = -INFINITY;
+                float x[NC][4], top[NC];
+                bool grown = false;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if ((live >> (8 * (i >> 1) + 2 * t4 + (i & 1))) & 1) top = fmaxf(top, fmaf(x[i], f, bias[i]));
+                for (int c = 0; c < NC; ++c) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[c][i] = sc[c][i >> 1][i & 1] + sc[c][i >> 1][2 + (i & 1)];
+                    if (live == 0xffffu) {
+                        top[c] = fmaxf(fmaxf(fmaf(x[c][0], f[c], bias[0]), fmaf(x[c][1], f[c], bias[1])),
+                                       fmaxf(fmaf(x[c][2], f[c], bias[2]), fmaf(x[c][3], f[c], bias[3])));
+                    } else {
+                        top[c] = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if ((live >> (8 * (i >> 1) + 2 * t4 + (i & 1))) & 1)
+                                top[c] = fmaxf(top[c], fmaf(x[c][i], f[c], bias[i]));
+                    }
+                    top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 1));
+                    top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 2));
+                    grown |= top[c] > m[c] + 3.f;  // (at the first unit m is -inf)
                 }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const bool grown = top > m + 3.f;  // (at the first unit m is -inf)
                 if (__any_sync(0xffffffffu, grown)) {
                     flush();
-                    const float mn = grown ? top : m;
-                    const float corr = m == -INFINITY ? 0.f : pa_exp2(m - mn);
-                    l *= corr;
 #pragma unroll
-                    for (int i = 0; i < 2 * KT; ++i) o[i][0] *= corr, o[i][1] *= corr;
-                    m = mn;
+                    for (int c = 0; c < NC; ++c) {
+                        const float mn = top[c] > m[c] + 3.f ? top[c] : m[c];
+                        const float corr = m[c] == -INFINITY ? 0.f : pa_exp2(m[c] - mn);
+                        l[c] *= corr;
+#pragma unroll
+                        for (int i = 0; i < 2 * KT; ++i) o[c][i][0] *= corr, o[c][i][1] *= corr;
+                        m[c] = mn;
+                    }
                 }
-                float w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = pa_exp2(fmaf(x[i], f, bias[i] - m)) * 4096.f;
-                if (live != 0xffffu) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!((live >> (8 * (i >> 1) + 2 * t4 + (i & 1))) & 1)) w[i] = 0.f;
-                }
-                l += (w[0] + w[1]) + (w[2] + w[3]);
                 // O += w V: the pieces of w as they stand are the A operand
-                uint32_t wa[4], w3[2];
-                wa[0] = pa_split<BF16>(w[0], w[1]);
-                wa[1] = pa_split<BF16>(w[0], w[1]);
-                wa[2] = pa_split<BF16>(w[2], w[3]);
-                wa[3] = pa_split<BF16>(w[2], w[3]);
-                if (BF16) w3[0] = pa_split<BF16>(w[0], w[1]), w3[1] = pa_split<BF16>(w[2], w[3]);
+                uint32_t wa[NC][4], w3[NC][2];
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    float w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = pa_exp2(fmaf(x[c][i], f[c], bias[i] - m[c])) * 4096.f;
+                    if (live != 0xffffu) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (!((live >> (8 * (i >> 1) + 2 * t4 + (i & 1))) & 1)) w[i] = 0.f;
+                    }
+                    l[c] += (w[0] + w[1]) + (w[2] + w[3]);
+                    wa[c][0] = pa_split<BF16>(w[0], w[1]);
+                    wa[c][1] = pa_split<BF16>(w[0], w[1]);
+                    wa[c][2] = pa_split<BF16>(w[2], w[3]);
+                    wa[c][3] = pa_split<BF16>(w[2], w[3]);
+                    if (BF16) w3[c][0] = pa_split<BF16>(w[0], w[1]), w3[c][1] = pa_split<BF16>(w[2], w[3]);
+                }
                 unrolled(std::make_index_sequence<KT>{}, [&](auto ic) {
                     constexpr int kt = decltype(ic)::value;
                     uint32_t b[4];
                     pa_ldsm_t_at<kt / 4 * 128>(b, v_at[kt % 4] + st);
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        if (FLUSH > 1) {
-                            float(&d)[4] = acc[(2 * kt + n) % (sizeof(acc) / sizeof(acc[0]))];
-                            pa_mma<BF16>(d, wa[0], wa[1], wa[2], wa[3], b[2 * n], b[2 * n + 1]);
-                            if (BF16) pa_mma<BF16>(d, w3[0], 0u, w3[1], 0u, b[2 * n], b[2 * n + 1]);
-                        } else {
-                            float d[4];
-                            pa_mma0<BF16>(d, wa[0], wa[1], wa[2], wa[3], b[2 * n], b[2 * n + 1]);
-                            if (BF16) pa_mma<BF16>(d, w3[0], 0u, w3[1], 0u, b[2 * n], b[2 * n + 1]);
-                            o[2 * kt + n][0] += d[0] + d[2];
-                            o[2 * kt + n][1] += d[1] + d[3];
+                    for (int c = 0; c < NC; ++c)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            if (FLUSH > 1) {
+                                float(&d)[4] = acc[c][FLUSH > 1 ? 2 * kt + n : 0];
+                                pa_mma<BF16>(d, wa[c][0], wa[c][1], wa[c][2], wa[c][3], b[2 * n], b[2 * n + 1]);
+                                if (BF16) pa_mma<BF16>(d, w3[c][0], 0u, w3[c][1], 0u, b[2 * n], b[2 * n + 1]);
+                            } else {
+                                float d[4];
+                                pa_mma0<BF16>(d, wa[c][0], wa[c][1], wa[c][2], wa[c][3], b[2 * n], b[2 * n + 1]);
+                                if (BF16) pa_mma<BF16>(d, w3[c][0], 0u, w3[c][1], 0u, b[2 * n], b[2 * n + 1]);
+                                o[c][2 * kt + n][0] += d[0] + d[2];
+                                o[c][2 * kt + n][1] += d[1] + d[3];
+                            }
                         }
-                    }
                 });
                 if (FLUSH > 1 && ++pending == FLUSH) flush();
             }
@@ -563,36 +603,39 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
             if (--turns == 0) {
                 const bool seg_end = cur.u + part == cur.nu;
                 flush();
-                l += __shfl_xor_sync(0xffffffffu, l, 1);
-                l += __shfl_xor_sync(0xffffffffu, l, 2);
-                if (seg_end && seg_from >= fb) {  // the whole segment
-                    const int j = cur.chunk * kPaHeads + g;
-                    const float inv = l > 0.f ? 1.f / l : 0.f;
-                    if (j < G) {
-                        float* dst = a.out + ((int64_t)cur.s * a.n_head + cur.head * G + j) * D + 2 * t4;
+                const bool whole = seg_end && seg_from >= fb;
+                float* p = seg_end ? head_piece(warp) : tail_piece(warp);
+                if (!seg_end) {  // the last piece of this warp: its ring is free
+                    pa_wait<0>();
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    l[c] += __shfl_xor_sync(0xffffffffu, l[c], 1);
+                    l[c] += __shfl_xor_sync(0xffffffffu, l[c], 2);
+                    const int r = kPaHeads * c + g, j = cur.chunk * NH + r;
+                    float scale = 1.f;
+                    float* dst = p + r * D;
+                    if (whole) {
+                        scale = l[c] > 0.f ? 1.f / l[c] : 0.f;
+                        dst = a.out + ((int64_t)cur.s * a.n_head + cur.head * G + j) * D;
+                    } else if (t4 == 0) {
+                        p[NH * D + r] = m[c], p[NH * D + NH + r] = l[c];
+                    }
+                    if (!whole || j < G)
 #pragma unroll
                         for (int i = 0; i < 2 * KT; ++i)
-                            *reinterpret_cast<float2*>(dst + 8 * i) = make_float2(o[i][0] * inv, o[i][1] * inv);
-                    }
-                } else {
-                    if (!seg_end) {  // the last piece of this warp: its ring is free
-                        pa_wait<0>();
-                        __syncwarp();
-                    }
-                    float* p = seg_end ? head_piece(warp) : tail_piece(warp);
-#pragma unroll
-                    for (int i = 0; i < 2 * KT; ++i)
-                        *reinterpret_cast<float2*>(p + g * D + 8 * i + 2 * t4) = make_float2(o[i][0], o[i][1]);
-                    if (t4 == 0) p[kPaHeads * D + g] = m, p[kPaHeads * D + kPaHeads + g] = l;
-                    if (lane == 0) {
-                        p[kPaHeads * D + 2 * kPaHeads] = mk;
-                        const int x = seg_end ? 0 : 1;
-                        sh.seg[x][warp] = (cur.s * a.kv.n_head_kv + cur.head) * a.chunks + cur.chunk;
-                        sh.from[x][warp] = seg_from;
-                        sh.nu[x][warp] = cur.nu;
-                        sh.row[x][warp] = cur.s * a.n_head + cur.head * G + cur.chunk * kPaHeads;
-                        sh.rows[x][warp] = min(kPaHeads, G - cur.chunk * kPaHeads);
-                    }
+                            *reinterpret_cast<float2*>(dst + 8 * i + 2 * t4) =
+                                make_float2(o[c][i][0] * scale, o[c][i][1] * scale);
+                }
+                if (!whole && lane == 0) {
+                    p[NH * D + 2 * NH] = mk;
+                    const int x = seg_end ? 0 : 1;
+                    sh.seg[x][warp] = (cur.s * a.kv.n_head_kv + cur.head) * a.chunks + cur.chunk;
+                    sh.from[x][warp] = seg_from;
+                    sh.nu[x][warp] = cur.nu;
+                    sh.row[x][warp] = cur.s * a.n_head + cur.head * G + cur.chunk * NH;
+                    sh.rows[x][warp] = min(NH, G - cur.chunk * NH);
                 }
                 to_do -= part;
                 if (to_do == 0) break;
@@ -616,7 +659,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
     const unsigned starts = __ballot_sync(0xffffffffu, tl >= 0 && tl != prev);
     const unsigned ends = __ballot_sync(0xffffffffu, hd >= 0 && hd == prev);     // head of the tail before
     const unsigned alone = __ballot_sync(0xffffffffu, hd >= 0 && hd != prev);
-    constexpr int AT_M = kPaHeads * D, AT_L = AT_M + kPaHeads, AT_MK = AT_L + kPaHeads, NV = PaJoint<D>::NV;
+    constexpr int AT_M = NH * D, AT_L = AT_M + NH, AT_MK = AT_L + NH, NV = PaJoint<D>::NV;
     const bool masked = MASK, has_col = 4 * lane < D;
     auto put_out = [&](int row, const PaJoint<D>& t) {
         const float inv = t.l > 0.f ? 1.f / t.l : 0.f;
@@ -673,9 +716,9 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
     unsigned got0 = 0, got1 = 0;
     const int my_j = warp + lane * W;
     if (my_j < sh.rows[open0 & 1][open0 >> 1])
-        got0 = atomicAdd(a.tickets + (int64_t)sh.seg[open0 & 1][open0 >> 1] * kPaHeads + my_j, 1u);
+        got0 = atomicAdd(a.tickets + (int64_t)sh.seg[open0 & 1][open0 >> 1] * NH + my_j, 1u);
     if (open1 >= 0 && my_j < sh.rows[open1 & 1][open1 >> 1])
-        got1 = atomicAdd(a.tickets + (int64_t)sh.seg[open1 & 1][open1 >> 1] * kPaHeads + my_j, 1u);
+        got1 = atomicAdd(a.tickets + (int64_t)sh.seg[open1 & 1][open1 >> 1] * NH + my_j, 1u);
     __threadfence();
 #pragma unroll 1
     for (int i = 0; i < 2; ++i) {
@@ -688,15 +731,15 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
 #pragma unroll 1
         for (int j = warp, x = 0; j < rows; j += W, ++x) {
             if (__shfl_sync(0xffffffffu, i ? got1 : got0, x) != (unsigned)(n - 1)) continue;
-            // 32 pieces at a time into this warp's ring, behind its tail piece
+            // up to 32 pieces at a time into this warp's ring, behind its tail piece
             // (which other warps may still be reading)
             const uint32_t buf = smem_u32(tail_piece(warp)) + (uint32_t)align256(PIECE * 4);
-            static_assert(32 * D * 4 + PIECE * 4 + 256 <= S * 2 * TILE, "32 rows of a head in a warp's ring");
+            constexpr int ROOM = (S * 2 * TILE - PIECE * 4 - 256) / (4 * D), BATCH = ROOM < 32 ? ROOM : 32;
             PaJoint<D> t;
             t.clear();
 #pragma unroll 1
-            for (int c = 0; c < n; c += 32) {
-                const int here = min(32, n - c);
+            for (int c = 0; c < n; c += BATCH) {
+                const int here = min(BATCH, n - c);
                 float pm = -INFINITY, pl = 0.f, pk = -INFINITY;
 #pragma unroll 4
                 for (int k = 0; k < here; ++k)
@@ -714,7 +757,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_attn_kernel(PagedAt
                 __syncwarp();
             }
             put_out(sh.row[at & 1][at >> 1] + j, t);
-            if (lane == 0) a.tickets[(int64_t)sh.seg[at & 1][at >> 1] * kPaHeads + j] = 0u;
+            if (lane == 0) a.tickets[(int64_t)sh.seg[at & 1][at >> 1] * NH + j] = 0u;
         }
     }
 }

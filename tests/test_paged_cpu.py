@@ -9,6 +9,10 @@ import torch
 
 import paged_ref as R
 
+# A call that is not refused would use the made-up addresses: never where there
+# is a device to use them.
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses must not reach a device")
+
 PTR = 4096  # an aligned address nothing reads
 
 
@@ -49,8 +53,10 @@ def test_plan_refuses_more_sequences_than_it_scans():
 BAD_KV = [dict(k=None), dict(v=None), dict(n_head_kv=0), dict(page_size=0), dict(n_pages=0), dict(k=PTR + 8),
           dict(v=PTR + 2), dict(k_page=8), dict(k_row=520), dict(k_head=2), dict(v_page=-16), dict(v_row=264),
           dict(v_head=8), dict(k_lo=None), dict(k_hi=None), dict(k_lo=PTR + 8), dict(k_hi=PTR + 4),
-          dict(page_size=1 << 20, n_pages=1 << 12), dict(k_page=1 << 36), dict(v_row=1 << 40)]
-UNSUPPORTED_KV = [dict(type=0), dict(type=2), dict(type=99), dict(head_dim=96), dict(head_dim=512), dict(head_dim=0)]
+          dict(page_size=1 << 20, n_pages=1 << 12)]
+UNSUPPORTED_KV = [dict(type=0), dict(type=2), dict(type=99), dict(head_dim=96), dict(head_dim=512), dict(head_dim=0),
+                  dict(k_page=1 << 36), dict(v_row=1 << 40), dict(k_page=1 << 34), dict(v_page=1 << 34),
+                  dict(v_head=1 << 36), dict(n_pages=1 << 26, k_page=1 << 10)]
 
 
 def calls(kv):
