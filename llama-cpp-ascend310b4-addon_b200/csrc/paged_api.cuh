@@ -322,6 +322,10 @@ int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, i
     a.n_head = n_head;
     a.n_sel = n_sel;
     a.max_blocks = max_blocks;
+    a.group = n_head / kv->n_head_kv;
+    a.unit_blocks = kPaTok / kv->page_size;
+    a.unit_rows = kPaTok % kv->page_size;
+    a.aligned = kv->page_size % kPaTok == 0;
     a.same_rows = kv->k_page == kv->v_page && kv->k_row == kv->v_row;
     a.near_rows = std::max(kv->k_row, kv->v_row) < ((int64_t)1 << 31) / kPaTok;
     return kv->type == B200_TYPE_BF16 ? launch_paged_attn<true>(a, (cudaStream_t)stream)

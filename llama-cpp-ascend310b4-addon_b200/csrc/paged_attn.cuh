@@ -88,6 +88,8 @@ struct PagedAttnArgs {
     unsigned int* tickets;  // [n_seq * n_head_kv * chunks][8 NC], zero between calls
     float scale;
     int n_seq, n_head, n_sel, max_blocks, chunks;
+    int group;              // query heads per KV head
+    int unit_blocks, unit_rows, aligned;  // 16 / page_size, 16 % page_size, page_size % 16 == 0
     int near_rows;          // 16 rows of a page span less than 2^31 bytes
     int same_rows;          // K and V have the same page and row strides
 };
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t4 = lane & 3;
-    const int ps = a.kv.page_size, G = a.n_head / a.kv.n_head_kv;
+    const int ps = a.kv.page_size, G = a.group;
     const int hh_n = a.kv.n_head_kv * a.chunks;
 
     if (tid < W) sh.seg[0][tid] = -1, sh.seg[1][tid] = -1;
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
         in.nu = pa_units(a, in.len);
         const int hh0 = (fb - range.base0) / in.nu;
         in.u = (fb - range.base0) - hh0 * in.nu;
-        in.head = hh0 / a.chunks;
+        in.head = a.chunks == 1 ? hh0 : hh0 / a.chunks;
         in.chunk = hh0 - in.head * a.chunks;
         cur = in;
         int seg_from = fb - in.u;  // first unit of the current segment
@@ -256,8 +258,8 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
         };
 
         // ---- producer: this lane looks after token lane & 15 of a unit ----
-        const int q16 = kPaTok / ps, r16 = kPaTok % ps;
-        const bool aligned = ps % kPaTok == 0;  // a unit lies in one page
+        const int q16 = a.unit_blocks, r16 = a.unit_rows;  // 16 = q16 ps + r16
+        const bool aligned = a.aligned != 0;               // a unit lies in one page
         const uint32_t lc = lane % LPR, lr = lane / LPR;  // this lane's 16 bytes of a row, its row of a copy
         // Offsets of pages and rows in 16-byte steps, in 32 bits: K and V span less
         // than 64 GiB each.  A unit of one page is copied at fixed steps from its

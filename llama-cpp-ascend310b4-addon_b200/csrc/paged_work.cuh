@@ -113,8 +113,9 @@ struct PaRangeShared {
 // The units of all sequences (units(s) for each of `segs` segments of sequence
 // s), in order, cut into equal ranges: [cb, ce) for this CTA, and that one
 // into [fb, fe) for this warp, which starts in sequence seq0, whose first unit
-// is base0.  Every CTA sums up the lengths for itself: up to 32 in each warp,
-// more across the CTA.  All threads call it; it ends with a CTA barrier.
+// is base0.  Every CTA sums up the lengths for itself: up to 128 in each warp
+// without a barrier, more across the CTA.  All threads call it; it ends with a
+// CTA barrier.
 template <int W>
 struct PaRange {
     int per_cta, cb, ce, fb, fe, seq0, base0;
@@ -122,9 +123,10 @@ struct PaRange {
     template <class U>
     __device__ __forceinline__ PaRange(PaRangeShared<W>& sh, int n_seq, int segs, U units) {
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-        const bool few = n_seq <= 32;
-        const int per = few ? 1 : (n_seq + 32 * W - 1) / (32 * W);
-        const int s_lo = min(n_seq, (few ? lane : tid) * per), s_hi = min(n_seq, s_lo + per);
+        const bool few = n_seq <= 128;
+        const int at = few ? lane : tid;
+        const int per = few ? (n_seq + 31) >> 5 : (n_seq + 32 * W - 1) / (32 * W);
+        const int s_lo = min(n_seq, at * per), s_hi = min(n_seq, s_lo + per);
         int mine = 0;
         for (int s = s_lo; s < s_hi; ++s) mine += units(s);
         int incl = mine;
@@ -155,9 +157,19 @@ struct PaRange {
         fb = min(ce, cb + per_warp * warp);
         fe = min(ce, fb + per_warp);
         if (few) {
-            const unsigned at = __ballot_sync(0xffffffffu, fb >= before && fb < before + mine * segs);
-            seq0 = at ? __ffs(at) - 1 : 0;
-            base0 = __shfl_sync(0xffffffffu, before, seq0);
+            const unsigned owner = __ballot_sync(0xffffffffu, fb >= before && fb < before + mine * segs);
+            seq0 = s_lo;
+            for (int s = s_lo; s < s_hi; ++s) {  // (no more than one owner, whose answer counts)
+                const int end = before + units(s) * segs;
+                if (fb < end) {
+                    seq0 = s;
+                    break;
+                }
+                before = end;
+            }
+            const int src = owner ? __ffs(owner) - 1 : 0;
+            seq0 = __shfl_sync(0xffffffffu, seq0, src);
+            base0 = __shfl_sync(0xffffffffu, before, src);
             __syncthreads();
         } else {
             for (int s = s_lo; s < s_hi; ++s) {
