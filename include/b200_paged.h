@@ -135,12 +135,15 @@ int b200_paged_select(const b200_paged_kv *kv, const float *q, int64_t q_stride,
  *   mask  f16, additive, row s at mask + s * mask_stride (elements), at least
  *         max_blocks * page_size entries, or NULL; finite or -inf.  Positions
  *         at -inf are left out whatever their key and value hold.
- *   out   f32 [n_seq][n_head][head_dim], 16-byte aligned; a sequence with no
- *         position gets zeros
+ *   out   f32 [n_seq][n_head][head_dim], 16-byte aligned, apart from q; a
+ *         sequence with no position gets zeros
+ * At most 2^30 units of 16 positions of a (sequence, KV head, 8 or 16 query
+ * heads) a call, counted at the table's width (B200_EUNSUPPORTED).
  * Products of K and V with q and w run on tensor cores; q and w enter as sums
  * of 16-bit parts (two of f16, three of bf16) that keep 22 bits of each.
  * The workspace must be zero-filled before its first use; every call leaves
- * it ready for the next.  Calls that share one must not overlap on the GPU. */
+ * it ready for the next, of any shape.  Calls that share one must not overlap
+ * on the GPU, and nothing else (b200_paged_select among it) may write to it. */
 size_t b200_paged_attn_workspace_size(int head_dim, int n_seq, int n_head, int n_head_kv);
 int b200_paged_attn(const b200_paged_kv *kv, const float *q, int64_t q_stride, int n_seq, int n_head,
                     const int32_t *block_table, int64_t table_stride, int max_blocks, const int32_t *seq_lens,

@@ -170,10 +170,6 @@ int paged_chunks(int head_dim, int n_head, int n_head_kv) {
     const int heads = paged_heads(head_dim, n_head, n_head_kv);
     return (n_head / n_head_kv + heads - 1) / heads;
 }
-size_t paged_pieces_bytes(int head_dim, int n_head, int n_head_kv) {
-    return align256((size_t)kPaCtas * 2 * pa_piece(head_dim, pa_groups(head_dim, n_head / n_head_kv)) * sizeof(float));
-}
-
 }  // namespace
 
 extern "C" {
@@ -247,7 +243,7 @@ int b200_paged_select(const b200_paged_kv* kv, const float* q, int64_t q_stride,
     CR_(check_paged_batch(kv, q, q_stride, n_seq, n_head, block_table, table_stride, max_blocks, seq_lens));
     if (!kv->k_lo || !sel || n_sel <= 0 || !workspace || !aligned16(workspace)) return B200_EINVAL;
     if (max_blocks > B200_PAGED_SELECT_MAX_BLOCKS) return B200_EUNSUPPORTED;
-    if ((int64_t)n_seq * kv->n_head_kv * paged_units(max_blocks) > INT32_MAX) return B200_EUNSUPPORTED;
+    if ((int64_t)n_seq * kv->n_head_kv * paged_units(max_blocks) > INT32_MAX / 2) return B200_EUNSUPPORTED;
     if (workspace_size < b200_paged_select_workspace_size(n_seq, kv->n_head_kv, max_blocks)) return B200_EINVAL;
     PagedSelectArgs a;
     a.lo = static_cast<const uint16_t*>(kv->k_lo);
@@ -282,7 +278,7 @@ size_t b200_paged_attn_workspace_size(int head_dim, int n_seq, int n_head, int n
     if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || n_seq < 0 || n_seq > 65535 || n_head <= 0 ||
         n_head > 65535 || n_head_kv <= 0 || n_head % n_head_kv)
         return 0;
-    return paged_pieces_bytes(head_dim, n_head, n_head_kv) +
+    return pa_piece_area() +
            align256((size_t)n_seq * n_head_kv * paged_chunks(head_dim, n_head, n_head_kv) *
                     paged_heads(head_dim, n_head, n_head_kv) * sizeof(unsigned int));
 }
@@ -297,12 +293,12 @@ int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, i
     if (!out || !aligned16(out) || !workspace || !aligned16(workspace) || (sel && n_sel <= 0) ||
         (reinterpret_cast<uintptr_t>(mask) & 1) ||
         (mask && n_seq > 1 && mask_stride < (int64_t)max_blocks * kv->page_size) ||
-        (sel && n_sel > INT32_MAX / kv->page_size) ||
+        (sel && n_sel > (INT32_MAX - 4096) / kv->page_size) ||
         workspace_size < b200_paged_attn_workspace_size(kv->head_dim, n_seq, n_head, kv->n_head_kv))
         return B200_EINVAL;
     const int64_t width = (int64_t)(sel ? n_sel : max_blocks) * kv->page_size;
     const int64_t segments = (int64_t)n_seq * kv->n_head_kv * paged_chunks(kv->head_dim, n_head, kv->n_head_kv);
-    if (segments * ((width + kPaTok - 1) / kPaTok) > INT32_MAX) return B200_EUNSUPPORTED;  // units are counted in int
+    if (segments * ((width + kPaTok - 1) / kPaTok) > INT32_MAX / 2) return B200_EUNSUPPORTED;  // units are counted in int
     PagedAttnArgs a;
     a.kv = *kv;
     a.q = q;
@@ -316,7 +312,7 @@ int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, i
     a.out = out;
     a.chunks = paged_chunks(kv->head_dim, n_head, kv->n_head_kv);
     a.pieces = static_cast<float*>(workspace);
-    a.tickets = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(workspace) + paged_pieces_bytes(kv->head_dim, n_head, kv->n_head_kv));
+    a.tickets = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(workspace) + pa_piece_area());
     a.scale = scale;
     a.n_seq = n_seq;
     a.n_head = n_head;

@@ -54,6 +54,14 @@ B200_HD constexpr int pa_warps(int D, int NC = 1) {
 B200_HD constexpr int pa_stages(int D, int NC = 1) { return NC == 2 ? (D == 64 ? 5 : 3) : D == 64 ? 4 : 3; }
 // Floats of one piece: o [8 NC][D], m [8 NC], l [8 NC], mask reference.
 B200_HD constexpr int pa_piece(int D, int NC = 1) { return kPaHeads * NC * (D + 2) + 4; }
+// Bytes of the workspace's piece area, the same for every shape: the tickets
+// behind it are zero whatever shapes used the workspace before.
+B200_HD constexpr size_t pa_piece_area() {
+    int most = pa_piece(256);
+    for (int D = 64; D <= 128; D *= 2)
+        if (pa_piece(D, 2) > most) most = pa_piece(D, 2);
+    return ((size_t)kPaCtas * 2 * most * sizeof(float) + 255) & ~(size_t)255;
+}
 B200_HD constexpr int pa_tile(int D) { return kPaTok * D * 2; }
 
 // Bookkeeping beside the ring and the pieces in shared memory.

@@ -262,6 +262,83 @@ def test_select_matches_reference(lens, page_size, heads, d, n_sel, dtype):
     np.testing.assert_array_equal(run_select(c, q, page_size, n_sel, dtype).cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,n_sel", [(8193, 500), (8194, 8100), (20001, 64), (3000, 1), (1025, 1024), (1026, 512)])
+def test_select_many_blocks(n, n_sel, dtype):
+    """More blocks than a CTA's threads hold at once, and around that number."""
+    r = rng(n + n_sel)
+    c, q = select_inputs(r, [n, n // 3], 1, 4, 2, 64, dtype)
+    lo, hi = R.bounds_of(c)
+    want = R.select_ref(q, lo, hi, c["table"], c["lens"], 1, n_sel)
+    np.testing.assert_array_equal(run_select(c, q, 1, n_sel, dtype).cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("n", [300, 2000, 9000])
+@pytest.mark.parametrize("kinds", [1, 2, 5])
+def test_select_crowds_of_equal_scores(n, kinds):
+    """Hundreds of blocks with the same keys: nothing but the 64-bit order and
+    the lower block decide."""
+    r = rng(n + kinds)
+    c = R.make_cache(r, [n], 1, 1, 64, "bf16")
+    few = R.rounded(r.standard_normal((kinds, 1, 64)), "bf16")
+    for b in range(n):
+        c["k"][c["table"][0, b], 0] = few[r.integers(kinds)]
+    q = r.standard_normal((1, 2, 64)).astype(np.float32)
+    lo, hi = R.bounds_of(c)
+    for n_sel in (2, n // 4, n // 2, n - 1):
+        want = R.select_ref(q, lo, hi, c["table"], c["lens"], 1, n_sel)
+        np.testing.assert_array_equal(run_select(c, q, 1, n_sel, "bf16").cpu().numpy(), want)
+
+
+def test_select_scores_that_differ_in_the_last_bits():
+    """Keys that differ by one step of their type in one channel: scores that
+    agree to six digits, in an order that 32 bits would not find."""
+    r = rng(14)
+    for dtype, step in (("f16", 2.0 ** -10), ("bf16", 2.0 ** -7)):
+        n = 600
+        c = R.make_cache(r, [n], 1, 1, 128, dtype)
+        base = R.rounded(1 + r.random(128) * 0.9, dtype)
+        for b in range(n):
+            row = base.copy()
+            row[r.integers(128)] -= step * int(r.integers(0, 3))
+            c["k"][c["table"][0, b], 0, 0] = row
+        q = r.standard_normal((1, 3, 128)).astype(np.float32)
+        q[:, :, ::7] *= 1e-4
+        lo, hi = R.bounds_of(c)
+        for n_sel in (10, 300):
+            want = R.select_ref(q, lo, hi, c["table"], c["lens"], 1, n_sel)
+            np.testing.assert_array_equal(run_select(c, q, 1, n_sel, dtype).cpu().numpy(), want)
+
+
+def test_select_not_finite():
+    """Infinite bounds rank first, NaN queries leave the lower blocks."""
+    r = rng(15)
+    c, q = select_inputs(r, [500], 1, 2, 1, 64, "f16")
+    q = np.abs(q) + 0.1
+    for b in (7, 300, 450):
+        c["k"][c["table"][0, b], 0, 0, 3] = np.inf
+    lo, hi = R.bounds_of(c)
+    want = R.select_ref(q, lo, hi, c["table"], c["lens"], 1, 6)
+    got = run_select(c, q, 1, 6, "f16").cpu().numpy()
+    np.testing.assert_array_equal(got, want)
+    assert set((7, 300, 450)) <= set(got[0, 0].tolist())
+    q[:] = np.nan
+    np.testing.assert_array_equal(run_select(c, q, 1, 6, "f16").cpu().numpy()[0, 0], [0, 1, 2, 3, 4, 499])
+
+
+@pytest.mark.parametrize("n_seq", [31, 33, 129, 400])
+def test_select_and_attn_of_many_sequences(n_seq):
+    r = rng(n_seq)
+    lens = [int(v) for v in r.integers(0, 60, n_seq)]
+    lens[0], lens[-1], lens[n_seq // 2] = 0, 0, 333
+    c, q = select_inputs(r, lens, 4, 6, 2, 64, "f16")
+    lo, hi = R.bounds_of(c)
+    want = R.select_ref(q, lo, hi, c["table"], c["lens"], 4, 5)
+    np.testing.assert_array_equal(run_select(c, q, 4, 5, "f16").cpu().numpy(), want)
+    check_attn(c, q, 4, "f16", 0.125)
+    check_attn(c, q, 4, "f16", 0.125, sel=want)
+
+
 @pytest.mark.parametrize("n_sel", [1, 2, 50, 66, 67, 99, 100, 101])
 def test_select_ties_take_the_lower_block(n_sel):
     r = rng(11)
@@ -398,6 +475,108 @@ def test_attn_selected_blocks(lens, page_size, hq, hkv, d, n_sel, dtype):
     check_attn(c, q, page_size, dtype, d ** -0.5, sel=sel)
     mask = make_mask(r, "holes", len(lens), c["table"].shape[1] * page_size)
     check_attn(c, q, page_size, dtype, d ** -0.5, sel=sel, mask=mask)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d,length,page_size", [(4, 1, 128, 30000, 16), (12, 1, 64, 50000, 48),
+                                                       (20, 1, 128, 9000, 16), (3, 1, 256, 20000, 100)])
+def test_attn_one_segment_over_every_cta(hq, hkv, d, length, page_size, dtype):
+    """A long sequence of one KV head: over a hundred pieces to join."""
+    r = rng(length + hq)
+    c = R.make_cache(r, [length], page_size, hkv, d, dtype)
+    q = r.standard_normal((1, hq, d)).astype(np.float32) * 2
+    check_attn(c, q, page_size, dtype, d ** -0.5)
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 1), (14, 2), (16, 1), (17, 1), (33, 1)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attn_group_sizes(hq, hkv, d):
+    r = rng(hq * d)
+    lens = [200, 3, 0, 90]
+    c = R.make_cache(r, lens, 16, hkv, d, "f16")
+    q = r.standard_normal((len(lens), hq, d)).astype(np.float32) * 2
+    mask = make_mask(r, "holes", len(lens), c["table"].shape[1] * 16)
+    check_attn(c, q, 16, "f16", d ** -0.5)
+    check_attn(c, q, 16, "f16", d ** -0.5, mask=mask)
+
+
+def test_attn_keys_and_values_in_different_layouts():
+    r = rng(44)
+    c = R.make_cache(r, [100, 37], 16, 2, 128, "f16")
+    q = r.standard_normal((2, 8, 128)).astype(np.float32)
+    for a, b in (("token", "head"), ("head", "gap"), ("gap", "token")):
+        cache = B().PagedKV(R.to_device(c, "f16", a)[0], R.to_device(c, "f16", b)[1])
+        got = B().paged_attn(cache, dev(q), i32(c["table"]), i32(c["lens"]), 0.1).cpu().numpy()
+        want, tol = R.attn_ref(c, q, 16, 0.1)
+        assert (np.abs(got - want) <= tol).all(), (a, b)
+
+
+def test_attn_one_workspace_for_all_shapes():
+    """Calls of other head dims, groups, batches and masks in between leave a
+    workspace ready for the next."""
+    bw = B()
+    r = rng(52)
+    ws = torch.zeros(4 << 20, dtype=torch.uint8, device="cuda")
+    for hq, hkv, d, n in ((3, 3, 256, 2), (4, 2, 64, 300), (12, 1, 128, 3), (64, 8, 128, 5), (1, 1, 256, 40), (14, 1, 64, 7),
+                          (8, 8, 64, 64), (3, 3, 256, 2)):
+        lens = [int(v) for v in r.integers(0, 9000 // n + 200, n)]
+        c = R.make_cache(r, lens, 16, hkv, d, "f16")
+        q = r.standard_normal((n, hq, d)).astype(np.float32)
+        assert ws.numel() >= bw.paged_attn_workspace_size(d, n, hq, hkv)
+        check_attn(c, q, 16, "f16", d ** -0.5, workspace=ws)
+
+
+def test_empty_batch_and_no_tokens():
+    bw = B()
+    k = torch.zeros((4, 16, 2, 64), dtype=torch.float16, device="cuda")
+    b = torch.zeros((4, 2, 64), dtype=torch.float16, device="cuda")
+    cache = bw.PagedKV(k, k.clone(), b, b.clone())
+    q = torch.zeros((0, 4, 64), device="cuda")
+    table, lens = torch.zeros((0, 3), dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")
+    assert bw.paged_attn(cache, q, table, lens, 1.0).shape == (0, 4, 64)
+    assert bw.paged_select(cache, q, table, lens, 2).shape == (0, 2, 2)
+    x = torch.zeros((0, 2, 64), device="cuda")
+    bw.paged_store(cache, x, x, torch.zeros(0, dtype=torch.int64, device="cuda"))
+    assert (cache.k == 0).all()
+
+
+FIRST_CALL = """
+import sys
+sys.path[:0] = {path!r}
+import torch, b200_decode as B
+k = torch.randn((8, 16, 2, 128), device="cuda").half()
+cache = B.PagedKV(k, k.clone(), k.amin(1).contiguous(), k.amax(1).contiguous())
+i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+table, lens, n_free, free, new = i32([[0, 1, 2, -1]]), i32([40]), i32([3]), i32([5, 6, 7, 0, 0, 0, 0, 0]), i32([3])
+x, q = torch.randn((3, 2, 128), device="cuda"), torch.randn((1, 4, 128), device="cuda")
+ws = torch.zeros(B.paged_attn_workspace_size(128, 1, 4, 2), dtype=torch.uint8, device="cuda")
+out_lens, out_free = i32([0]), i32([0])
+def step():
+    p = B.paged_plan(new, lens, table, free, n_free, 16, 3, seq_lens_out=out_lens, n_free_out=out_free)
+    B.paged_store(cache, x, x, p.slots)
+    sel = B.paged_select(cache, q, table, p.seq_lens, 2)
+    return B.paged_attn(cache, q, table, p.seq_lens, 0.1, workspace=ws), \
+        B.paged_attn(cache, q, table, p.seq_lens, 0.1, sel=sel)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+g.replay()
+want = step()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) and a.abs().sum() > 0 for a, b in zip(got, want))
+assert int(out_lens.item()) == 43 and B.device_status() == 0
+print("captured")
+"""
+
+
+def test_first_calls_of_a_process_can_be_captured():
+    import os
+    import subprocess
+    import sys
+
+    here = os.path.dirname(os.path.abspath(B().__file__))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL.format(path=[here])], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
 
 
 def test_attn_selected_blocks_any_order_repeats_and_gaps():
