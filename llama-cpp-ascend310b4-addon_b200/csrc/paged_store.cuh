@@ -35,8 +35,8 @@ struct PagedStoreArgs {
     int64_t n_tokens;
 };
 
-constexpr int kStoreThreads = 256;
-constexpr int kStoreTile = 32;  // tokens whose runs one CTA looks for, at most
+constexpr int kStoreThreads = 128;
+constexpr int kStoreTile = 64;  // tokens whose runs one CTA looks for, at most
 constexpr int kStoreRows = 2;   // rows a thread has in flight
 
 // CTA (tile of `tile` tokens, head): the runs of tokens of one page that begin
@@ -45,7 +45,7 @@ constexpr int kStoreRows = 2;   // rows a thread has in flight
 // row; a page's bounds are theirs alone, so they meet in shared memory once per
 // run, without atomics.  Bound by memory: 12 bytes per element.
 template <bool BF16, int D>
-__global__ void __launch_bounds__(kStoreThreads, 4) paged_store_kernel(PagedStoreArgs a, int tile) {
+__global__ void __launch_bounds__(kStoreThreads, 6) paged_store_kernel(PagedStoreArgs a, int tile) {
     constexpr int LPR = D / 8;                // lanes per row, 8 values each
     constexpr int RPP = kStoreThreads / LPR;  // rows per pass
     constexpr int W = kStoreThreads / 32;
@@ -56,15 +56,16 @@ __global__ void __launch_bounds__(kStoreThreads, 4) paged_store_kernel(PagedStor
     auto slot_of = [&](int64_t t) -> int64_t { return t >= 0 && t < a.n_tokens ? a.slots[t] : -1; };
     auto page_of = [&](int64_t s) -> int { return s >= 0 && s < n_slots ? (int)((unsigned)s / (unsigned)ps) : -1; };
     const int64_t first = (int64_t)blockIdx.x * tile;
-    unsigned starts;
-    {
-        const int64_t s = lane < tile ? slot_of(first + lane) : -1;
+    unsigned long long starts = 0;
+    for (int base = 0; base < tile; base += 32) {
+        const int x = base + lane;
+        const int64_t s = x < tile ? slot_of(first + x) : -1;
         if (s >= n_slots) record_status(B200_DEVSTATUS_BOUNDS);
-        const int page = page_of(s), before = page_of(slot_of(first + lane - 1));
-        starts = __ballot_sync(0xffffffffu, page >= 0 && page != before);
+        const int page = page_of(s), before = page_of(slot_of(first + x - 1));
+        starts |= (unsigned long long)__ballot_sync(0xffffffffu, page >= 0 && page != before) << base;
     }
     for (; starts != 0; starts &= starts - 1) {
-        const int64_t t0 = first + __ffs(starts) - 1;
+        const int64_t t0 = first + __ffsll(starts) - 1;
         const int page = page_of(slot_of(t0));
         float lo[8], hi[8];
 #pragma unroll
