@@ -501,7 +501,11 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
                     __syncwarp();
                 }
                 // S = q K^T: 8 heads (high parts, low parts) x 16 positions
-                float sc[NC][2][4];
+                // Chains of at most 4 k steps, added up outside the tensor core, which
+                // truncates every addition; bf16's third parts in a chain of their
+                // own, where what is truncated is 2^-16 as large.
+                constexpr int CHAINS = (KT + 3) / 4;
+                float sc[NC][2][CHAINS][4], s3[NC][2][4];
                 unrolled(std::make_index_sequence<KT>{}, [&](auto ic) {
                     constexpr int kt = decltype(ic)::value, k3 = BF16 ? kt : 0;
                     uint32_t b[4];
@@ -511,9 +515,14 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
 #pragma unroll
                         for (int n = 0; n < 2; ++n) {
                             const uint32_t(&q)[4] = qf[c][kt];
-                            if (kt == 0) pa_mma0<BF16>(sc[c][n], q[0], q[1], q[2], q[3], b[2 * n], b[2 * n + 1]);
-                            else pa_mma<BF16>(sc[c][n], q[0], q[1], q[2], q[3], b[2 * n], b[2 * n + 1]);
-                            if (BF16) pa_mma<BF16>(sc[c][n], q3[c][k3][0], 0u, q3[c][k3][1], 0u, b[2 * n], b[2 * n + 1]);
+                            float(&d)[4] = sc[c][n][kt / 4];
+                            if (kt % 4 == 0) pa_mma0<BF16>(d, q[0], q[1], q[2], q[3], b[2 * n], b[2 * n + 1]);
+                            else pa_mma<BF16>(d, q[0], q[1], q[2], q[3], b[2 * n], b[2 * n + 1]);
+                            if (BF16) {
+                                const uint32_t(&r)[2] = q3[c][k3];
+                                if (kt == 0) pa_mma0<BF16>(s3[c][n], r[0], 0u, r[1], 0u, b[2 * n], b[2 * n + 1]);
+                                else pa_mma<BF16>(s3[c][n], r[0], 0u, r[1], 0u, b[2 * n], b[2 * n + 1]);
+                            }
                         }
                 });
                 float bias[4] = {};
@@ -539,7 +548,15 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[c][i] = sc[c][i >> 1][i & 1] + sc[c][i >> 1][2 + (i & 1)];
+                    for (int i = 0; i < 4; ++i) {
+                        float lows = BF16 ? s3[c][i >> 1][i & 1] : 0.f, highs = 0.f;
+#pragma unroll
+                        for (int y = 0; y < CHAINS; ++y) {
+                            highs += sc[c][i >> 1][y][i & 1];
+                            lows += sc[c][i >> 1][y][2 + (i & 1)];
+                        }
+                        x[c][i] = highs + lows;
+                    }
                     if (live == 0xffffu) {
                         top[c] = fmaxf(fmaxf(fmaf(x[c][0], f[c], bias[0]), fmaf(x[c][1], f[c], bias[1])),
                                        fmaxf(fmaf(x[c][2], f[c], bias[2]), fmaf(x[c][3], f[c], bias[3])));
