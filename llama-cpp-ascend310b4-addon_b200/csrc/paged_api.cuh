@@ -244,6 +244,7 @@ int b200_paged_select(const b200_paged_kv* kv, const float* q, int64_t q_stride,
     if (!kv->k_lo || !sel || n_sel <= 0 || !workspace || !aligned16(workspace)) return B200_EINVAL;
     if (max_blocks > B200_PAGED_SELECT_MAX_BLOCKS) return B200_EUNSUPPORTED;
     if ((int64_t)n_seq * kv->n_head_kv * paged_units(max_blocks) > INT32_MAX / 2) return B200_EUNSUPPORTED;
+    if (kv->n_pages > ((int64_t)1 << 35) / kv->n_head_kv / kv->head_dim) return B200_EUNSUPPORTED;  // bounds below 64 GiB
     if (workspace_size < b200_paged_select_workspace_size(n_seq, kv->n_head_kv, max_blocks)) return B200_EINVAL;
     PagedSelectArgs a;
     a.lo = static_cast<const uint16_t*>(kv->k_lo);

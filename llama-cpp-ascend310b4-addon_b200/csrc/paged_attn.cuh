@@ -32,8 +32,6 @@
 // outside the tensor core, which truncates its own.
 #pragma once
 
-#include <utility>
-
 #include "../../include/b200_paged.h"
 #include "args.h"
 #include "common.cuh"
@@ -102,12 +100,6 @@ struct PagedAttnArgs {
     int same_rows;          // K and V have the same page and row strides
 };
 
-// f(integral_constant<I>) for I of the sequence.
-template <size_t... I, class F>
-__device__ __forceinline__ void unrolled(std::index_sequence<I...>, F f) {
-    (f(std::integral_constant<int, (int)I>{}), ...);
-}
-
 // Where a warp is in its range: unit u of nu of the segment (s, head, chunk).
 struct PaCursor {
     int s, head, chunk, u, nu, len;
@@ -149,15 +141,6 @@ __device__ __forceinline__ float4 pa_lds4(uint32_t addr) {
                  : "r"(addr)
                  : "memory");
     return v;
-}
-
-// p + I * step in one instruction.
-template <int I>
-__device__ __forceinline__ const uint8_t* pa_step(const uint8_t* p, uint32_t step) {
-    if (I == 0) return p;
-    uint64_t r;
-    asm("mad.wide.u32 %0, %1, %2, %3;" : "=l"(r) : "r"(step), "n"(I), "l"(p));
-    return reinterpret_cast<const uint8_t*>(r);
 }
 
 // One head of a segment being joined by one warp: the unnormalised values of

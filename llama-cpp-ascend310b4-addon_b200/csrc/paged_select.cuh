@@ -112,7 +112,13 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_score_kernel(PagedS
     int to_issue = range.fe - range.fb, to_do = to_issue;
 
     // producer: lane & 15 looks after one block of the unit; the pages of the
-    // unit after it are on their way
+    // unit after it are on their way.  Offsets in 16-byte steps, in 32 bits.
+    const uint32_t lc = lane % LPR, lr = lane / LPR;
+    constexpr int SW = 8 / RPI;  // the swizzle repeats after 8 rows
+    uint32_t dst_of[SW];
+#pragma unroll
+    for (int i = 0; i < SW; ++i) dst_of[i] = ring + lr * RB + ((lc ^ ((i * RPI + lr) & 7)) << 4);
+    const uint8_t *hi = reinterpret_cast<const uint8_t*>(a.hi + 8 * lc), *lo = reinterpret_cast<const uint8_t*>(a.lo + 8 * lc);
     auto page_of = [&](const Cursor& c) -> int {
         const int b = kPaTok * c.u + (lane & 15);
         return b < c.nb ? a.table[c.s * a.table_stride + b] : -1;
@@ -120,9 +126,10 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_score_kernel(PagedS
     int page_next = page_of(in);
     auto issue = [&](int stage) {
         if (to_issue > 0) {
-            const int page = page_next, head = in.head;
+            const int page = page_next;
             const bool ok = (unsigned)page < (unsigned)a.n_pages;
             if (!ok && kPaTok * in.u + (lane & 15) < in.nb) record_status(B200_DEVSTATUS_BOUNDS);
+            const uint32_t row = ok ? ((uint32_t)page * H + in.head) * LPR : 0u;
             --to_issue;
             if (to_issue > 0) {
                 if (advance(in)) page_next = page_of(in);
@@ -130,27 +137,35 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_score_kernel(PagedS
             }
             const unsigned valid = __ballot_sync(0xffffffffu, ok) & 0xffffu;
             if (lane == 0) sh.valid[warp][stage] = valid;
-            const uint32_t st = ring + stage * (2 * TILE), c = lane % LPR;
-#pragma unroll
-            for (int i = 0; i < kPaTok / RPI; ++i) {
-                const int r = i * RPI + lane / LPR;
-                const bool on = (valid >> r) & 1;
-                const int p = __shfl_sync(0xffffffffu, page, r);
-                const int64_t at = on ? ((int64_t)p * H + head) * D + 8 * c : 0;
-                const uint32_t d = st + r * RB + ((c ^ (r & 7)) << 4);
-                pa_cp16(d, a.hi + at, on);
-                pa_cp16(d + TILE, a.lo + at, on);
-            }
+            const uint32_t at = stage * (2 * TILE);
+            unrolled(std::make_index_sequence<kPaTok / RPI>{}, [&](auto ic) {
+                constexpr int I = decltype(ic)::value, OFF = I / SW * (SW * RPI * RB) + I % SW * (RPI * RB);
+                const uint32_t x = __shfl_sync(0xffffffffu, row, I * RPI + lr);
+                if (valid == 0xffffu) {
+                    pa_cp16_at<OFF>(dst_of[I % SW] + at, pa_step<16>(hi, x));
+                    pa_cp16_at<OFF + TILE>(dst_of[I % SW] + at, pa_step<16>(lo, x));
+                } else {
+                    const bool on = (valid >> (I * RPI + lr)) & 1;
+                    pa_cp16(dst_of[I % SW] + at + OFF, pa_step<16>(hi, x), on);
+                    pa_cp16(dst_of[I % SW] + at + OFF + TILE, pa_step<16>(lo, x), on);
+                }
+            });
         }
         pa_commit();
     };
 
     // consumer
-    uint32_t qf[KT][4], q3[BF16 ? KT : 1][2], plus[KT][2];  // plus: all ones where q > 0
+    // q+ and q- apart where registers allow, else q and the mask of its positive
+    // entries
+    constexpr bool APART = D <= 128;
+    uint32_t qf[APART ? 2 : 1][KT][4], q3[APART ? 2 : 1][BF16 ? KT : 1][2], plus[APART ? 1 : KT][2];
     bool new_q = true;
     int stage = 0, ahead = 0;
     float up = 1.f;
     const int mi = lane >> 3, ri = lane & 7;
+    uint32_t b_at[4];  // this lane's ldmatrix rows, as K's in the attention kernel
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b_at[i] = ring + (8 * (mi >> 1) + ri) * RB + (((2 * i + (mi & 1)) ^ ri) << 4);
 #pragma unroll 1
     for (int turn = 1 - S; to_do > 0; ++turn) {
         if (turn >= 0) {
@@ -190,7 +205,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_score_kernel(PagedS
             up = __uint_as_float((unsigned)(127 - ex) << 23);
             if (lane == 0 && cur.u == 0) a.group[sh_] = make_float2(up, sum * up);
         }
-        const uint32_t hst = ring + stage * (2 * TILE), lst = hst + TILE;
+        const uint32_t st = stage * (2 * TILE);
         float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         unsigned top = 0;
 #pragma unroll 1
@@ -201,40 +216,52 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_score_kernel(PagedS
 #pragma unroll
                 for (int i = 0; i < 2 * KT; ++i) {
                     float x = v[i].x * up, y = v[i].y * up;
-                    plus[i >> 1][i & 1] = (x > 0.f ? 0xffffu : 0u) | (y > 0.f ? 0xffff0000u : 0u);
-                    qf[i >> 1][2 * (i & 1)] = pa_split<BF16>(x, y);
-                    qf[i >> 1][2 * (i & 1) + 1] = pa_split<BF16>(x, y);
-                    if (BF16) q3[i >> 1][i & 1] = pa_split<BF16>(x, y);
+                    const uint32_t pos = (x > 0.f ? 0xffffu : 0u) | (y > 0.f ? 0xffff0000u : 0u);
+                    const int kt = i >> 1, e = i & 1;
+                    const uint32_t p0 = pa_split<BF16>(x, y), p1 = pa_split<BF16>(x, y);
+                    const uint32_t p2 = BF16 ? pa_split<BF16>(x, y) : 0u;
+                    if (APART) {
+#pragma unroll
+                        for (int half = 0; half < (APART ? 2 : 1); ++half) {
+                            const uint32_t m = half ? ~pos : pos;
+                            qf[half][kt][2 * e] = p0 & m;
+                            qf[half][kt][2 * e + 1] = p1 & m;
+                            if (BF16) q3[half][BF16 ? kt : 0][e] = p2 & m;
+                        }
+                    } else {
+                        plus[APART ? 0 : kt][e] = pos;
+                        qf[0][kt][2 * e] = p0;
+                        qf[0][kt][2 * e + 1] = p1;
+                        if (BF16) q3[0][BF16 ? kt : 0][e] = p2;
+                    }
                 }
             }
-            // two k steps at a time from zero, added up outside the tensor core,
+            // four k steps at a time from zero, added up outside the tensor core,
             // which truncates: the bound on the sum is what keeps the undecided few
-            float sc[4] = {};
+            float sc[4] = {}, d[2][4];
+            unrolled(std::make_index_sequence<2 * KT>{}, [&](auto ic) {
+                constexpr int half = decltype(ic)::value / KT, kt = decltype(ic)::value % KT, k3 = BF16 ? kt : 0;
+                constexpr int from = APART ? half : 0, km = APART ? 0 : kt;
+                uint32_t b[4];
+                pa_ldsm_at<half * TILE + kt / 4 * 128>(b, b_at[kt % 4] + st);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {  // q+ with hi, then q- with lo
+                for (int i = 0; i < 4; ++i) top = max16_abs<BF16>(top, b[i]);
+                // q+ with hi, then q- with lo
+                const uint32_t m0 = APART ? 0xffffffffu : half ? ~plus[km][0] : plus[km][0];
+                const uint32_t m1 = APART ? 0xffffffffu : half ? ~plus[km][1] : plus[km][1];
+                const uint32_t(&q)[4] = qf[from][kt];
+                const uint32_t a0 = q[0] & m0, a1 = q[1] & m0, a2 = q[2] & m1, a3 = q[3] & m1;
 #pragma unroll
-                for (int kt = 0; kt < KT; kt += 2) {
-                    float d[2][4];
-#pragma unroll
-                    for (int y = kt; y < kt + 2; ++y) {
-                        uint32_t b[4];
-                        const int r = 8 * (mi >> 1) + ri, c = 2 * y + (mi & 1);
-                        pa_ldsm(b, (half ? lst : hst) + r * RB + ((c ^ ri) << 4));
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) top = max16_abs<BF16>(top, b[i]);
-                        const uint32_t m0 = half ? ~plus[y][0] : plus[y][0], m1 = half ? ~plus[y][1] : plus[y][1];
-                        const uint32_t a0 = qf[y][0] & m0, a1 = qf[y][1] & m0, a2 = qf[y][2] & m1, a3 = qf[y][3] & m1;
-#pragma unroll
-                        for (int n = 0; n < 2; ++n) {
-                            if (y == kt) pa_mma0<BF16>(d[n], a0, a1, a2, a3, b[2 * n], b[2 * n + 1]);
-                            else pa_mma<BF16>(d[n], a0, a1, a2, a3, b[2 * n], b[2 * n + 1]);
-                            if (BF16) pa_mma<BF16>(d[n], q3[y][0] & m0, 0u, q3[y][1] & m1, 0u, b[2 * n], b[2 * n + 1]);
-                        }
-                    }
+                for (int n = 0; n < 2; ++n) {
+                    if (kt % 4 == 0) pa_mma0<BF16>(d[n], a0, a1, a2, a3, b[2 * n], b[2 * n + 1]);
+                    else pa_mma<BF16>(d[n], a0, a1, a2, a3, b[2 * n], b[2 * n + 1]);
+                    if (BF16)
+                        pa_mma<BF16>(d[n], q3[from][k3][0] & m0, 0u, q3[from][k3][1] & m1, 0u, b[2 * n], b[2 * n + 1]);
+                }
+                if (kt % 4 == 3)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) sc[i] += d[i >> 1][i & 1] + d[i >> 1][2 + (i & 1)];
-                }
-            }
+            });
 #pragma unroll
             for (int i = 0; i < 4; ++i) best[i] = fmaxf(best[i], sc[i]);
         }
@@ -404,12 +431,12 @@ __global__ void __launch_bounds__(kTopkThreads) paged_topk_kernel(PagedSelectArg
     __syncthreads();
     // eps, with q' = q 2^-ex, whose largest entry is in [1, 2), M = max |bound| and
     // S = M max_j sum |q'_jd|: the parts of q' leave out at most 2^-23 of each
-    // entry, in all D 2^-23 M; a chain of two instructions (bf16: four) truncates
-    // its 33 (67) terms below 2^-24 of the largest, in all 67 2^-24 S; adding high
-    // and low halves and the D / 16 chains rounds D / 16 + 1 times by 2^-24 S at
+    // entry, in all D 2^-23 M; a chain of four instructions (bf16: eight) truncates
+    // its 67 (135) terms below 2^-24 of the largest, in all 135 2^-24 S; adding high
+    // and low halves and the D / 32 chains rounds D / 32 + 1 times by 2^-24 S at
     // most.  1e-30 covers what underflows.
     const float biggest = BF16 ? __uint_as_float(s_top << 16) : h2f((uint16_t)s_top);
-    const float eps = biggest * (D * 0x1p-23f + group.y * (70 + D / 16) * 0x1p-24f) * 1.01f + 1e-30f;
+    const float eps = biggest * (D * 0x1p-23f + group.y * (140 + D / 32) * 0x1p-24f) * 1.01f + 1e-30f;
     const bool sure = eps < 1e30f;  // not: bounds or queries that are not finite, nothing is decided by the scores
     float tau = 0.f;
     if (sure) {

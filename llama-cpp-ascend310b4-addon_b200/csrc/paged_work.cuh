@@ -3,6 +3,8 @@
 // pages with f32 operands.
 #pragma once
 
+#include <utility>
+
 #include "common.cuh"
 #include "paged_store.cuh"
 
@@ -104,6 +106,21 @@ __device__ __forceinline__ float pa_warp_max(float v) {
     asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
 }
+// f(integral_constant<I>) for I of the sequence.
+template <size_t... I, class F>
+__device__ __forceinline__ void unrolled(std::index_sequence<I...>, F f) {
+    (f(std::integral_constant<int, (int)I>{}), ...);
+}
+
+// p + I * step in one instruction.
+template <int I>
+__device__ __forceinline__ const uint8_t* pa_step(const uint8_t* p, uint32_t step) {
+    if (I == 0) return p;
+    uint64_t r;
+    asm("mad.wide.u32 %0, %1, %2, %3;" : "=l"(r) : "r"(step), "n"(I), "l"(p));
+    return reinterpret_cast<const uint8_t*>(r);
+}
+
 template <int W>
 struct PaRangeShared {
     int part[W];           // prefix-sum partials
