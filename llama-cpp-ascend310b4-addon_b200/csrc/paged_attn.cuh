@@ -4,7 +4,7 @@
 //   out_j = sum_p w_p v_p / sum_p w_p,  w_p = 2^(f q_j . k_p + bias_p - m)
 //
 // with f = scale log2(e) and m the running maximum.  Per cached token and KV
-// head K and V are 4 D bytes for 4 D G flops (G <= 8 query heads a pass), so
+// head K and V are 4 D bytes for 4 D G flops (G <= 16 query heads a pass), so
 // the kernel is bound by reading the cache; the arithmetic only has to keep
 // up, and the split only has to keep every SM reading until the end.
 //
@@ -223,16 +223,18 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
     };
     auto tail_piece = [&](int w) -> float* { return reinterpret_cast<float*>(pa_sm + w * (S * 2 * TILE)); };
 
-    if (fb < fe) {
-        PaCursor in, cur;
-        in.s = range.seq0;
-        in.len = pa_len(a, in.s);
-        in.nu = pa_units(a, in.len);
-        const int hh0 = (fb - range.base0) / in.nu;
+    PaCursor in;
+    in.s = range.seq0;
+    in.len = fb < fe ? pa_len(a, in.s) : 0;
+    in.nu = pa_units(a, in.len);
+    // (lengths that change while the kernel runs give wrong results, but no
+    // address outside the tensors: a position that does not fit ends the warp)
+    const int hh0 = in.nu > 0 ? (fb - range.base0) / in.nu : hh_n;
+    if ((unsigned)hh0 < (unsigned)hh_n) {
         in.u = (fb - range.base0) - hh0 * in.nu;
         in.head = a.chunks == 1 ? hh0 : hh0 / a.chunks;
         in.chunk = hh0 - in.head * a.chunks;
-        cur = in;
+        PaCursor cur = in;
         int seg_from = fb - in.u;  // first unit of the current segment
         int to_issue = fe - fb, to_do = to_issue;
 
@@ -303,8 +305,11 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
             }
         };
         // another segment, or the next 32 entries of this one's list
-        auto refill = [&]() {
-            if (in.u == in.nu) fresh = pa_next(a, in);
+        auto refill = [&]() -> bool {
+            if (in.u == in.nu) {
+                if (!pa_next(a, in)) return false;
+                fresh = true;
+            }
             const unsigned vt = (unsigned)in.u * kPaTok + (lane & 15);
             bi = (int)(vt / (unsigned)ps);
             row = (int)(vt - (unsigned)bi * (unsigned)ps);
@@ -322,17 +327,20 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
             // units that begin before entry w0 + 32
             const long long here = ((long long)(w0 + 32) * ps - (long long)in.u * kPaTok + kPaTok - 1) / kPaTok;
             run = (int)min((long long)(in.nu - in.u), here);
+            return true;
         };
         auto issue = [&](int stage) {
             if (MASK) flush_mask();
             if (to_issue > 0) {
-                if (run == 0) {
-                    refill();
-                } else {
+                if (run != 0) {
                     bi += q16;
                     row += r16;
                     if (row >= ps) row -= ps, ++bi;
+                } else if (!refill()) {
+                    to_issue = 0;
                 }
+            }
+            if (to_issue > 0) {
                 const int x = bi - w0;  // 0 .. 31, 46 where a unit spans pages
                 int page = __shfl_sync(0xffffffffu, p0, x & 31), blk = bi;
                 if (a.sel != nullptr) blk = __shfl_sync(0xffffffffu, b0, x & 31);

@@ -94,7 +94,8 @@ __global__ void __launch_bounds__(32 * pa_warps(D), 1) paged_score_kernel(PagedS
     in.s = range.seq0;
     in.nb = blocks(in.s);
     in.nu = paged_units(in.nb);
-    in.head = (range.fb - range.base0) / in.nu;
+    in.head = in.nu > 0 ? (range.fb - range.base0) / in.nu : H;
+    if ((unsigned)in.head >= (unsigned)H) return;  // the lengths changed while the kernel runs
     in.u = (range.fb - range.base0) - in.head * in.nu;
     cur = in;
     auto advance = [&](Cursor& c) -> bool {
