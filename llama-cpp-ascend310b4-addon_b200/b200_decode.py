@@ -763,7 +763,10 @@ def _paged_batch(what, cache, q, block_table, seq_lens):
             or seq_lens.shape != shape[:1] or not seq_lens.is_contiguous()):
         _bad(what, "block_table must be int32 [n_seq, max_blocks] with contiguous rows and seq_lens int32 [n_seq], "
                    "on the cache's device")
-    q, ld = _rows_f32(what, "q", q, n_head * cache.head_dim, dev)
+    row = n_head * cache.head_dim
+    if q.dtype == torch.float32 and q.device == dev and q.is_contiguous() and q.data_ptr() % 16 == 0:
+        return q, row, n_seq, n_head
+    q, ld = _rows_f32(what, "q", q, row, dev)
     return q, ld, n_seq, n_head
 
 

@@ -679,13 +679,12 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
     const unsigned alone = __ballot_sync(0xffffffffu, hd >= 0 && hd != prev);
     constexpr int AT_M = NH * D, AT_L = AT_M + NH, AT_MK = AT_L + NH, NV = PaJoint<D>::NV;
     const bool masked = MASK, has_col = 4 * lane < D;
-    auto put_out = [&](int row, const PaJoint<D>& t) {
-        const float inv = t.l > 0.f ? 1.f / t.l : 0.f;
-        float4* out = reinterpret_cast<float4*>(a.out + (int64_t)row * D) + lane;
+    auto put = [&](float* row, const PaJoint<D>& t, float scale) {
+        float4* out = reinterpret_cast<float4*>(row) + lane;
         if (has_col)
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                out[32 * i] = make_float4(t.v[i].x * inv, t.v[i].y * inv, t.v[i].z * inv, t.v[i].w * inv);
+                out[32 * i] = make_float4(t.v[i].x * scale, t.v[i].y * scale, t.v[i].z * scale, t.v[i].w * scale);
     };
     int open0 = -1, open1 = -1;  // segments cut by the CTA's borders: where to find them in sh (2 * warp + slot)
 #pragma unroll 1
@@ -711,19 +710,12 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
             }
             t.add(n, pm, pl, pk, masked, smem_u32(tail_piece(w0) + j * D), S * 2 * TILE, closed ? n - 1 : -1,
                   smem_u32(head_piece(w0 + n - 1) + j * D));
-            if (whole) {
-                put_out(sh.row[slot][w0] + j, t);
-            } else {
-                float* p = a.pieces + (int64_t)(2 * blockIdx.x + (from >= cb ? 1 : 0)) * PIECE;
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (has_col) __stcg(reinterpret_cast<float4*>(p + j * D + 4 * lane + 128 * i), t.v[i]);
-                if (lane == 0) {
-                    __stcg(p + AT_M + j, t.m);
-                    __stcg(p + AT_L + j, t.l);
-                    __stcg(p + AT_MK, t.mk);
-                }
-            }
+            // the output, or this CTA's piece of the segment (one path: most of what
+            // this costs is fetching its instructions)
+            float* p = a.pieces + (int64_t)(2 * blockIdx.x + (from >= cb ? 1 : 0)) * PIECE;
+            const float inv = t.l > 0.f ? 1.f / t.l : 0.f;
+            put(whole ? a.out + (int64_t)(sh.row[slot][w0] + j) * D : p + j * D, t, whole ? inv : 1.f);
+            if (!whole && lane == 0) p[AT_M + j] = t.m, p[AT_L + j] = t.l, p[AT_MK] = t.mk;
         }
     }
     if (open0 < 0) return;
@@ -774,7 +766,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
                 t.add(here, pm, pl, pk, masked, buf, 4 * D, -1, 0u);
                 __syncwarp();
             }
-            put_out(sh.row[at & 1][at >> 1] + j, t);
+            put(a.out + (int64_t)(sh.row[at & 1][at >> 1] + j) * D, t, t.l > 0.f ? 1.f / t.l : 0.f);
             if (lane == 0) a.tickets[(int64_t)sh.seg[at & 1][at >> 1] * NH + j] = 0u;
         }
     }
