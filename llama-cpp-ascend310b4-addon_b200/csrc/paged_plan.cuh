@@ -7,6 +7,8 @@
 // sequences are.  The call is bound by latency (a few hundred KB at most): one
 // cluster of up to 8 CTAs, each with the sums of all sequences, so nothing but
 // one barrier separates reading the lengths from replacing them in place.
+// Measured: 64 sequences with one token each 4.0 us, 1024 mixed ones with 25000
+// tokens 15.5 us (60 us on one CTA).
 #pragma once
 
 #include <cooperative_groups.h>
