@@ -19,6 +19,8 @@
  * [0, max_blocks * page_size] is never followed: the access is skipped (the
  * length clamped) and B200_DEVSTATUS_BOUNDS recorded (b200_device_status).
  *
+ * A batch has at most 65535 sequences and 65535 query heads (B200_EINVAL).
+ *
  * The reference serves one sequence over one contiguous cache; these are the
  * counterparts of its attention step, its SET_ROWS and its kv_lengths input
  * (patch:1370-1432, patch:1179-1184, patch:2009-2023) for many sequences.

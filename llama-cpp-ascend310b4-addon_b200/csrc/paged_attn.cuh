@@ -30,7 +30,7 @@
 // high parts of q (and of the weights w) and rows 8-15 with the low parts, so
 // one instruction gives both products and f16 keeps 22 bits of q and w: their
 // own rounding stays below that of the f32 sums.  q is scaled by a power of
-// two into f16's range, w by 2^12 out of f16's subnormals.  bf16 takes a third
+// two into f16's range, w (f16 pages) by 2^12 out of f16's subnormals.  bf16 takes a third
 // part in a second instruction.  Sums over positions are f32 additions
 // outside the tensor core, which truncates its own.  (tcgen05 has no use for 8
 // rows of heads; mma.sync keeps the tensor pipe 19% busy.)
@@ -402,6 +402,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
         // additions stay below the rounding of one f32.  m is the weights'
         // reference: it follows the running maximum only when that has grown by
         // 2^3, which w has room for (w <= 2^15 in f16), so o is rarely rescaled.
+        constexpr float W_UP = BF16 ? 1.f : 4096.f;  // bf16 has no subnormals to keep out of
         constexpr int FLUSH = D * NC <= 128 ? 4 : 1;  // (the others lack the registers)
         float o[NC][2 * KT][2], acc[NC][FLUSH > 1 ? 2 * KT : 1][4];
         float m[NC], l[NC], f[NC], mk = -INFINITY;
@@ -589,7 +590,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
                 for (int c = 0; c < NC; ++c) {
                     float w[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = pa_exp2(fmaf(x[c][i], f[c], bias[i] - m[c])) * 4096.f;
+                    for (int i = 0; i < 4; ++i) w[i] = pa_exp2(fmaf(x[c][i], f[c], bias[i] - m[c])) * W_UP;
                     if (live != 0xffffu) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)

@@ -415,7 +415,7 @@ def check_attn(c, q, page_size, dtype, scale, mask=None, sel=None, layout="token
 
 
 LENS = [([1], 16), ([37], 16), ([0, 1, 15, 16, 17, 0], 16), ([127, 128, 129, 255, 256, 257], 32), ([63, 500, 5], 5),
-        ([1000], 1), ([2048, 3, 777], 100), ([4160], 16), ([9000, 0, 1], 64)]
+        ([1000], 1), ([2048, 3, 777], 100), ([4160], 16), ([9000, 0, 1], 64), ([5000, 4096, 17], 2048), ([2500, 1], 1000)]
 SHAPES = [(12, 2, 128), (24, 2, 64), (4, 4, 256), (64, 8, 128), (8, 8, 64), (16, 4, 256), (40, 1, 128)]
 
 
@@ -602,6 +602,18 @@ def test_attn_peaked_and_extreme_queries(dtype):
                        (1.0, -0.3)):
         q = (r.standard_normal((2, 8, 128)) * mag).astype(np.float32)
         check_attn(c, q, 16, dtype, scale)
+
+
+def test_attn_values_at_the_end_of_their_range():
+    """f16 values of 60000, bf16 values of 1e36: the weighted sums stay in
+    range as far as f32 sums of weights of at most one would."""
+    r = rng(32)
+    for dtype, big in (("f16", 6e4), ("bf16", 1e36)):
+        c = R.make_cache(r, [40, 3], 16, 2, 128, dtype)
+        live = ~np.isnan(c["v"])
+        c["v"][live] = R.rounded(np.sign(c["v"][live]) * big * (0.5 + 0.5 * r.random(live.sum())), dtype)
+        q = r.standard_normal((2, 8, 128)).astype(np.float32)
+        check_attn(c, q, 16, dtype, 0.1)
 
 
 def test_attn_strided_queries_tables_and_masks():
