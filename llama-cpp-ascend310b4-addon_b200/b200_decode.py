@@ -821,7 +821,8 @@ def paged_attn(cache: PagedKV, q, block_table, seq_lens, scale: float, mask=None
     q f32 [n_seq, n_head, head_dim]; block_table int32 [n_seq, max_blocks];
     seq_lens int32 [n_seq]; mask f16 [n_seq, >= max_blocks * page_size]
     additive or None; sel int32 [n_seq, n_head_kv, n_sel] (paged_select) or
-    None for every block.  Returns f32 [n_seq, n_head, head_dim]; zeros where
+    None for every block.  Returns f32 [n_seq, n_head, head_dim] (out, which must
+    not overlap q); zeros where
     nothing is attended to.  workspace: uint8 of paged_attn_workspace_size
     bytes, zero-filled before its first use and not shared by calls that
     overlap on the GPU; allocated and cleared for this call when not given."""
@@ -844,9 +845,10 @@ def paged_attn(cache: PagedKV, q, block_table, seq_lens, scale: float, mask=None
             _bad("paged_attn", "sel must be a contiguous int32 [n_seq, n_head_kv, n_sel]")
         sel_ptr, n_sel = sel.data_ptr(), s[2]
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.dtype != torch.float32 or out.device != dev or not out.is_contiguous() or out.shape != q.shape:
-        _bad("paged_attn", "out must be a contiguous f32 [n_seq, n_head, head_dim]")
+        out = torch.empty_like(q)  # rows of contiguous heads: contiguous
+    elif (out.dtype != torch.float32 or out.device != dev or not out.is_contiguous() or out.shape != q.shape
+          or (out.data_ptr() == q.data_ptr() and n_seq)):
+        _bad("paged_attn", "out must be a contiguous f32 [n_seq, n_head, head_dim] apart from q")
     if workspace is None:
         size = paged_attn_workspace_size(cache.head_dim, n_seq, n_head, cache.n_head_kv)
         workspace = torch.zeros(size, dtype=torch.uint8, device=dev)

@@ -402,6 +402,9 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
         // additions stay below the rounding of one f32.  m is the weights'
         // reference: it follows the running maximum only when that has grown by
         // 2^3, which w has room for (w <= 2^15 in f16), so o is rarely rescaled.
+        // bf16's third parts take rows 0-7 of an instruction; two groups share one
+        constexpr bool PAIR = BF16 && NC == 2;
+        constexpr int THIRDS = PAIR ? 1 : NC;
         constexpr float W_UP = BF16 ? 1.f : 4096.f;  // bf16 has no subnormals to keep out of
         constexpr int FLUSH = D * NC <= 128 ? 4 : 1;  // (the others lack the registers)
         float o[NC][2 * KT][2], acc[NC][FLUSH > 1 ? 2 * KT : 1][4];
@@ -506,7 +509,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
                 // truncates every addition; bf16's third parts in a chain of their
                 // own, where what is truncated is 2^-16 as large.
                 constexpr int CHAINS = (KT + 3) / 4;
-                float sc[NC][2][CHAINS][4], s3[NC][2][4];
+                float sc[NC][2][CHAINS][4], s3[THIRDS][2][4];
                 unrolled(std::make_index_sequence<KT>{}, [&](auto ic) {
                     constexpr int kt = decltype(ic)::value, k3 = BF16 ? kt : 0;
                     uint32_t b[4];
@@ -519,10 +522,11 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
                             float(&d)[4] = sc[c][n][kt / 4];
                             if (kt % 4 == 0) pa_mma0<BF16>(d, q[0], q[1], q[2], q[3], b[2 * n], b[2 * n + 1]);
                             else pa_mma<BF16>(d, q[0], q[1], q[2], q[3], b[2 * n], b[2 * n + 1]);
-                            if (BF16) {
+                            if (BF16 && c < THIRDS) {
                                 const uint32_t(&r)[2] = q3[c][k3];
-                                if (kt == 0) pa_mma0<BF16>(s3[c][n], r[0], 0u, r[1], 0u, b[2 * n], b[2 * n + 1]);
-                                else pa_mma<BF16>(s3[c][n], r[0], 0u, r[1], 0u, b[2 * n], b[2 * n + 1]);
+                                const uint32_t r1 = PAIR ? q3[NC - 1][k3][0] : 0u, r3 = PAIR ? q3[NC - 1][k3][1] : 0u;
+                                if (kt == 0) pa_mma0<BF16>(s3[c][n], r[0], r1, r[1], r3, b[2 * n], b[2 * n + 1]);
+                                else pa_mma<BF16>(s3[c][n], r[0], r1, r[1], r3, b[2 * n], b[2 * n + 1]);
                             }
                         }
                 });
@@ -550,7 +554,8 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
                 for (int c = 0; c < NC; ++c) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float lows = BF16 ? s3[c][i >> 1][i & 1] : 0.f, highs = 0.f;
+                        float lows = !BF16 ? 0.f : PAIR ? s3[0][i >> 1][2 * c + (i & 1)] : s3[PAIR ? 0 : c][i >> 1][i & 1];
+                        float highs = 0.f;
 #pragma unroll
                         for (int y = 0; y < CHAINS; ++y) {
                             highs += sc[c][i >> 1][y][i & 1];
@@ -607,6 +612,15 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
                     constexpr int kt = decltype(ic)::value;
                     uint32_t b[4];
                     pa_ldsm_t_at<kt / 4 * 128>(b, v_at[kt % 4] + st);
+                    if (PAIR) {
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            float d[4];
+                            pa_mma0<BF16>(d, w3[0][0], w3[NC - 1][0], w3[0][1], w3[NC - 1][1], b[2 * n], b[2 * n + 1]);
+                            o[0][2 * kt + n][0] += d[0], o[0][2 * kt + n][1] += d[1];
+                            o[NC - 1][2 * kt + n][0] += d[2], o[NC - 1][2 * kt + n][1] += d[3];
+                        }
+                    }
 #pragma unroll
                     for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -614,11 +628,11 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(Pag
                             if (FLUSH > 1) {
                                 float(&d)[4] = acc[c][FLUSH > 1 ? 2 * kt + n : 0];
                                 pa_mma<BF16>(d, wa[c][0], wa[c][1], wa[c][2], wa[c][3], b[2 * n], b[2 * n + 1]);
-                                if (BF16) pa_mma<BF16>(d, w3[c][0], 0u, w3[c][1], 0u, b[2 * n], b[2 * n + 1]);
+                                if (BF16 && !PAIR) pa_mma<BF16>(d, w3[c][0], 0u, w3[c][1], 0u, b[2 * n], b[2 * n + 1]);
                             } else {
                                 float d[4];
                                 pa_mma0<BF16>(d, wa[c][0], wa[c][1], wa[c][2], wa[c][3], b[2 * n], b[2 * n + 1]);
-                                if (BF16) pa_mma<BF16>(d, w3[c][0], 0u, w3[c][1], 0u, b[2 * n], b[2 * n + 1]);
+                                if (BF16 && !PAIR) pa_mma<BF16>(d, w3[c][0], 0u, w3[c][1], 0u, b[2 * n], b[2 * n + 1]);
                                 o[c][2 * kt + n][0] += d[0] + d[2];
                                 o[c][2 * kt + n][1] += d[1] + d[3];
                             }

@@ -724,7 +724,7 @@ def test_refusals_of_the_python_layer_on_device():
            dict(mask=torch.zeros((2, 32), device="cuda")),
            dict(sel=torch.zeros((2, 1, 3), dtype=torch.int32, device="cuda")),
            dict(sel=torch.zeros((2, 2, 0), dtype=torch.int32, device="cuda")),
-           dict(out=torch.zeros((2, 4, 64), device="cuda")),
+           dict(out=torch.zeros((2, 4, 64), device="cuda")), dict(out=q),
            dict(workspace=torch.zeros(64, device="cuda")),
            dict(workspace=torch.zeros(8, dtype=torch.uint8, device="cuda"))]
     for over in bad:
