@@ -55,11 +55,14 @@ int launch_paged_plan(const PagedPlanArgs& a, cudaStream_t st) {
         }
     }
     // one cluster: every CTA scans the sequences, and each takes its share of
-    // the token rows
+    // the token rows.  One CTA alone, launched without a cluster, up to a token
+    // row per thread: 64 sequences with one token each 3.4 us against 4.0 on
+    // two CTAs, 1024 sequences 6.5 against 7.1; twice the rows 7.6 against 6.9
     const int rows = std::max(a.max_tokens, a.n_seq);
+    const int ctas = a.max_tokens <= kPlanThreads ? 1 : (a.max_tokens + 2 * kPlanThreads - 1) / (2 * kPlanThreads) + 1;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3((unsigned)std::min(kPlanThreads, (rows + 63) / 64 * 64), 1, 1);
-    cfg.gridDim = dim3((unsigned)std::min(kPlanCtas, (a.max_tokens + 2 * kPlanThreads - 1) / (2 * kPlanThreads) + 1), 1, 1);
+    cfg.gridDim = dim3((unsigned)std::min(kPlanCtas, ctas), 1, 1);
     cfg.dynamicSmemBytes = plan_smem_bytes(a.n_seq);
     cfg.stream = st;
     cudaLaunchAttribute at;
@@ -68,7 +71,7 @@ int launch_paged_plan(const PagedPlanArgs& a, cudaStream_t st) {
     at.val.clusterDim.y = 1;
     at.val.clusterDim.z = 1;
     cfg.attrs = &at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cfg.gridDim.x > 1 ? 1 : 0;
     return cuda_status(cudaLaunchKernelEx(&cfg, paged_plan_kernel, a));
 }
 
