@@ -254,21 +254,14 @@ def prepare(case, seed):
 
 # ---------------------------------------------------------------- own calls
 
-_module = None
-
-
 def _package():
-    """The framework's module, imported once as a program does."""
-    global _module
-    if _module is None:
-        here = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-        path = os.path.join(here, "llama-cpp-ascend310b4-addon_b200")
-        if path not in sys.path:
-            sys.path.insert(0, path)
-        import b200_decode
+    here = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    path = os.path.join(here, "llama-cpp-ascend310b4-addon_b200")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import b200_decode
 
-        _module = b200_decode
-    return _module
+    return b200_decode
 
 
 def _run_own(s):
@@ -281,13 +274,13 @@ def _run_own(s):
     if "cache" not in s:  # the handle a program keeps for its cache
         if s["op"] == "store":
             n = s["n_pages"]
-            s["stored"] = dict(k=s["k_all"][:n], v=s["v_all"][:n], lo=s["lo_all"][:n], hi=s["hi_all"][:n])
-            s["cache"] = B.PagedKV(s["stored"]["k"], s["stored"]["v"], k_lo=s["stored"]["lo"], k_hi=s["stored"]["hi"])
+            s["cache"] = B.PagedKV(s["k_all"][:n], s["v_all"][:n], k_lo=s["lo_all"][:n], k_hi=s["hi_all"][:n])
         else:
             s["cache"] = B.PagedKV(s["k"], s["v"], k_lo=s.get("lo"), k_hi=s.get("hi"))
     if s["op"] == "store":
         B.paged_store(s["cache"], s["new_k"], s["new_v"], s["slots"])
-        return s["stored"]
+        n = s["n_pages"]
+        return dict(k=s["k_all"][:n], v=s["v_all"][:n], lo=s["lo_all"][:n], hi=s["hi_all"][:n])
     if s["op"] == "select":
         return B.paged_select(s["cache"], s["q"], s["table"], s["seq_lens"], s["k_blocks"], workspace=s["workspace"])
     return B.paged_attn(s["cache"], s["q"], s["table"], s["seq_lens"], s["scale"], mask=s["mask_rows"], sel=s["sel"],
