@@ -116,7 +116,9 @@ int b200_paged_store(const b200_paged_kv *kv, const float *k, int64_t k_ld, cons
  * the n_sel - 1 blocks of largest score among the others (ties: the lower
  * block; NaN scores come last), in ascending order, then -1 where the
  * sequence has fewer blocks.  A block whose page index is out of range is
- * scored as NaN.  q as in b200_paged_attn; workspace: 16-byte aligned, no
+ * scored as NaN.  A product that is NaN (a NaN bound, 0 times an infinite one)
+ * makes the score NaN.  (b200_paged_store leaves lo = +inf and hi = -inf in a
+ * channel whose every key is NaN.)  q as in b200_paged_attn; workspace: 16-byte aligned, no
  * initial contents needed, not shared by calls that overlap on the GPU. */
 size_t b200_paged_select_workspace_size(int n_seq, int n_head_kv, int max_blocks);
 int b200_paged_select(const b200_paged_kv *kv, const float *q, int64_t q_stride, int n_seq, int n_head,

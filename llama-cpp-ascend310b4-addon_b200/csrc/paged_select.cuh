@@ -310,6 +310,9 @@ __device__ __forceinline__ float from_order_key(unsigned k) {
     return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k);
 }
 
+// The larger of two products; NaN where either is (fmax would drop it).
+__device__ __forceinline__ double larger_or_nan(double x, double y) { return x > y || x != x ? x : y; }
+
 // One warp: the 64-bit score of block b for query head j of KV head h, every
 // lane.
 template <bool BF16, int D>
@@ -324,8 +327,8 @@ __device__ __forceinline__ double exact_score(const PagedSelectArgs& a, int s, i
         const float2 lo = unpack16<BF16>(*reinterpret_cast<const uint32_t*>(a.lo + at + e));
         const float2 hi = unpack16<BF16>(*reinterpret_cast<const uint32_t*>(a.hi + at + e));
         const float2 v = *reinterpret_cast<const float2*>(q + e);
-        x += fmax((double)v.x * lo.x, (double)v.x * hi.x);
-        x += fmax((double)v.y * lo.y, (double)v.y * hi.y);
+        x += larger_or_nan((double)v.x * lo.x, (double)v.x * hi.x);
+        x += larger_or_nan((double)v.y * lo.y, (double)v.y * hi.y);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
