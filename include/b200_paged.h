@@ -118,8 +118,9 @@ int b200_paged_store(const b200_paged_kv *kv, const float *k, int64_t k_ld, cons
  * sequence has fewer blocks.  A block whose page index is out of range is
  * scored as NaN.  A product that is NaN (a NaN bound, 0 times an infinite one)
  * makes the score NaN.  (b200_paged_store leaves lo = +inf and hi = -inf in a
- * channel whose every key is NaN.)  q as in b200_paged_attn; workspace: 16-byte aligned, no
- * initial contents needed, not shared by calls that overlap on the GPU. */
+ * channel whose every key is NaN.)  q as in b200_paged_attn; workspace: 16-byte
+ * aligned, no initial contents needed, not shared by calls that overlap on the
+ * GPU. */
 size_t b200_paged_select_workspace_size(int n_seq, int n_head_kv, int max_blocks);
 int b200_paged_select(const b200_paged_kv *kv, const float *q, int64_t q_stride, int n_seq, int n_head,
                       const int32_t *block_table, int64_t table_stride, int max_blocks, const int32_t *seq_lens,
@@ -141,6 +142,12 @@ int b200_paged_select(const b200_paged_kv *kv, const float *q, int64_t q_stride,
  *         at -inf are left out whatever their key and value hold.
  *   out   f32 [n_seq][n_head][head_dim], 16-byte aligned, apart from q; a
  *         sequence with no position gets zeros
+ * Keys, values and queries may be infinite or NaN (b200_paged_store makes
+ * infinities of values past the f16 range): a score of -inf has weight 0, and
+ * zeros come out where every weight is 0; a score that is +inf or NaN makes its
+ * head's output NaN; infinite values make their columns infinite, or NaN where
+ * both signs or a weight of 0 (below 2^-126 of the largest) meet them.  A
+ * sequence whose every page holds such values takes up to 60 times as long.
  * At most 2^30 units of 16 positions of a (sequence, KV head, 8 or 16 query
  * heads) a call, counted at the table's width (B200_EUNSUPPORTED).
  * Products of K and V with q and w run on tensor cores; q and w enter as sums
