@@ -18,12 +18,19 @@ int check_paged_kv(const b200_paged_kv* kv) {
     if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256) return B200_EUNSUPPORTED;
     const int64_t strides = kv->k_page | kv->k_row | kv->k_head | kv->v_page | kv->v_row | kv->v_head;
     if (!aligned16(kv->k) || !aligned16(kv->v) || (strides & 15) || strides < 0) return B200_EINVAL;
-    // the last byte of K and of V: offsets are counted in 16-byte steps in 32 bits
+    // the last byte of K and of V: offsets are counted in 16-byte steps in 32 bits.
+    // Each term is compared by division first, so the sums cannot wrap around
     const int64_t span = (int64_t)1 << 36;
-    if ((strides >> 36) || kv->n_pages > span / std::max<int64_t>(1, std::max(kv->k_page, kv->v_page)) ||
-        (kv->n_pages - 1) * kv->k_page + (kv->page_size - 1) * kv->k_row + (kv->n_head_kv - 1) * kv->k_head >= span ||
-        (kv->n_pages - 1) * kv->v_page + (kv->page_size - 1) * kv->v_row + (kv->n_head_kv - 1) * kv->v_head >= span)
-        return B200_EUNSUPPORTED;
+    const int64_t last[3] = {kv->n_pages - 1, kv->page_size - 1, kv->n_head_kv - 1};
+    const int64_t steps[2][3] = {{kv->k_page, kv->k_row, kv->k_head}, {kv->v_page, kv->v_row, kv->v_head}};
+    for (const auto& step : steps) {
+        int64_t end = 0;
+        for (int i = 0; i < 3; ++i) {
+            if (step[i] >= span || (step[i] > 0 && last[i] > span / step[i])) return B200_EUNSUPPORTED;
+            end += last[i] * step[i];
+        }
+        if (end >= span) return B200_EUNSUPPORTED;
+    }
     if ((kv->k_lo == nullptr) != (kv->k_hi == nullptr) || !aligned16(kv->k_lo) || !aligned16(kv->k_hi))
         return B200_EINVAL;
     return B200_OK;
