@@ -235,10 +235,12 @@ def test_attn_selected_blocks_with_an_overflowed_key():
 
 def test_attn_bf16_values_near_the_largest():
     """A value of 3e38 at the position of the largest weight: the weighted sum
-    stays in f32's range, as it does with weights of at most one."""
+    stays in f32's range, as it does with weights of at most one.  Of 60000
+    positions the kernel takes several units of 16 with one reference for their
+    weights."""
     r = rng(9)
-    for d in (64, 128, 256):
-        c = R.make_cache(r, [40], 16, 1, d, "bf16")
+    for d, n in ((64, 40), (128, 40), (256, 40), (64, 60000), (128, 60000), (256, 60000)):
+        c = R.make_cache(r, [n], 16, 1, d, "bf16")
         c["k"][~np.isnan(c["k"])] = 0.0
         put(c, "k", 0, [20], 16, 0, 1.75)  # e^1.75 = 2^2.52 times the others' weight
         c["v"][~np.isnan(c["v"])] = 1.0
