@@ -65,11 +65,11 @@ int launch_paged_plan(const PagedPlanArgs& a, cudaStream_t st) {
     // the token rows.  One CTA alone, launched without a cluster, up to a token
     // row per thread: 64 sequences with one token each 3.4 us against 4.0 on
     // two CTAs, 1024 sequences 6.5 against 7.1; twice the rows 7.6 against 6.9
-    const int rows = std::max(a.max_tokens, a.n_seq);
-    const int ctas = a.max_tokens <= kPlanThreads ? 1 : (a.max_tokens + 2 * kPlanThreads - 1) / (2 * kPlanThreads) + 1;
+    const int64_t tokens = a.max_tokens, rows = std::max<int64_t>(tokens, a.n_seq);
+    const int64_t ctas = tokens <= kPlanThreads ? 1 : (tokens + 2 * kPlanThreads - 1) / (2 * kPlanThreads) + 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3((unsigned)std::min(kPlanThreads, (rows + 63) / 64 * 64), 1, 1);
-    cfg.gridDim = dim3((unsigned)std::min(kPlanCtas, ctas), 1, 1);
+    cfg.blockDim = dim3((unsigned)std::min<int64_t>(kPlanThreads, (rows + 63) / 64 * 64), 1, 1);
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>(kPlanCtas, ctas), 1, 1);
     cfg.dynamicSmemBytes = plan_smem_bytes(a.n_seq);
     cfg.stream = st;
     cudaLaunchAttribute at;

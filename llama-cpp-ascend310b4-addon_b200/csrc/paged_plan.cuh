@@ -149,8 +149,10 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
     };
     auto blocks_of = [&](int tokens) { return (int)(((unsigned)tokens + (unsigned)ps - 1u) / (unsigned)ps); };
 
-    const int at = blockIdx.x * blockDim.x + tid, step = gridDim.x * blockDim.x;
-    for (int t = at; t < a.max_tokens; t += step) {
+    // unsigned: a step past the last of 2^31 - 2 rows or pages must not wrap around
+    const unsigned at = blockIdx.x * blockDim.x + tid, step = gridDim.x * blockDim.x;
+    for (unsigned u = at; u < (unsigned)a.max_tokens; u += step) {
+        const int t = (int)u;
         int64_t slot = -1;
         int pos = -1;
         if (t < s_cu[n]) {
@@ -172,11 +174,13 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
         a.slots[t] = slot;
         a.positions[t] = pos;
     }
-    for (int r = at; r < got; r += step) {
+    for (unsigned u = at; u < (unsigned)got; u += step) {
+        const int r = (int)u;
         const int i = find_segment(s_need, n, r);
         a.table[i * a.table_stride + blocks_of(s_old[i]) + (r - s_need[i])] = popped(r);
     }
-    for (int r = at; r < n_back; r += step) {
+    for (unsigned u = at; u < (unsigned)n_back; u += step) {
+        const int r = (int)u;
         const int page = given_back(r);
         if ((unsigned)page >= (unsigned)a.n_pages) record_status(B200_DEVSTATUS_BOUNDS);
         a.free_pages[n0 + r] = page;
@@ -184,7 +188,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedPlanArgs 
     // every CTA has read the lengths and the page count
     if (gridDim.x > 1) cooperative_groups::this_cluster().sync();
     else __syncthreads();
-    for (int i = at; i < n; i += step) {
+    for (int i = (int)at; i < n; i += (int)step) {
         const int old = s_old[i];
         int len = old >= 0 ? old : ~old;
         if (a.new_lens[i] < 0) len = 0;
