@@ -18,6 +18,9 @@
  * used.  A page index outside [0, n_pages) or a length outside
  * [0, max_blocks * page_size] is never followed: the access is skipped (the
  * length clamped) and B200_DEVSTATUS_BOUNDS recorded (b200_device_status).
+ * Lengths, tables, lists and masks must not change while a call that reads them
+ * runs: it then still touches nothing outside its tensors, but its results are
+ * wrong, and an attention workspace has to be zero-filled again.
  *
  * A batch has at most 65535 sequences and 65535 query heads (B200_EINVAL).
  *

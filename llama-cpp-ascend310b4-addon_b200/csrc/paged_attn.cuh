@@ -337,8 +337,9 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(con
     in.s = range.seq0;
     in.len = fb < fe ? pa_len(a, in.s) : 0;
     in.nu = pa_units(a, in.len);
-    // (lengths that change while the kernel runs give wrong results, but no
-    // address outside the tensors: a position that does not fit ends the warp)
+    // (lengths that change while the kernel runs give wrong results and tickets
+    // that do not end at zero, but no address outside the tensors: a position that
+    // does not fit ends the warp, and no piece is looked for past the grid)
     const int hh0 = in.nu > 0 ? (fb - range.base0) / in.nu : hh_n;
     if ((unsigned)hh0 < (unsigned)hh_n) {
         in.u = (fb - range.base0) - hh0 * in.nu;
@@ -873,7 +874,7 @@ __global__ void __launch_bounds__(32 * pa_warps(D, NC), 1) paged_attn_kernel(con
         const int at = i ? open1 : open0;
         if (at < 0) break;
         const int from = sh.from[at & 1][at >> 1], rows = sh.rows[at & 1][at >> 1];
-        const int c0 = from / per_cta, n = (from + sh.nu[at & 1][at >> 1] - 1) / per_cta - c0 + 1;
+        const int c0 = from / per_cta, n = pa_pieces(from, sh.nu[at & 1][at >> 1], per_cta, (int)gridDim.x);
         // piece k: slot 1 of CTA c0, where the segment starts, then slot 0 of the next CTAs
         auto piece = [&](int k) -> const float* { return a.pieces + (int64_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * PIECE; };
 #pragma unroll 1

@@ -604,7 +604,8 @@ __global__ void __launch_bounds__(kTopkThreads) paged_topk_kernel(PagedSelectArg
             tied += total;
         }
         int at = done + block_prefix(__popc(take), part, total);
-        for (; take != 0; take &= take - 1) out[at++] = (t * T + tid) * per + __ffs(take) - 1;
+        for (; take != 0; take &= take - 1, ++at)
+            if (at < need) out[at] = (t * T + tid) * per + __ffs(take) - 1;  // (more only if lengths changed meanwhile)
         done += total;
     }
     if (tid == 0) out[need] = m;
