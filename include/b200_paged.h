@@ -142,7 +142,9 @@ int b200_paged_select(const b200_paged_kv *kv, const float *q, int64_t q_stride,
  *         [n_head][head_dim] contiguous, 16-byte aligned
  *   mask  f16, additive, row s at mask + s * mask_stride (elements), at least
  *         max_blocks * page_size entries, or NULL; finite or -inf.  Positions
- *         at -inf are left out whatever their key and value hold.
+ *         at -inf are left out whatever their key and value hold.  A stride of
+ *         0 gives every sequence the same row, as table_stride 0 does (here
+ *         and in b200_paged_select).
  *   out   f32 [n_seq][n_head][head_dim], 16-byte aligned, apart from q; a
  *         sequence with no position gets zeros
  * Keys, values and queries may be infinite or NaN (b200_paged_store makes

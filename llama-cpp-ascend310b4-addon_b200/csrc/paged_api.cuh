@@ -43,7 +43,9 @@ int check_paged_batch(const b200_paged_kv* kv, const float* q, int64_t q_stride,
         n_head > 65535)
         return B200_EINVAL;
     if (!aligned16(q) || (q_stride & 3) || (n_seq > 1 && q_stride < (int64_t)n_head * kv->head_dim)) return B200_EINVAL;
-    if (max_blocks <= 0 || (n_seq > 1 && table_stride < max_blocks) || max_blocks > INT32_MAX / kv->page_size)
+    // (a row stride of 0: one row for every sequence)
+    if (max_blocks <= 0 || (n_seq > 1 && table_stride != 0 && table_stride < max_blocks) ||
+        max_blocks > INT32_MAX / kv->page_size)
         return B200_EINVAL;
     return B200_OK;
 }
@@ -303,7 +305,7 @@ int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, i
     CR_(check_paged_batch(kv, q, q_stride, n_seq, n_head, block_table, table_stride, max_blocks, seq_lens));
     if (!out || !aligned16(out) || !workspace || !aligned16(workspace) || (sel && n_sel <= 0) ||
         (reinterpret_cast<uintptr_t>(mask) & 1) ||
-        (mask && n_seq > 1 && mask_stride < (int64_t)max_blocks * kv->page_size) ||
+        (mask && n_seq > 1 && mask_stride != 0 && mask_stride < (int64_t)max_blocks * kv->page_size) ||
         (sel && n_sel > (INT32_MAX - 4096) / kv->page_size) ||
         workspace_size < b200_paged_attn_workspace_size(kv->head_dim, n_seq, n_head, kv->n_head_kv))
         return B200_EINVAL;

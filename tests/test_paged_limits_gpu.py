@@ -49,3 +49,35 @@ def test_plan_with_the_most_token_rows(max_tokens):
         assert bool((slots[at:at + (1 << 28)] == -1).all()) and bool((positions[at:at + (1 << 28)] == -1).all()), at
     del slots, positions, p
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n_seq", [2, 5, 140])
+def test_one_row_of_table_and_mask_for_every_sequence(n_seq):
+    """Expanded tensors (row stride 0): many queries of one cached prompt, one
+    mask for the whole batch; the same bits as with rows written out."""
+    bw = B()
+    r = rng(n_seq)
+    ps, d = 16, 64
+    c = R.make_cache(r, [300], ps, 2, d, "f16")
+    dk, dv = R.to_device(c, "f16")
+    lo, hi = R.bounds_of(c)
+    cache = bw.PagedKV(dk, dv, dev(lo).half(), dev(hi).half())
+    q = r.standard_normal((n_seq, 8, d)).astype(np.float32)
+    lens = r.integers(0, 301, n_seq).astype(np.int32)
+    width = c["table"].shape[1]
+    mask = r.standard_normal((1, width * ps)).astype(np.float16)
+    mask[0, ::3] = -np.inf
+    table = i32(c["table"]).expand(n_seq, width)
+    full = table.contiguous()
+    dmask = dev(mask).expand(n_seq, width * ps)
+    assert table.stride(0) == dmask.stride(0) == 0 and full.stride(0) == width
+    dq, dl = dev(q), i32(lens)
+    for m, fm in ((None, None), (dmask, dmask.contiguous())):
+        for sel in (None, bw.paged_select(cache, dq, table, dl, 4)):
+            got = bw.paged_attn(cache, dq, table, dl, 0.125, mask=m, sel=sel)
+            assert torch.equal(got, bw.paged_attn(cache, dq, full, dl, 0.125, mask=fm, sel=sel))
+    assert torch.equal(bw.paged_select(cache, dq, table, dl, 4), bw.paged_select(cache, dq, full, dl, 4))
+    want, tol = R.attn_ref(dict(c, table=np.repeat(c["table"], n_seq, 0), lens=lens), q, ps, 0.125,
+                           np.repeat(mask, n_seq, 0))
+    got = bw.paged_attn(cache, dq, table, dl, 0.125, mask=dmask).cpu().numpy()
+    assert (np.abs(got - want) <= tol).all()
