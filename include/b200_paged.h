@@ -145,8 +145,8 @@ int b200_paged_select(const b200_paged_kv *kv, const float *q, int64_t q_stride,
  *         at -inf are left out whatever their key and value hold.  A stride of
  *         0 gives every sequence the same row, as table_stride 0 does (here
  *         and in b200_paged_select).
- *   out   f32 [n_seq][n_head][head_dim], 16-byte aligned, apart from q; a
- *         sequence with no position gets zeros
+ *   out   f32 [n_seq][n_head][head_dim], 16-byte aligned, apart from q's rows
+ *         (B200_EINVAL); a sequence with no position gets zeros
  * Keys, values and queries may be infinite or NaN (b200_paged_store makes
  * infinities of values past the f16 range): a score of -inf has weight 0, and
  * zeros come out where every weight is 0; a score that is +inf or NaN makes its

@@ -50,6 +50,15 @@ int check_paged_batch(const b200_paged_kv* kv, const float* q, int64_t q_stride,
     return B200_OK;
 }
 
+// Whether `size` bytes at out meet one of n rows of `row` bytes, `stride` bytes
+// apart from q on.
+bool meets_rows(const void* out, int64_t size, const void* q, int64_t stride, int64_t row, int64_t n) {
+    const int64_t ahead = reinterpret_cast<intptr_t>(out) - reinterpret_cast<intptr_t>(q);
+    // the first row that ends behind out's first byte
+    const int64_t s = ahead < row ? 0 : n == 1 || stride == 0 ? n : (ahead - row) / stride + 1;
+    return s < n && s * stride < ahead + size;
+}
+
 bool g_paged_plan_attr[kMaxDevices];
 
 int launch_paged_plan(const PagedPlanArgs& a, cudaStream_t st) {
@@ -309,6 +318,8 @@ int b200_paged_attn(const b200_paged_kv* kv, const float* q, int64_t q_stride, i
         (sel && n_sel > (INT32_MAX - 4096) / kv->page_size) ||
         workspace_size < b200_paged_attn_workspace_size(kv->head_dim, n_seq, n_head, kv->n_head_kv))
         return B200_EINVAL;
+    const int64_t row = (int64_t)n_head * kv->head_dim * (int64_t)sizeof(float);
+    if (meets_rows(out, n_seq * row, q, q_stride * (int64_t)sizeof(float), row, n_seq)) return B200_EINVAL;
     const int64_t width = (int64_t)(sel ? n_sel : max_blocks) * kv->page_size;
     const int64_t segments = (int64_t)n_seq * kv->n_head_kv * paged_chunks(kv->head_dim, n_head, kv->n_head_kv);
     if (segments * ((width + kPaTok - 1) / kPaTok) > INT32_MAX / 2) return B200_EUNSUPPORTED;  // units are counted in int

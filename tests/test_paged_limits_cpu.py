@@ -189,3 +189,23 @@ def test_work_ranges_on_the_host(tmp_path):
     assert r.returncode == 0, r.stderr[-2000:]
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, (r.returncode, r.stdout)
+
+
+@no_device
+@pytest.mark.parametrize("n_seq,q_stride,out,meets", [
+    (2, 512, 0, True), (2, 512, 16, True), (2, 512, -16, True), (2, 512, 4096 - 16, True), (2, 512, -4096 + 16, True),
+    (2, 512, 4096, False), (2, 512, -4096, False), (1, 512, 2048, False), (1, 512, 2032, True), (1, 0, 2048, False),
+    (1, 0, -2048, False), (1, 0, 16, True),
+    # rows of a wider matrix: out behind the last row, in a gap of three rows, or past that
+    (3, 2048, 2 * 8192 + 2048, False), (3, 2048, 2 * 8192 + 2032, True), (1, 2048, 2048, False), (3, 2048, 2048, False),
+    (3, 2048, 2064, True),
+    (3, 2048, -6144, False), (3, 2048, -6144 + 16, True), (2, 4096, 2048, False), (2, 4096, 2032, True),
+    (2, 4096, 16384 - 4096, False), (2, 4096, 16384 - 4080, True)])
+def test_attn_refuses_an_output_that_meets_the_queries(n_seq, q_stride, out, meets):
+    """Rows of 4 heads x 128 f32, 2048 bytes; `out` bytes from the first query."""
+    bw = B()
+    kv = bw._PagedKVStruct(bw.TYPE_F16, 128, 2, 16, 8, PTR, PTR, 16 * 512, 512, 256, 16 * 512, 512, 256, None, None)
+    at = 1 << 20
+    rc = bw.lib().b200_paged_attn(C.byref(kv), at, q_stride, n_seq, 4, PTR, 4, 4, PTR, None, 0, None, 0, 1.0, at + out, PTR,
+                                  1 << 30, None)
+    assert (rc == bw.EINVAL) == meets
