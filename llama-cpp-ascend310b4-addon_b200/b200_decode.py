@@ -821,9 +821,9 @@ def paged_attn(cache: PagedKV, q, block_table, seq_lens, scale: float, mask=None
     q f32 [n_seq, n_head, head_dim]; block_table int32 [n_seq, max_blocks];
     seq_lens int32 [n_seq]; mask f16 [n_seq, >= max_blocks * page_size]
     additive or None; sel int32 [n_seq, n_head_kv, n_sel] (paged_select) or
-    None for every block.  Returns f32 [n_seq, n_head, head_dim] (out, which must
-    not overlap q); zeros where
-    nothing is attended to.  workspace: uint8 of paged_attn_workspace_size
+    None for every block.  block_table and mask may be one row expanded to the
+    batch.  Returns f32 [n_seq, n_head, head_dim] (out, which must not overlap q);
+    zeros where nothing is attended to.  workspace: uint8 of paged_attn_workspace_size
     bytes, zero-filled before its first use and not shared by calls that
     overlap on the GPU; allocated and cleared for this call when not given."""
     torch = _torch()

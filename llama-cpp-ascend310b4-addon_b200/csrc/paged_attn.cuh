@@ -16,9 +16,9 @@
 // ring of cp.async stages (each row of K and V found through the block table,
 // so any page size and layout works), never waiting for another warp; the
 // ring runs ahead across segment borders.  What decides the rate at the power
-// cap, where the SM clock is 1.5 GHz, is the instructions per unit (359 with
-// 16-row pages; with 539 the same stream was 17% slower), hence the fixed copy
-// steps and offsets and the single counter per side below.
+// cap, where the SM clock is 1.5 GHz, is the instructions per unit (about 375
+// with 16-row pages; with 539 the same stream was 17% slower), hence the fixed
+// copy steps and offsets and the single counter per side below.
 //
 // Join.  A segment inside one warp's range is written straight to the output.
 // The pieces of a cut segment meet in shared memory once per CTA, and those
@@ -36,8 +36,8 @@
 // rows of heads; mma.sync keeps the tensor pipe 19% busy.)
 //
 // Measured on a B200 whose copy runs at 6458 GB/s, 64/8 heads x 128, f16: 8
-// sequences of 32768 to 131072 tokens 507 us, 6.73 TB/s; 48 of 0 to 8192 120 us,
-// 5.98 TB/s; one of 4160 14.2 us, of which the start takes 3 us, two units per
+// sequences of 32768 to 131072 tokens 505 us, 6.76 TB/s; 48 of 0 to 8192 123 us,
+// 5.83 TB/s; one of 4160 14.9 us, of which the start takes 3 us, two units per
 // warp 3 us and joining the pieces 5 us.
 #pragma once
 

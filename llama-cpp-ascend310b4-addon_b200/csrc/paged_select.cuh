@@ -6,7 +6,7 @@
 // head the scores around the last place of the selection lie that close
 // together, so 32 bits would pick blocks by rounding.  But only the few
 // blocks around that place need 64 bits.  The first kernel reads all bounds
-// once and finds every score to within a proven eps on the tensor cores; the
+// once and finds every score to within a bound eps on the tensor cores; the
 // second finds the need-th largest of those, tau.  The exact need-th largest
 // score is within eps of tau, so a block above tau + 2 eps is chosen and one
 // below tau - 2 eps is not, whatever the rounding; the blocks in between
@@ -19,10 +19,11 @@
 // the f64 pipe and the selects that feed it.
 //
 // Measured: 26300 blocks x 8 KV heads x 128 dims (108 MB of bounds), 128 chosen
-// per head, 34.8 us: 17 us of stream at the copy rate and 8 us of start and
+// per head, 35.5 us: 17 us of stream at the copy rate and 8 us of start and
 // drain in the first kernel, 8 us in the second; all in 64 bits 292 us as a
-// plain kernel.  The error of the first kernel's scores was below 2% of eps over
-// 72 shapes and distributions.
+// plain kernel.  eps assumes how the tensor core truncates (below, where it is
+// computed); the error of the first kernel's scores was below 2% of eps over 72
+// shapes and distributions.
 #pragma once
 
 #include "../../include/b200_paged.h"
@@ -441,8 +442,9 @@ __global__ void __launch_bounds__(kTopkThreads) paged_topk_kernel(PagedSelectArg
     __syncthreads();
     // eps, with q' = q 2^-ex, whose largest entry is in [1, 2), M = max |bound| and
     // S = M max_j sum |q'_jd|: the parts of q' leave out at most 2^-23 of each
-    // entry, in all D 2^-23 M; a chain of four instructions (bf16: eight) truncates
-    // its 67 (135) terms below 2^-24 of the largest, in all 135 2^-24 S; adding high
+    // entry, in all D 2^-23 M; a chain of four instructions (bf16: eight) is assumed
+    // to truncate its 67 (135) terms below 2^-24 of the largest (no document says
+    // how the tensor core rounds), in all 135 2^-24 S; adding high
     // and low halves and the D / 32 chains rounds D / 32 + 1 times by 2^-24 S at
     // most.  1e-30 covers what underflows.
     const float biggest = BF16 ? __uint_as_float(s_top << 16) : h2f((uint16_t)s_top);

@@ -45,8 +45,10 @@ constexpr int kStoreRows = 2;   // rows a thread has in flight
 // row; a page's bounds are theirs alone, so they meet in shared memory once per
 // run, without atomics.  12 bytes per element; bound by the latency of slots,
 // then rows: with two rows a thread and 80 registers 8192 tokens x 8 x 128 take
-// 25.4 us (4.0 TB/s), 64 decode tokens 3.6 us; four rows a thread (126
-// registers, half the CTAs) took 31 and 6.0 us.
+// 24.3 us (4.2 TB/s), 64 decode tokens 3.85 us; four rows a thread (126
+// registers, half the CTAs) took 31 and 6.0 us.  Meant for pages of 16 to 64
+// rows: with pages of 1 the same tokens take 220 us (most lanes idle), with
+// pages of 2048 207 us (one CTA per page and head).
 template <bool BF16, int D>
 __global__ void __launch_bounds__(kStoreThreads, 6) paged_store_kernel(PagedStoreArgs a, int tile) {
     constexpr int LPR = D / 8;                // lanes per row, 8 values each
