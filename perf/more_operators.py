@@ -377,15 +377,13 @@ def _plain_fork(s):
     one = torch.ones_like(new)
     held = torch.zeros(n_pages + 1, dtype=torch.int64, device=dev)
     held.scatter_add_(0, new.reshape(-1), one.reshape(-1))
-    # pages that nobody holds any more, in the order of the rows that held them first
-    e = torch.arange(n * width, device=dev)
-    first = torch.full((n_pages + 1,), n * width, dtype=torch.int64, device=dev)
-    first.scatter_reduce_(0, old.reshape(-1), e, "amin")
-    freed = (old_live & (held[old] == 0)).reshape(-1) & (first[old.reshape(-1)] == e)
+    # pages that nobody holds any more, in ascending order
+    was = torch.zeros_like(held).scatter_add_(0, old.reshape(-1), one.reshape(-1))
+    freed = ((was > 0) & (held == 0))[:n_pages]
     n0 = s["n_free"].long()
     at = torch.where(freed, n0 + freed.cumsum(0) - 1, n_pages)
     stack = torch.cat([s["free_pages"], s["free_pages"].new_zeros(1)])
-    stack.scatter_(0, at, old.reshape(-1).int())
+    stack.scatter_(0, at, torch.arange(n_pages, device=dev).int())
     pool = n0 + freed.sum()
     # rows whose last page is not full need it alone
     tail = k % ps
@@ -530,13 +528,9 @@ def _exact_fork(s):
     for i, row in enumerate(new):
         for b, p in enumerate(row):
             holders.setdefault(p, []).append((i, (b + 1) * ps > got[i]))
-    seen = set()
-    for row, n in zip(old, lens):
-        for p in row[: _ceil(n, ps)]:
-            if p not in holders and p not in seen:
-                seen.add(p)
-                stack[top] = p
-                top += 1
+    for p in sorted({p for row, n in zip(old, lens) for p in row[: _ceil(n, ps)] if p not in holders}):
+        stack[top] = p
+        top += 1
     copies = []
     for i, row in enumerate(new):
         copies.append((-1, -1, 0))
