@@ -266,6 +266,25 @@ int b200_add_f32(const float *a, const float *b, float *y, int64_t n, b200_strea
  * n / nb rows of a (a norm weight). */
 int b200_mul_f32(const float *a, const float *b, float *y, int64_t n, int64_t nb, b200_stream_t stream);
 int b200_argmax_f32(const float *x, int64_t n, int32_t *out, b200_stream_t stream);
+/* Log probabilities of rows of logits (f32, f16 or B200_TYPE_BF16 values,
+ * `type`; row r at logits + r * ld elements, aligned to its type), in one pass:
+ *   logprob[r]          x[tokens[r]] - log sum_i exp(x[i]); 0 for a negative
+ *                       token, and for one past the vocabulary, which is
+ *                       recorded (B200_DEVSTATUS_BOUNDS).  NULL with tokens.
+ *   entropy[r]          -sum_i p_i log p_i in nats, p = softmax(x); or NULL
+ *   top_ids[r][i], top_logprobs[r][i], i < k (contiguous): the k largest
+ *                       logits in descending order, ties by the lower id, NaN
+ *                       last; k = 0: none (NULL both)
+ * Tokens ruled out by a logit of -inf have probability 0.  A row with a NaN or
+ * +inf, or with nothing but -inf, has NaN for every logprob and its entropy.
+ * Sums are kept in 32 bits per thread and joined in a fixed order; the largest
+ * logit is left out of them, so that log probabilities near 0 keep their
+ * digits.  0 <= k <= min(B200_LOGPROBS_MAX_K, n_vocab), 1 <= n_vocab < 2^31
+ * (B200_EINVAL). */
+#define B200_LOGPROBS_MAX_K 32
+int b200_token_logprobs(const void *logits, int type, int64_t ld, int64_t n_rows, int64_t n_vocab,
+                        const int32_t *tokens, int k, float *logprob, float *entropy, int32_t *top_ids,
+                        float *top_logprobs, b200_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Weight upload in chunks.  Replaces the reference's TensorSetTracker and the

@@ -1,8 +1,8 @@
 /*
- * b200_paged.h -- C ABI of batched single-token decode over a paged
- * key-value cache: page allocation and slot maps, the K/V store, block
- * selection for sparse attention, and attention of one new token per
- * sequence.
+ * b200_paged.h -- C ABI of batched decode over a paged key-value cache: page
+ * allocation and slot maps, the K/V store, block selection for sparse
+ * attention, attention of one new token per sequence and of chunks of new
+ * tokens, sequences that share pages, and copies of pages.
  *
  * The conventions are those of b200_decode.h: plain C, device pointers of the
  * device current on the calling thread, byte strides where stated, an int
@@ -165,6 +165,85 @@ int b200_paged_attn(const b200_paged_kv *kv, const float *q, int64_t q_stride, i
                     const int32_t *block_table, int64_t table_stride, int max_blocks, const int32_t *seq_lens,
                     const void *mask, int64_t mask_stride, const int32_t *sel, int n_sel, float scale, float *out,
                     void *workspace, size_t workspace_size, b200_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Attention of a chunk of new tokens per sequence (prompts, draft tokens; the
+ * rows of one b200_paged_plan step whose K and V are stored):
+ *   out[t][j] = sum_p w_p v_p / sum_p w_p,
+ *   w_p = exp(scale * q[t][j] . k_p + mask[s][p])
+ * for the token rows t = cu[s] + i of sequence s, i < n = cu[s + 1] - cu[s].
+ * The sequence's seq_lens[s] tokens include these n, so row t stands at
+ * position P = seq_lens[s] - n + i and sees the positions p <= P, with
+ * window > 0 only those with p > P - window.
+ *   q     16-bit values of the cache's type, row t at q + t * q_stride
+ *         (elements, a multiple of 8), heads [n_head][head_dim] contiguous,
+ *         16-byte aligned
+ *   cu    int32 [n_seq + 1], ascending, within [0, n_tokens]; the rows before
+ *         cu[0] and from cu[n_seq] on are neither read nor written.  Other
+ *         values are clamped and recorded (B200_DEVSTATUS_BOUNDS).
+ *   mask  as in b200_paged_attn: one row per sequence
+ *   out   16-bit values of the cache's type [n_tokens][n_head][head_dim],
+ *         16-byte aligned, apart from q's rows (B200_EINVAL); a row that sees no
+ *         position gets zeros
+ * A sequence that b200_paged_plan did not serve has rows in cu but its old
+ * length: its rows come out as if its last n tokens were the new ones.
+ * Scores, weights' sums and outputs are kept in 32 bits; the weights enter the
+ * product with V rounded to the cache's type, as the output is.  Infinities and
+ * NaN as in b200_paged_attn, where a weight counts as 0 below 2^-24 of the
+ * largest for f16, 2^-120 for bf16; a position that a row does not see leaves no
+ * trace in it.  n_tokens * n_head < 2^31 (B200_EUNSUPPORTED).
+ * workspace: 16-byte aligned, no initial contents needed, not shared by calls
+ * that overlap on the GPU. */
+size_t b200_paged_prefill_workspace_size(int head_dim, int64_t n_tokens, int n_seq, int n_head, int n_head_kv);
+int b200_paged_prefill(const b200_paged_kv *kv, const void *q, int64_t q_stride, int64_t n_tokens, int n_head,
+                       const int32_t *block_table, int64_t table_stride, int n_seq, int max_blocks,
+                       const int32_t *seq_lens, const int32_t *cu, const void *mask, int64_t mask_stride, int window,
+                       float scale, void *out, void *workspace, size_t workspace_size, b200_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Sequences that fork, change places, give tokens back or end: row s of the
+ * table becomes the first min(keep[s], seq_lens[src[s]]) tokens of row src[s]
+ * as it was before the call (src[s] < 0: an empty row).  Rows that go on
+ * unchanged name themselves and their length; a row may be named any number
+ * of times.  Full pages are shared: from then on a page may stand in several
+ * rows, and it goes back to the stack when a call leaves it in none (in
+ * ascending order of pages, on top of free_pages[n_free[0]]).  The page of a
+ * block that is not full receives the next tokens, so it stays with one row:
+ * the lowest of those that end in it, if no row holds it in full.  Every other
+ * row gets a page from the top of the stack (in ascending order of rows) and
+ * an entry in the copy list, for b200_paged_copy on every layer's cache before
+ * the next store: copy_src[s], copy_dst[s] and copy_rows[s] (-1, -1, 0 for a
+ * row without one).  Without a page left a row ends with its last full block.
+ *   block_table, table_out  int32 [n_seq][max_blocks] with row strides of at
+ *         least max_blocks, the same tensor (and stride) or apart; entries past
+ *         a row's new blocks become -1
+ *   seq_lens_out, n_free_out  may be seq_lens and n_free; with all three apart
+ *         the call can be repeated
+ * Every owner of a page has to be a row of this table: a prefix that is kept
+ * for later is a row like any other.  A row that shares pages must end here
+ * (src < 0), not by a negative new_lens of b200_paged_plan, which would hand
+ * its pages out again.  Pages out of range stay in their row and are passed over
+ * (B200_DEVSTATUS_BOUNDS), as a src of n_seq or more, which counts as -1.
+ * workspace: 16-byte aligned, no initial contents needed, not shared by calls
+ * that overlap on the GPU.  n_seq * max_blocks < 2^31 (B200_EUNSUPPORTED). */
+size_t b200_paged_fork_workspace_size(int n_seq, int max_blocks, int64_t n_pages);
+int b200_paged_fork(const int32_t *src, const int32_t *keep, const int32_t *seq_lens, int n_seq,
+                    const int32_t *block_table, int64_t table_stride, int max_blocks, int page_size,
+                    int32_t *free_pages, int64_t n_pages, const int32_t *n_free, int32_t *table_out,
+                    int64_t table_out_stride, int32_t *seq_lens_out, int32_t *n_free_out, int32_t *copy_src,
+                    int32_t *copy_dst, int32_t *copy_rows, void *workspace, size_t workspace_size,
+                    b200_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Contents of pages: the first rows[i] rows (NULL: all) of K and V of page
+ * src[i], and where the cache has them the page's key bounds, to page dst[i],
+ * for i < n.  An entry with a negative src or dst, no rows or src = dst copies
+ * nothing; pages out of range are skipped and rows clamped
+ * (B200_DEVSTATUS_BOUNDS).  The pages of dst differ and none of them is in
+ * src.  The bounds of a page of which a part is copied are those of the whole
+ * page: still bounds of its keys. */
+int b200_paged_copy(const b200_paged_kv *kv, const int32_t *src, const int32_t *dst, const int32_t *rows, int64_t n,
+                    b200_stream_t stream);
 
 #ifdef __cplusplus
 }

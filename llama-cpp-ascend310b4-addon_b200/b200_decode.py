@@ -129,6 +129,7 @@ def _declare(L):
         "b200_swiglu_f32": (C.c_int, [P, P, P, I64, P]),
         "b200_add_f32": (C.c_int, [P, P, P, I64, P]),
         "b200_argmax_f32": (C.c_int, [P, I64, P, P]),
+        "b200_token_logprobs": (C.c_int, [P, C.c_int, I64, I64, I64, P, C.c_int, P, P, P, P, P]),
         "b200_paged_plan": (
             C.c_int,
             [P, P, C.c_int, P, I64, C.c_int, C.c_int, P, I64, P, I64, P, P, P, P, P, P],
@@ -144,6 +145,17 @@ def _declare(L):
             C.c_int,
             [P, P, I64, C.c_int, C.c_int, P, I64, C.c_int, P, P, I64, P, C.c_int, C.c_float, P, P, C.c_size_t, P],
         ),
+        "b200_paged_prefill_workspace_size": (C.c_size_t, [C.c_int, I64, C.c_int, C.c_int, C.c_int]),
+        "b200_paged_prefill": (
+            C.c_int,
+            [P, P, I64, I64, C.c_int, P, I64, C.c_int, C.c_int, P, P, P, I64, C.c_int, C.c_float, P, P, C.c_size_t, P],
+        ),
+        "b200_paged_fork_workspace_size": (C.c_size_t, [C.c_int, C.c_int, I64]),
+        "b200_paged_fork": (
+            C.c_int,
+            [P, P, P, C.c_int, P, I64, C.c_int, C.c_int, P, I64, P, P, I64, P, P, P, P, P, P, C.c_size_t, P],
+        ),
+        "b200_paged_copy": (C.c_int, [P, P, P, P, I64, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -567,6 +579,56 @@ def argmax(x):
     return out
 
 
+LOGPROBS_MAX_K = 32
+
+
+class TokenLogprobs:
+    """Result of token_logprobs."""
+
+    __slots__ = ("logprob", "entropy", "top_ids", "top_logprobs")
+
+    def __init__(self, logprob, entropy, top_ids, top_logprobs):
+        self.logprob, self.entropy, self.top_ids, self.top_logprobs = logprob, entropy, top_ids, top_logprobs
+
+
+def token_logprobs(logits, tokens=None, k: int = 0) -> TokenLogprobs:
+    """Log probabilities of given tokens under rows of logits, with the rows'
+    entropy and k most likely alternatives (b200_token_logprobs).
+
+    logits f32, f16 or bf16 [n_rows, n_vocab] with contiguous rows (a row
+    stride and an address of any alignment work); tokens int32 [n_rows]
+    (negative: none, log probability 0) or None.  Returns logprob f32 [n_rows]
+    (None without tokens), entropy f32 [n_rows] in nats, and for k > 0 top_ids
+    int32 and top_logprobs f32 [n_rows, k] in descending order, ties by the
+    lower id (None for k = 0; k at most LOGPROBS_MAX_K and n_vocab)."""
+    torch = _torch()
+    types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+    if logits.dtype not in types:
+        raise B200Unsupported(EUNSUPPORTED, f"token_logprobs of {logits.dtype}")
+    dev, shape = logits.device, logits.shape
+    if dev.type != "cuda" or len(shape) != 2 or shape[1] == 0 or (logits.stride(1) != 1 and shape[1] > 1):
+        _bad("token_logprobs", "logits must be [n_rows, n_vocab] with contiguous rows on a CUDA device")
+    rows, vocab = shape
+    if not 0 <= k <= min(LOGPROBS_MAX_K, vocab):
+        _bad("token_logprobs", f"k must be from 0 to {min(LOGPROBS_MAX_K, vocab)}")
+    if rows > 1 and logits.stride(0) < vocab:
+        logits = logits.contiguous()  # rows that overlap, as an expanded one
+    i32 = torch.int32
+    logprob = top_ids = top_logprobs = None
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    if tokens is not None:
+        if tokens.dtype != i32 or tokens.device != dev or tokens.shape != shape[:1] or not tokens.is_contiguous():
+            _bad("token_logprobs", "tokens must be a contiguous int32 [n_rows] on the logits' device")
+        logprob = torch.empty_like(entropy)
+    if k:
+        top_ids = torch.empty((rows, k), dtype=i32, device=dev)
+        top_logprobs = torch.empty((rows, k), dtype=torch.float32, device=dev)
+    _launch("token_logprobs", dev, lib().b200_token_logprobs, logits.data_ptr(), types[logits.dtype], logits.stride(0),
+            rows, vocab, None if tokens is None else tokens.data_ptr(), k,
+            *(None if t is None else t.data_ptr() for t in (logprob, entropy, top_ids, top_logprobs)))
+    return TokenLogprobs(logprob, entropy, top_ids, top_logprobs)
+
+
 def kv_lengths_from_mask(mask_f16: np.ndarray) -> np.ndarray:
     m = np.ascontiguousarray(mask_f16, dtype=np.float16)
     if m.ndim == 1:
@@ -581,10 +643,12 @@ def kv_lengths_from_mask(mask_f16: np.ndarray) -> np.ndarray:
 
 
 # ------------------------------------------------- paged key-value cache
-# Batched single-token decode over fixed-size pages (include/b200_paged.h):
-# one step is paged_plan (pages and slots for the step's tokens), then per
-# layer paged_store (the layer's K/V rows into their slots) and paged_attn,
-# for long contexts with paged_select before it.  Every call is asynchronous
+# Batched decode over fixed-size pages (include/b200_paged.h): one step is
+# paged_plan (pages and slots for the step's tokens), then per layer paged_store
+# (the layer's K/V rows into their slots) and paged_attn, for long contexts with
+# paged_select before it, or paged_prefill where sequences append several tokens.
+# Between steps paged_fork lets sequences share pages and paged_copy copies the
+# pages that they cannot share.  Every call is asynchronous
 # on the current stream and may be captured into a CUDA graph; what varies
 # from step to step (lengths, tables, free pages) stays on the device.
 
@@ -858,3 +922,143 @@ def paged_attn(cache: PagedKV, q, block_table, seq_lens, scale: float, mask=None
             block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), mask_ptr,
             mask_stride, sel_ptr, n_sel, scale, out.data_ptr(), workspace.data_ptr(), workspace.numel())
     return out
+
+
+def paged_prefill_workspace_size(head_dim: int, n_tokens: int, n_seq: int, n_head: int, n_head_kv: int) -> int:
+    return int(lib().b200_paged_prefill_workspace_size(head_dim, n_tokens, n_seq, n_head, n_head_kv))
+
+
+def paged_prefill(cache: PagedKV, q, block_table, seq_lens, cu, scale: float, mask=None, window: int = 0, out=None,
+                  workspace=None):
+    """Attention of a chunk of new tokens per sequence over its cached tokens,
+    the new ones among them (stored before): prompts, draft tokens, and single
+    tokens beside them.
+
+    q [n_tokens, n_head, head_dim] of the cache's type (rows may be strided);
+    block_table int32 [n_seq, max_blocks]; seq_lens int32 [n_seq] with the new
+    tokens; cu int32 [n_seq + 1] (paged_plan): the rows of sequence s are
+    cu[s] .. cu[s + 1] - 1, the last at position seq_lens[s] - 1, and each sees
+    the positions up to its own, with window > 0 the last window of them.  mask
+    f16 [n_seq, >= max_blocks * page_size], additive over positions, or None.
+    Returns out [n_tokens, n_head, head_dim] of the cache's type (apart from
+    q); rows that no sequence has are left as they are, rows that see nothing
+    become zero.  workspace: uint8 of paged_prefill_workspace_size bytes, not
+    shared by calls that overlap on the GPU; allocated when not given."""
+    torch = _torch()
+    dev, dtype, shape = cache.device, cache.k.dtype, q.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim or q.dtype != dtype or q.device != dev:
+        _bad("paged_prefill", "q must be [n_tokens, n_head, head_dim] of the cache's type and device")
+    n_tokens, n_head, d = shape
+    if n_head == 0 or n_head % cache.n_head_kv:
+        _bad("paged_prefill", "n_head must be a multiple of the cache's n_head_kv")
+    row = n_head * d
+    strides = q.stride()
+    if strides[2] != 1 or (strides[1] != d and n_head > 1) or strides[0] % 8 or q.data_ptr() % 16 \
+            or (n_tokens > 1 and strides[0] < row):
+        q = q.clone(memory_format=torch.contiguous_format)
+        strides = q.stride()
+    i32, ts = torch.int32, block_table.shape
+    if (block_table.dtype != i32 or block_table.device != dev or len(ts) != 2 or ts[1] == 0
+            or block_table.stride(1) != 1 or seq_lens.dtype != i32 or seq_lens.device != dev
+            or seq_lens.shape != ts[:1] or not seq_lens.is_contiguous() or cu.dtype != i32 or cu.device != dev
+            or cu.dim() != 1 or cu.numel() < ts[0] + 1 or not cu.is_contiguous()):
+        _bad("paged_prefill", "block_table must be int32 [n_seq, max_blocks] with contiguous rows, seq_lens int32 "
+                              "[n_seq] and cu int32 [n_seq + 1], on the cache's device")
+    if window < 0 or window >= 2**31:
+        _bad("paged_prefill", "window must be from 0 to 2^31 - 1")
+    if mask is None:
+        mask_ptr, mask_stride = None, 0
+    else:
+        if (mask.dtype != torch.float16 or mask.device != dev or mask.dim() != 2 or mask.shape[0] != ts[0]
+                or mask.shape[1] < ts[1] * cache.page_size or mask.stride(1) != 1):
+            _bad("paged_prefill", "mask must be f16 [n_seq, >= max_blocks * page_size] with contiguous rows")
+        mask_ptr, mask_stride = mask.data_ptr(), mask.stride(0)
+    if out is None:
+        out = torch.empty((n_tokens, n_head, d), dtype=dtype, device=dev)
+    elif out.dtype != dtype or out.device != dev or not out.is_contiguous() or out.shape != shape:
+        _bad("paged_prefill", "out must be a contiguous [n_tokens, n_head, head_dim] of the cache's type")
+    if workspace is None:
+        size = paged_prefill_workspace_size(d, n_tokens, ts[0], n_head, cache.n_head_kv)
+        workspace = torch.empty(size, dtype=torch.uint8, device=dev)
+    else:
+        _check_workspace("paged_prefill", workspace, dev)
+    _launch("paged_prefill", dev, lib().b200_paged_prefill, cache._ref, q.data_ptr(), strides[0], n_tokens, n_head,
+            block_table.data_ptr(), block_table.stride(0), ts[0], ts[1], seq_lens.data_ptr(), cu.data_ptr(), mask_ptr,
+            mask_stride, window, scale, out.data_ptr(), workspace.data_ptr(), workspace.numel())
+    return out
+
+
+class PagedFork:
+    """Result of paged_fork."""
+
+    __slots__ = ("block_table", "seq_lens", "n_free", "copy_src", "copy_dst", "copy_rows")
+
+    def __init__(self, block_table, seq_lens, n_free, copy_src, copy_dst, copy_rows):
+        self.block_table, self.seq_lens, self.n_free = block_table, seq_lens, n_free
+        self.copy_src, self.copy_dst, self.copy_rows = copy_src, copy_dst, copy_rows
+
+
+def paged_fork_workspace_size(n_seq: int, max_blocks: int, n_pages: int) -> int:
+    return int(lib().b200_paged_fork_workspace_size(n_seq, max_blocks, n_pages))
+
+
+def paged_fork(src, keep, seq_lens, block_table, free_pages, n_free, page_size: int, table_out=None,
+               seq_lens_out=None, n_free_out=None, workspace=None) -> PagedFork:
+    """Rows of the block table become prefixes of other rows: forks, beams that
+    change places, rejected tokens taken back, sequences that end.
+
+    Row s gets the first min(keep[s], seq_lens[src[s]]) tokens of row src[s] as
+    it was (src int32 [n_seq], negative: an empty row; keep int32 [n_seq]).
+    Full pages are shared; the page of a last block that is not full stays with
+    the lowest of the rows that end in it (if none holds it in full), the others
+    get a free page each and an entry in the copy list.  Pages that no row holds
+    any more go back to the stack.  block_table, seq_lens and n_free are updated
+    in place unless table_out, seq_lens_out and n_free_out are given.  Returns
+    those with copy_src, copy_dst and copy_rows int32 [n_seq] (-1, -1, 0: nothing
+    to copy), for paged_copy on the cache of every layer.  A sequence that shares
+    pages must end here, not by paged_plan.  workspace: uint8 of
+    paged_fork_workspace_size bytes, not shared by calls that overlap on the
+    GPU; allocated when not given."""
+    torch = _torch()
+    dev, i32, shape, table = seq_lens.device, torch.int32, seq_lens.shape, block_table.shape
+    if len(shape) != 1 or dev.type != "cuda" or shape[0] == 0 or src.shape != shape or keep.shape != shape:
+        _bad("paged_fork", "src, keep and seq_lens must be [n_seq] on a CUDA device, n_seq >= 1")
+    n = shape[0]
+    table_out = block_table if table_out is None else table_out
+    seq_lens_out = seq_lens if seq_lens_out is None else seq_lens_out
+    n_free_out = n_free if n_free_out is None else n_free_out
+    for t in (block_table, table_out):
+        if (t.dtype != i32 or t.device != dev or len(t.shape) != 2 or t.shape != table or t.shape[0] != n
+                or t.shape[1] == 0 or t.stride(1) != 1):
+            _bad("paged_fork", "block_table and table_out must be int32 [n_seq, max_blocks] with contiguous rows")
+    for t in (src, keep, seq_lens, seq_lens_out, free_pages, n_free, n_free_out):
+        if t.dtype != i32 or t.device != dev or not t.is_contiguous() or t.dim() != 1:
+            _bad("paged_fork", "src, keep, seq_lens, free_pages and n_free must be contiguous int32 vectors on one device")
+    if seq_lens_out.shape != shape or n_free.numel() != 1 or n_free_out.numel() != 1 or free_pages.numel() == 0:
+        _bad("paged_fork", "seq_lens_out must be [n_seq], n_free and n_free_out [1], free_pages [n_pages]")
+    if workspace is None:
+        size = paged_fork_workspace_size(n, table[1], free_pages.numel())
+        workspace = torch.empty(size, dtype=torch.uint8, device=dev)
+    else:
+        _check_workspace("paged_fork", workspace, dev)
+    copies = torch.empty((3, n), dtype=i32, device=dev)
+    at = copies.data_ptr()
+    _launch("paged_fork", dev, lib().b200_paged_fork, src.data_ptr(), keep.data_ptr(), seq_lens.data_ptr(), n,
+            block_table.data_ptr(), block_table.stride(0), table[1], page_size, free_pages.data_ptr(),
+            free_pages.numel(), n_free.data_ptr(), table_out.data_ptr(), table_out.stride(0), seq_lens_out.data_ptr(),
+            n_free_out.data_ptr(), at, at + 4 * n, at + 8 * n, workspace.data_ptr(), workspace.numel())
+    return PagedFork(table_out, seq_lens_out, n_free_out, *copies.unbind(0))
+
+
+def paged_copy(cache: PagedKV, src, dst, rows=None):
+    """Pages src[i] of the cache to pages dst[i] (int32 [n]; an entry with a
+    negative one is skipped): the first rows[i] rows of K and V (int32 [n];
+    None: all) and the page's key bounds.  The pages of dst differ and none of
+    them is in src, as paged_fork makes them."""
+    torch = _torch()
+    dev = cache.device
+    for t in (src, dst) if rows is None else (src, dst, rows):
+        if t.dtype != torch.int32 or t.device != dev or t.dim() != 1 or t.shape != src.shape or not t.is_contiguous():
+            _bad("paged_copy", "src, dst and rows must be contiguous int32 [n] on the cache's device")
+    _launch("paged_copy", dev, lib().b200_paged_copy, cache._ref, src.data_ptr(), dst.data_ptr(),
+            None if rows is None else rows.data_ptr(), src.numel())

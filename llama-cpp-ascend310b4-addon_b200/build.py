@@ -11,6 +11,7 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -23,6 +24,7 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 SOURCES = [
     "kernels.cu",
+    "scoring.cu",
     "host.cpp",
     "model.cpp",
     "upload.cpp",
@@ -41,12 +43,19 @@ def nvcc() -> str:
 
 
 def _deps(src: str) -> list[str]:
-    """The source and the headers it may include: host .cpp files see only
-    the .h headers; the device unit (.cu) sees every header."""
-    host = src.endswith(".cpp")
-    own = [os.path.join(CSRC, f) for f in os.listdir(CSRC)
-           if f == src or f.endswith(".h") or (not host and f.endswith(".cuh"))]
-    return own + [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE)]
+    """The source and every file it includes by a quoted name, in turn."""
+    seen, todo = [], [os.path.join(CSRC, src)]
+    while todo:
+        path = todo.pop()
+        if path in seen or not os.path.exists(path):
+            continue
+        seen.append(path)
+        with open(path) as f:
+            names = re.findall(r'^\s*#include "([^"]+)"', f.read(), re.M)
+        for name in names:
+            here = os.path.normpath(os.path.join(os.path.dirname(path), name))
+            todo.append(here if os.path.exists(here) else os.path.join(INCLUDE, name))
+    return seen
 
 
 def _compile(src: str, force: bool) -> str:

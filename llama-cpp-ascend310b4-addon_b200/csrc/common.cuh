@@ -14,12 +14,13 @@
 namespace b200 {
 
 // Device status word: kernels OR a B200_DEVSTATUS_* bit in when a bounded wait
-// expires or a runtime bound check fails.  Read with b200_device_status().
-__device__ unsigned int g_status;
+// expires or a runtime bound check fails.  Read with b200_device_status(),
+// which joins the words of the device translation units (one each).
+static __device__ unsigned int g_status;
 
 // Limit of one bounded wait in nanoseconds (2 s unless b200_set_wait_timeout
 // changed it for this device).
-__device__ unsigned long long g_wait_timeout_ns = 2000000000ull;
+static __device__ unsigned long long g_wait_timeout_ns = 2000000000ull;
 
 // True once any bounded wait on this device has expired (the status word's
 // TIMEOUT bit, read without caching).  Waits that depend on another kernel,

@@ -32,3 +32,8 @@ int b200i_finish(b200::StepState* state, cudaStream_t st);
 // A quantised-activation image (GemvArgs::xq_in layout, U blocks) as ggml
 // block_q8_0 rows (U x 34 bytes).
 int b200i_image_to_q8_0(const uint8_t* img, int64_t U, uint8_t* out, cudaStream_t st);
+
+// The device status word and the wait limit of the second device translation
+// unit (scoring.cu): ORs its word into *status, clears it on request.
+int b200i_scoring_status(unsigned int* status, int reset);
+int b200i_scoring_timeout(unsigned long long ns);

@@ -21,6 +21,7 @@
 #include "gemm_small.cuh"
 #include "gemm_tc.cuh"
 #include "gemv.cuh"
+#include "host_util.h"
 #include "internal.h"
 #include "model_ops.cuh"
 #include "ops.cuh"
@@ -29,18 +30,11 @@ using namespace b200;
 
 namespace {
 
-constexpr int kMaxDevices = 64;
 constexpr size_t kSmemBudget = 200 * 1024;
 
 int g_sms[kMaxDevices];
 std::mutex g_attr_mu;
 bool g_attr_done[kMaxDevices][5][2][9][2];
-
-int current_device() {
-    int d = 0;
-    cudaGetDevice(&d);
-    return d;
-}
 
 int sm_count(int dev) {
     if (dev < 0 || dev >= kMaxDevices) return 148;
@@ -61,20 +55,6 @@ int stage_cap() {
     }();
     return cap;
 }
-
-int cuda_status(cudaError_t e) {
-    if (e != cudaSuccess) {
-        fprintf(stderr, "b200_decode: CUDA error %s (%s)\n", cudaGetErrorName(e), cudaGetErrorString(e));
-        return B200_ECUDA;
-    }
-    return B200_OK;
-}
-
-#define CR_(x)                        \
-    do {                              \
-        const int r_ = (x);           \
-        if (r_ != B200_OK) return r_; \
-    } while (0)
 
 // Opts a GEMV instantiation into large dynamic shared memory, once per device.
 // Done before any stream capture (b200i_prepare_device) so that capturing a
@@ -122,14 +102,6 @@ size_t gemv_smem_bytes(int fmt, const GemvPlan& p, int stages, int64_t rows_per_
     return (size_t)gemv_x_bytes(fmt, p) + (size_t)kGemvWarps * stages * (size_t)p.stage_bytes +
            (size_t)kGemvWarps * stages * sizeof(uint64_t) + kGemvWarps * sizeof(double) +
            (p.rpc > 1 ? 0 : (size_t)(2 * rows_per_cta) * sizeof(float));
-}
-
-// Launch attribute for programmatic dependent launch (see b200i_gemv).
-cudaLaunchAttribute pdl_attr() {
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    return at;
 }
 
 template <int FMT, bool DEBUG, int UPL>
@@ -211,8 +183,6 @@ int launch_gemv_t(GemvArgs a, const GemvPlan& p, cudaStream_t st, bool pdl) {
     }
     return launch_gemv_u<FMT, DEBUG, 0>(a, p, st, pdl);
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // ggml rows -> packed rows (layout in args.h).  One thread per (row, unit).
 __global__ void repack_kernel(int type, const uint8_t* src0, const uint8_t* src1, int interleave, uint8_t* dst,
@@ -603,7 +573,8 @@ const char* b200_strerror(int code) {
 
 int b200_set_wait_timeout(uint64_t ns) {
     const unsigned long long v = ns == 0 ? 2000000000ull : (unsigned long long)ns;
-    return cuda_status(cudaMemcpyToSymbol(g_wait_timeout_ns, &v, sizeof(v)));
+    CR_(cuda_status(cudaMemcpyToSymbol(g_wait_timeout_ns, &v, sizeof(v))));
+    return b200i_scoring_timeout(v);
 }
 
 int b200_tp_allreduce_f32(float* x, const float* const* parts, int world, int rank, int64_t n,
@@ -638,9 +609,9 @@ int b200_device_status(unsigned int* status, int reset) {
     if (rc) return rc;
     if (reset) {
         const unsigned int z = 0;
-        rc = cuda_status(cudaMemcpyToSymbol(g_status, &z, sizeof(unsigned int)));
+        CR_(cuda_status(cudaMemcpyToSymbol(g_status, &z, sizeof(unsigned int))));
     }
-    return rc;
+    return b200i_scoring_status(status, reset);
 }
 
 int64_t b200_packed_row_stride(int type, int64_t n, int64_t k) {
