@@ -25,6 +25,7 @@
 #include "args.h"
 #include "common.cuh"
 #include "gemm_small.cuh"  // tma_load_2d
+#include "tcgen05.cuh"
 
 namespace b200 {
 
@@ -42,52 +43,12 @@ struct TcArgs {
 B200_HD constexpr uint32_t tc_stage_bytes(int bn) { return (uint32_t)(kTcBM + bn) * 128u; }
 B200_HD constexpr size_t tc_smem_bytes(int bn) { return (size_t)kTcStages * tc_stage_bytes(bn) + 1024; }
 
-// Shared-memory matrix descriptor of a K-major operand tile in the 128-byte
-// swizzle layout: rows of 128 bytes, 8-row groups 1024 bytes apart (stride
-// byte offset), start address 1024-aligned (base offset 0), descriptor
-// version 1 (bits 46-47), layout 2 = 128-byte swizzle (bits 61-63).  The
-// leading byte offset is unused for this layout (one swizzle row spans the
-// stage's K).  Advancing K by 16 halves within the row adds 32 bytes to the
-// start address (2 in its 16-byte units).
-__device__ __forceinline__ uint64_t tc_desc_sw128(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-
 // Instruction descriptor of kind::f16: D f32 (bits 4-5 = 1), A and B f16
 // (bits 7-9, 10-12 = 0), both K-major (bits 15, 16 = 0), N >> 3 in bits
 // 17-22, M >> 4 in bits 24-28.
 template <int BN>
 __device__ __forceinline__ constexpr uint32_t tc_idesc_f16() {
     return (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kTcBM >> 4) << 24);
-}
-
-__device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, uint64_t da, uint64_t db, uint32_t idesc, int acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(da), "l"(db), "r"(idesc), "r"(acc));
-}
-
-// Arrives on `bar` once every tcgen05 operation this thread issued before
-// has completed.
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// 16 consecutive 32-bit columns of this warp's 32 lanes (lane = thread).
-__device__ __forceinline__ void tc_ld_x16(uint32_t (&r)[16], uint32_t taddr) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 // K runs in segments of kTcSegKb k-blocks (512 halves).  A segment's MMAs

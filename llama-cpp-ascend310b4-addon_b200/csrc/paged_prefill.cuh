@@ -1,11 +1,21 @@
 // paged_prefill.cuh -- attention of a chunk of new tokens per sequence over the
-// paged cache.
+// paged cache, on the 5th-generation tensor cores.
+//
+// Rows are (token, query head of the KV head) pairs, flat within a sequence and
+// a KV head: every one of them reads the same keys, so a tile of 128 rows is full
+// whatever the number of heads to a KV head.  A unit is one or two such tiles of
+// one (sequence, KV head) with the tiles of keys that any of its rows sees; a
+// launch lays all units end to end (plan kernel), cuts the line of key tiles into
+// equal ranges, one per SM, whatever lengths and heads are (main kernel), and
+// joins the units that a cut went through (finish kernel).  Three launches, a few
+// hundred bytes of schedule, results that do not depend on timing.
 #pragma once
 
 #include "../../include/b200_paged.h"
 #include "args.h"
 #include "common.cuh"
 #include "paged_store.cuh"
+#include "tcgen05.cuh"
 
 namespace b200 {
 
@@ -21,7 +31,29 @@ struct PagedPrefillArgs {
     uint16_t* out;
     int n_tokens, n_head, group, n_seq, max_blocks, window;
     float scale;
+    // workspace
+    struct PfHeader* header;
+    int4* desc;         // two per unit: {sequence, first flat row, first key tile, key tiles}, {first, n, len, -}
+    int64_t* prefix;    // [units + 1] key tiles of the units before
+    int2* bad;          // rows to compute again: {flat (token, head), unit}
+    float4* piece_ml;   // [2 * CTAs][tiles][128] {reference, sum, mask reference, -} of cut units
+    float4* piece_o;    // [2 * CTAs][tiles][D / 4][128] their sums of weighted values
 };
+
+struct PfHeader {
+    int64_t total;    // key tiles of all units of one KV head
+    int64_t per_cta;  // of all KV heads' units, to a CTA
+    int units, n_bad;
+};
+
+constexpr int kPfCtas = 148;   // one per SM
+constexpr int kPfRows = 128;   // rows of a tile: the lanes of tensor memory
+// Key tiles and row tiles of a unit by head dim: two row tiles take turns between
+// the tensor core and the exponentials; at head dim 256 the outputs of one fill
+// half of tensor memory, and two score buffers of 64 keys take its place.
+B200_HD constexpr int pf_tiles(int d) { return d == 256 ? 1 : 2; }
+B200_HD constexpr int pf_keys(int d) { return d == 256 ? 64 : 128; }
+B200_HD constexpr int pf_stages(int d) { return d == 64 ? 8 : 5; }
 
 // The tokens of sequence s: rows first .. first + n - 1 of q, the last of them
 // at position len - 1.
@@ -102,22 +134,742 @@ __device__ void pf_row(const PagedPrefillArgs& a, int s, const PfSeq& sq, int i,
             sum == 0.f ? 0u : pack16<BF16>(o[e] * inv, o[e + 1] * inv);
 }
 
-// A warp per (row, head).
-template <bool BF16, int D>
-__global__ void __launch_bounds__(256) paged_prefill_rows_kernel(const __grid_constant__ PagedPrefillArgs a) {
-    const int64_t task = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t t = task / a.n_head;
-    const int head = (int)(task - t * a.n_head);
-    if (t >= a.n_tokens) return;
-    int lo = 0, hi = a.n_seq;  // the sequence of row t: cu[lo] <= t < cu[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.cu[mid] <= t) lo = mid;
-        else hi = mid;
+// ------------------------------------------------------------------- plan
+
+// Exclusive sum of v over the CTA's 1024 threads; the total in *total.
+__device__ __forceinline__ int64_t pf_scan(int64_t v, int64_t* part, int64_t* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
     }
-    const PfSeq sq = pf_seq(a, lo, head == 0 && (threadIdx.x & 31) == 0);
-    if (t < sq.first || t >= sq.first + sq.n) return;
-    pf_row<BF16, D>(a, lo, sq, (int)(t - sq.first), head);
+    __syncthreads();
+    if (lane == 31) part[warp] = x;
+    __syncthreads();
+    const int64_t w = part[lane];
+    int64_t sum = w, before = lane < warp ? w : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    *total = sum;
+    return before + x - v;
+}
+
+constexpr int kPfPlanThreads = 1024;
+
+// The units of one KV head in order of sequences and rows.  One CTA: latency only.
+__global__ void __launch_bounds__(kPfPlanThreads) paged_prefill_plan_kernel(const __grid_constant__ PagedPrefillArgs a,
+                                                                            int rows, int keys) {
+    __shared__ int64_t part[32], s_base[kPfPlanThreads + 1];
+    __shared__ PfSeq s_seq[kPfPlanThreads];
+    const int tid = threadIdx.x;
+    int64_t units = 0, tiles = 0, sum;
+    for (int base = 0; base < a.n_seq; base += kPfPlanThreads) {
+        const int s = base + tid, count = min(kPfPlanThreads, a.n_seq - base);
+        PfSeq q = {0, 0, 0};
+        if (s < a.n_seq) q = pf_seq(a, s, true);
+        const int64_t at = pf_scan(((int64_t)q.n * a.group + rows - 1) / rows, part, &sum);
+        s_base[tid] = at;
+        s_seq[tid] = q;
+        if (tid == 0) s_base[count] = sum;
+        __syncthreads();
+        for (int64_t u0 = 0; u0 < sum; u0 += kPfPlanThreads) {
+            const int64_t u = u0 + tid;
+            int64_t cost = 0;
+            int4 d0, d1;
+            if (u < sum) {
+                int lo = 0, hi = count;  // s_base[lo] <= u < s_base[hi]
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (s_base[mid] <= u) lo = mid;
+                    else hi = mid;
+                }
+                const PfSeq t = s_seq[lo];
+                const int row0 = (int)(u - s_base[lo]) * rows;
+                const int row1 = (int)min((int64_t)row0 + rows, (int64_t)t.n * a.group) - 1;
+                const int at0 = t.len - t.n + row0 / a.group, at1 = t.len - t.n + row1 / a.group;
+                const int first = a.window > 0 ? max(0, max(-1, at0) - a.window + 1) / keys : 0;
+                cost = at1 < 0 ? 1 : at1 / keys - first + 1;
+                d0 = make_int4(base + lo, row0, first, (int)cost);
+                d1 = make_int4(t.first, t.n, t.len, 0);
+            }
+            int64_t more;
+            const int64_t before = tiles + pf_scan(cost, part, &more);
+            if (u < sum) {
+                a.desc[2 * (units + u)] = d0;
+                a.desc[2 * (units + u) + 1] = d1;
+                a.prefix[units + u] = before;
+            }
+            tiles += more;
+        }
+        units += sum;
+        __syncthreads();  // s_base and s_seq are read no more
+    }
+    if (tid == 0) {
+        a.prefix[units] = tiles;
+        const int64_t all = tiles * a.kv.n_head_kv;
+        a.header->total = tiles;
+        a.header->per_cta = max((int64_t)1, (all + kPfCtas - 1) / kPfCtas);
+        a.header->units = (int)units;
+        a.header->n_bad = 0;
+    }
+}
+
+// Largest u with prefix[u] <= x, for prefix[0] = 0 <= x < prefix[n]; a warp together.
+__device__ __forceinline__ int pf_find(const int64_t* prefix, int n, int64_t x) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = n;  // prefix[lo] <= x < prefix[hi]
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const unsigned below = __ballot_sync(0xffffffffu, at < hi && prefix[at] <= x);
+        const int last = 31 - __clz((int)below);
+        lo += last * step;
+        hi = min(hi, lo + step);
+    }
+    return lo;
+}
+
+// A unit, or the part of one that lies in a CTA's range.
+struct PfUnit {
+    int u, s, h, row0, first, n, len, tile0;  // tile0: the unit's first key tile
+    int tb, te, cost;                      // key tiles tb .. te - 1 of cost
+};
+// Walks over a range of the line of key tiles of all KV heads' units.
+struct PfWalk {
+    int64_t w, w1;
+    int u, h;
+    __device__ __forceinline__ bool next(const PagedPrefillArgs& a, int units, int64_t total, PfUnit& x) {
+        if (w >= w1) return false;
+        const int4 d0 = __ldg(a.desc + 2 * (int64_t)u), d1 = __ldg(a.desc + 2 * (int64_t)u + 1);
+        const int64_t start = h * total + __ldg(reinterpret_cast<const long long*>(a.prefix) + u);
+        x.u = u, x.s = d0.x, x.row0 = d0.y, x.tile0 = d0.z, x.cost = d0.w;
+        x.first = d1.x, x.n = d1.y, x.len = d1.z;
+        x.h = h;
+        x.tb = (int)(w - start);
+        x.te = (int)min((int64_t)x.cost, x.tb + (w1 - w));
+        w += x.te - x.tb;
+        if (x.te == x.cost && ++u == units) u = 0, ++h;
+        return true;
+    }
+};
+
+// ------------------------------------------------------------------- main
+
+template <int D>
+struct PfShared {
+    static constexpr int ST = pf_stages(D);
+    uint64_t q_full, q_empty, full[ST], empty[ST], s_full[2], p_ready[2], o_done[2], done;
+    uint32_t tmem;
+    int aborted, u, h;
+    float tmax[ST][4];                       // largest mask entry of each warp's rows
+    alignas(16) uint16_t bias[ST][pf_keys(D)];  // mask of the tile whose values a stage holds
+};
+template <int D>
+B200_HD constexpr int pf_stage_bytes() { return pf_keys(D) * D * 2; }
+template <int D>
+B200_HD constexpr int pf_q_bytes() { return pf_tiles(D) * kPfRows * D * 2; }
+template <int D>
+B200_HD constexpr int pf_smem() { return pf_q_bytes<D>() + pf_stages(D) * pf_stage_bytes<D>() + 1024; }
+
+// Place of key tile t's K and V in the order of loads K0 K1 V0 K2 V1 .. of n tiles.
+__device__ __forceinline__ int pf_k_place(int t) { return t == 0 ? 0 : 2 * t - 1; }
+__device__ __forceinline__ int pf_v_place(int t, int n) { return t == n - 1 ? 2 * n - 1 : 2 * t + 2; }
+
+__device__ __forceinline__ void pf_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// A warp's wait: the same answer for every lane.
+__device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
+}
+__device__ __forceinline__ void pf_cp16(uint32_t dst, const void* src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ float pf_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+constexpr int kPfThreads = 512;     // two softmax warpgroups, copies, tensor-core issue
+constexpr int kPfLag = 2;           // tiles of copies in flight behind the one being issued
+constexpr float kPfLazy = 8.f;      // the reference stays until the maximum passes it by 2^8
+// f16 weights are taken times 2^7: 2^15 at most with the lazy reference, and 2^-31 of
+// the reference is still a value
+template <bool BF16>
+constexpr float kPfShift = BF16 ? 0.f : 7.f;
+
+template <bool BF16, int D, bool MASK>
+__global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __grid_constant__ PagedPrefillArgs a) {
+    constexpr int NT = pf_tiles(D), KT = pf_keys(D), ST = pf_stages(D), STAGE = pf_stage_bytes<D>();
+    constexpr int QTILE = kPfRows * D * 2, QHALF = kPfRows * 128, KHALF = KT * 128;
+    constexpr uint32_t O_COL = NT == 2 ? 2 * KT : 256;  // scores from column 0, outputs from here
+    constexpr uint32_t S_STEP = NT == 2 ? KT : 128;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ PfShared<D> sh;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, role = warp >> 2;
+    const uint32_t q_smem = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = q_smem + pf_q_bytes<D>();
+
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        mbar_init(&sh.q_full, 128);
+        mbar_init(&sh.q_empty, 1);
+        for (int i = 0; i < ST; ++i) mbar_init(&sh.full[i], 128), mbar_init(&sh.empty[i], 1);
+        for (int j = 0; j < 2; ++j) mbar_init(&sh.s_full[j], 1), mbar_init(&sh.p_ready[j], 4), mbar_init(&sh.o_done[j], 1);
+        mbar_init(&sh.done, 1);
+        sh.aborted = 0;
+        mbar_fence_init();
+    }
+    griddep_wait();  // the schedule
+    const int units = a.header->units;
+    const int64_t total = a.header->total, per_cta = a.header->per_cta;
+    PfWalk walk;
+    walk.w = min(total * a.kv.n_head_kv, per_cta * blockIdx.x);
+    walk.w1 = min(total * a.kv.n_head_kv, walk.w + per_cta);
+    if (warp == 0 && walk.w < walk.w1) {
+        const int h = (int)(walk.w / total), u = pf_find(a.prefix, units, walk.w - h * total);
+        if (lane == 0) sh.h = h, sh.u = u;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    walk.u = sh.u, walk.h = sh.h;
+    const uint32_t tmem = sh.tmem;
+    PfUnit x;
+
+    if (role == 2) {
+        // ---- copies: keys and values by pages into 128-byte swizzled rows
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        const int pt = tid - 256, pw = pt >> 5;
+        constexpr int CH = D / 8;            // 16-byte pieces of a row
+        constexpr int RPI = 32 / CH;         // rows a warp copies at once
+        constexpr int RPW = KT / 4;          // rows of a tile that a warp copies
+        uint64_t* late[kPfLag] = {};         // barriers of tiles in flight, the oldest first
+        auto flush = [&] {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < kPfLag; ++i) {
+                if (late[i]) pf_arrive(late[i]);
+                late[i] = nullptr;
+            }
+        };
+        auto issued = [&](uint64_t* bar) {
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (late[0]) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kPfLag) : "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                pf_arrive(late[0]);
+            }
+#pragma unroll
+            for (int i = 0; i + 1 < kPfLag; ++i) late[i] = late[i + 1];
+            late[kPfLag - 1] = bar;
+        };
+        // (a wait that is not over at once: what is in flight may be what it waits for)
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            bool there = mbar_try_wait(bar, parity);
+            if (!there) {
+                flush();
+                there = mbar_wait_bounded(bar, parity);
+            }
+            return __all_sync(0xffffffffu, there) != 0;
+        };
+        int stage = 0, unit = 0;
+        uint32_t lap = 0;  // parity of the ring's lap
+        bool ok = true;
+        const int ps = a.kv.page_size;
+        const uint64_t krow = a.kv.k_row >> 4, vrow = a.kv.v_row >> 4, kpage = a.kv.k_page >> 4, vpage = a.kv.v_page >> 4;
+        while (ok && walk.next(a, units, total, x)) {
+            const int n = x.te - x.tb, rows = min(NT * kPfRows, x.n * a.group - x.row0);
+            const int at1 = x.len - x.n + (x.row0 + rows - 1) / a.group;  // the last position that a row sees
+            if (unit && !(ok = wait(&sh.q_empty, (unit - 1) & 1))) break;
+            for (int r0 = pw * RPI; r0 < rows; r0 += 4 * RPI) {
+                const int r = r0 + lane / CH, c = lane % CH;
+                if (r >= rows) continue;
+                const int flat = x.row0 + r, i = flat / a.group, g = flat - i * a.group;
+                const uint16_t* src = a.q + (int64_t)(x.first + i) * a.q_stride + (x.h * a.group + g) * D + c * 8;
+                const int rr = r & (kPfRows - 1);
+                pf_cp16(q_smem + (r / kPfRows) * QTILE + (c >> 3) * QHALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), src,
+                        true);
+            }
+            issued(&sh.q_full);
+            const uint8_t* kb = static_cast<const uint8_t*>(a.kv.k) + x.h * a.kv.k_head;
+            const uint8_t* vb = static_cast<const uint8_t*>(a.kv.v) + x.h * a.kv.v_head;
+            const int32_t* table = a.table + x.s * a.table_stride;
+            const uint16_t* mask = MASK ? a.mask + x.s * a.mask_stride : nullptr;
+            // a lane's row of a tile: its place in 16-byte steps, or ~0 for none
+            uint32_t k_off = ~0u, v_off = ~0u, v_next = ~0u;
+            uint16_t bias = 0, bias_next = 0;
+            constexpr uint16_t kNone = 0xfc00;  // -inf
+            auto find = [&](int t) {
+                const int p = (x.tile0 + x.tb + t) * KT + pw * RPW + lane;
+                bool on = lane < RPW && p <= at1;
+                k_off = v_next = ~0u;
+                bias_next = kNone;
+                if (MASK && on) {
+                    bias_next = __ldg(mask + p);
+                    on = bias_next != kNone;
+                }
+                if (on) {
+                    const int b = (int)((unsigned)p / (unsigned)ps), page = __ldg(table + b);
+                    if ((unsigned)page < (unsigned)a.kv.n_pages) {
+                        const unsigned r = (unsigned)p - (unsigned)b * (unsigned)ps;
+                        k_off = (uint32_t)((unsigned)page * kpage + r * krow);
+                        v_next = (uint32_t)((unsigned)page * vpage + r * vrow);
+                    } else {
+                        record_status(B200_DEVSTATUS_BOUNDS);
+                        bias_next = kNone;
+                    }
+                }
+            };
+            auto copy = [&](const uint8_t* base, uint32_t off) {
+                if (!(ok = wait(&sh.empty[stage], lap ^ 1u))) return;
+                const uint32_t dst = ring + stage * STAGE;
+#pragma unroll 8
+                for (int j = 0; j < RPW; j += RPI) {
+                    const int rl = j + lane / CH, c = lane % CH, r = pw * RPW + rl;
+                    const uint32_t o = __shfl_sync(0xffffffffu, off, rl);
+                    pf_cp16(dst + (c >> 3) * KHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                            o == ~0u ? base : base + ((uint64_t)o << 4) + c * 16, o != ~0u);
+                }
+                issued(&sh.full[stage]);
+                if (++stage == ST) stage = 0, lap ^= 1u;
+            };
+            for (int t = 0; t <= n && ok; ++t) {
+                if (t < n) {
+                    find(t);
+                    copy(kb, k_off);
+                    if (!ok) break;
+                }
+                if (t > 0) {
+                    if (MASK) {
+                        // (before the tile's copies are waited for, after its stage is free)
+                        if (!(ok = wait(&sh.empty[stage], lap ^ 1u))) break;
+                        if (lane < RPW) sh.bias[stage][pw * RPW + lane] = bias;
+                        const float m = warp_max(lane < RPW ? h2f(bias) : -INFINITY);
+                        if (lane == 0) sh.tmax[stage][pw] = m;
+                    }
+                    copy(vb, v_off);
+                }
+                v_off = v_next;
+                bias = bias_next;
+            }
+            ++unit;
+        }
+        flush();
+        if (!ok) sh.aborted = 1;
+    } else if (role == 3) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == 12 && lane == 0) {
+            // ---- tensor-core issue
+            constexpr uint32_t type = BF16 ? (1u << 7) | (1u << 10) : 0u;
+            const uint32_t negate = a.scale < 0.f ? 1u << 13 : 0u;  // of q
+            const uint32_t idesc_s = (1u << 4) | type | negate | ((uint32_t)(KT >> 3) << 17) | ((uint32_t)(kPfRows >> 4) << 24);
+            const uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kPfRows >> 4) << 24);
+            int base = 0, unit = 0;            // ring places before this unit
+            uint32_t ready[2] = {0, 0};        // parities of p_ready
+            bool ok = true;
+            auto stage_of = [&](int place) { return place % ST; };
+            auto parity_of = [&](int place) { return (uint32_t)(place / ST) & 1u; };
+            auto scores = [&](int j, uint32_t d, int stage) {
+                const uint64_t da = tc_desc_sw128(q_smem + j * QTILE), db = tc_desc_sw128(ring + stage * STAGE);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    tc_mma_f16(d, da + (uint64_t)(((k >> 2) * QHALF + (k & 3) * 32) >> 4),
+                               db + (uint64_t)(((k >> 2) * KHALF + (k & 3) * 32) >> 4), idesc_s, k > 0);
+            };
+            auto values = [&](uint32_t d, uint32_t p, int stage, bool add) {
+                const uint64_t db = tc_desc_sw128_mn(ring + stage * STAGE, KHALF);
+#pragma unroll
+                for (int k = 0; k < KT / 16; ++k)
+                    tc_mma_f16_ts(d, p + k * 8, db + (uint64_t)((k * 2048) >> 4), idesc_o, add || k > 0);
+            };
+            while (ok && walk.next(a, units, total, x)) {
+                const int n = x.te - x.tb;
+                const bool two = NT == 2 && x.n * a.group - x.row0 > kPfRows;
+                if (!(ok = mbar_wait_bounded(&sh.q_full, unit & 1))) break;
+                int k_at = base;
+                if (!(ok = mbar_wait_bounded(&sh.full[stage_of(k_at)], parity_of(k_at)))) break;
+                tc_fence_after();
+                scores(0, tmem, stage_of(k_at));
+                tc_commit(&sh.s_full[0]);
+                if (two) {
+                    scores(1, tmem + S_STEP, stage_of(k_at));
+                    tc_commit(&sh.s_full[1]);
+                }
+                tc_commit(&sh.empty[stage_of(k_at)]);
+                if (n == 1) tc_commit(&sh.q_empty);
+                for (int t = 0; t < n && ok; ++t) {
+                    const bool more = t + 1 < n;
+                    k_at = base + pf_k_place(t + 1);
+                    const int v_at = base + pf_v_place(t, n);
+                    if (more && !(ok = mbar_wait_bounded(&sh.full[stage_of(k_at)], parity_of(k_at)))) break;
+                    if (NT == 1 && more) {
+                        // the other score buffer: its weights went into the product before
+                        tc_fence_after();
+                        scores(0, tmem + ((t + 1) & 1) * S_STEP, stage_of(k_at));
+                        tc_commit(&sh.s_full[(t + 1) & 1]);
+                        tc_commit(&sh.empty[stage_of(k_at)]);
+                        if (t + 2 == n) tc_commit(&sh.q_empty);
+                    }
+                    if (!(ok = mbar_wait_bounded(&sh.full[stage_of(v_at)], parity_of(v_at)))) break;
+                    if (NT == 1) {
+                        if (!(ok = mbar_wait_bounded(&sh.p_ready[t & 1], ready[t & 1]))) break;
+                        ready[t & 1] ^= 1u;
+                        tc_fence_after();
+                        values(tmem + O_COL, tmem + (t & 1) * S_STEP, stage_of(v_at), t > 0);
+                        tc_commit(&sh.o_done[0]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            if (j == 1 && !two) break;
+                            if (!(ok = mbar_wait_bounded(&sh.p_ready[j], ready[j]))) break;
+                            ready[j] ^= 1u;
+                            tc_fence_after();
+                            values(tmem + O_COL + j * D, tmem + j * S_STEP, stage_of(v_at), t > 0);
+                            tc_commit(&sh.o_done[j]);
+                            if (more) {
+                                scores(j, tmem + j * S_STEP, stage_of(k_at));
+                                tc_commit(&sh.s_full[j]);
+                            }
+                        }
+                        if (!ok) break;
+                        if (more) tc_commit(&sh.empty[stage_of(k_at)]);
+                        if (t + 2 == n) tc_commit(&sh.q_empty);
+                    }
+                    tc_commit(&sh.empty[stage_of(v_at)]);
+                }
+                base += 2 * n;
+                ++unit;
+            }
+            if (!ok) sh.aborted = 1;
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: a row to a thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        const int j = role;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t o_addr = tmem + lanes + O_COL + (NT == 2 ? j * D : 0);
+        const int row = (warp & 3) * 32 + lane;
+        const float scale2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.17549435e-38f);
+        int base = 0;
+        uint32_t s_par[2] = {0, 0}, o_par = 0;  // o_par: products into this tile's outputs so far
+        bool ok = j < NT, first_unit = true;
+        while (ok && walk.next(a, units, total, x)) {
+            const int n = x.te - x.tb, count = x.n * a.group;
+            const bool first_in_range = first_unit;
+            first_unit = false;
+            if (j * kPfRows >= count - x.row0) {  // no rows for this tile
+                base += 2 * n;
+                continue;
+            }
+            const int flat = x.row0 + j * kPfRows + row;
+            const bool real = flat < count, any = x.row0 + j * kPfRows + (warp & 3) * 32 < count;
+            const int i = flat / a.group;
+            const int at = real ? max(-1, x.len - x.n + i) : -1;
+            float ref = -INFINITY, l = 0.f, c_ref = -INFINITY;
+            for (int t = 0; t < n; ++t) {
+                const int sb = NT == 2 ? j : (t & 1);
+                const uint32_t s_addr = tmem + lanes + sb * S_STEP;
+                if (!(ok = pf_wait(&sh.s_full[sb], s_par[sb]))) break;
+                s_par[sb] ^= 1u;
+                const int v_at = base + pf_v_place(t, n), v_stage = v_at % ST;
+                if (MASK && !(ok = pf_wait(&sh.full[v_stage], (uint32_t)(v_at / ST) & 1u))) break;
+                tc_fence_after();
+                if (any) {
+                    uint32_t s[KT / 32][32];
+#pragma unroll
+                    for (int c = 0; c < KT / 32; ++c) tc_ld_x32(s[c], s_addr + 32 * c);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < KT / 32; ++c) tc_loaded(s[c]);
+                    // columns lo .. hi are seen
+                    const int p0 = (x.tile0 + x.tb + t) * KT;
+                    const int hi = at - p0, lo = a.window > 0 ? max(0, at - a.window + 1) - p0 : 0;
+                    const bool edge = __any_sync(0xffffffffu, hi < KT - 1 || lo > 0);
+                    if (MASK) {
+                        const uint4* b = reinterpret_cast<const uint4*>(sh.bias[v_stage]);
+                        float cm;
+                        if (edge) {
+                            cm = -INFINITY;
+#pragma unroll
+                            for (int c = 0; c < KT; c += 8) {
+                                const uint4 w = b[c / 8];
+                                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                                for (int e = 0; e < 8; e += 2) {
+                                    const float2 f = unpack16<false>(ws[e / 2]);
+                                    if (c + e >= lo && c + e <= hi) cm = fmaxf(cm, f.x);
+                                    if (c + e + 1 >= lo && c + e + 1 <= hi) cm = fmaxf(cm, f.y);
+                                }
+                            }
+                        } else {
+                            cm = fmaxf(fmaxf(sh.tmax[v_stage][0], sh.tmax[v_stage][1]),
+                                       fmaxf(sh.tmax[v_stage][2], sh.tmax[v_stage][3]));
+                        }
+                        // the mask relative to the largest entry that the row has seen:
+                        // a row of lowest values keeps its scores' bits
+                        if (cm > c_ref) {
+                            ref += (c_ref - cm) * 1.4426950408889634f;
+                            c_ref = cm;
+                        }
+                        const float c0 = c_ref == -INFINITY ? 0.f : c_ref;
+#pragma unroll
+                        for (int c = 0; c < KT; c += 8) {
+                            const uint4 w = b[c / 8];
+                            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                            for (int e = 0; e < 8; e += 2) {
+                                const float2 f = unpack16<false>(ws[e / 2]);
+                                uint32_t* y = &s[c >> 5][(c & 31) + e];
+                                y[0] = __float_as_uint(fmaf(__uint_as_float(y[0]), scale2, (f.x - c0) * 1.4426950408889634f));
+                                y[1] = __float_as_uint(fmaf(__uint_as_float(y[1]), scale2, (f.y - c0) * 1.4426950408889634f));
+                            }
+                        }
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int c = 0; c < KT; ++c)
+                            if (c < lo || c > hi) s[c >> 5][c & 31] = 0xff800000u;
+                    }
+                    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < KT; c += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            m[e] = fmaxf(m[e], fmaxf(__uint_as_float(s[c >> 5][(c & 31) + 2 * e]),
+                                                     __uint_as_float(s[c >> 5][(c & 31) + 2 * e + 1])));
+                    float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                    if (!MASK) top *= scale2;
+                    const bool moves = top > ref + kPfLazy;
+                    if (__any_sync(0xffffffffu, moves)) {
+                        const float f = moves ? pf_exp2(ref - top) : 1.f;
+                        l *= f;
+                        if (moves) ref = top;
+                        if (t > 0) {
+                            if (!(ok = pf_wait(&sh.o_done[j], (o_par + 1u) & 1u))) break;
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 32) {
+                                uint32_t o[32];
+                                tc_ld_x32(o, o_addr + c);
+                                tc_wait_ld();
+                                tc_loaded(o);
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                                tc_st_x32(o_addr + c, o);
+                            }
+                        }
+                    }
+                    const float off = (ref == -INFINITY ? 0.f : -ref) + kPfShift<BF16>;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c0 = 0; c0 < KT; c0 += 64) {
+                        uint32_t p[32];
+#pragma unroll
+                        for (int c = 0; c < 64; c += 2) {
+                            const uint32_t* y = &s[(c0 + c) >> 5][(c0 + c) & 31];
+                            const float x0 = __uint_as_float(y[0]), x1 = __uint_as_float(y[1]);
+                            const float e0 = pf_exp2(MASK ? x0 + off : fmaf(x0, scale2, off));
+                            const float e1 = pf_exp2(MASK ? x1 + off : fmaf(x1, scale2, off));
+                            sum[(c >> 1) & 1] += e0;
+                            sum[2 + ((c >> 1) & 1)] += e1;
+                            p[c >> 1] = pack16<BF16>(e0, e1);
+                        }
+                        tc_st_x32(s_addr + c0 / 2, p);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tc_wait_st();
+                }
+                ++o_par;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) pf_arrive(&sh.p_ready[sb]);
+            }
+            if (!ok) break;
+            base += 2 * n;
+            // ---- the unit's outputs, or this CTA's piece of them
+            if (!(ok = pf_wait(&sh.o_done[j], (o_par + 1u) & 1u))) break;
+            tc_fence_after();
+            if (!any) continue;
+            if (n == x.cost) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                float odd = l * 0.f;  // NaN where anything is not finite
+                const int g = flat - i * a.group;
+                const int64_t out_row = (int64_t)(x.first + i) * a.n_head + x.h * a.group + g;
+                uint4* to = reinterpret_cast<uint4*>(a.out + out_row * D);
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tc_ld_x32(o, o_addr + c);
+                    tc_wait_ld();
+                    tc_loaded(o);
+                    uint32_t w[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float y0 = __uint_as_float(o[2 * e]), y1 = __uint_as_float(o[2 * e + 1]);
+                        odd = fmaf(y0, 0.f, fmaf(y1, 0.f, odd));
+                        w[e] = l == 0.f ? 0u : pack16<BF16>(y0 * inv, y1 * inv);
+                    }
+                    if (real)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            to[c / 8 + e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+                }
+                const bool again = real && l != 0.f && odd != 0.f;
+                const unsigned votes = __ballot_sync(0xffffffffu, again);
+                if (votes) {
+                    int at_list = 0;
+                    if (lane == 0) at_list = atomicAdd(&a.header->n_bad, __popc(votes));
+                    at_list = __shfl_sync(0xffffffffu, at_list, 0) + __popc(votes & ((1u << lane) - 1u));
+                    if (again) a.bad[at_list] = make_int2((int)out_row, x.u);
+                }
+            } else {
+                const int slot = 2 * blockIdx.x + (first_in_range ? 0 : 1);
+                float4* ml = a.piece_ml + ((int64_t)slot * NT + j) * kPfRows + row;
+                float4* po = a.piece_o + ((int64_t)slot * NT + j) * (D / 4) * kPfRows + row;
+                if (real) *ml = make_float4(ref, l, c_ref, 0.f);
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tc_ld_x32(o, o_addr + c);
+                    tc_wait_ld();
+                    tc_loaded(o);
+                    if (real)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            po[(c / 4 + e) * kPfRows] =
+                                make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                            __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+                }
+            }
+            tc_fence_before();
+        }
+        if (!ok && j < NT) sh.aborted = 1;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 12 * 32) tc_commit(&sh.done);  // every product issued has ended
+    if (warp == 12) {
+        mbar_wait_drain(&sh.done, 0);
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// ----------------------------------------------------------------- finish
+
+constexpr int kPfFinishThreads = 256;
+
+// CTA (cut, 32 rows): the pieces of the unit that the cut is the first to go
+// through, joined in order.  Then the rows that infinities or NaN met, and which
+// no product of whole tiles can tell apart from positions they do not see.
+template <bool BF16, int D>
+__global__ void __launch_bounds__(kPfFinishThreads) paged_prefill_finish_kernel(const __grid_constant__ PagedPrefillArgs a) {
+    constexpr int NT = pf_tiles(D), W = kPfFinishThreads / 32, CPW = D / 4 / W;  // float4 columns to a warp
+    __shared__ int s_odd[W][32];
+    griddep_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t total = a.header->total, per = a.header->per_cta, all = total * a.kv.n_head_kv;
+    const int64_t cut = (int64_t)(blockIdx.y + 1) * per;
+    if (cut < all) {
+        const int h = (int)(cut / total), u = pf_find(a.prefix, a.header->units, cut - h * total);
+        const int64_t start = h * total + a.prefix[u], end = h * total + a.prefix[u + 1];
+        const int c0 = (int)(start / per), c1 = (int)((end - 1) / per);
+        if (start < cut && c0 == (int)blockIdx.y) {
+            const int4 d0 = a.desc[2 * (int64_t)u], d1 = a.desc[2 * (int64_t)u + 1];
+            const int r0 = blockIdx.x * 32, j = r0 / kPfRows, row = (r0 & (kPfRows - 1)) + lane;
+            const int flat = d0.y + r0 + lane;
+            const bool real = flat < d1.y * a.group;
+            if (d0.y + r0 < d1.y * a.group) {
+                auto slot = [&](int c) { return (int64_t)(2 * c + (c == c0 && start > c0 * per ? 1 : 0)) * NT + j; };
+                // references of all pieces first
+                float cm = -INFINITY, top = -INFINITY;
+                if (a.mask)
+                    for (int c = c0; c <= c1; ++c)
+                        if (real) cm = fmaxf(cm, a.piece_ml[slot(c) * kPfRows + row].z);
+                auto moved = [&](const float4& ml) {
+                    return a.mask && ml.z != cm ? ml.x + (ml.z - cm) * 1.4426950408889634f : ml.x;
+                };
+                for (int c = c0; c <= c1; ++c)
+                    if (real) top = fmaxf(top, moved(a.piece_ml[slot(c) * kPfRows + row]));
+                float l = 0.f;
+                float4 o[CPW];
+#pragma unroll
+                for (int e = 0; e < CPW; ++e) o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int c = c0; c <= c1; ++c) {
+                    if (!real) break;
+                    const float4 ml = a.piece_ml[slot(c) * kPfRows + row];
+                    const float ref = moved(ml), f = ref == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : pf_exp2(ref - top);
+                    l = fmaf(f, ml.y, l);
+                    const float4* po = a.piece_o + (slot(c) * (D / 4) + warp * CPW) * kPfRows + row;
+                    if (f != 0.f)
+#pragma unroll
+                        for (int e = 0; e < CPW; ++e) {
+                            const float4 y = po[e * kPfRows];
+                            o[e].x = fmaf(f, y.x, o[e].x), o[e].y = fmaf(f, y.y, o[e].y);
+                            o[e].z = fmaf(f, y.z, o[e].z), o[e].w = fmaf(f, y.w, o[e].w);
+                        }
+                    else  // a weight of 0 meets what is not finite
+#pragma unroll
+                        for (int e = 0; e < CPW; ++e) {
+                            const float4 y = po[e * kPfRows];
+                            const float z = (y.x + y.y + y.z + y.w) * 0.f;
+                            o[e].x += z;
+                        }
+                }
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const int i = flat / a.group, g = flat - i * a.group;
+                const int64_t out_row = (int64_t)(d1.x + i) * a.n_head + h * a.group + g;
+                float odd = l * 0.f;
+                uint32_t w[2 * CPW];
+#pragma unroll
+                for (int e = 0; e < CPW; ++e) {
+                    odd += o[e].x * 0.f + o[e].y * 0.f + o[e].z * 0.f + o[e].w * 0.f;
+                    w[2 * e] = l == 0.f ? 0u : pack16<BF16>(o[e].x * inv, o[e].y * inv);
+                    w[2 * e + 1] = l == 0.f ? 0u : pack16<BF16>(o[e].z * inv, o[e].w * inv);
+                }
+                if (real) {
+                    uint2* to = reinterpret_cast<uint2*>(a.out + out_row * D) + warp * CPW;
+#pragma unroll
+                    for (int e = 0; e < CPW; ++e) to[e] = make_uint2(w[2 * e], w[2 * e + 1]);
+                }
+                s_odd[warp][lane] = real && l != 0.f && odd != 0.f;
+                __syncthreads();
+                bool again = false;
+#pragma unroll
+                for (int v = 0; v < W; ++v) again |= s_odd[v][lane] != 0;
+                unsigned votes = __ballot_sync(0xffffffffu, again);
+                PfSeq sq;
+                sq.first = d1.x, sq.n = d1.y, sq.len = d1.z;
+                for (int k = 0; votes; votes &= votes - 1, ++k)
+                    if (k % W == warp) {
+                        const int r = d0.y + r0 + __ffs(votes) - 1, t = r / a.group;
+                        pf_row<BF16, D>(a, d0.x, sq, t, h * a.group + r - t * a.group);
+                    }
+            }
+        }
+    }
+    const int n_bad = a.header->n_bad;
+    const int cta = blockIdx.y * gridDim.x + blockIdx.x, ctas = gridDim.x * gridDim.y;
+    for (int64_t b = (int64_t)cta * W + warp; b < n_bad; b += (int64_t)ctas * W) {
+        const int2 e = a.bad[b];
+        const int4 d1 = a.desc[2 * (int64_t)e.y + 1];
+        PfSeq sq;
+        sq.first = d1.x, sq.n = d1.y, sq.len = d1.z;
+        const int t = e.x / a.n_head;
+        pf_row<BF16, D>(a, a.desc[2 * (int64_t)e.y].x, sq, t - sq.first, e.x - t * a.n_head);
+    }
 }
 
 }  // namespace b200

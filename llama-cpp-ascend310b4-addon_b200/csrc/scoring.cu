@@ -33,12 +33,13 @@ int b200i_scoring_timeout(unsigned long long ns) {
 
 namespace {
 
-// kernel<<<grid, threads, 0, st>>>(a), programmatically dependent on the launch before.
+// kernel<<<grid, threads, smem, st>>>(a), programmatically dependent on the launch before.
 template <class A>
-int launch_after(void (*kernel)(A), dim3 grid, int threads, cudaStream_t st, const A& a) {
+int launch_after(void (*kernel)(A), dim3 grid, int threads, cudaStream_t st, const A& a, int smem = 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
     cudaLaunchAttribute at = pdl_attr();
     cfg.attrs = &at;
@@ -48,11 +49,32 @@ int launch_after(void (*kernel)(A), dim3 grid, int threads, cudaStream_t st, con
 
 // ------------------------------------------------------------------ prefill
 
+bool g_prefill_attr[kMaxDevices][2][3][2];
+std::mutex g_attr_mu;
+
+template <bool BF16, int D, bool MASK>
+int launch_prefill_main(const PagedPrefillArgs& a, cudaStream_t st) {
+    const int dev = current_device();
+    if (dev < 0 || dev >= kMaxDevices) return B200_EINVAL;
+    {
+        bool& done = g_prefill_attr[dev][BF16][D == 64 ? 0 : D == 128 ? 1 : 2][MASK];
+        std::lock_guard<std::mutex> lk(g_attr_mu);
+        if (!done) {
+            CR_(cuda_status(cudaFuncSetAttribute(paged_prefill_kernel<BF16, D, MASK>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, pf_smem<D>())));
+            done = true;
+        }
+    }
+    return launch_after(paged_prefill_kernel<BF16, D, MASK>, dim3(kPfCtas), kPfThreads, st, a, pf_smem<D>());
+}
+
 template <bool BF16, int D>
 int launch_prefill_d(const PagedPrefillArgs& a, cudaStream_t st) {
-    const int64_t warps = (int64_t)a.n_tokens * a.n_head;
-    paged_prefill_rows_kernel<BF16, D><<<(unsigned)((warps + 7) / 8), 256, 0, st>>>(a);
-    return cuda_status(cudaGetLastError());
+    paged_prefill_plan_kernel<<<1, kPfPlanThreads, 0, st>>>(a, pf_tiles(D) * kPfRows, pf_keys(D));
+    CR_(cuda_status(cudaGetLastError()));
+    CR_(a.mask ? (launch_prefill_main<BF16, D, true>(a, st)) : (launch_prefill_main<BF16, D, false>(a, st)));
+    return launch_after(paged_prefill_finish_kernel<BF16, D>, dim3(pf_tiles(D) * kPfRows / 32, kPfCtas - 1),
+                        kPfFinishThreads, st, a);
 }
 
 template <bool BF16>
@@ -62,6 +84,23 @@ int launch_prefill(const PagedPrefillArgs& a, cudaStream_t st) {
         case 128: return launch_prefill_d<BF16, 128>(a, st);
         default: return launch_prefill_d<BF16, 256>(a, st);
     }
+}
+
+struct PrefillLayout {
+    size_t desc, prefix, bad, ml, o, total;
+};
+
+PrefillLayout prefill_layout(int head_dim, int64_t n_tokens, int64_t n_seq, int64_t n_head, int64_t n_head_kv) {
+    const int64_t rows = pf_tiles(head_dim) * kPfRows;
+    const int64_t units = n_tokens * (n_head / n_head_kv) / rows + n_seq;
+    PrefillLayout l;
+    l.desc = 256;
+    l.prefix = l.desc + align256((size_t)units * 2 * sizeof(int4));
+    l.bad = l.prefix + align256((size_t)(units + 1) * sizeof(int64_t));
+    l.ml = l.bad + align256((size_t)(n_tokens * n_head) * sizeof(int2));
+    l.o = l.ml + (size_t)2 * kPfCtas * rows * sizeof(float4);
+    l.total = l.o + (size_t)2 * kPfCtas * rows * head_dim * sizeof(float);
+    return l;
 }
 
 // --------------------------------------------------------------------- fork
@@ -112,7 +151,7 @@ size_t b200_paged_prefill_workspace_size(int head_dim, int64_t n_tokens, int n_s
     if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || n_tokens < 0 || n_tokens > INT32_MAX || n_seq < 0 ||
         n_seq > 65535 || n_head <= 0 || n_head > 65535 || n_head_kv <= 0 || n_head % n_head_kv)
         return 0;
-    return 256;
+    return prefill_layout(head_dim, n_tokens, n_seq, n_head, n_head_kv).total;
 }
 
 int b200_paged_prefill(const b200_paged_kv* kv, const void* q, int64_t q_stride, int64_t n_tokens, int n_head,
@@ -123,7 +162,7 @@ int b200_paged_prefill(const b200_paged_kv* kv, const void* q, int64_t q_stride,
     if (n_seq == 0 || n_tokens == 0) return B200_OK;
     const int64_t row = (int64_t)n_head * kv->head_dim;
     if (!q || !block_table || !seq_lens || !cu || !out || !workspace || n_seq < 0 || n_seq > 65535 || n_tokens < 0 ||
-        n_head <= 0 || n_head % kv->n_head_kv || n_head > 65535 || window < 0)
+        n_head <= 0 || n_head % kv->n_head_kv || n_head > 65535 || window < 0 || scale != scale)
         return B200_EINVAL;
     if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || (q_stride & 7) || (n_tokens > 1 && q_stride < row))
         return B200_EINVAL;
@@ -155,8 +194,17 @@ int b200_paged_prefill(const b200_paged_kv* kv, const void* q, int64_t q_stride,
     a.group = n_head / kv->n_head_kv;
     a.n_seq = n_seq;
     a.max_blocks = max_blocks;
-    a.window = window;
+    // (a window of every position is none)
+    a.window = window >= (int64_t)max_blocks * kv->page_size ? 0 : window;
     a.scale = scale;
+    const PrefillLayout l = prefill_layout(kv->head_dim, n_tokens, n_seq, n_head, kv->n_head_kv);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    a.header = reinterpret_cast<PfHeader*>(ws);
+    a.desc = reinterpret_cast<int4*>(ws + l.desc);
+    a.prefix = reinterpret_cast<int64_t*>(ws + l.prefix);
+    a.bad = reinterpret_cast<int2*>(ws + l.bad);
+    a.piece_ml = reinterpret_cast<float4*>(ws + l.ml);
+    a.piece_o = reinterpret_cast<float4*>(ws + l.o);
     return kv->type == B200_TYPE_BF16 ? launch_prefill<true>(a, (cudaStream_t)stream)
                                       : launch_prefill<false>(a, (cudaStream_t)stream);
 }
