@@ -691,6 +691,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     tc_wait_st();
                 }
+                // (one score buffer: the scores came after the product before.  Two: the parity
+                // of o_done says which product ended only if none is passed over)
+                if (NT == 1 && t > 0 && !(ok = pf_wait(&sh.o_done[0], (o_par + 1u) & 1u))) break;
                 ++o_par;
                 tc_fence_before();
                 __syncwarp();

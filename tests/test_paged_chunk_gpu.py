@@ -85,6 +85,39 @@ def test_chunks(past, new, ps, hq, hkv, d, dtype):
     check(c, q, cu, ps, dtype)
 
 
+@pytest.mark.parametrize("past,new,ps,hq,hkv,d,dtype", [([500], [1000], 16, 16, 4, 256, "f16"),
+                                                        ([2000, 500, 600, 100], [700] * 4, 24, 8, 2, 256, "bf16"),
+                                                        ([900, 0], [600, 1500], 16, 16, 8, 128, "bf16"),
+                                                        ([900, 0], [600, 1500], 64, 24, 8, 64, "f16")])
+def test_ranges_of_many_tiles_and_units(past, new, ps, hq, hkv, d, dtype):
+    """Work for every SM: ranges that hold the end of a unit, whole ones and the start of another."""
+    _, c, cu, q = make(past, new, ps, hq, hkv, d, dtype)
+    check(c, q, cu, ps, dtype)
+    check(c, q, cu, ps, dtype, window=700)
+
+
+@pytest.mark.parametrize("d,ps", [(64, 16), (128, 24), (256, 64)])
+def test_every_tile_counts_once(d, ps):
+    """Keys of 0 and values that name their position: every weight is 1 / length,
+    over 300 sequences of 1 to 8 tiles of keys in ranges that cut them anywhere."""
+    bw, n, most = B(), 300, 8 * 128
+    r = rng(d)
+    lens = r.integers(1, most + 1, n)
+    nb = R.ceil_div(most, ps)
+    v = torch.zeros((n * nb, ps, 1, d), dtype=torch.float16, device="cuda")
+    table = torch.randperm(n * nb, device="cuda", generator=torch.Generator("cuda").manual_seed(d)).int().view(n, nb)
+    pos = torch.arange(nb * ps, device="cuda")
+    width = R.ceil_div(most, d)  # positions that share a channel
+    v[table[:, pos // ps].long(), pos % ps, 0, (pos // width) % d] = 1
+    cache = bw.PagedKV(torch.zeros_like(v), v)
+    q = torch.randn((n, 1, d), device="cuda").half()
+    out = bw.paged_prefill(cache, q, table, i32(lens), i32(np.arange(n + 1)), 1.0)[:, 0].double()
+    end = dev(lens)[:, None]
+    want = ((end - torch.arange(d, device="cuda") * width).clamp(0, width)).double() / end
+    # sums of whole numbers below 2^24 are exact; the quotient is rounded in f32 twice and to f16
+    assert ((out - want).abs() <= want * (2.0 ** -11 + 2.0 ** -22) + 2.0 ** -25).all()
+
+
 @pytest.mark.parametrize("window", [1, 2, 100, 129, 1000])
 @pytest.mark.parametrize("past,new,ps,hq,hkv,d,dtype", [([0], [300], 16, 8, 2, 128, "f16"),
                                                         ([700, 0, 130], [50, 200, 1], 24, 12, 2, 64, "bf16"),
