@@ -5,7 +5,6 @@
 // code.  Host-side code elsewhere (graph runner, backend, decode driver)
 // reaches the kernels through include/b200_decode.h and internal.h.
 #include <cuda_runtime.h>
-#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <cmath>
@@ -368,20 +367,6 @@ int set_fa_attrs() {
     std::lock_guard<std::mutex> lk(g_attr_mu);
     CR_(fa_cluster_probe<64>(dev));
     return fa_cluster_probe<128>(dev);
-}
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no link
-// against the driver library).
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    }();
-    return fn;
 }
 
 // K or V cache view [D, Hkv, n_kv] (byte strides nb2 per head, nb1 per

@@ -20,6 +20,11 @@
 namespace b200 {
 
 struct PagedPrefillArgs {
+    // [page][head][row][channel] views of K and V for boxes of box rows of a page by
+    // 64 channels, and [KV head][token][head][channel] of q for boxes of 128 rows
+    CUtensorMap map_k, map_v, map_q;
+    int box;    // 0: pages have no 8 rows in a row that start at a multiple of 8
+    int q_box;  // tokens of 128 rows; 0: the heads of a KV head do not divide 128
     b200_paged_kv kv;
     const uint16_t* q;
     int64_t q_stride;
@@ -34,20 +39,23 @@ struct PagedPrefillArgs {
     // workspace
     struct PfHeader* header;
     int4* desc;         // two per unit: {sequence, first flat row, first key tile, key tiles}, {first, n, len, -}
-    int64_t* prefix;    // [units + 1] key tiles of the units before
+    int64_t* prefix;    // [units + 1] steps of the units before
     int2* bad;          // rows to compute again: {flat (token, head), unit}
     float4* piece_ml;   // [2 * CTAs][tiles][128] {reference, sum, mask reference, -} of cut units
     float4* piece_o;    // [2 * CTAs][tiles][D / 4][128] their sums of weighted values
 };
 
 struct PfHeader {
-    int64_t total;    // key tiles of all units of one KV head
+    int64_t total;    // steps of all units of one KV head
     int64_t per_cta;  // of all KV heads' units, to a CTA
     int units, n_bad;
 };
 
 constexpr int kPfCtas = 148;   // one per SM
 constexpr int kPfRows = 128;   // rows of a tile: the lanes of tensor memory
+// A unit counts as many steps as it has key tiles and these: its queries, the first
+// scores and the outputs, which nothing overlaps.
+constexpr int kPfUnitSteps = 2;
 // Key tiles and row tiles of a unit by head dim: two row tiles take turns between
 // the tensor core and the exponentials; at head dim 256 the outputs of one fill
 // half of tensor memory, and two score buffers of 64 keys take its place.
@@ -179,7 +187,7 @@ __global__ void __launch_bounds__(kPfPlanThreads) paged_prefill_plan_kernel(cons
         __syncthreads();
         for (int64_t u0 = 0; u0 < sum; u0 += kPfPlanThreads) {
             const int64_t u = u0 + tid;
-            int64_t cost = 0;
+            int64_t steps = 0;
             int4 d0, d1;
             if (u < sum) {
                 int lo = 0, hi = count;  // s_base[lo] <= u < s_base[hi]
@@ -193,12 +201,13 @@ __global__ void __launch_bounds__(kPfPlanThreads) paged_prefill_plan_kernel(cons
                 const int row1 = (int)min((int64_t)row0 + rows, (int64_t)t.n * a.group) - 1;
                 const int at0 = t.len - t.n + row0 / a.group, at1 = t.len - t.n + row1 / a.group;
                 const int first = a.window > 0 ? max(0, max(-1, at0) - a.window + 1) / keys : 0;
-                cost = at1 < 0 ? 1 : at1 / keys - first + 1;
-                d0 = make_int4(base + lo, row0, first, (int)cost);
+                const int cost = at1 < 0 ? 1 : at1 / keys - first + 1;
+                steps = cost + kPfUnitSteps;
+                d0 = make_int4(base + lo, row0, first, cost);
                 d1 = make_int4(t.first, t.n, t.len, 0);
             }
             int64_t more;
-            const int64_t before = tiles + pf_scan(cost, part, &more);
+            const int64_t before = tiles + pf_scan(steps, part, &more);
             if (u < sum) {
                 a.desc[2 * (units + u)] = d0;
                 a.desc[2 * (units + u) + 1] = d1;
@@ -243,17 +252,20 @@ struct PfWalk {
     int64_t w, w1;
     int u, h;
     __device__ __forceinline__ bool next(const PagedPrefillArgs& a, int units, int64_t total, PfUnit& x) {
-        if (w >= w1) return false;
-        const int4 d0 = __ldg(a.desc + 2 * (int64_t)u), d1 = __ldg(a.desc + 2 * (int64_t)u + 1);
-        const int64_t start = h * total + __ldg(reinterpret_cast<const long long*>(a.prefix) + u);
-        x.u = u, x.s = d0.x, x.row0 = d0.y, x.tile0 = d0.z, x.cost = d0.w;
-        x.first = d1.x, x.n = d1.y, x.len = d1.z;
-        x.h = h;
-        x.tb = (int)(w - start);
-        x.te = (int)min((int64_t)x.cost, x.tb + (w1 - w));
-        w += x.te - x.tb;
-        if (x.te == x.cost && ++u == units) u = 0, ++h;
-        return true;
+        while (w < w1) {
+            const int4 d0 = __ldg(a.desc + 2 * (int64_t)u), d1 = __ldg(a.desc + 2 * (int64_t)u + 1);
+            // the unit's first key tile, and where the range starts and ends from there
+            const int64_t start = h * total + __ldg(reinterpret_cast<const long long*>(a.prefix) + u) + kPfUnitSteps;
+            x.u = u, x.s = d0.x, x.row0 = d0.y, x.tile0 = d0.z, x.cost = d0.w;
+            x.first = d1.x, x.n = d1.y, x.len = d1.z;
+            x.h = h;
+            x.tb = (int)max((int64_t)0, w - start);
+            x.te = (int)min((int64_t)x.cost, w1 - start);
+            w = start + x.cost;
+            if (++u == units) u = 0, ++h;
+            if (x.tb < x.te) return true;
+        }
+        return false;
     }
 };
 
@@ -265,7 +277,7 @@ struct PfShared {
     uint64_t q_full, q_empty, full[ST], empty[ST], s_full[2], p_ready[2], o_done[2], done;
     uint32_t tmem;
     int aborted, u, h;
-    float tmax[ST][4];                       // largest mask entry of each warp's rows
+    float tmax[ST][2];                       // largest mask entry of each warp's rows
     alignas(16) uint16_t bias[ST][pf_keys(D)];  // mask of the tile whose values a stage holds
 };
 template <int D>
@@ -282,6 +294,13 @@ __device__ __forceinline__ int pf_v_place(int t, int n) { return t == n - 1 ? 2 
 __device__ __forceinline__ void pf_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void pf_tma(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
 // A warp's wait: the same answer for every lane.
 __device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
@@ -295,8 +314,36 @@ __device__ __forceinline__ float pf_exp2(float x) {
     return y;
 }
 
-constexpr int kPfThreads = 512;     // two softmax warpgroups, copies, tensor-core issue
-constexpr int kPfLag = 2;           // tiles of copies in flight behind the one being issued
+// Two f32 in one register pair: one instruction adds or multiplies both.
+__device__ __forceinline__ uint64_t pf_pair(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 pf_unpair(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t pf_fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t pf_add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ float pf_max3(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+
+constexpr int kPfThreads = 384;     // two softmax warpgroups; two warps of copies, tensor-core issue
+constexpr int kPfCopyThreads = 64;
+constexpr int kPfIssueWarp = 10;
 constexpr float kPfLazy = 8.f;      // the reference stays until the maximum passes it by 2^8
 // f16 weights are taken times 2^7: 2^15 at most with the lazy reference, and 2^-31 of
 // the reference is still a value
@@ -314,16 +361,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, role = warp >> 2;
     const uint32_t q_smem = (smem_u32(smem_raw) + 1023u) & ~1023u, ring = q_smem + pf_q_bytes<D>();
 
-    if (warp == 12) {
+    if (warp == kPfIssueWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
                      "r"(512)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (tid == 0) {
-        mbar_init(&sh.q_full, 128);
+        mbar_init(&sh.q_full, kPfCopyThreads);
         mbar_init(&sh.q_empty, 1);
-        for (int i = 0; i < ST; ++i) mbar_init(&sh.full[i], 128), mbar_init(&sh.empty[i], 1);
+        for (int i = 0; i < ST; ++i) mbar_init(&sh.full[i], kPfCopyThreads + (MASK ? 2 : 0)), mbar_init(&sh.empty[i], 1);
         for (int j = 0; j < 2; ++j) mbar_init(&sh.s_full[j], 1), mbar_init(&sh.p_ready[j], 4), mbar_init(&sh.o_done[j], 1);
         mbar_init(&sh.done, 1);
         sh.aborted = 0;
@@ -347,129 +394,168 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
     PfUnit x;
 
     if (role == 2) {
-        // ---- copies: keys and values by pages into 128-byte swizzled rows
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-        const int pt = tid - 256, pw = pt >> 5;
-        constexpr int CH = D / 8;            // 16-byte pieces of a row
-        constexpr int RPI = 32 / CH;         // rows a warp copies at once
-        constexpr int RPW = KT / 4;          // rows of a tile that a warp copies
-        uint64_t* late[kPfLag] = {};         // barriers of tiles in flight, the oldest first
-        auto flush = [&] {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-#pragma unroll
-            for (int i = 0; i < kPfLag; ++i) {
-                if (late[i]) pf_arrive(late[i]);
-                late[i] = nullptr;
-            }
-        };
-        auto issued = [&](uint64_t* bar) {
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (late[0]) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(kPfLag) : "memory");
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                pf_arrive(late[0]);
-            }
-#pragma unroll
-            for (int i = 0; i + 1 < kPfLag; ++i) late[i] = late[i + 1];
-            late[kPfLag - 1] = bar;
-        };
-        // (a wait that is not over at once: what is in flight may be what it waits for)
-        auto wait = [&](uint64_t* bar, uint32_t parity) {
-            bool there = mbar_try_wait(bar, parity);
-            if (!there) {
-                flush();
-                there = mbar_wait_bounded(bar, parity);
-            }
-            return __all_sync(0xffffffffu, there) != 0;
-        };
-        int stage = 0, unit = 0;
-        uint32_t lap = 0;  // parity of the ring's lap
-        bool ok = true;
-        const int ps = a.kv.page_size;
-        const uint64_t krow = a.kv.k_row >> 4, vrow = a.kv.v_row >> 4, kpage = a.kv.k_page >> 4, vpage = a.kv.v_page >> 4;
-        while (ok && walk.next(a, units, total, x)) {
-            const int n = x.te - x.tb, rows = min(NT * kPfRows, x.n * a.group - x.row0);
-            const int at1 = x.len - x.n + (x.row0 + rows - 1) / a.group;  // the last position that a row sees
-            if (unit && !(ok = wait(&sh.q_empty, (unit - 1) & 1))) break;
-            for (int r0 = pw * RPI; r0 < rows; r0 += 4 * RPI) {
-                const int r = r0 + lane / CH, c = lane % CH;
-                if (r >= rows) continue;
-                const int flat = x.row0 + r, i = flat / a.group, g = flat - i * a.group;
-                const uint16_t* src = a.q + (int64_t)(x.first + i) * a.q_stride + (x.h * a.group + g) * D + c * 8;
-                const int rr = r & (kPfRows - 1);
-                pf_cp16(q_smem + (r / kPfRows) * QTILE + (c >> 3) * QHALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), src,
-                        true);
-            }
-            issued(&sh.q_full);
-            const uint8_t* kb = static_cast<const uint8_t*>(a.kv.k) + x.h * a.kv.k_head;
-            const uint8_t* vb = static_cast<const uint8_t*>(a.kv.v) + x.h * a.kv.v_head;
-            const int32_t* table = a.table + x.s * a.table_stride;
-            const uint16_t* mask = MASK ? a.mask + x.s * a.mask_stride : nullptr;
-            // a lane's row of a tile: its place in 16-byte steps, or ~0 for none
-            uint32_t k_off = ~0u, v_off = ~0u, v_next = ~0u;
-            uint16_t bias = 0, bias_next = 0;
-            constexpr uint16_t kNone = 0xfc00;  // -inf
-            auto find = [&](int t) {
-                const int p = (x.tile0 + x.tb + t) * KT + pw * RPW + lane;
-                bool on = lane < RPW && p <= at1;
-                k_off = v_next = ~0u;
-                bias_next = kNone;
-                if (MASK && on) {
-                    bias_next = __ldg(mask + p);
-                    on = bias_next != kNone;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (tid < 256 + kPfCopyThreads) {
+            // ---- copies: keys and values by pages into 128-byte swizzled rows.  The
+            // barrier of a tile counts its copies' ends; the thread that issues the
+            // products puts the fence between the copies' writes and the tensor core
+            const int pw = warp - 8;
+            constexpr int CH = D / 8;            // 16-byte pieces of a row
+            constexpr int RPI = 32 / CH;         // rows a warp copies at once
+            constexpr int RPW = KT / 2, RPL = RPW / 32;  // rows of a tile to a warp, to a lane
+            auto issued = [&](uint64_t* bar) {
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+            };
+            // a warp's share of a barrier where TMA copies `bytes` for it
+            auto expects = [&](uint64_t* bar, uint32_t bytes, uint32_t arrivals) {
+                if (lane == 0) {
+                    if (bytes) mbar_arrive_expect_tx(bar, bytes);
+                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
+                                 "r"(arrivals - (bytes ? 1u : 0u))
+                                 : "memory");
                 }
-                if (on) {
-                    const int b = (int)((unsigned)p / (unsigned)ps), page = __ldg(table + b);
-                    if ((unsigned)page < (unsigned)a.kv.n_pages) {
-                        const unsigned r = (unsigned)p - (unsigned)b * (unsigned)ps;
-                        k_off = (uint32_t)((unsigned)page * kpage + r * krow);
-                        v_next = (uint32_t)((unsigned)page * vpage + r * vrow);
-                    } else {
-                        record_status(B200_DEVSTATUS_BOUNDS);
-                        bias_next = kNone;
+                __syncwarp();
+            };
+            constexpr int HALVES = D / 64, MINE = HALVES / 2;  // blocks of 64 channels; of each warp
+            int stage = 0, unit = 0;
+            uint32_t lap = 0;  // parity of the ring's lap
+            bool ok = true;
+            const int ps = a.kv.page_size;
+            const uint64_t krow = a.kv.k_row >> 4, vrow = a.kv.v_row >> 4, kpage = a.kv.k_page >> 4, vpage = a.kv.v_page >> 4;
+            while (ok && walk.next(a, units, total, x)) {
+                const int n = x.te - x.tb, rows = min(NT * kPfRows, x.n * a.group - x.row0);
+                const int at1 = x.len - x.n + (x.row0 + rows - 1) / a.group;  // the last position that a row sees
+                if (unit && !(ok = pf_wait(&sh.q_empty, (unit - 1) & 1))) break;
+                if (a.q_box) {
+                    // 128 rows of 64 channels to a copy; rows past the sequence's are not used
+                    const int tiles = (rows + kPfRows - 1) / kPfRows;
+                    const int mine = tiles * (HALVES == 1 ? 1 - pw : MINE);
+                    expects(&sh.q_full, (uint32_t)(mine * QHALF), 32);
+                    if (lane < mine) {
+                        const int j = HALVES == 1 ? lane : lane / MINE, hf = HALVES == 1 ? 0 : 2 * (lane % MINE) + pw;
+                        pf_tma(q_smem + j * QTILE + hf * QHALF, &a.map_q, hf * 64, 0, x.first + x.row0 / a.group + j * a.q_box,
+                               x.h, &sh.q_full);
                     }
+                } else {
+#pragma unroll 4
+                    for (int r0 = pw * RPI; r0 < rows; r0 += 2 * RPI) {
+                        const int r = r0 + lane / CH, c = lane % CH;
+                        if (r >= rows) continue;
+                        const int flat = x.row0 + r, i = flat / a.group, g = flat - i * a.group;
+                        const uint16_t* src = a.q + (int64_t)(x.first + i) * a.q_stride + (x.h * a.group + g) * D + c * 8;
+                        const int rr = r & (kPfRows - 1);
+                        pf_cp16(q_smem + (r / kPfRows) * QTILE + (c >> 3) * QHALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), src,
+                                true);
+                    }
+                    issued(&sh.q_full);
                 }
-            };
-            auto copy = [&](const uint8_t* base, uint32_t off) {
-                if (!(ok = wait(&sh.empty[stage], lap ^ 1u))) return;
-                const uint32_t dst = ring + stage * STAGE;
-#pragma unroll 8
-                for (int j = 0; j < RPW; j += RPI) {
-                    const int rl = j + lane / CH, c = lane % CH, r = pw * RPW + rl;
-                    const uint32_t o = __shfl_sync(0xffffffffu, off, rl);
-                    pf_cp16(dst + (c >> 3) * KHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4),
-                            o == ~0u ? base : base + ((uint64_t)o << 4) + c * 16, o != ~0u);
-                }
-                issued(&sh.full[stage]);
-                if (++stage == ST) stage = 0, lap ^= 1u;
-            };
-            for (int t = 0; t <= n && ok; ++t) {
-                if (t < n) {
-                    find(t);
-                    copy(kb, k_off);
-                    if (!ok) break;
-                }
-                if (t > 0) {
+                const uint8_t* kb = static_cast<const uint8_t*>(a.kv.k) + x.h * a.kv.k_head;
+                const uint8_t* vb = static_cast<const uint8_t*>(a.kv.v) + x.h * a.kv.v_head;
+                const int32_t* table = a.table + x.s * a.table_stride;
+                const uint16_t* mask = MASK ? a.mask + x.s * a.mask_stride : nullptr;
+                // a lane's rows of a tile: their places in 16-byte steps, or ~0 for none
+                uint32_t k_off[RPL], v_off[RPL], v_next[RPL];
+                uint16_t bias[RPL], bias_next[RPL];
+                constexpr uint16_t kNone = 0xfc00;  // -inf
+                auto find = [&](int t) {
+#pragma unroll
+                    for (int e = 0; e < RPL; ++e) {
+                        const int p = (x.tile0 + x.tb + t) * KT + pw * RPW + 32 * e + lane;
+                        bool on = p <= at1;
+                        k_off[e] = v_next[e] = ~0u;
+                        bias_next[e] = kNone;
+                        if (MASK && on) {
+                            bias_next[e] = __ldg(mask + p);
+                            on = bias_next[e] != kNone;
+                        }
+                        if (on) {
+                            const int b = (int)((unsigned)p / (unsigned)ps), page = __ldg(table + b);
+                            if ((unsigned)page < (unsigned)a.kv.n_pages) {
+                                const unsigned r = (unsigned)p - (unsigned)b * (unsigned)ps;
+                                k_off[e] = (uint32_t)((unsigned)page * kpage + r * krow);
+                                v_next[e] = (uint32_t)((unsigned)page * vpage + r * vrow);
+                            } else {
+                                record_status(B200_DEVSTATUS_BOUNDS);
+                                bias_next[e] = kNone;
+                            }
+                        }
+                    }
+                };
+                auto copy = [&](const uint8_t* base, const uint32_t (&off)[RPL]) {
+                    const uint32_t dst = ring + stage * STAGE;
+#pragma unroll
+                    for (int j = 0; j < RPW; j += RPI) {
+                        const int rl = j + lane / CH, c = lane % CH, r = pw * RPW + rl;
+                        const uint32_t o = __shfl_sync(0xffffffffu, off[j / 32], rl & 31);
+                        pf_cp16(dst + (c >> 3) * KHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                                o == ~0u ? base : base + ((uint64_t)o << 4) + c * 16, o != ~0u);
+                    }
+                    issued(&sh.full[stage]);
                     if (MASK) {
-                        // (before the tile's copies are waited for, after its stage is free)
-                        if (!(ok = wait(&sh.empty[stage], lap ^ 1u))) break;
-                        if (lane < RPW) sh.bias[stage][pw * RPW + lane] = bias;
-                        const float m = warp_max(lane < RPW ? h2f(bias) : -INFINITY);
-                        if (lane == 0) sh.tmax[stage][pw] = m;
+                        __syncwarp();
+                        if (lane == 0) pf_arrive(&sh.full[stage]);  // the mask entries are written
                     }
-                    copy(vb, v_off);
+                    if (++stage == ST) stage = 0, lap ^= 1u;
+                };
+                // a tile that is seen whole goes by TMA, a box to a lane
+                const int boxes = a.box ? KT / a.box : 0;
+                int page = 0, row = 0, v_page = 0, v_row = 0;
+                bool whole = false, v_whole = false;
+                auto find_boxes = [&](int t) {
+                    const int p = (x.tile0 + x.tb + t) * KT;
+                    whole = !MASK && boxes > 0 && p + KT - 1 <= at1;
+                    if (whole && lane < boxes) {
+                        const unsigned at = (unsigned)p + (unsigned)lane * (unsigned)a.box, b = at / (unsigned)ps;
+                        page = __ldg(table + b);
+                        row = (int)(at - b * (unsigned)ps);
+                    }
+                };
+                auto copy_boxes = [&](const CUtensorMap* map, int pg, int r) {
+                    uint64_t* bar = &sh.full[stage];
+                    expects(bar, HALVES == 1 ? (pw ? 0u : STAGE) : STAGE / 2, 32);
+                    if (lane < boxes && (HALVES > 1 || pw == 0))
+#pragma unroll
+                        for (int hf = HALVES == 1 ? 0 : pw; hf < HALVES; hf += 2)
+                            pf_tma(ring + stage * STAGE + hf * KHALF + lane * a.box * 128, map, hf * 64, r, x.h, pg, bar);
+                    if (++stage == ST) stage = 0, lap ^= 1u;
+                };
+                find_boxes(0);
+                for (int t = 0; t <= n; ++t) {
+                    if (t < n) {
+                        whole = whole && __all_sync(0xffffffffu, lane >= boxes || (unsigned)page < (unsigned)a.kv.n_pages);
+                        if (!whole) find(t);
+                        if (!(ok = pf_wait(&sh.empty[stage], lap ^ 1u))) break;
+                        if (whole) copy_boxes(&a.map_k, page, row);
+                        else copy(kb, k_off);
+                    }
+                    const bool now_whole = whole;
+                    const int now_page = page, now_row = row;
+                    if (t + 1 < n) find_boxes(t + 1);
+                    if (t > 0) {
+                        if (!(ok = pf_wait(&sh.empty[stage], lap ^ 1u))) break;
+                        if (v_whole) {
+                            copy_boxes(&a.map_v, v_page, v_row);
+                        } else if (MASK) {
+                            float m = -INFINITY;
+#pragma unroll
+                            for (int e = 0; e < RPL; ++e) {
+                                sh.bias[stage][pw * RPW + 32 * e + lane] = bias[e];
+                                m = fmaxf(m, h2f(bias[e]));
+                            }
+                            m = warp_max(m);
+                            if (lane == 0) sh.tmax[stage][pw] = m;
+                        }
+                        if (!v_whole) copy(vb, v_off);
+                    }
+                    v_whole = now_whole, v_page = now_page, v_row = now_row;
+#pragma unroll
+                    for (int e = 0; e < RPL; ++e) v_off[e] = v_next[e], bias[e] = bias_next[e];
                 }
-                v_off = v_next;
-                bias = bias_next;
+                ++unit;
             }
-            ++unit;
-        }
-        flush();
-        if (!ok) sh.aborted = 1;
-    } else if (role == 3) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-        if (warp == 12 && lane == 0) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (!ok) sh.aborted = 1;
+        } else if (warp == kPfIssueWarp && lane == 0) {
             // ---- tensor-core issue
             constexpr uint32_t type = BF16 ? (1u << 7) | (1u << 10) : 0u;
             const uint32_t negate = a.scale < 0.f ? 1u << 13 : 0u;  // of q
@@ -478,6 +564,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
             int base = 0, unit = 0;            // ring places before this unit
             uint32_t ready[2] = {0, 0};        // parities of p_ready
             bool ok = true;
+            auto landed = [&](uint64_t* bar, uint32_t parity) {
+                const bool there = mbar_wait_bounded(bar, parity);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                return there;
+            };
             auto stage_of = [&](int place) { return place % ST; };
             auto parity_of = [&](int place) { return (uint32_t)(place / ST) & 1u; };
             auto scores = [&](int j, uint32_t d, int stage) {
@@ -496,9 +587,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
             while (ok && walk.next(a, units, total, x)) {
                 const int n = x.te - x.tb;
                 const bool two = NT == 2 && x.n * a.group - x.row0 > kPfRows;
-                if (!(ok = mbar_wait_bounded(&sh.q_full, unit & 1))) break;
+                if (!(ok = landed(&sh.q_full, unit & 1))) break;
                 int k_at = base;
-                if (!(ok = mbar_wait_bounded(&sh.full[stage_of(k_at)], parity_of(k_at)))) break;
+                if (!(ok = landed(&sh.full[stage_of(k_at)], parity_of(k_at)))) break;
                 tc_fence_after();
                 scores(0, tmem, stage_of(k_at));
                 tc_commit(&sh.s_full[0]);
@@ -512,7 +603,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                     const bool more = t + 1 < n;
                     k_at = base + pf_k_place(t + 1);
                     const int v_at = base + pf_v_place(t, n);
-                    if (more && !(ok = mbar_wait_bounded(&sh.full[stage_of(k_at)], parity_of(k_at)))) break;
+                    if (more && !(ok = landed(&sh.full[stage_of(k_at)], parity_of(k_at)))) break;
                     if (NT == 1 && more) {
                         // the other score buffer: its weights went into the product before
                         tc_fence_after();
@@ -521,7 +612,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         tc_commit(&sh.empty[stage_of(k_at)]);
                         if (t + 2 == n) tc_commit(&sh.q_empty);
                     }
-                    if (!(ok = mbar_wait_bounded(&sh.full[stage_of(v_at)], parity_of(v_at)))) break;
+                    if (!(ok = landed(&sh.full[stage_of(v_at)], parity_of(v_at)))) break;
                     if (NT == 1) {
                         if (!(ok = mbar_wait_bounded(&sh.p_ready[t & 1], ready[t & 1]))) break;
                         ready[t & 1] ^= 1u;
@@ -556,7 +647,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
         __syncwarp();
     } else {
         // ---- softmax: a row to a thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int j = role;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t o_addr = tmem + lanes + O_COL + (NT == 2 ? j * D : 0);
@@ -564,11 +655,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
         const float scale2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.17549435e-38f);
         int base = 0;
         uint32_t s_par[2] = {0, 0}, o_par = 0;  // o_par: products into this tile's outputs so far
-        bool ok = j < NT, first_unit = true;
+        bool ok = j < NT;
         while (ok && walk.next(a, units, total, x)) {
             const int n = x.te - x.tb, count = x.n * a.group;
-            const bool first_in_range = first_unit;
-            first_unit = false;
             if (j * kPfRows >= count - x.row0) {  // no rows for this tile
                 base += 2 * n;
                 continue;
@@ -587,24 +676,19 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                 if (MASK && !(ok = pf_wait(&sh.full[v_stage], (uint32_t)(v_at / ST) & 1u))) break;
                 tc_fence_after();
                 if (any) {
-                    uint32_t s[KT / 32][32];
-#pragma unroll
-                    for (int c = 0; c < KT / 32; ++c) tc_ld_x32(s[c], s_addr + 32 * c);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int c = 0; c < KT / 32; ++c) tc_loaded(s[c]);
                     // columns lo .. hi are seen
                     const int p0 = (x.tile0 + x.tb + t) * KT;
                     const int hi = at - p0, lo = a.window > 0 ? max(0, at - a.window + 1) - p0 : 0;
                     const bool edge = __any_sync(0xffffffffu, hi < KT - 1 || lo > 0);
+                    const uint4* entries = reinterpret_cast<const uint4*>(sh.bias[v_stage]);
+                    float c0 = 0.f;
                     if (MASK) {
-                        const uint4* b = reinterpret_cast<const uint4*>(sh.bias[v_stage]);
                         float cm;
                         if (edge) {
                             cm = -INFINITY;
-#pragma unroll
+#pragma unroll 4
                             for (int c = 0; c < KT; c += 8) {
-                                const uint4 w = b[c / 8];
+                                const uint4 w = entries[c / 8];
                                 const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                                 for (int e = 0; e < 8; e += 2) {
@@ -614,8 +698,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                                 }
                             }
                         } else {
-                            cm = fmaxf(fmaxf(sh.tmax[v_stage][0], sh.tmax[v_stage][1]),
-                                       fmaxf(sh.tmax[v_stage][2], sh.tmax[v_stage][3]));
+                            cm = fmaxf(sh.tmax[v_stage][0], sh.tmax[v_stage][1]);
                         }
                         // the mask relative to the largest entry that the row has seen:
                         // a row of lowest values keeps its scores' bits
@@ -623,33 +706,49 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                             ref += (c_ref - cm) * 1.4426950408889634f;
                             c_ref = cm;
                         }
-                        const float c0 = c_ref == -INFINITY ? 0.f : c_ref;
+                        c0 = c_ref == -INFINITY ? 0.f : c_ref;
+                    }
+                    // 32 scores as loaded: with a mask times scale2 and the entries added,
+                    // -inf where the row does not see
+                    auto ready = [&](uint32_t (&s)[32], int c) {
+                        if (MASK) {
 #pragma unroll
-                        for (int c = 0; c < KT; c += 8) {
-                            const uint4 w = b[c / 8];
-                            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                            for (int k = 0; k < 32; k += 8) {
+                                const uint4 w = entries[(c + k) / 8];
+                                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                            for (int e = 0; e < 8; e += 2) {
-                                const float2 f = unpack16<false>(ws[e / 2]);
-                                uint32_t* y = &s[c >> 5][(c & 31) + e];
-                                y[0] = __float_as_uint(fmaf(__uint_as_float(y[0]), scale2, (f.x - c0) * 1.4426950408889634f));
-                                y[1] = __float_as_uint(fmaf(__uint_as_float(y[1]), scale2, (f.y - c0) * 1.4426950408889634f));
+                                for (int e = 0; e < 8; e += 2) {
+                                    const float2 f = unpack16<false>(ws[e / 2]);
+                                    s[k + e] = __float_as_uint(
+                                        fmaf(__uint_as_float(s[k + e]), scale2, (f.x - c0) * 1.4426950408889634f));
+                                    s[k + e + 1] = __float_as_uint(
+                                        fmaf(__uint_as_float(s[k + e + 1]), scale2, (f.y - c0) * 1.4426950408889634f));
+                                }
                             }
                         }
+                        if (edge) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (c + e < lo || c + e > hi) s[e] = 0xff800000u;
+                        }
+                    };
+                    // two passes over the scores in 32 columns each, the next ones on their way
+                    uint32_t s[2][32];
+                    float m[2] = {-INFINITY, -INFINITY};
+                    tc_ld_x32(s[0], s_addr);
+#pragma unroll
+                    for (int c = 0; c < KT / 32; ++c) {
+                        tc_wait_ld();
+                        tc_loaded(s[c & 1]);
+                        tc_ld_x32(s[(c + 1) & 1], s_addr + 32 * ((c + 1) % (KT / 32)));
+                        ready(s[c & 1], 32 * c);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            m[0] = pf_max3(m[0], __uint_as_float(s[c & 1][e]), __uint_as_float(s[c & 1][e + 1]));
+                            m[1] = pf_max3(m[1], __uint_as_float(s[c & 1][e + 2]), __uint_as_float(s[c & 1][e + 3]));
+                        }
                     }
-                    if (edge) {
-#pragma unroll
-                        for (int c = 0; c < KT; ++c)
-                            if (c < lo || c > hi) s[c >> 5][c & 31] = 0xff800000u;
-                    }
-                    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int c = 0; c < KT; c += 8)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            m[e] = fmaxf(m[e], fmaxf(__uint_as_float(s[c >> 5][(c & 31) + 2 * e]),
-                                                     __uint_as_float(s[c >> 5][(c & 31) + 2 * e + 1])));
-                    float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                    float top = fmaxf(m[0], m[1]);
                     if (!MASK) top *= scale2;
                     const bool moves = top > ref + kPfLazy;
                     if (__any_sync(0xffffffffu, moves)) {
@@ -672,23 +771,28 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         }
                     }
                     const float off = (ref == -INFINITY ? 0.f : -ref) + kPfShift<BF16>;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const uint64_t off2 = pf_pair(off, off), scale22 = pf_pair(scale2, scale2);
+                    uint64_t sum = pf_pair(0.f, 0.f);
+                    uint32_t p[32];
 #pragma unroll
-                    for (int c0 = 0; c0 < KT; c0 += 64) {
-                        uint32_t p[32];
+                    for (int c = 0; c < KT / 32; ++c) {
+                        tc_wait_ld();
+                        tc_loaded(s[c & 1]);
+                        if (c + 1 < KT / 32) tc_ld_x32(s[(c + 1) & 1], s_addr + 32 * (c + 1));
+                        ready(s[c & 1], 32 * c);
 #pragma unroll
-                        for (int c = 0; c < 64; c += 2) {
-                            const uint32_t* y = &s[(c0 + c) >> 5][(c0 + c) & 31];
-                            const float x0 = __uint_as_float(y[0]), x1 = __uint_as_float(y[1]);
-                            const float e0 = pf_exp2(MASK ? x0 + off : fmaf(x0, scale2, off));
-                            const float e1 = pf_exp2(MASK ? x1 + off : fmaf(x1, scale2, off));
-                            sum[(c >> 1) & 1] += e0;
-                            sum[2 + ((c >> 1) & 1)] += e1;
-                            p[c >> 1] = pack16<BF16>(e0, e1);
+                        for (int e = 0; e < 32; e += 2) {
+                            const uint64_t y = pf_pair(__uint_as_float(s[c & 1][e]), __uint_as_float(s[c & 1][e + 1]));
+                            const float2 z = pf_unpair(MASK ? pf_add2(y, off2) : pf_fma2(y, scale22, off2));
+                            const float e0 = pf_exp2(z.x), e1 = pf_exp2(z.y);
+                            sum = pf_add2(sum, pf_pair(e0, e1));
+                            p[(c & 1) * 16 + e / 2] = pack16<BF16>(e0, e1);
                         }
-                        tc_st_x32(s_addr + c0 / 2, p);
+                        // (over scores that both passes have read)
+                        if (c & 1) tc_st_x32(s_addr + 32 * (c >> 1), p);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    const float2 both = pf_unpair(sum);
+                    l += both.x + both.y;
                     tc_wait_st();
                 }
                 // (one score buffer: the scores came after the product before.  Two: the parity
@@ -738,7 +842,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                     if (again) a.bad[at_list] = make_int2((int)out_row, x.u);
                 }
             } else {
-                const int slot = 2 * blockIdx.x + (first_in_range ? 0 : 1);
+                // at most one unit goes on from the CTA before, and one goes on in the next
+                const int slot = 2 * blockIdx.x + (x.tb > 0 ? 0 : 1);
                 float4* ml = a.piece_ml + ((int64_t)slot * NT + j) * kPfRows + row;
                 float4* po = a.piece_o + ((int64_t)slot * NT + j) * (D / 4) * kPfRows + row;
                 if (real) *ml = make_float4(ref, l, c_ref, 0.f);
@@ -762,8 +867,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
     }
     tc_fence_before();
     __syncthreads();
-    if (tid == 12 * 32) tc_commit(&sh.done);  // every product issued has ended
-    if (warp == 12) {
+    if (tid == kPfIssueWarp * 32) tc_commit(&sh.done);  // every product issued has ended
+    if (warp == kPfIssueWarp) {
         mbar_wait_drain(&sh.done, 0);
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
@@ -787,15 +892,15 @@ __global__ void __launch_bounds__(kPfFinishThreads) paged_prefill_finish_kernel(
     const int64_t cut = (int64_t)(blockIdx.y + 1) * per;
     if (cut < all) {
         const int h = (int)(cut / total), u = pf_find(a.prefix, a.header->units, cut - h * total);
-        const int64_t start = h * total + a.prefix[u], end = h * total + a.prefix[u + 1];
-        const int c0 = (int)(start / per), c1 = (int)((end - 1) / per);
-        if (start < cut && c0 == (int)blockIdx.y) {
-            const int4 d0 = a.desc[2 * (int64_t)u], d1 = a.desc[2 * (int64_t)u + 1];
+        const int4 d0 = a.desc[2 * (int64_t)u], d1 = a.desc[2 * (int64_t)u + 1];
+        const int64_t start = h * total + a.prefix[u] + kPfUnitSteps;  // its first key tile
+        const int c0 = (int)(start / per), c1 = (int)((start + d0.w - 1) / per);
+        if (c0 == (int)blockIdx.y && c1 > c0) {
             const int r0 = blockIdx.x * 32, j = r0 / kPfRows, row = (r0 & (kPfRows - 1)) + lane;
             const int flat = d0.y + r0 + lane;
             const bool real = flat < d1.y * a.group;
             if (d0.y + r0 < d1.y * a.group) {
-                auto slot = [&](int c) { return (int64_t)(2 * c + (c == c0 && start > c0 * per ? 1 : 0)) * NT + j; };
+                auto slot = [&](int c) { return (int64_t)(2 * c + (c == c0 ? 1 : 0)) * NT + j; };
                 // references of all pieces first
                 float cm = -INFINITY, top = -INFINITY;
                 if (a.mask)

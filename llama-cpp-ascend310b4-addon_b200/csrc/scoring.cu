@@ -86,6 +86,24 @@ int launch_prefill(const PagedPrefillArgs& a, cudaStream_t st) {
     }
 }
 
+// A 16-bit view of four dimensions, the first contiguous, for boxes of 64 values by
+// b1 by b2; false where TMA has no such view.
+bool encode_view(CUtensorMap* m, const void* base, const int64_t (&dims)[4], const int64_t (&strides)[3], int b1, int b2) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+    if (!enc) return false;
+    cuuint64_t d[4], st[3];
+    for (int i = 0; i < 4; ++i) d[i] = (cuuint64_t)dims[i];
+    for (int i = 0; i < 3; ++i) {
+        const bool single = dims[i + 1] == 1;
+        if (!single && (strides[i] <= 0 || strides[i] >= (int64_t)1 << 40)) return false;
+        st[i] = single ? 16 : (cuuint64_t)strides[i];
+    }
+    const cuuint32_t box[4] = {64, (cuuint32_t)b1, (cuuint32_t)b2, 1}, step[4] = {1, 1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), d, st, box, step,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 struct PrefillLayout {
     size_t desc, prefix, bad, ml, o, total;
 };
@@ -178,8 +196,20 @@ int b200_paged_prefill(const b200_paged_kv* kv, const void* q, int64_t q_stride,
         return B200_EINVAL;
     if (q_stride > INT64_MAX / 4 / n_tokens) return B200_EINVAL;
     if (meets_rows(out, n_tokens * row * 2, q, q_stride * 2, row * 2, n_tokens)) return B200_EINVAL;
-    PagedPrefillArgs a;
+    PagedPrefillArgs a = {};
     a.kv = *kv;
+    // rows of a page to a box: the largest power of two that divides the page, 8 (a
+    // group of the swizzle) at least, a tile of keys at most
+    a.box = std::min(kv->page_size & -kv->page_size, pf_keys(kv->head_dim));
+    const int64_t d = kv->head_dim, group = n_head / kv->n_head_kv;
+    const int64_t page_dims[4] = {d, kv->page_size, kv->n_head_kv, kv->n_pages};
+    if (a.box < 8 || !encode_view(&a.map_k, kv->k, page_dims, {kv->k_row, kv->k_head, kv->k_page}, a.box, 1) ||
+        !encode_view(&a.map_v, kv->v, page_dims, {kv->v_row, kv->v_head, kv->v_page}, a.box, 1))
+        a.box = 0;
+    a.q_box = kPfRows % group == 0 ? (int)(kPfRows / group) : 0;
+    if (a.q_box && !encode_view(&a.map_q, q, {d, group, n_tokens, kv->n_head_kv}, {d * 2, q_stride * 2, group * d * 2},
+                                (int)group, a.q_box))
+        a.q_box = 0;
     a.q = static_cast<const uint16_t*>(q);
     a.q_stride = q_stride;
     a.table = block_table;
