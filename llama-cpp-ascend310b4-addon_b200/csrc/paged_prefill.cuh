@@ -40,6 +40,8 @@ struct PagedPrefillArgs {
     struct PfHeader* header;
     int4* desc;         // two per unit: {sequence, first flat row, first key tile, key tiles}, {first, n, len, -}
     int64_t* prefix;    // [units + 1] steps of the units before
+    int2* start;        // [CTAs] {unit, KV head} that a CTA's range starts in
+    int2* cut;          // [CTAs] the one that begins in a CTA's range and goes on past it; unit -1: none
     int2* bad;          // rows to compute again: {flat (token, head), unit}
     float4* piece_ml;   // [2 * CTAs][tiles][128] {reference, sum, mask reference, -} of cut units
     float4* piece_o;    // [2 * CTAs][tiles][D / 4][128] their sums of weighted values
@@ -174,6 +176,7 @@ __global__ void __launch_bounds__(kPfPlanThreads) paged_prefill_plan_kernel(cons
                                                                             int rows, int keys) {
     __shared__ int64_t part[32], s_base[kPfPlanThreads + 1];
     __shared__ PfSeq s_seq[kPfPlanThreads];
+    __shared__ int64_t s_prefix[kPfPlanThreads + 1];
     const int tid = threadIdx.x;
     int64_t units = 0, tiles = 0, sum;
     for (int base = 0; base < a.n_seq; base += kPfPlanThreads) {
@@ -212,45 +215,51 @@ __global__ void __launch_bounds__(kPfPlanThreads) paged_prefill_plan_kernel(cons
                 a.desc[2 * (units + u)] = d0;
                 a.desc[2 * (units + u) + 1] = d1;
                 a.prefix[units + u] = before;
+                if (units + u < kPfPlanThreads) s_prefix[units + u] = before;
             }
             tiles += more;
         }
         units += sum;
         __syncthreads();  // s_base and s_seq are read no more
     }
+    const int64_t all = tiles * a.kv.n_head_kv, per = max((int64_t)1, (all + kPfCtas - 1) / kPfCtas);
     if (tid == 0) {
         a.prefix[units] = tiles;
-        const int64_t all = tiles * a.kv.n_head_kv;
         a.header->total = tiles;
-        a.header->per_cta = max((int64_t)1, (all + kPfCtas - 1) / kPfCtas);
+        a.header->per_cta = per;
         a.header->units = (int)units;
         a.header->n_bad = 0;
     }
-}
-
-// Largest u with prefix[u] <= x, for prefix[0] = 0 <= x < prefix[n]; a warp together.
-__device__ __forceinline__ int pf_find(const int64_t* prefix, int n, int64_t x) {
-    const int lane = threadIdx.x & 31;
-    int lo = 0, hi = n;  // prefix[lo] <= x < prefix[hi]
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-        const unsigned below = __ballot_sync(0xffffffffu, at < hi && prefix[at] <= x);
-        const int last = 31 - __clz((int)below);
-        lo += last * step;
-        hi = min(hi, lo + step);
+    // where every CTA starts (the loops above end with a barrier behind the last prefix)
+    if (tid < kPfCtas && tid * per < all) {
+        const int64_t h = tid * per / tiles, x = tid * per - h * tiles;
+        const int64_t* prefix = units <= kPfPlanThreads ? s_prefix : a.prefix;
+        int lo = 0, hi = (int)units;  // prefix[lo] <= x < prefix[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (prefix[mid] <= x) lo = mid;
+            else hi = mid;
+        }
+        a.start[tid] = make_int2(lo, (int)h);
     }
-    return lo;
 }
 
 // A unit, or the part of one that lies in a CTA's range.
 struct PfUnit {
     int u, s, h, row0, first, n, len, tile0;  // tile0: the unit's first key tile
     int tb, te, cost;                      // key tiles tb .. te - 1 of cost
+    int shift;                             // the first of them to be done, from tb
+    // key tile of step t: all in turn, from `shift` on
+    __device__ __forceinline__ int tile(int t) const {
+        const int n = te - tb, i = t + shift;
+        return tile0 + tb + (i < n ? i : i - n);
+    }
 };
 // Walks over a range of the line of key tiles of all KV heads' units.
 struct PfWalk {
     int64_t w, w1;
     int u, h;
+    int steps;  // done by this CTA
     __device__ __forceinline__ bool next(const PagedPrefillArgs& a, int units, int64_t total, PfUnit& x) {
         while (w < w1) {
             const int4 d0 = __ldg(a.desc + 2 * (int64_t)u), d1 = __ldg(a.desc + 2 * (int64_t)u + 1);
@@ -263,7 +272,14 @@ struct PfWalk {
             x.te = (int)min((int64_t)x.cost, w1 - start);
             w = start + x.cost;
             if (++u == units) u = 0, ++h;
-            if (x.tb < x.te) return true;
+            if (x.tb < x.te) {
+                // units of one long sequence are done in step: CTAs that are at the same
+                // step read the same keys, from the L2 cache all but one of them
+                const int at = steps % x.cost;
+                x.shift = at >= x.tb && at < x.te ? at - x.tb : 0;
+                steps += x.te - x.tb + kPfUnitSteps;
+                return true;
+            }
         }
         return false;
     }
@@ -276,7 +292,7 @@ struct PfShared {
     static constexpr int ST = pf_stages(D);
     uint64_t q_full, q_empty, full[ST], empty[ST], s_full[2], p_ready[2], o_done[2], done;
     uint32_t tmem;
-    int aborted, u, h;
+    int aborted;
     float tmax[ST][2];                       // largest mask entry of each warp's rows
     alignas(16) uint16_t bias[ST][pf_keys(D)];  // mask of the tile whose values a stage holds
 };
@@ -382,14 +398,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
     PfWalk walk;
     walk.w = min(total * a.kv.n_head_kv, per_cta * blockIdx.x);
     walk.w1 = min(total * a.kv.n_head_kv, walk.w + per_cta);
-    if (warp == 0 && walk.w < walk.w1) {
-        const int h = (int)(walk.w / total), u = pf_find(a.prefix, units, walk.w - h * total);
-        if (lane == 0) sh.h = h, sh.u = u;
-    }
+    const int2 start = a.start[blockIdx.x];  // (not used by a CTA without work)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    walk.u = sh.u, walk.h = sh.h;
+    walk.u = start.x, walk.h = start.y, walk.steps = 0;
     const uint32_t tmem = sh.tmem;
     PfUnit x;
 
@@ -422,7 +435,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
             bool ok = true;
             const int ps = a.kv.page_size;
             const uint64_t krow = a.kv.k_row >> 4, vrow = a.kv.v_row >> 4, kpage = a.kv.k_page >> 4, vpage = a.kv.v_page >> 4;
+            int2 cut = make_int2(-1, 0);
             while (ok && walk.next(a, units, total, x)) {
+                if (x.tb == 0 && x.te < x.cost) cut = make_int2(x.u, x.h);
                 const int n = x.te - x.tb, rows = min(NT * kPfRows, x.n * a.group - x.row0);
                 const int at1 = x.len - x.n + (x.row0 + rows - 1) / a.group;  // the last position that a row sees
                 if (unit && !(ok = pf_wait(&sh.q_empty, (unit - 1) & 1))) break;
@@ -460,7 +475,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                 auto find = [&](int t) {
 #pragma unroll
                     for (int e = 0; e < RPL; ++e) {
-                        const int p = (x.tile0 + x.tb + t) * KT + pw * RPW + 32 * e + lane;
+                        const int p = x.tile(t) * KT + pw * RPW + 32 * e + lane;
                         bool on = p <= at1;
                         k_off[e] = v_next[e] = ~0u;
                         bias_next[e] = kNone;
@@ -502,7 +517,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                 int page = 0, row = 0, v_page = 0, v_row = 0;
                 bool whole = false, v_whole = false;
                 auto find_boxes = [&](int t) {
-                    const int p = (x.tile0 + x.tb + t) * KT;
+                    const int p = x.tile(t) * KT;
                     whole = !MASK && boxes > 0 && p + KT - 1 <= at1;
                     if (whole && lane < boxes) {
                         const unsigned at = (unsigned)p + (unsigned)lane * (unsigned)a.box, b = at / (unsigned)ps;
@@ -553,6 +568,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                 }
                 ++unit;
             }
+            if (tid == 256) a.cut[blockIdx.x] = cut;
             asm volatile("cp.async.wait_all;" ::: "memory");
             if (!ok) sh.aborted = 1;
         } else if (warp == kPfIssueWarp && lane == 0) {
@@ -677,7 +693,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                 tc_fence_after();
                 if (any) {
                     // columns lo .. hi are seen
-                    const int p0 = (x.tile0 + x.tb + t) * KT;
+                    const int p0 = x.tile(t) * KT;
                     const int hi = at - p0, lo = a.window > 0 ? max(0, at - a.window + 1) - p0 : 0;
                     const bool edge = __any_sync(0xffffffffu, hi < KT - 1 || lo > 0);
                     const uint4* entries = reinterpret_cast<const uint4*>(sh.bias[v_stage]);
@@ -732,20 +748,20 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                                 if (c + e < lo || c + e > hi) s[e] = 0xff800000u;
                         }
                     };
-                    // two passes over the scores in 32 columns each, the next ones on their way
-                    uint32_t s[2][32];
+                    // the row's scores in registers, 32 at a time, the next ones on their way
+                    uint32_t s[KT / 32][32];
                     float m[2] = {-INFINITY, -INFINITY};
                     tc_ld_x32(s[0], s_addr);
 #pragma unroll
                     for (int c = 0; c < KT / 32; ++c) {
                         tc_wait_ld();
-                        tc_loaded(s[c & 1]);
-                        tc_ld_x32(s[(c + 1) & 1], s_addr + 32 * ((c + 1) % (KT / 32)));
-                        ready(s[c & 1], 32 * c);
+                        tc_loaded(s[c]);
+                        if (c + 1 < KT / 32) tc_ld_x32(s[c + 1], s_addr + 32 * (c + 1));
+                        ready(s[c], 32 * c);
 #pragma unroll
                         for (int e = 0; e < 32; e += 4) {
-                            m[0] = pf_max3(m[0], __uint_as_float(s[c & 1][e]), __uint_as_float(s[c & 1][e + 1]));
-                            m[1] = pf_max3(m[1], __uint_as_float(s[c & 1][e + 2]), __uint_as_float(s[c & 1][e + 3]));
+                            m[0] = pf_max3(m[0], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+                            m[1] = pf_max3(m[1], __uint_as_float(s[c][e + 2]), __uint_as_float(s[c][e + 3]));
                         }
                     }
                     float top = fmaxf(m[0], m[1]);
@@ -776,19 +792,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                     uint32_t p[32];
 #pragma unroll
                     for (int c = 0; c < KT / 32; ++c) {
-                        tc_wait_ld();
-                        tc_loaded(s[c & 1]);
-                        if (c + 1 < KT / 32) tc_ld_x32(s[(c + 1) & 1], s_addr + 32 * (c + 1));
-                        ready(s[c & 1], 32 * c);
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
-                            const uint64_t y = pf_pair(__uint_as_float(s[c & 1][e]), __uint_as_float(s[c & 1][e + 1]));
+                            const uint64_t y = pf_pair(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
                             const float2 z = pf_unpair(MASK ? pf_add2(y, off2) : pf_fma2(y, scale22, off2));
                             const float e0 = pf_exp2(z.x), e1 = pf_exp2(z.y);
                             sum = pf_add2(sum, pf_pair(e0, e1));
                             p[(c & 1) * 16 + e / 2] = pack16<BF16>(e0, e1);
                         }
-                        // (over scores that both passes have read)
+                        // (over the scores, which are all in registers)
                         if (c & 1) tc_st_x32(s_addr + 32 * (c >> 1), p);
                     }
                     const float2 both = pf_unpair(sum);
@@ -879,8 +891,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
 
 constexpr int kPfFinishThreads = 256;
 
-// CTA (cut, 32 rows): the pieces of the unit that the cut is the first to go
-// through, joined in order.  Then the rows that infinities or NaN met, and which
+// CTA (CTA of the main kernel, 32 rows): the pieces of the unit that begins in that
+// one's range and goes on past it, joined in order.  Then the rows that infinities or NaN met, and which
 // no product of whole tiles can tell apart from positions they do not see.
 template <bool BF16, int D>
 __global__ void __launch_bounds__(kPfFinishThreads) paged_prefill_finish_kernel(const __grid_constant__ PagedPrefillArgs a) {
@@ -888,84 +900,87 @@ __global__ void __launch_bounds__(kPfFinishThreads) paged_prefill_finish_kernel(
     __shared__ int s_odd[W][32];
     griddep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t total = a.header->total, per = a.header->per_cta, all = total * a.kv.n_head_kv;
-    const int64_t cut = (int64_t)(blockIdx.y + 1) * per;
-    if (cut < all) {
-        const int h = (int)(cut / total), u = pf_find(a.prefix, a.header->units, cut - h * total);
+    const int2 cut = a.cut[blockIdx.y];
+    if (cut.x >= 0) {
+        const int u = cut.x, h = cut.y, c0 = blockIdx.y;
         const int4 d0 = a.desc[2 * (int64_t)u], d1 = a.desc[2 * (int64_t)u + 1];
-        const int64_t start = h * total + a.prefix[u] + kPfUnitSteps;  // its first key tile
-        const int c0 = (int)(start / per), c1 = (int)((start + d0.w - 1) / per);
-        if (c0 == (int)blockIdx.y && c1 > c0) {
-            const int r0 = blockIdx.x * 32, j = r0 / kPfRows, row = (r0 & (kPfRows - 1)) + lane;
-            const int flat = d0.y + r0 + lane;
-            const bool real = flat < d1.y * a.group;
-            if (d0.y + r0 < d1.y * a.group) {
-                auto slot = [&](int c) { return (int64_t)(2 * c + (c == c0 ? 1 : 0)) * NT + j; };
-                // references of all pieces first
-                float cm = -INFINITY, top = -INFINITY;
-                if (a.mask)
-                    for (int c = c0; c <= c1; ++c)
-                        if (real) cm = fmaxf(cm, a.piece_ml[slot(c) * kPfRows + row].z);
-                auto moved = [&](const float4& ml) {
-                    return a.mask && ml.z != cm ? ml.x + (ml.z - cm) * 1.4426950408889634f : ml.x;
-                };
-                for (int c = c0; c <= c1; ++c)
-                    if (real) top = fmaxf(top, moved(a.piece_ml[slot(c) * kPfRows + row]));
-                float l = 0.f;
-                float4 o[CPW];
+        const int r0 = blockIdx.x * 32, j = r0 / kPfRows, row = (r0 & (kPfRows - 1)) + lane;
+        const int flat = d0.y + r0 + lane;
+        const bool real = flat < d1.y * a.group;
+        if (d0.y + r0 < d1.y * a.group) {
+            // the CTA of the unit's last key tile
+            const int64_t last = h * a.header->total + a.prefix[u] + kPfUnitSteps + d0.w - 1;
+            const int pieces = (int)(last / a.header->per_cta) - c0 + 1;
+            // piece k: the last of CTA c0's range, then the first of each one's
+            auto slot = [&](int k) { return (int64_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * NT + j; };
+            float cm = -INFINITY, top = -INFINITY, l = 0.f;
+            float4 o[CPW];
 #pragma unroll
-                for (int e = 0; e < CPW; ++e) o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int c = c0; c <= c1; ++c) {
-                    if (!real) break;
-                    const float4 ml = a.piece_ml[slot(c) * kPfRows + row];
-                    const float ref = moved(ml), f = ref == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : pf_exp2(ref - top);
-                    l = fmaf(f, ml.y, l);
-                    const float4* po = a.piece_o + (slot(c) * (D / 4) + warp * CPW) * kPfRows + row;
-                    if (f != 0.f)
+            for (int e = 0; e < CPW; ++e) o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+            constexpr int AT_ONCE = 4;
+            for (int k0 = 0; k0 < pieces && real; k0 += AT_ONCE) {
+                float4 ml[AT_ONCE], y[AT_ONCE][CPW];
 #pragma unroll
-                        for (int e = 0; e < CPW; ++e) {
-                            const float4 y = po[e * kPfRows];
-                            o[e].x = fmaf(f, y.x, o[e].x), o[e].y = fmaf(f, y.y, o[e].y);
-                            o[e].z = fmaf(f, y.z, o[e].z), o[e].w = fmaf(f, y.w, o[e].w);
+                for (int k = 0; k < AT_ONCE; ++k) {
+                    if (k0 + k >= pieces) continue;
+                    const int64_t at = slot(k0 + k);
+                    ml[k] = a.piece_ml[at * kPfRows + row];
+                    const float4* po = a.piece_o + (at * (D / 4) + warp * CPW) * kPfRows + row;
+#pragma unroll
+                    for (int e = 0; e < CPW; ++e) y[k][e] = po[e * kPfRows];
+                }
+#pragma unroll
+                for (int k = 0; k < AT_ONCE; ++k) {
+                    if (k0 + k >= pieces) continue;
+                    float ref = ml[k].x;
+                    if (a.mask) {  // relative to the largest mask entry so far
+                        if (ml[k].z > cm) {
+                            top += (cm - ml[k].z) * 1.4426950408889634f;
+                            cm = ml[k].z;
+                        } else if (ml[k].z < cm) {
+                            ref += (ml[k].z - cm) * 1.4426950408889634f;
                         }
-                    else  // a weight of 0 meets what is not finite
-#pragma unroll
-                        for (int e = 0; e < CPW; ++e) {
-                            const float4 y = po[e * kPfRows];
-                            const float z = (y.x + y.y + y.z + y.w) * 0.f;
-                            o[e].x += z;
-                        }
-                }
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                const int i = flat / a.group, g = flat - i * a.group;
-                const int64_t out_row = (int64_t)(d1.x + i) * a.n_head + h * a.group + g;
-                float odd = l * 0.f;
-                uint32_t w[2 * CPW];
-#pragma unroll
-                for (int e = 0; e < CPW; ++e) {
-                    odd += o[e].x * 0.f + o[e].y * 0.f + o[e].z * 0.f + o[e].w * 0.f;
-                    w[2 * e] = l == 0.f ? 0u : pack16<BF16>(o[e].x * inv, o[e].y * inv);
-                    w[2 * e + 1] = l == 0.f ? 0u : pack16<BF16>(o[e].z * inv, o[e].w * inv);
-                }
-                if (real) {
-                    uint2* to = reinterpret_cast<uint2*>(a.out + out_row * D) + warp * CPW;
-#pragma unroll
-                    for (int e = 0; e < CPW; ++e) to[e] = make_uint2(w[2 * e], w[2 * e + 1]);
-                }
-                s_odd[warp][lane] = real && l != 0.f && odd != 0.f;
-                __syncthreads();
-                bool again = false;
-#pragma unroll
-                for (int v = 0; v < W; ++v) again |= s_odd[v][lane] != 0;
-                unsigned votes = __ballot_sync(0xffffffffu, again);
-                PfSeq sq;
-                sq.first = d1.x, sq.n = d1.y, sq.len = d1.z;
-                for (int k = 0; votes; votes &= votes - 1, ++k)
-                    if (k % W == warp) {
-                        const int r = d0.y + r0 + __ffs(votes) - 1, t = r / a.group;
-                        pf_row<BF16, D>(a, d0.x, sq, t, h * a.group + r - t * a.group);
                     }
+                    const float now = fmaxf(top, ref), base = now == -INFINITY ? 0.f : now;
+                    const float fo = pf_exp2(top - base), f = pf_exp2(ref - base);
+                    l = fo * l + f * ml[k].y;
+                    top = now;
+#pragma unroll
+                    for (int e = 0; e < CPW; ++e) {
+                        o[e].x = fo * o[e].x + f * y[k][e].x, o[e].y = fo * o[e].y + f * y[k][e].y;
+                        o[e].z = fo * o[e].z + f * y[k][e].z, o[e].w = fo * o[e].w + f * y[k][e].w;
+                    }
+                }
             }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const int i = flat / a.group, g = flat - i * a.group;
+            const int64_t out_row = (int64_t)(d1.x + i) * a.n_head + h * a.group + g;
+            float odd = l * 0.f;
+            uint32_t w[2 * CPW];
+#pragma unroll
+            for (int e = 0; e < CPW; ++e) {
+                odd += o[e].x * 0.f + o[e].y * 0.f + o[e].z * 0.f + o[e].w * 0.f;
+                w[2 * e] = l == 0.f ? 0u : pack16<BF16>(o[e].x * inv, o[e].y * inv);
+                w[2 * e + 1] = l == 0.f ? 0u : pack16<BF16>(o[e].z * inv, o[e].w * inv);
+            }
+            if (real) {
+                uint2* to = reinterpret_cast<uint2*>(a.out + out_row * D) + warp * CPW;
+#pragma unroll
+                for (int e = 0; e < CPW; ++e) to[e] = make_uint2(w[2 * e], w[2 * e + 1]);
+            }
+            s_odd[warp][lane] = real && l != 0.f && odd != 0.f;
+            __syncthreads();
+            bool again = false;
+#pragma unroll
+            for (int v = 0; v < W; ++v) again |= s_odd[v][lane] != 0;
+            unsigned votes = __ballot_sync(0xffffffffu, again);
+            PfSeq sq;
+            sq.first = d1.x, sq.n = d1.y, sq.len = d1.z;
+            for (int k = 0; votes; votes &= votes - 1, ++k)
+                if (k % W == warp) {
+                    const int r = d0.y + r0 + __ffs(votes) - 1, t = r / a.group;
+                    pf_row<BF16, D>(a, d0.x, sq, t, h * a.group + r - t * a.group);
+                }
         }
     }
     const int n_bad = a.header->n_bad;

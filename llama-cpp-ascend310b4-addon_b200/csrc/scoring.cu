@@ -73,7 +73,7 @@ int launch_prefill_d(const PagedPrefillArgs& a, cudaStream_t st) {
     paged_prefill_plan_kernel<<<1, kPfPlanThreads, 0, st>>>(a, pf_tiles(D) * kPfRows, pf_keys(D));
     CR_(cuda_status(cudaGetLastError()));
     CR_(a.mask ? (launch_prefill_main<BF16, D, true>(a, st)) : (launch_prefill_main<BF16, D, false>(a, st)));
-    return launch_after(paged_prefill_finish_kernel<BF16, D>, dim3(pf_tiles(D) * kPfRows / 32, kPfCtas - 1),
+    return launch_after(paged_prefill_finish_kernel<BF16, D>, dim3(pf_tiles(D) * kPfRows / 32, kPfCtas),
                         kPfFinishThreads, st, a);
 }
 
@@ -105,14 +105,16 @@ bool encode_view(CUtensorMap* m, const void* base, const int64_t (&dims)[4], con
 }
 
 struct PrefillLayout {
-    size_t desc, prefix, bad, ml, o, total;
+    size_t start, cut, desc, prefix, bad, ml, o, total;
 };
 
 PrefillLayout prefill_layout(int head_dim, int64_t n_tokens, int64_t n_seq, int64_t n_head, int64_t n_head_kv) {
     const int64_t rows = pf_tiles(head_dim) * kPfRows;
     const int64_t units = n_tokens * (n_head / n_head_kv) / rows + n_seq;
     PrefillLayout l;
-    l.desc = 256;
+    l.start = 256;
+    l.cut = l.start + align256(kPfCtas * sizeof(int2));
+    l.desc = l.cut + align256(kPfCtas * sizeof(int2));
     l.prefix = l.desc + align256((size_t)units * 2 * sizeof(int4));
     l.bad = l.prefix + align256((size_t)(units + 1) * sizeof(int64_t));
     l.ml = l.bad + align256((size_t)(n_tokens * n_head) * sizeof(int2));
@@ -230,6 +232,8 @@ int b200_paged_prefill(const b200_paged_kv* kv, const void* q, int64_t q_stride,
     const PrefillLayout l = prefill_layout(kv->head_dim, n_tokens, n_seq, n_head, kv->n_head_kv);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     a.header = reinterpret_cast<PfHeader*>(ws);
+    a.start = reinterpret_cast<int2*>(ws + l.start);
+    a.cut = reinterpret_cast<int2*>(ws + l.cut);
     a.desc = reinterpret_cast<int4*>(ws + l.desc);
     a.prefix = reinterpret_cast<int64_t*>(ws + l.prefix);
     a.bad = reinterpret_cast<int2*>(ws + l.bad);
