@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(kPfPlanThreads) paged_prefill_plan_kernel(cons
     __shared__ PfSeq s_seq[kPfPlanThreads];
     __shared__ int64_t s_prefix[kPfPlanThreads + 1];
     const int tid = threadIdx.x;
+    griddep_launch_dependents();
     int64_t units = 0, tiles = 0, sum;
     for (int base = 0; base < a.n_seq; base += kPfPlanThreads) {
         const int s = base + tid, count = min(kPfPlanThreads, a.n_seq - base);
@@ -290,11 +291,14 @@ struct PfWalk {
 template <int D>
 struct PfShared {
     static constexpr int ST = pf_stages(D);
-    uint64_t q_full, q_empty, full[ST], empty[ST], s_full[2], p_ready[2], o_done[2], done;
+    uint64_t q_full, q_empty, full[ST], empty[ST], s_full[2], p_ready[2], o_done[2], fix, done;
     uint32_t tmem;
     int aborted;
-    float tmax[ST][2];                       // largest mask entry of each warp's rows
-    alignas(16) uint16_t bias[ST][pf_keys(D)];  // mask of the tile whose values a stage holds
+    float tmax[4][2];  // the largest of each copying warp's rows
+    // mask entries of the last tiles.  Those of V's tile i are written when its stage is
+    // free: then the tile before i - 2 (i - 3 with 8 stages) has been through the softmax
+    static constexpr int NB = ST == 8 ? 4 : 3;
+    alignas(16) float bias[NB][pf_keys(D)];
 };
 template <int D>
 B200_HD constexpr int pf_stage_bytes() { return pf_keys(D) * D * 2; }
@@ -324,6 +328,9 @@ __device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t parity) {
 __device__ __forceinline__ void pf_cp16(uint32_t dst, const void* src, bool on) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void pf_cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ float pf_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -349,6 +356,11 @@ __device__ __forceinline__ uint64_t pf_fma2(uint64_t x, uint64_t y, uint64_t z) 
 __device__ __forceinline__ uint64_t pf_add2(uint64_t x, uint64_t y) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t pf_mul2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
     return r;
 }
 __device__ __forceinline__ float pf_max3(float x, float y, float z) {
@@ -388,11 +400,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
         mbar_init(&sh.q_empty, 1);
         for (int i = 0; i < ST; ++i) mbar_init(&sh.full[i], kPfCopyThreads + (MASK ? 2 : 0)), mbar_init(&sh.empty[i], 1);
         for (int j = 0; j < 2; ++j) mbar_init(&sh.s_full[j], 1), mbar_init(&sh.p_ready[j], 4), mbar_init(&sh.o_done[j], 1);
+        mbar_init(&sh.fix, 2);
         mbar_init(&sh.done, 1);
         sh.aborted = 0;
         mbar_fence_init();
     }
     griddep_wait();  // the schedule
+    griddep_launch_dependents();
     const int units = a.header->units;
     const int64_t total = a.header->total, per_cta = a.header->per_cta;
     PfWalk walk;
@@ -422,16 +436,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
             // a warp's share of a barrier where TMA copies `bytes` for it
             auto expects = [&](uint64_t* bar, uint32_t bytes, uint32_t arrivals) {
                 if (lane == 0) {
-                    if (bytes) mbar_arrive_expect_tx(bar, bytes);
-                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
-                                 "r"(arrivals - (bytes ? 1u : 0u))
-                                 : "memory");
+                    if (bytes) mbar_arrive_expect_tx(bar, bytes), --arrivals;
+                    if (arrivals)
+                        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(arrivals)
+                                     : "memory");
                 }
                 __syncwarp();
             };
             constexpr int HALVES = D / 64, MINE = HALVES / 2;  // blocks of 64 channels; of each warp
-            int stage = 0, unit = 0;
-            uint32_t lap = 0;  // parity of the ring's lap
+            int stage = 0, unit = 0, tiles = 0;
+            uint32_t lap = 0, fix = 0;  // parities of the ring's lap and of sh.fix
             bool ok = true;
             const int ps = a.kv.page_size;
             const uint64_t krow = a.kv.k_row >> 4, vrow = a.kv.v_row >> 4, kpage = a.kv.k_page >> 4, vpage = a.kv.v_page >> 4;
@@ -452,15 +466,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                                x.h, &sh.q_full);
                     }
                 } else {
+                    // (token, head) of the lane's row, one step of 2 RPI rows after the other
+                    int r = pw * RPI + lane / CH, i = (x.row0 + r) / a.group, g = x.row0 + r - i * a.group;
+                    const int c = lane % CH, di = 2 * RPI / a.group, dg = 2 * RPI - di * a.group;
 #pragma unroll 4
-                    for (int r0 = pw * RPI; r0 < rows; r0 += 2 * RPI) {
-                        const int r = r0 + lane / CH, c = lane % CH;
-                        if (r >= rows) continue;
-                        const int flat = x.row0 + r, i = flat / a.group, g = flat - i * a.group;
+                    for (; r < rows; r += 2 * RPI) {
                         const uint16_t* src = a.q + (int64_t)(x.first + i) * a.q_stride + (x.h * a.group + g) * D + c * 8;
                         const int rr = r & (kPfRows - 1);
-                        pf_cp16(q_smem + (r / kPfRows) * QTILE + (c >> 3) * QHALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), src,
-                                true);
+                        pf_cp16(q_smem + (r / kPfRows) * QTILE + (c >> 3) * QHALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), src);
+                        i += di, g += dg;
+                        if (g >= a.group) g -= a.group, ++i;
                     }
                     issued(&sh.q_full);
                 }
@@ -468,101 +483,140 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                 const uint8_t* vb = static_cast<const uint8_t*>(a.kv.v) + x.h * a.kv.v_head;
                 const int32_t* table = a.table + x.s * a.table_stride;
                 const uint16_t* mask = MASK ? a.mask + x.s * a.mask_stride : nullptr;
-                // a lane's rows of a tile: their places in 16-byte steps, or ~0 for none
-                uint32_t k_off[RPL], v_off[RPL], v_next[RPL];
-                uint16_t bias[RPL], bias_next[RPL];
-                constexpr uint16_t kNone = 0xfc00;  // -inf
-                auto find = [&](int t) {
-#pragma unroll
-                    for (int e = 0; e < RPL; ++e) {
-                        const int p = x.tile(t) * KT + pw * RPW + 32 * e + lane;
-                        bool on = p <= at1;
-                        k_off[e] = v_next[e] = ~0u;
-                        bias_next[e] = kNone;
-                        if (MASK && on) {
-                            bias_next[e] = __ldg(mask + p);
-                            on = bias_next[e] != kNone;
-                        }
-                        if (on) {
-                            const int b = (int)((unsigned)p / (unsigned)ps), page = __ldg(table + b);
-                            if ((unsigned)page < (unsigned)a.kv.n_pages) {
-                                const unsigned r = (unsigned)p - (unsigned)b * (unsigned)ps;
-                                k_off[e] = (uint32_t)((unsigned)page * kpage + r * krow);
-                                v_next[e] = (uint32_t)((unsigned)page * vpage + r * vrow);
-                            } else {
-                                record_status(B200_DEVSTATUS_BOUNDS);
-                                bias_next[e] = kNone;
-                            }
-                        }
-                    }
+                // by TMA, a box of a page to a lane: its page and row
+                struct Boxes {
+                    int page, row, rows;  // rows: of the tile, that any query sees
+                    bool on;              // this way, not the other
                 };
-                auto copy = [&](const uint8_t* base, const uint32_t (&off)[RPL]) {
-                    const uint32_t dst = ring + stage * STAGE;
-#pragma unroll
-                    for (int j = 0; j < RPW; j += RPI) {
-                        const int rl = j + lane / CH, c = lane % CH, r = pw * RPW + rl;
-                        const uint32_t o = __shfl_sync(0xffffffffu, off[j / 32], rl & 31);
-                        pf_cp16(dst + (c >> 3) * KHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4),
-                                o == ~0u ? base : base + ((uint64_t)o << 4) + c * 16, o != ~0u);
+                auto find_boxes = [&](int t) {
+                    const int p0 = x.tile(t) * KT;
+                    Boxes b;
+                    b.page = b.row = 0;
+                    b.rows = min(KT, max(0, at1 + 1 - p0));
+                    b.on = a.box > 0;
+                    if (b.on && lane * a.box < b.rows) {
+                        const unsigned at = (unsigned)p0 + (unsigned)(lane * a.box), blk = at / (unsigned)ps;
+                        b.page = __ldg(table + blk);
+                        b.row = (int)(at - blk * (unsigned)ps);
                     }
-                    issued(&sh.full[stage]);
+                    return b;
+                };
+                auto send_boxes = [&](const CUtensorMap* map, const Boxes& b, uint64_t* bar, uint32_t arrivals) {
+                    const int boxes = (b.rows + a.box - 1) / a.box;
+                    expects(bar, (uint32_t)(boxes * a.box * 128 * (HALVES == 1 ? 1 - pw : MINE)), arrivals);
+                    if (lane < boxes)
+#pragma unroll
+                        for (int hf = pw; hf < HALVES; hf += 2)
+                            pf_tma(ring + stage * STAGE + hf * KHALF + lane * a.box * 128, map, hf * 64, b.row, x.h, b.page,
+                                   bar);
+                };
+                auto advance = [&] {
                     if (MASK) {
                         __syncwarp();
                         if (lane == 0) pf_arrive(&sh.full[stage]);  // the mask entries are written
                     }
                     if (++stage == ST) stage = 0, lap ^= 1u;
                 };
-                // a tile that is seen whole goes by TMA, a box to a lane
-                const int boxes = a.box ? KT / a.box : 0;
-                int page = 0, row = 0, v_page = 0, v_row = 0;
-                bool whole = false, v_whole = false;
-                auto find_boxes = [&](int t) {
-                    const int p = x.tile(t) * KT;
-                    whole = !MASK && boxes > 0 && p + KT - 1 <= at1;
-                    if (whole && lane < boxes) {
-                        const unsigned at = (unsigned)p + (unsigned)lane * (unsigned)a.box, b = at / (unsigned)ps;
-                        page = __ldg(table + b);
-                        row = (int)(at - b * (unsigned)ps);
+                auto k_boxes = [&](const Boxes& b) {
+                    send_boxes(&a.map_k, b, &sh.full[stage], 32);  // rows that no query sees: what was there
+                    advance();
+                };
+                auto v_boxes = [&](const Boxes& b) {
+                    if (b.rows == KT) {
+                        send_boxes(&a.map_v, b, &sh.full[stage], 32);
+                    } else {
+                        // a weight of 0 meets every value: rows that no query sees become 0
+                        send_boxes(&a.map_v, b, &sh.fix, 1);
+                        if (!(ok = pf_wait(&sh.fix, fix))) return;
+                        fix ^= 1u;
+                        const int per = (KT - b.rows) * 8;  // 16-byte pieces of a block of 64 channels
+                        for (int hf = 0; hf < HALVES; ++hf)
+                            for (int e = pw * 32 + lane; e < per; e += kPfCopyThreads)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                                                 ring + stage * STAGE + hf * KHALF + b.rows * 128 + e * 16),
+                                             "r"(0)
+                                             : "memory");
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        expects(&sh.full[stage], 0, 32);
+                    }
+                    advance();
+                };
+                // by cp.async, a lane's rows of a tile: their places in 16-byte steps, or ~0 for none
+                uint32_t k_off[RPL], v_off[RPL], v_next[RPL];
+                auto find_rows = [&](int t) {
+#pragma unroll
+                    for (int e = 0; e < RPL; ++e) {
+                        const int p = x.tile(t) * KT + pw * RPW + 32 * e + lane;
+                        k_off[e] = v_next[e] = ~0u;
+                        if (p > at1) continue;
+                        const int b = (int)((unsigned)p / (unsigned)ps), page = __ldg(table + b);
+                        if ((unsigned)page < (unsigned)a.kv.n_pages) {
+                            const unsigned r = (unsigned)p - (unsigned)b * (unsigned)ps;
+                            k_off[e] = (uint32_t)((unsigned)page * kpage + r * krow);
+                            v_next[e] = (uint32_t)((unsigned)page * vpage + r * vrow);
+                        } else {
+                            record_status(B200_DEVSTATUS_BOUNDS);
+                        }
                     }
                 };
-                auto copy_boxes = [&](const CUtensorMap* map, int pg, int r) {
-                    uint64_t* bar = &sh.full[stage];
-                    expects(bar, HALVES == 1 ? (pw ? 0u : STAGE) : STAGE / 2, 32);
-                    if (lane < boxes && (HALVES > 1 || pw == 0))
+                auto copy_rows = [&](const uint8_t* base, const uint32_t (&off)[RPL]) {
+                    bool all = true;
 #pragma unroll
-                        for (int hf = HALVES == 1 ? 0 : pw; hf < HALVES; hf += 2)
-                            pf_tma(ring + stage * STAGE + hf * KHALF + lane * a.box * 128, map, hf * 64, r, x.h, pg, bar);
-                    if (++stage == ST) stage = 0, lap ^= 1u;
+                    for (int e = 0; e < RPL; ++e) all = all && off[e] != ~0u;
+                    all = __all_sync(0xffffffffu, all);
+                    const uint32_t dst = ring + stage * STAGE;
+#pragma unroll
+                    for (int j = 0; j < RPW; j += RPI) {
+                        const int rl = j + lane / CH, c = lane % CH, r = pw * RPW + rl;
+                        const uint32_t o = __shfl_sync(0xffffffffu, off[j / 32], rl & 31);
+                        const uint32_t to = dst + (c >> 3) * KHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                        if (all) pf_cp16(to, base + ((uint64_t)o << 4) + c * 16);
+                        else pf_cp16(to, o == ~0u ? base : base + ((uint64_t)o << 4) + c * 16, o != ~0u);
+                    }
+                    issued(&sh.full[stage]);
+                    advance();
                 };
-                find_boxes(0);
+                // the mask entries of a lane's rows
+                uint16_t bias[RPL], bias_next[RPL];
+                auto find_mask = [&](int t) {
+                    if (MASK)
+#pragma unroll
+                        for (int e = 0; e < RPL; ++e) {
+                            const int p = x.tile(t) * KT + pw * RPW + 32 * e + lane;
+                            bias_next[e] = p <= at1 ? __ldg(mask + p) : (uint16_t)0xfc00;  // -inf
+                        }
+                };
+                auto put_mask = [&] {
+                    float m = -INFINITY;
+                    const int at = tiles++ % PfShared<D>::NB;
+#pragma unroll
+                    for (int e = 0; e < RPL; ++e) {
+                        sh.bias[at][pw * RPW + 32 * e + lane] = h2f(bias[e]);
+                        m = fmaxf(m, h2f(bias[e]));
+                    }
+                    m = warp_max(m);
+                    if (lane == 0) sh.tmax[at][pw] = m;
+                };
+                Boxes now = find_boxes(0), before = now;
                 for (int t = 0; t <= n; ++t) {
                     if (t < n) {
-                        whole = whole && __all_sync(0xffffffffu, lane >= boxes || (unsigned)page < (unsigned)a.kv.n_pages);
-                        if (!whole) find(t);
+                        now.on = now.on && __all_sync(0xffffffffu, (unsigned)now.page < (unsigned)a.kv.n_pages);
+                        if (!now.on) find_rows(t);
+                        find_mask(t);
                         if (!(ok = pf_wait(&sh.empty[stage], lap ^ 1u))) break;
-                        if (whole) copy_boxes(&a.map_k, page, row);
-                        else copy(kb, k_off);
+                        if (now.on) k_boxes(now);
+                        else copy_rows(kb, k_off);
                     }
-                    const bool now_whole = whole;
-                    const int now_page = page, now_row = row;
-                    if (t + 1 < n) find_boxes(t + 1);
+                    const Boxes next = t + 1 < n ? find_boxes(t + 1) : now;
                     if (t > 0) {
                         if (!(ok = pf_wait(&sh.empty[stage], lap ^ 1u))) break;
-                        if (v_whole) {
-                            copy_boxes(&a.map_v, v_page, v_row);
-                        } else if (MASK) {
-                            float m = -INFINITY;
-#pragma unroll
-                            for (int e = 0; e < RPL; ++e) {
-                                sh.bias[stage][pw * RPW + 32 * e + lane] = bias[e];
-                                m = fmaxf(m, h2f(bias[e]));
-                            }
-                            m = warp_max(m);
-                            if (lane == 0) sh.tmax[stage][pw] = m;
-                        }
-                        if (!v_whole) copy(vb, v_off);
+                        if (MASK) put_mask();
+                        if (before.on) v_boxes(before);
+                        else copy_rows(vb, v_off);
+                        if (!ok) break;
                     }
-                    v_whole = now_whole, v_page = now_page, v_row = now_row;
+                    before = now, now = next;
 #pragma unroll
                     for (int e = 0; e < RPL; ++e) v_off[e] = v_next[e], bias[e] = bias_next[e];
                 }
@@ -669,7 +723,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
         const uint32_t o_addr = tmem + lanes + O_COL + (NT == 2 ? j * D : 0);
         const int row = (warp & 3) * 32 + lane;
         const float scale2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.17549435e-38f);
-        int base = 0;
+        int base = 0;  // places before the unit
         uint32_t s_par[2] = {0, 0}, o_par = 0;  // o_par: products into this tile's outputs so far
         bool ok = j < NT;
         while (ok && walk.next(a, units, total, x)) {
@@ -696,25 +750,23 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                     const int p0 = x.tile(t) * KT;
                     const int hi = at - p0, lo = a.window > 0 ? max(0, at - a.window + 1) - p0 : 0;
                     const bool edge = __any_sync(0xffffffffu, hi < KT - 1 || lo > 0);
-                    const uint4* entries = reinterpret_cast<const uint4*>(sh.bias[v_stage]);
+                    const int v_bias = (base / 2 + t) % PfShared<D>::NB;
+                    const float4* entries = reinterpret_cast<const float4*>(sh.bias[v_bias]);
                     float c0 = 0.f;
                     if (MASK) {
                         float cm;
                         if (edge) {
                             cm = -INFINITY;
-#pragma unroll 4
-                            for (int c = 0; c < KT; c += 8) {
-                                const uint4 w = entries[c / 8];
-                                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                                for (int e = 0; e < 8; e += 2) {
-                                    const float2 f = unpack16<false>(ws[e / 2]);
-                                    if (c + e >= lo && c + e <= hi) cm = fmaxf(cm, f.x);
-                                    if (c + e + 1 >= lo && c + e + 1 <= hi) cm = fmaxf(cm, f.y);
-                                }
+#pragma unroll 8
+                            for (int c = 0; c < KT; c += 4) {
+                                const float4 w = entries[c / 4];
+                                if (c >= lo && c <= hi) cm = fmaxf(cm, w.x);
+                                if (c + 1 >= lo && c + 1 <= hi) cm = fmaxf(cm, w.y);
+                                if (c + 2 >= lo && c + 2 <= hi) cm = fmaxf(cm, w.z);
+                                if (c + 3 >= lo && c + 3 <= hi) cm = fmaxf(cm, w.w);
                             }
                         } else {
-                            cm = fmaxf(sh.tmax[v_stage][0], sh.tmax[v_stage][1]);
+                            cm = fmaxf(sh.tmax[v_bias][0], sh.tmax[v_bias][1]);
                         }
                         // the mask relative to the largest entry that the row has seen:
                         // a row of lowest values keeps its scores' bits
@@ -724,22 +776,23 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         }
                         c0 = c_ref == -INFINITY ? 0.f : c_ref;
                     }
+                    const uint64_t scale22 = pf_pair(scale2, scale2), minus = pf_pair(-c0, -c0);
+                    const uint64_t log2e2 = pf_pair(1.4426950408889634f, 1.4426950408889634f);
                     // 32 scores as loaded: with a mask times scale2 and the entries added,
                     // -inf where the row does not see
                     auto ready = [&](uint32_t (&s)[32], int c) {
                         if (MASK) {
 #pragma unroll
-                            for (int k = 0; k < 32; k += 8) {
-                                const uint4 w = entries[(c + k) / 8];
-                                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                                for (int e = 0; e < 8; e += 2) {
-                                    const float2 f = unpack16<false>(ws[e / 2]);
-                                    s[k + e] = __float_as_uint(
-                                        fmaf(__uint_as_float(s[k + e]), scale2, (f.x - c0) * 1.4426950408889634f));
-                                    s[k + e + 1] = __float_as_uint(
-                                        fmaf(__uint_as_float(s[k + e + 1]), scale2, (f.y - c0) * 1.4426950408889634f));
-                                }
+                            for (int k = 0; k < 32; k += 4) {
+                                const float4 w = entries[(c + k) / 4];
+                                const uint64_t w0 = pf_mul2(pf_add2(pf_pair(w.x, w.y), minus), log2e2);
+                                const uint64_t w1 = pf_mul2(pf_add2(pf_pair(w.z, w.w), minus), log2e2);
+                                const float2 y0 = pf_unpair(pf_fma2(
+                                    pf_pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), scale22, w0));
+                                const float2 y1 = pf_unpair(pf_fma2(
+                                    pf_pair(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])), scale22, w1));
+                                s[k] = __float_as_uint(y0.x), s[k + 1] = __float_as_uint(y0.y);
+                                s[k + 2] = __float_as_uint(y1.x), s[k + 3] = __float_as_uint(y1.y);
                             }
                         }
                         if (edge) {
@@ -748,15 +801,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                                 if (c + e < lo || c + e > hi) s[e] = 0xff800000u;
                         }
                     };
-                    // the row's scores in registers, 32 at a time, the next ones on their way
+                    // the row's scores in registers: a load of tensor memory takes longer
+                    // than all that is done with 32 of them
                     uint32_t s[KT / 32][32];
                     float m[2] = {-INFINITY, -INFINITY};
-                    tc_ld_x32(s[0], s_addr);
+#pragma unroll
+                    for (int c = 0; c < KT / 32; ++c) tc_ld_x32(s[c], s_addr + 32 * c);
+                    tc_wait_ld();
 #pragma unroll
                     for (int c = 0; c < KT / 32; ++c) {
-                        tc_wait_ld();
                         tc_loaded(s[c]);
-                        if (c + 1 < KT / 32) tc_ld_x32(s[c + 1], s_addr + 32 * (c + 1));
                         ready(s[c], 32 * c);
 #pragma unroll
                         for (int e = 0; e < 32; e += 4) {
@@ -787,21 +841,21 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         }
                     }
                     const float off = (ref == -INFINITY ? 0.f : -ref) + kPfShift<BF16>;
-                    const uint64_t off2 = pf_pair(off, off), scale22 = pf_pair(scale2, scale2);
+                    const uint64_t off2 = pf_pair(off, off);
                     uint64_t sum = pf_pair(0.f, 0.f);
-                    uint32_t p[32];
 #pragma unroll
                     for (int c = 0; c < KT / 32; ++c) {
+                        uint32_t p[16];
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
                             const uint64_t y = pf_pair(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
                             const float2 z = pf_unpair(MASK ? pf_add2(y, off2) : pf_fma2(y, scale22, off2));
                             const float e0 = pf_exp2(z.x), e1 = pf_exp2(z.y);
                             sum = pf_add2(sum, pf_pair(e0, e1));
-                            p[(c & 1) * 16 + e / 2] = pack16<BF16>(e0, e1);
+                            p[e / 2] = pack16<BF16>(e0, e1);
                         }
                         // (over the scores, which are all in registers)
-                        if (c & 1) tc_st_x32(s_addr + 32 * (c >> 1), p);
+                        tc_st_x16(s_addr + 16 * c, p);
                     }
                     const float2 both = pf_unpair(sum);
                     l += both.x + both.y;
@@ -828,22 +882,26 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                 const int64_t out_row = (int64_t)(x.first + i) * a.n_head + x.h * a.group + g;
                 uint4* to = reinterpret_cast<uint4*>(a.out + out_row * D);
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    tc_ld_x32(o, o_addr + c);
+                for (int c = 0; c < D; c += 64) {
+                    uint32_t o[2][32];
+                    tc_ld_x32(o[0], o_addr + c);
+                    tc_ld_x32(o[1], o_addr + c + 32);
                     tc_wait_ld();
-                    tc_loaded(o);
-                    uint32_t w[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float y0 = __uint_as_float(o[2 * e]), y1 = __uint_as_float(o[2 * e + 1]);
-                        odd = fmaf(y0, 0.f, fmaf(y1, 0.f, odd));
-                        w[e] = l == 0.f ? 0u : pack16<BF16>(y0 * inv, y1 * inv);
+                    for (int b = 0; b < 2; ++b) {
+                        tc_loaded(o[b]);
+                        uint32_t w[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float y0 = __uint_as_float(o[b][2 * e]), y1 = __uint_as_float(o[b][2 * e + 1]);
+                            odd = fmaf(y0, 0.f, fmaf(y1, 0.f, odd));
+                            w[e] = l == 0.f ? 0u : pack16<BF16>(y0 * inv, y1 * inv);
+                        }
+                        if (real)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                to[c / 8 + 4 * b + e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
                     }
-                    if (real)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            to[c / 8 + e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
                 }
                 const bool again = real && l != 0.f && odd != 0.f;
                 const unsigned votes = __ballot_sync(0xffffffffu, again);
@@ -860,17 +918,21 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                 float4* po = a.piece_o + ((int64_t)slot * NT + j) * (D / 4) * kPfRows + row;
                 if (real) *ml = make_float4(ref, l, c_ref, 0.f);
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    tc_ld_x32(o, o_addr + c);
+                for (int c = 0; c < D; c += 64) {
+                    uint32_t o[2][32];
+                    tc_ld_x32(o[0], o_addr + c);
+                    tc_ld_x32(o[1], o_addr + c + 32);
                     tc_wait_ld();
-                    tc_loaded(o);
-                    if (real)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            po[(c / 4 + e) * kPfRows] =
-                                make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                                            __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+                    for (int b = 0; b < 2; ++b) {
+                        tc_loaded(o[b]);
+                        if (real)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                po[(c / 4 + 8 * b + e) * kPfRows] =
+                                    make_float4(__uint_as_float(o[b][4 * e]), __uint_as_float(o[b][4 * e + 1]),
+                                                __uint_as_float(o[b][4 * e + 2]), __uint_as_float(o[b][4 * e + 3]));
+                    }
                 }
             }
             tc_fence_before();
