@@ -13,9 +13,10 @@
 // The k largest: the k-th largest of the threads' largest logits is a lower bound
 // of the k-th largest of all, and of the thread with the r-th largest only its
 // k - r largest can be among them.  So a thread keeps its largest vector alone
-// in the pass; then the threads' winners are sorted (32 to a warp by
-// shuffles, merged by halves), and the owners of the first k are read again for
-// what else they hold above the k-th.  Keys are (order-preserving bits, inverted
+// in the pass.  The k-th largest of 64 groups of threads bounds from below which
+// threads can matter (a few more than k, as a rule); their winners are sorted by
+// one warp, and the owners of the first k are read again for what else they hold
+// above the k-th.  Keys are (order-preserving bits, inverted
 // id): all differ, ties go to the lower id, NaN is smallest.
 //
 // A row is read once by a cluster of up to 8 CTAs, whose lists and sums meet in
@@ -41,7 +42,7 @@ struct LogprobsArgs {
     int32_t* top_ids;
 };
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpBatch = 4;       // vectors of 16 bytes in flight per thread
 constexpr int kLpMaxCtas = 8;
@@ -158,9 +159,16 @@ struct LpType {
     }
 };
 
+constexpr int kLpGroups = 64;                     // groups of neighbouring threads
+constexpr int kLpGroup = kLpThreads / kLpGroups;  // threads in each
+static_assert(kLpGroups >= B200_LOGPROBS_MAX_K, "k of the groups bound the k-th largest");
+
 struct LpShared {
     LpSums sums[kLpWarps];
-    LpKey list[kLpWarps][32];
+    alignas(16) float group[kLpGroups];  // largest logit of a group
+    LpKey winner[kLpThreads];  // largest keys of the threads above the bound
+    LpKey first[32];           // the first of them, descending
+    int n_winners;
     LpKey found[kLpFound];
     int n_found;
     // the first CTA's: what the cluster's CTAs found
@@ -186,7 +194,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const __grid_const
     const uint4* vecs = reinterpret_cast<const uint4*>(row + (int64_t)head * T::kSize);
     const int per = (n_vec + ctas - 1) / ctas;
     const int v0 = min(n_vec, cta * per), v1 = min(n_vec, v0 + per);
-    if (tid == 0) sh.n_found = 0;
+    if (tid == 0) sh.n_found = sh.n_winners = 0;
     __syncthreads();
 
     LpSums c = {-INFINITY, 0.f, 0.f, 0.f};
@@ -216,7 +224,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const __grid_const
     for (; v + (kLpBatch - 1) * kLpThreads < v1; v += kLpBatch * kLpThreads) {
         uint4 w[kLpBatch];
 #pragma unroll
-        for (int j = 0; j < kLpBatch; ++j) w[j] = __ldg(vecs + v + j * kLpThreads);
+        for (int j = 0; j < kLpBatch; ++j) w[j] = __ldcs(vecs + v + j * kLpThreads);
         batch(w, v, true);
     }
     if (v < v1) {
@@ -253,22 +261,46 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const __grid_const
             }
             return best_key;
         };
-        LpKey key = 0;
-        if (odd) {
-            for (int u = v0 + tid; u < v1; u += kLpThreads) key = vector_best(u, ~0ull, key);
-        } else if (best_v < v1) {
-            key = vector_best(best_v, ~0ull, 0);
-        }
-        key = lp_sort(key);
-        sh.list[warp][lane] = key;
+        const bool some = v0 + tid < v1;
+        float group = some ? best : -INFINITY;
+#pragma unroll
+        for (int o = 1; o < kLpGroup; o <<= 1) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, o));
+        if (tid % kLpGroup == 0) sh.group[tid / kLpGroup] = group;
         __syncthreads();
-        // every warp merges all lists for itself: no more barriers
-        key = sh.list[0][lane];
-#pragma unroll 1
-        for (int w = 1; w < kLpWarps; ++w) {
-            const LpKey other = sh.list[w][lane];
-            if (__shfl_sync(0xffffffffu, other, 0) > __shfl_sync(0xffffffffu, key, 31)) key = lp_merge(key, other);
+        // how many groups exceed this lane's: the k-th largest (ties by any order)
+        float bound = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < kLpGroups / 32; ++h) {
+            const float mine_g = sh.group[32 * h + lane];
+            int above = 0, same = 0;
+#pragma unroll 4
+            for (int g = 0; g < kLpGroups; g += 4) {
+                const float4 w = *reinterpret_cast<const float4*>(sh.group + g);
+                above += (w.x > mine_g) + (w.y > mine_g) + (w.z > mine_g) + (w.w > mine_g);
+                same += (w.x == mine_g) + (w.y == mine_g) + (w.z == mine_g) + (w.w == mine_g);
+            }
+            const unsigned is = __ballot_sync(0xffffffffu, above < a.k && above + same >= a.k);
+            if (is) bound = __shfl_sync(0xffffffffu, mine_g, __ffs(is) - 1);
         }
+        if (odd || (some && best >= bound)) {
+            LpKey key = 0;
+            if (odd)
+                for (int u = v0 + tid; u < v1; u += kLpThreads) key = vector_best(u, ~0ull, key);
+            else
+                key = vector_best(best_v, ~0ull, 0);
+            sh.winner[atomicAdd(&sh.n_winners, 1)] = key;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            LpKey top = 0;
+            for (int f = 0; f < sh.n_winners; f += 32) {
+                const LpKey other = lp_sort(f + lane < sh.n_winners ? sh.winner[f + lane] : 0);
+                top = f ? lp_merge(top, other) : other;
+            }
+            sh.first[lane] = top;
+        }
+        __syncthreads();
+        const LpKey key = sh.first[lane];
         const LpKey least = __shfl_sync(0xffffffffu, key, a.k - 1);
         for (int i = warp; i < a.k; i += kLpWarps) {
             LpKey last = __shfl_sync(0xffffffffu, key, i);

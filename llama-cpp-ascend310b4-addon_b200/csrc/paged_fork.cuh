@@ -4,7 +4,7 @@
 // Which pages go back and which rows need a page of their own follows from who
 // holds each page before and after the call, so every entry leaves marks on its
 // page in one pass and everything else is read from the marks.
-//   mark   (a warp per row and 1024 entries): old entries set was[p], new
+//   mark   (a warp per row and 256 entries): old entries set was[p], new
 //          ones full[p], or tails[p]
 //          (the largest n_seq - s, so the lowest row) where the row's last block
 //          is not full.  Only tails needs an atomic, and a maximum does not
@@ -48,7 +48,8 @@ struct PagedForkArgs {
 };
 
 constexpr int kForkRowThreads = 256;
-constexpr int kForkCols = 1024;   // entries of a row that one warp takes, at least
+constexpr int kForkCols = 256;    // entries of a row that one warp takes, at least
+constexpr int kForkAtOnce = 4;    // entries a lane has in flight
 constexpr int kForkThreads = 1024;
 constexpr int kForkPer = 16;      // pages per thread
 constexpr int kForkPages = kForkThreads * kForkPer;
@@ -88,18 +89,25 @@ __global__ void __launch_bounds__(kForkRowThreads) paged_fork_mark_kernel(PagedF
     const int32_t* mine = a.table + s * a.table_stride;
     const int32_t* from = a.table + max(r.src, 0) * a.table_stride;
     bool bad = false;
-    for (int b = b0 + lane; b < min(b1, max(r.old_b, r.blocks)); b += 32) {
-        if (b < r.old_b) {
-            const int p = mine[b];
-            if (a.staged) a.staged[(int64_t)s * a.max_blocks + b] = p;
-            if ((unsigned)p < (unsigned)a.n_pages) a.was[p] = 1;
-            else bad = true;
+    const int end = min(b1, max(r.old_b, r.blocks));
+    for (int b = b0 + lane; b < end; b += 32 * kForkAtOnce) {
+        int p[kForkAtOnce], q[kForkAtOnce];
+#pragma unroll
+        for (int e = 0; e < kForkAtOnce; ++e) {
+            p[e] = b + 32 * e < min(end, r.old_b) ? mine[b + 32 * e] : -1;
+            q[e] = b + 32 * e < min(end, r.blocks) ? from[b + 32 * e] : -1;
         }
-        if (b < r.blocks) {
-            const int p = from[b];
-            if ((unsigned)p < (unsigned)a.n_pages) {
-                if (b + 1 == r.blocks && r.tail) atomicMax(a.tails + p, (unsigned)(a.n_seq - s));
-                else a.full[p] = 1;
+#pragma unroll
+        for (int e = 0; e < kForkAtOnce; ++e) {
+            const int at = b + 32 * e;
+            if (at < min(end, r.old_b)) {
+                if (a.staged) a.staged[(int64_t)s * a.max_blocks + at] = p[e];
+                if ((unsigned)p[e] < (unsigned)a.n_pages) a.was[p[e]] = 1;
+                else bad = true;
+            }
+            if ((unsigned)q[e] < (unsigned)a.n_pages) {
+                if (at + 1 == r.blocks && r.tail) atomicMax(a.tails + q[e], (unsigned)(a.n_seq - s));
+                else a.full[q[e]] = 1;
             }
         }
     }
@@ -226,9 +234,16 @@ __global__ void __launch_bounds__(kForkThreads) paged_fork_write_kernel(PagedFor
     const int32_t* from = old + src * old_stride;
     int32_t* to = a.out + s * a.out_stride;
     const int whole = rank >= 0 ? blocks - 1 : blocks;  // entries taken as they are
-    for (int b = b0 + lane; b < b1; b += 32)
-        if (b < whole) to[b] = from[b];
-        else if (b >= blocks) to[b] = -1;
+    for (int b = b0 + lane; b < b1; b += 32 * kForkAtOnce) {
+        int p[kForkAtOnce];
+#pragma unroll
+        for (int e = 0; e < kForkAtOnce; ++e) p[e] = b + 32 * e < min(b1, whole) ? from[b + 32 * e] : -1;
+#pragma unroll
+        for (int e = 0; e < kForkAtOnce; ++e) {
+            const int at = b + 32 * e;
+            if (at < b1 && (at < whole || at >= blocks)) to[at] = p[e];
+        }
+    }
     if (b0 != 0 || lane != 0) return;
     const bool served = rank >= 0 && rank < got;
     a.seq_lens_out[s] = rank >= 0 && !served ? len - tail : len;

@@ -14,6 +14,7 @@
 #include "../../include/b200_paged.h"
 #include "args.h"
 #include "common.cuh"
+#include "f32_pairs.cuh"
 #include "paged_store.cuh"
 #include "tcgen05.cuh"
 
@@ -335,38 +336,6 @@ __device__ __forceinline__ float pf_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-
-// Two f32 in one register pair: one instruction adds or multiplies both.
-__device__ __forceinline__ uint64_t pf_pair(float x, float y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ float2 pf_unpair(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t pf_fma2(uint64_t x, uint64_t y, uint64_t z) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-    return r;
-}
-__device__ __forceinline__ uint64_t pf_add2(uint64_t x, uint64_t y) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return r;
-}
-__device__ __forceinline__ uint64_t pf_mul2(uint64_t x, uint64_t y) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return r;
-}
-__device__ __forceinline__ float pf_max3(float x, float y, float z) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
-    return r;
 }
 
 constexpr int kPfThreads = 384;     // two softmax warpgroups; two warps of copies, tensor-core issue
@@ -776,8 +745,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         }
                         c0 = c_ref == -INFINITY ? 0.f : c_ref;
                     }
-                    const uint64_t scale22 = pf_pair(scale2, scale2), minus = pf_pair(-c0, -c0);
-                    const uint64_t log2e2 = pf_pair(1.4426950408889634f, 1.4426950408889634f);
+                    const uint64_t scale22 = f2_pair(scale2, scale2), minus = f2_pair(-c0, -c0);
+                    const uint64_t log2e2 = f2_pair(1.4426950408889634f, 1.4426950408889634f);
                     // 32 scores as loaded: with a mask times scale2 and the entries added,
                     // -inf where the row does not see
                     auto ready = [&](uint32_t (&s)[32], int c) {
@@ -785,12 +754,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
 #pragma unroll
                             for (int k = 0; k < 32; k += 4) {
                                 const float4 w = entries[(c + k) / 4];
-                                const uint64_t w0 = pf_mul2(pf_add2(pf_pair(w.x, w.y), minus), log2e2);
-                                const uint64_t w1 = pf_mul2(pf_add2(pf_pair(w.z, w.w), minus), log2e2);
-                                const float2 y0 = pf_unpair(pf_fma2(
-                                    pf_pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), scale22, w0));
-                                const float2 y1 = pf_unpair(pf_fma2(
-                                    pf_pair(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])), scale22, w1));
+                                const uint64_t w0 = f2_mul(f2_add(f2_pair(w.x, w.y), minus), log2e2);
+                                const uint64_t w1 = f2_mul(f2_add(f2_pair(w.z, w.w), minus), log2e2);
+                                const float2 y0 = f2_unpair(f2_fma(
+                                    f2_pair(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), scale22, w0));
+                                const float2 y1 = f2_unpair(f2_fma(
+                                    f2_pair(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])), scale22, w1));
                                 s[k] = __float_as_uint(y0.x), s[k + 1] = __float_as_uint(y0.y);
                                 s[k + 2] = __float_as_uint(y1.x), s[k + 3] = __float_as_uint(y1.y);
                             }
@@ -814,8 +783,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         ready(s[c], 32 * c);
 #pragma unroll
                         for (int e = 0; e < 32; e += 4) {
-                            m[0] = pf_max3(m[0], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-                            m[1] = pf_max3(m[1], __uint_as_float(s[c][e + 2]), __uint_as_float(s[c][e + 3]));
+                            m[0] = f_max3(m[0], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+                            m[1] = f_max3(m[1], __uint_as_float(s[c][e + 2]), __uint_as_float(s[c][e + 3]));
                         }
                     }
                     float top = fmaxf(m[0], m[1]);
@@ -841,23 +810,23 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         }
                     }
                     const float off = (ref == -INFINITY ? 0.f : -ref) + kPfShift<BF16>;
-                    const uint64_t off2 = pf_pair(off, off);
-                    uint64_t sum = pf_pair(0.f, 0.f);
+                    const uint64_t off2 = f2_pair(off, off);
+                    uint64_t sum = f2_pair(0.f, 0.f);
 #pragma unroll
                     for (int c = 0; c < KT / 32; ++c) {
                         uint32_t p[16];
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
-                            const uint64_t y = pf_pair(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-                            const float2 z = pf_unpair(MASK ? pf_add2(y, off2) : pf_fma2(y, scale22, off2));
+                            const uint64_t y = f2_pair(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+                            const float2 z = f2_unpair(MASK ? f2_add(y, off2) : f2_fma(y, scale22, off2));
                             const float e0 = pf_exp2(z.x), e1 = pf_exp2(z.y);
-                            sum = pf_add2(sum, pf_pair(e0, e1));
+                            sum = f2_add(sum, f2_pair(e0, e1));
                             p[e / 2] = pack16<BF16>(e0, e1);
                         }
                         // (over the scores, which are all in registers)
                         tc_st_x16(s_addr + 16 * c, p);
                     }
-                    const float2 both = pf_unpair(sum);
+                    const float2 both = f2_unpair(sum);
                     l += both.x + both.y;
                     tc_wait_st();
                 }

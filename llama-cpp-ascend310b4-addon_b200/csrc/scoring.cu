@@ -193,7 +193,9 @@ int b200_paged_prefill(const b200_paged_kv* kv, const void* q, int64_t q_stride,
     if ((reinterpret_cast<uintptr_t>(mask) & 1) ||
         (mask && n_seq > 1 && mask_stride != 0 && mask_stride < (int64_t)max_blocks * kv->page_size))
         return B200_EINVAL;
-    if (n_tokens > INT32_MAX / n_head) return B200_EUNSUPPORTED;  // rows are counted in int
+    // rows and positions are counted in int, a tile past the last
+    if (n_tokens > INT32_MAX / n_head || (int64_t)max_blocks * kv->page_size > INT32_MAX - kPfRows)
+        return B200_EUNSUPPORTED;
     if (workspace_size < b200_paged_prefill_workspace_size(kv->head_dim, n_tokens, n_seq, n_head, kv->n_head_kv))
         return B200_EINVAL;
     if (q_stride > INT64_MAX / 4 / n_tokens) return B200_EINVAL;
@@ -362,10 +364,12 @@ int b200_token_logprobs(const void* logits, int type, int64_t ld, int64_t n_rows
     a.entropy = entropy;
     a.top_ids = top_ids;
     a.top_logprobs = top_logprobs;
-    // CTAs to a row: as many as keep the GPU's 148 SMs busy with two each, while
-    // every thread still gets a batch
+    // CTAs to a row: a doubling while the grid stays within two CTAs to a place on the
+    // GPU (8 of them on each of 148 SMs) and every thread gets a vector.  More of
+    // them even out the last wave but pay the selection's 6 us each: 1024 rows of
+    // 151936 take 131 us with one, 119 with two, 128 with four
     a.ctas = 1;
-    while (a.ctas < kLpMaxCtas && 2 * a.ctas * n_rows <= 296 &&
+    while (a.ctas < kLpMaxCtas && 2 * a.ctas * n_rows <= 2 * 8 * 148 &&
            n_vocab * size / 16 / (2 * a.ctas) >= kLpThreads)
         a.ctas *= 2;
     if (n_rows * a.ctas > INT32_MAX) return B200_EUNSUPPORTED;

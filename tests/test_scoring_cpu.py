@@ -39,6 +39,8 @@ def test_prefill_refuses(over):
 
 def test_prefill_refuses_more_rows_than_it_counts():
     assert prefill(n_tokens=1 << 29, out=PTR + (1 << 45)) == B().EUNSUPPORTED
+    assert prefill(max_blocks=(1 << 27) - 1, table_stride=1 << 27) == B().EUNSUPPORTED  # the last tile passes 2^31
+    assert prefill(scale=float("nan")) == B().EINVAL
 
 
 @pytest.mark.parametrize("over", BAD_KV)
