@@ -42,7 +42,8 @@ struct PagedPrefillArgs {
     int4* desc;         // two per unit: {sequence, first flat row, first key tile, key tiles}, {first, n, len, -}
     int64_t* prefix;    // [units + 1] steps of the units before
     int2* start;        // [CTAs] {unit, KV head} that a CTA's range starts in
-    int2* cut;          // [CTAs] the one that begins in a CTA's range and goes on past it; unit -1: none
+    int4* cut;          // [CTAs] two for the unit that begins in a CTA's range and goes on past it:
+                        // {sequence, KV head, first flat row, pieces (0: no such unit)}, {first, n, len, -}
     int2* bad;          // rows to compute again: {flat (token, head), unit}
     float4* piece_ml;   // [2 * CTAs][tiles][128] {reference, sum, mask reference, -} of cut units
     float4* piece_o;    // [2 * CTAs][tiles][D / 4][128] their sums of weighted values
@@ -424,9 +425,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
             bool ok = true;
             const int ps = a.kv.page_size;
             const uint64_t krow = a.kv.k_row >> 4, vrow = a.kv.v_row >> 4, kpage = a.kv.k_page >> 4, vpage = a.kv.v_page >> 4;
-            int2 cut = make_int2(-1, 0);
+            int4 cut = make_int4(0, 0, 0, 0), cut_seq = cut;
             while (ok && walk.next(a, units, total, x)) {
-                if (x.tb == 0 && x.te < x.cost) cut = make_int2(x.u, x.h);
+                if (x.tb == 0 && x.te < x.cost) {
+                    // its last key tile's CTA; walk.w is one past that tile
+                    cut = make_int4(x.s, x.h, x.row0, (int)((walk.w - 1) / per_cta) - (int)blockIdx.x + 1);
+                    cut_seq = make_int4(x.first, x.n, x.len, 0);
+                }
                 const int n = x.te - x.tb, rows = min(NT * kPfRows, x.n * a.group - x.row0);
                 const int at1 = x.len - x.n + (x.row0 + rows - 1) / a.group;  // the last position that a row sees
                 if (unit && !(ok = pf_wait(&sh.q_empty, (unit - 1) & 1))) break;
@@ -597,7 +602,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                 }
                 ++unit;
             }
-            if (tid == 256) a.cut[blockIdx.x] = cut;
+            if (tid == 256) a.cut[2 * blockIdx.x] = cut, a.cut[2 * blockIdx.x + 1] = cut_seq;
             asm volatile("cp.async.wait_all;" ::: "memory");
             if (!ok) sh.aborted = 1;
         } else if (warp == kPfIssueWarp && lane == 0) {
@@ -943,24 +948,21 @@ __global__ void __launch_bounds__(kPfFinishThreads) paged_prefill_finish_kernel(
     __shared__ int s_odd[W][32];
     griddep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int2 cut = a.cut[blockIdx.y];
-    if (cut.x >= 0) {
-        const int u = cut.x, h = cut.y, c0 = blockIdx.y;
-        const int4 d0 = a.desc[2 * (int64_t)u], d1 = a.desc[2 * (int64_t)u + 1];
+    const int4 cut = a.cut[2 * blockIdx.y], d1 = a.cut[2 * blockIdx.y + 1];
+    const int n_bad = a.header->n_bad;
+    if (cut.w > 0) {
+        const int h = cut.y, c0 = blockIdx.y, pieces = cut.w;
         const int r0 = blockIdx.x * 32, j = r0 / kPfRows, row = (r0 & (kPfRows - 1)) + lane;
-        const int flat = d0.y + r0 + lane;
+        const int flat = cut.z + r0 + lane;
         const bool real = flat < d1.y * a.group;
-        if (d0.y + r0 < d1.y * a.group) {
-            // the CTA of the unit's last key tile
-            const int64_t last = h * a.header->total + a.prefix[u] + kPfUnitSteps + d0.w - 1;
-            const int pieces = (int)(last / a.header->per_cta) - c0 + 1;
+        if (cut.z + r0 < d1.y * a.group) {
             // piece k: the last of CTA c0's range, then the first of each one's
             auto slot = [&](int k) { return (int64_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * NT + j; };
             float cm = -INFINITY, top = -INFINITY, l = 0.f;
             float4 o[CPW];
 #pragma unroll
             for (int e = 0; e < CPW; ++e) o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-            constexpr int AT_ONCE = 4;
+            constexpr int AT_ONCE = D == 256 ? 2 : 4;
             for (int k0 = 0; k0 < pieces && real; k0 += AT_ONCE) {
                 float4 ml[AT_ONCE], y[AT_ONCE][CPW];
 #pragma unroll
@@ -1021,12 +1023,11 @@ __global__ void __launch_bounds__(kPfFinishThreads) paged_prefill_finish_kernel(
             sq.first = d1.x, sq.n = d1.y, sq.len = d1.z;
             for (int k = 0; votes; votes &= votes - 1, ++k)
                 if (k % W == warp) {
-                    const int r = d0.y + r0 + __ffs(votes) - 1, t = r / a.group;
-                    pf_row<BF16, D>(a, d0.x, sq, t, h * a.group + r - t * a.group);
+                    const int r = cut.z + r0 + __ffs(votes) - 1, t = r / a.group;
+                    pf_row<BF16, D>(a, cut.x, sq, t, h * a.group + r - t * a.group);
                 }
         }
     }
-    const int n_bad = a.header->n_bad;
     const int cta = blockIdx.y * gridDim.x + blockIdx.x, ctas = gridDim.x * gridDim.y;
     for (int64_t b = (int64_t)cta * W + warp; b < n_bad; b += (int64_t)ctas * W) {
         const int2 e = a.bad[b];

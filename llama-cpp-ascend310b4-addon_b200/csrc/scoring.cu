@@ -114,7 +114,7 @@ PrefillLayout prefill_layout(int head_dim, int64_t n_tokens, int64_t n_seq, int6
     PrefillLayout l;
     l.start = 256;
     l.cut = l.start + align256(kPfCtas * sizeof(int2));
-    l.desc = l.cut + align256(kPfCtas * sizeof(int2));
+    l.desc = l.cut + align256(2 * kPfCtas * sizeof(int4));
     l.prefix = l.desc + align256((size_t)units * 2 * sizeof(int4));
     l.bad = l.prefix + align256((size_t)(units + 1) * sizeof(int64_t));
     l.ml = l.bad + align256((size_t)(n_tokens * n_head) * sizeof(int2));
@@ -238,7 +238,7 @@ int b200_paged_prefill(const b200_paged_kv* kv, const void* q, int64_t q_stride,
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     a.header = reinterpret_cast<PfHeader*>(ws);
     a.start = reinterpret_cast<int2*>(ws + l.start);
-    a.cut = reinterpret_cast<int2*>(ws + l.cut);
+    a.cut = reinterpret_cast<int4*>(ws + l.cut);
     a.desc = reinterpret_cast<int4*>(ws + l.desc);
     a.prefix = reinterpret_cast<int64_t*>(ws + l.prefix);
     a.bad = reinterpret_cast<int2*>(ws + l.bad);
