@@ -189,9 +189,12 @@ int b200_paged_attn(const b200_paged_kv *kv, const float *q, int64_t q_stride, i
  * length: its rows come out as if its last n tokens were the new ones.
  * Scores, weights' sums and outputs are kept in 32 bits; the weights enter the
  * product with V rounded to the cache's type, as the output is.  Infinities and
- * NaN as in b200_paged_attn, where a weight counts as 0 below 2^-24 of the
- * largest for f16, 2^-120 for bf16; a position that a row does not see leaves no
- * trace in it.  n_tokens * n_head < 2^31 (B200_EUNSUPPORTED).
+ * NaN as in b200_paged_attn, a weight counting as 0 below 2^-149 of the largest:
+ * a row that meets any (in positions it does not see too) is computed again in
+ * f32, a warp to a row, which takes up to 60 times as long and leaves no trace of
+ * what it does not see.  n_tokens * n_head and max_blocks * page_size stay 128
+ * below 2^31 (B200_EUNSUPPORTED); a scale that is NaN is refused (B200_EINVAL).
+ * Fast for pages that four rows divide, best from 16 rows on.
  * workspace: 16-byte aligned, no initial contents needed, not shared by calls
  * that overlap on the GPU. */
 size_t b200_paged_prefill_workspace_size(int head_dim, int64_t n_tokens, int n_seq, int n_head, int n_head_kv);

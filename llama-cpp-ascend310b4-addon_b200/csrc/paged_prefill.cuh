@@ -53,6 +53,7 @@ struct PfHeader {
     int64_t total;    // steps of all units of one KV head
     int64_t per_cta;  // of all KV heads' units, to a CTA
     int units, n_bad;
+    int whole;  // CTA c has unit c and nothing else
 };
 
 constexpr int kPfCtas = 148;   // one per SM
@@ -61,6 +62,10 @@ constexpr int kPfRows = 128;   // rows of a tile: the lanes of tensor memory
 // scores and the outputs, which nothing overlaps.  (8192 tokens: 1174 us with 2,
 // 1099 with 4, 1128 with 6; 33 ragged sequences 93, 98, 97.)
 constexpr int kPfUnitSteps = 4;
+// A unit stays whole on a CTA of its own where all find one and the largest has at most
+// this many steps more than an equal range: a second unit's start and the pieces'
+// join would cost as much.  (512 tokens, 64/8 heads x 128: 33.7 us cut, 29.0 whole.)
+constexpr int kPfWholeSteps = 6;
 // Key tiles and row tiles of a unit by head dim: two row tiles take turns between
 // the tensor core and the exponentials; at head dim 256 the outputs of one fill
 // half of tensor memory, and two score buffers of 64 keys take its place.
@@ -183,6 +188,7 @@ __global__ void __launch_bounds__(kPfPlanThreads) paged_prefill_plan_kernel(cons
     const int tid = threadIdx.x;
     griddep_launch_dependents();
     int64_t units = 0, tiles = 0, sum;
+    int largest = 0;
     for (int base = 0; base < a.n_seq; base += kPfPlanThreads) {
         const int s = base + tid, count = min(kPfPlanThreads, a.n_seq - base);
         PfSeq q = {0, 0, 0};
@@ -222,20 +228,25 @@ __global__ void __launch_bounds__(kPfPlanThreads) paged_prefill_plan_kernel(cons
                 if (units + u < kPfPlanThreads) s_prefix[units + u] = before;
             }
             tiles += more;
+            largest = max(largest, (int)min(steps, (int64_t)INT32_MAX));
         }
         units += sum;
         __syncthreads();  // s_base and s_seq are read no more
     }
     const int64_t all = tiles * a.kv.n_head_kv, per = max((int64_t)1, (all + kPfCtas - 1) / kPfCtas);
+    const bool whole = __syncthreads_or(largest > per + kPfWholeSteps) == 0 && units * a.kv.n_head_kv <= kPfCtas;
     if (tid == 0) {
         a.prefix[units] = tiles;
+        a.header->whole = whole;
         a.header->total = tiles;
         a.header->per_cta = per;
         a.header->units = (int)units;
         a.header->n_bad = 0;
     }
     // where every CTA starts (the loops above end with a barrier behind the last prefix)
-    if (tid < kPfCtas && tid * per < all) {
+    if (whole) {
+        if (tid < units * a.kv.n_head_kv) a.start[tid] = make_int2((int)(tid % units), (int)(tid / units));
+    } else if (tid < kPfCtas && tid * per < all) {
         const int64_t h = tid * per / tiles, x = tid * per - h * tiles;
         const int64_t* prefix = units <= kPfPlanThreads ? s_prefix : a.prefix;
         int lo = 0, hi = (int)units;  // prefix[lo] <= x < prefix[hi]
@@ -389,6 +400,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
     walk.w = min(total * a.kv.n_head_kv, per_cta * blockIdx.x);
     walk.w1 = min(total * a.kv.n_head_kv, walk.w + per_cta);
     const int2 start = a.start[blockIdx.x];  // (not used by a CTA without work)
+    if (a.header->whole) {
+        walk.w = walk.w1 = 0;
+        if ((int64_t)blockIdx.x < (int64_t)units * a.kv.n_head_kv) {
+            walk.w = start.y * total + a.prefix[start.x];
+            walk.w1 = start.y * total + a.prefix[start.x + 1];
+        }
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

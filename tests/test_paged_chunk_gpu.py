@@ -75,6 +75,7 @@ SHAPES = [
     ([17], [129], 16, 32, 2, 128), ([4000], [1], 16, 64, 8, 128), ([0], [1030], 128, 8, 1, 128),
     ([10, 20, 30, 40, 50], [3, 0, 2, 0, 1], 7, 20, 4, 128), ([9000], [17], 16, 12, 2, 128), ([600], [300], 8, 130, 1, 64),
     ([40], [3], 16, 300, 1, 128), ([200], [257], 16, 1, 1, 256),
+    ([0], [512], 16, 64, 8, 128), ([0, 100, 30], [400, 0, 250], 16, 32, 8, 64), ([64], [300], 16, 16, 4, 256),
 ]
 
 
