@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
             int stage = 0, unit = 0, tiles = 0;
             uint32_t lap = 0, fix = 0;  // parities of the ring's lap and of sh.fix
             bool ok = true;
-            const int ps = a.kv.page_size;
+            const int ps = a.kv.page_size, box_log = __ffs(a.box) - 1;
             const uint64_t krow = a.kv.k_row >> 4, vrow = a.kv.v_row >> 4, kpage = a.kv.k_page >> 4, vpage = a.kv.v_page >> 4;
             int4 cut = make_int4(0, 0, 0, 0), cut_seq = cut;
             while (ok && walk.next(a, units, total, x)) {
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                     return b;
                 };
                 auto send_boxes = [&](const CUtensorMap* map, const Boxes& b, uint64_t* bar, uint32_t arrivals) {
-                    const int boxes = (b.rows + a.box - 1) / a.box;
+                    const int boxes = (b.rows + a.box - 1) >> box_log;
                     expects(bar, (uint32_t)(boxes * a.box * 128 * (HALVES == 1 ? 1 - pw : MINE)), arrivals);
                     if (lane < boxes)
 #pragma unroll
@@ -596,7 +596,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                     m = warp_max(m);
                     if (lane == 0) sh.tmax[at][pw] = m;
                 };
-                Boxes now = find_boxes(0), before = now;
+                // (pages are looked up two tiles ahead: a look-up takes as long as a tile)
+                Boxes now = find_boxes(0), next = n > 1 ? find_boxes(1) : now, before = now;
                 for (int t = 0; t <= n; ++t) {
                     if (t < n) {
                         now.on = now.on && __all_sync(0xffffffffu, (unsigned)now.page < (unsigned)a.kv.n_pages);
@@ -606,7 +607,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         if (now.on) k_boxes(now);
                         else copy_rows(kb, k_off);
                     }
-                    const Boxes next = t + 1 < n ? find_boxes(t + 1) : now;
+                    const Boxes later = t + 2 < n ? find_boxes(t + 2) : next;
                     if (t > 0) {
                         if (!(ok = pf_wait(&sh.empty[stage], lap ^ 1u))) break;
                         if (MASK) put_mask();
@@ -614,7 +615,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         else copy_rows(vb, v_off);
                         if (!ok) break;
                     }
-                    before = now, now = next;
+                    before = now, now = next, next = later;
 #pragma unroll
                     for (int e = 0; e < RPL; ++e) v_off[e] = v_next[e], bias[e] = bias_next[e];
                 }
