@@ -38,6 +38,7 @@ struct PagedPrefillArgs {
     int n_tokens, n_head, group, n_seq, max_blocks, window;
     float scale;
     // workspace
+    int64_t max_units;  // there is room for, and for n_tokens * n_head rows in bad
     struct PfHeader* header;
     int4* desc;         // two per unit: {sequence, first flat row, first key tile, key tiles}, {first, n, len, -}
     int64_t* prefix;    // [units + 1] steps of the units before
@@ -198,6 +199,10 @@ __global__ void __launch_bounds__(kPfPlanThreads) paged_prefill_plan_kernel(cons
         s_seq[tid] = q;
         if (tid == 0) s_base[count] = sum;
         __syncthreads();
+        if (units + sum > a.max_units) {  // starts that go back name rows more than once: what passes the room is left out
+            if (tid == 0) record_status(B200_DEVSTATUS_BOUNDS);
+            sum = a.max_units - units;
+        }
         for (int64_t u0 = 0; u0 < sum; u0 += kPfPlanThreads) {
             const int64_t u = u0 + tid;
             int64_t steps = 0;
@@ -914,7 +919,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                     int at_list = 0;
                     if (lane == 0) at_list = atomicAdd(&a.header->n_bad, __popc(votes));
                     at_list = __shfl_sync(0xffffffffu, at_list, 0) + __popc(votes & ((1u << lane) - 1u));
-                    if (again) a.bad[at_list] = make_int2((int)out_row, x.u);
+                    if (again && at_list < a.n_tokens * a.n_head) a.bad[at_list] = make_int2((int)out_row, x.u);
                 }
             } else {
                 // at most one unit goes on from the CTA before, and one goes on in the next
@@ -968,7 +973,7 @@ __global__ void __launch_bounds__(kPfFinishThreads) paged_prefill_finish_kernel(
     griddep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int4 cut = a.cut[2 * blockIdx.y], d1 = a.cut[2 * blockIdx.y + 1];
-    const int n_bad = a.header->n_bad;
+    const int n_bad = min(a.header->n_bad, a.n_tokens * a.n_head);
     if (cut.w > 0) {
         const int h = cut.y, c0 = blockIdx.y, pieces = cut.w;
         const int r0 = blockIdx.x * 32, j = r0 / kPfRows, row = (r0 & (kPfRows - 1)) + lane;

@@ -105,18 +105,19 @@ bool encode_view(CUtensorMap* m, const void* base, const int64_t (&dims)[4], con
 }
 
 struct PrefillLayout {
+    int64_t units;  // at most
     size_t start, cut, desc, prefix, bad, ml, o, total;
 };
 
 PrefillLayout prefill_layout(int head_dim, int64_t n_tokens, int64_t n_seq, int64_t n_head, int64_t n_head_kv) {
     const int64_t rows = pf_tiles(head_dim) * kPfRows;
-    const int64_t units = n_tokens * (n_head / n_head_kv) / rows + n_seq;
     PrefillLayout l;
+    l.units = n_tokens * (n_head / n_head_kv) / rows + n_seq;
     l.start = 256;
     l.cut = l.start + align256(kPfCtas * sizeof(int2));
     l.desc = l.cut + align256(2 * kPfCtas * sizeof(int4));
-    l.prefix = l.desc + align256((size_t)units * 2 * sizeof(int4));
-    l.bad = l.prefix + align256((size_t)(units + 1) * sizeof(int64_t));
+    l.prefix = l.desc + align256((size_t)l.units * 2 * sizeof(int4));
+    l.bad = l.prefix + align256((size_t)(l.units + 1) * sizeof(int64_t));
     l.ml = l.bad + align256((size_t)(n_tokens * n_head) * sizeof(int2));
     l.o = l.ml + (size_t)2 * kPfCtas * rows * sizeof(float4);
     l.total = l.o + (size_t)2 * kPfCtas * rows * head_dim * sizeof(float);
@@ -236,6 +237,7 @@ int b200_paged_prefill(const b200_paged_kv* kv, const void* q, int64_t q_stride,
     a.scale = scale;
     const PrefillLayout l = prefill_layout(kv->head_dim, n_tokens, n_seq, n_head, kv->n_head_kv);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
+    a.max_units = l.units;
     a.header = reinterpret_cast<PfHeader*>(ws);
     a.start = reinterpret_cast<int2*>(ws + l.start);
     a.cut = reinterpret_cast<int4*>(ws + l.cut);

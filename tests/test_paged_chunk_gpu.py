@@ -220,6 +220,21 @@ def test_lengths_that_the_plan_did_not_serve_and_bad_rows():
     assert B().device_status(reset=True) == BOUNDS
 
 
+def test_starts_that_go_back_and_forth_stay_in_the_workspace():
+    """Every other sequence names all rows: far more units than there is room for."""
+    bw, n = B(), 400
+    _, c, cu, q = make([0], [64], 16, 64, 8, 128, "f16", pad=0)
+    dk, dv = R.to_device(c, "f16")
+    dv[c["table"][0, 0], 3, :, 5] = float("inf")  # and every row is computed again
+    size = bw.paged_prefill_workspace_size(128, 64, n, 64, 8)
+    ws = torch.full((size + 4096,), 0x3C, dtype=torch.uint8, device="cuda")
+    starts = i32([0 if i % 2 == 0 else 64 for i in range(n + 1)])
+    out = bw.paged_prefill(bw.PagedKV(dk, dv), q, i32(c["table"]).expand(n, -1), i32([64] * n), starts, 0.1,
+                           workspace=ws[:size])
+    assert bw.device_status(reset=True) == BOUNDS
+    assert (ws[size:] == 0x3C).all() and torch.isfinite(out[:, :, :5].float()).all()
+
+
 def test_bad_pages_are_recorded_and_passed_over():
     _, c, cu, q = make([64], [16], 16, 8, 2, 128, "f16")
     good = run(c, q, cu, "f16", 0.1)
