@@ -194,7 +194,7 @@ int b200_paged_attn(const b200_paged_kv *kv, const float *q, int64_t q_stride, i
  * f32, a warp to a row, which takes up to 60 times as long and leaves no trace of
  * what it does not see.  n_tokens * n_head and max_blocks * page_size stay 128
  * below 2^31 (B200_EUNSUPPORTED); a scale that is NaN is refused (B200_EINVAL).
- * Fast for pages that four rows divide, best from 16 rows on.
+ * Fastest for pages of a multiple of 8 rows.
  * workspace: 16-byte aligned, no initial contents needed, not shared by calls
  * that overlap on the GPU. */
 size_t b200_paged_prefill_workspace_size(int head_dim, int64_t n_tokens, int n_seq, int n_head, int n_head_kv);

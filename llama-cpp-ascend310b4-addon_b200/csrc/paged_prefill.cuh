@@ -24,7 +24,7 @@ struct PagedPrefillArgs {
     // [page][head][row][channel] views of K and V for boxes of box rows of a page by
     // 64 channels, and [KV head][token][head][channel] of q for boxes of 128 rows
     CUtensorMap map_k, map_v, map_q;
-    int box;    // 0: a page has no four rows in a row that start at a multiple of four
+    int box;    // 0: a page has no eight rows in a row that start at a multiple of eight
     int q_box;  // tokens of 128 rows; 0: the heads of a KV head do not divide 128
     b200_paged_kv kv;
     const uint16_t* q;
@@ -60,9 +60,9 @@ struct PfHeader {
 constexpr int kPfCtas = 148;   // one per SM
 constexpr int kPfRows = 128;   // rows of a tile: the lanes of tensor memory
 // A unit counts as many steps as it has key tiles and these: its queries, the first
-// scores and the outputs, which nothing overlaps.  (8192 tokens: 1174 us with 2,
-// 1099 with 4, 1128 with 6; 33 ragged sequences 93, 98, 97.)
-constexpr int kPfUnitSteps = 4;
+// scores and the outputs, which nothing overlaps.  (8192 tokens: 1105 us with 2,
+// 1077 with 3, 1094 with 4; 33 ragged sequences 76, 76, 79.)
+constexpr int kPfUnitSteps = 3;
 // A unit stays whole on a CTA of its own where all find one and the largest has at most
 // this many steps more than an equal range: a second unit's start and the pieces'
 // join would cost as much.  (512 tokens, 64/8 heads x 128: 33.7 us cut, 29.0 whole.)
@@ -345,9 +345,26 @@ __device__ __forceinline__ uint32_t pf_bits(int lo, int hi) {
     const int l = max(lo, 0), h = min(hi, 31);
     return h < l ? 0u : (0xffffffffu >> (31 - h + l)) << l;
 }
+// Waits of this kernel: the clock and the limit are read once in 4096 tries that found
+// nothing, by as few instructions as can be: there are twenty such places, and what
+// they take of the instruction cache costs the others (8192 tokens 1231 -> 1115 us).
+__device__ __forceinline__ bool pf_wait_one(uint64_t* bar, uint32_t parity) {
+    unsigned long long began = 0;
+#pragma unroll 1
+    for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i)
+        if ((i & 4095u) == 0) {
+            const unsigned long long now = globaltimer();
+            if (began == 0) began = now;
+            if (now - began > g_wait_timeout_ns) {
+                record_status(B200_DEVSTATUS_TIMEOUT);
+                return false;
+            }
+        }
+    return true;
+}
 // A warp's wait: the same answer for every lane.
 __device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
+    return __all_sync(0xffffffffu, pf_wait_one(bar, parity));
 }
 __device__ __forceinline__ void pf_cp16(uint32_t dst, const void* src, bool on) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
@@ -420,7 +437,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
     PfUnit x;
 
     if (role == 2) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         if (tid < 256 + kPfCopyThreads) {
             // ---- copies: keys and values by pages into 128-byte swizzled rows.  The
             // barrier of a tile counts its copies' ends; the thread that issues the
@@ -520,20 +537,18 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                     }
                     if (++stage == ST) stage = 0, lap ^= 1u;
                 };
-                auto k_boxes = [&](const Boxes& b) {
-                    send_boxes(&a.map_k, b, &sh.full[stage], 32);  // rows that no query sees: what was there
-                    advance();
-                };
-                auto v_boxes = [&](const Boxes& b) {
-                    if (b.rows == KT) {
-                        send_boxes(&a.map_v, b, &sh.full[stage], 32);
-                    } else {
+                auto copy_boxes = [&](const Boxes& b, bool value) {
+                    const bool part = value && b.rows < KT;
+                    // (rows of K that no query sees: what was there)
+                    send_boxes(value ? &a.map_v : &a.map_k, b, part ? &sh.fix : &sh.full[stage], part ? 1 : 32);
+                    if (part) {
                         // a weight of 0 meets every value: rows that no query sees become 0
-                        send_boxes(&a.map_v, b, &sh.fix, 1);
                         if (!(ok = pf_wait(&sh.fix, fix))) return;
                         fix ^= 1u;
                         const int per = (KT - b.rows) * 8;  // 16-byte pieces of a block of 64 channels
+#pragma unroll 1
                         for (int hf = 0; hf < HALVES; ++hf)
+#pragma unroll 1
                             for (int e = pw * 32 + lane; e < per; e += kPfCopyThreads)
                                 asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
                                                  ring + stage * STAGE + hf * KHALF + b.rows * 128 + e * 16),
@@ -543,7 +558,6 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         __syncwarp();
                         expects(&sh.full[stage], 0, 32);
                     }
-                    advance();
                 };
                 // by cp.async, a lane's rows of a tile: their places in 16-byte steps, or ~0 for none
                 uint32_t k_off[RPL], v_off[RPL], v_next[RPL];
@@ -564,21 +578,17 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                     }
                 };
                 auto copy_rows = [&](const uint8_t* base, const uint32_t (&off)[RPL]) {
-                    bool all = true;
-#pragma unroll
-                    for (int e = 0; e < RPL; ++e) all = all && off[e] != ~0u;
-                    all = __all_sync(0xffffffffu, all);
                     const uint32_t dst = ring + stage * STAGE;
 #pragma unroll
-                    for (int j = 0; j < RPW; j += RPI) {
-                        const int rl = j + lane / CH, c = lane % CH, r = pw * RPW + rl;
-                        const uint32_t o = __shfl_sync(0xffffffffu, off[j / 32], rl & 31);
-                        const uint32_t to = dst + (c >> 3) * KHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                        if (all) pf_cp16(to, base + ((uint64_t)o << 4) + c * 16);
-                        else pf_cp16(to, o == ~0u ? base : base + ((uint64_t)o << 4) + c * 16, o != ~0u);
-                    }
+                    for (int e = 0; e < RPL; ++e)
+#pragma unroll (D == 256 ? 8 : 16)
+                        for (int j = 0; j < 32; j += RPI) {
+                            const int rl = j + lane / CH, c = lane % CH, r = pw * RPW + 32 * e + rl;
+                            const uint32_t o = __shfl_sync(0xffffffffu, off[e], rl);
+                            pf_cp16(dst + (c >> 3) * KHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                                    o == ~0u ? base : base + ((uint64_t)o << 4) + c * 16, o != ~0u);
+                        }
                     issued(&sh.full[stage]);
-                    advance();
                 };
                 // the mask entries of a lane's rows
                 uint16_t bias[RPL], bias_next[RPL];
@@ -603,22 +613,27 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                 };
                 // (pages are looked up two tiles ahead: a look-up takes as long as a tile)
                 Boxes now = find_boxes(0), next = n > 1 ? find_boxes(1) : now, before = now;
-                for (int t = 0; t <= n; ++t) {
+#pragma unroll 1
+                for (int t = 0; t <= n && ok; ++t) {
                     if (t < n) {
                         now.on = now.on && __all_sync(0xffffffffu, (unsigned)now.page < (unsigned)a.kv.n_pages);
                         if (!now.on) find_rows(t);
                         find_mask(t);
+                    }
+                    if (t < n) {
                         if (!(ok = pf_wait(&sh.empty[stage], lap ^ 1u))) break;
-                        if (now.on) k_boxes(now);
+                        if (now.on) copy_boxes(now, false);
                         else copy_rows(kb, k_off);
+                        advance();
                     }
                     const Boxes later = t + 2 < n ? find_boxes(t + 2) : next;
                     if (t > 0) {
                         if (!(ok = pf_wait(&sh.empty[stage], lap ^ 1u))) break;
                         if (MASK) put_mask();
-                        if (before.on) v_boxes(before);
+                        if (before.on) copy_boxes(before, true);
                         else copy_rows(vb, v_off);
                         if (!ok) break;
+                        advance();
                     }
                     before = now, now = next, next = later;
 #pragma unroll
@@ -639,7 +654,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
             uint32_t ready[2] = {0, 0};        // parities of p_ready
             bool ok = true;
             auto landed = [&](uint64_t* bar, uint32_t parity) {
-                const bool there = mbar_wait_bounded(bar, parity);
+                const bool there = pf_wait_one(bar, parity);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 return there;
             };
@@ -690,7 +705,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                     }
                     if (!(ok = landed(&sh.full[stage_of(v_at)], parity_of(v_at)))) break;
                     if (NT == 1) {
-                        if (!(ok = mbar_wait_bounded(&sh.p_ready[t & 1], ready[t & 1]))) break;
+                        if (!(ok = pf_wait_one(&sh.p_ready[t & 1], ready[t & 1]))) break;
                         ready[t & 1] ^= 1u;
                         tc_fence_after();
                         values(tmem + O_COL, tmem + (t & 1) * S_STEP, stage_of(v_at), t > 0);
@@ -699,7 +714,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             if (j == 1 && !two) break;
-                            if (!(ok = mbar_wait_bounded(&sh.p_ready[j], ready[j]))) break;
+                            if (!(ok = pf_wait_one(&sh.p_ready[j], ready[j]))) break;
                             ready[j] ^= 1u;
                             tc_fence_after();
                             values(tmem + O_COL + j * D, tmem + j * S_STEP, stage_of(v_at), t > 0);
@@ -723,7 +738,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
         __syncwarp();
     } else {
         // ---- softmax: a row to a thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int j = role;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t o_addr = tmem + lanes + O_COL + (NT == 2 ? j * D : 0);

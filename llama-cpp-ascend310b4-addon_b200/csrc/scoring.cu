@@ -204,14 +204,13 @@ int b200_paged_prefill(const b200_paged_kv* kv, const void* q, int64_t q_stride,
     PagedPrefillArgs a = {};
     a.kv = *kv;
     // Rows of a page to a box: the largest power of two that divides the page, a tile
-    // of keys at most; four at least, so that a warp has a lane for each box.  (The
-    // swizzle goes by the address in shared memory: a box may start at any row.)
-    // 8192 tokens, 64/8 heads x 128: pages of 64 1150 us, of 8 1256, of 100 (boxes of
-    // four) 1620, by rows 2200; pages of 5 go by rows, 2220.
+    // of keys at most, eight (a group of the swizzle) at least; other pages go row by
+    // row.  8192 tokens, 64/8 heads x 128: pages of 64 1090 us, of 24 1095, of 5 by
+    // rows 1476, of 100 in boxes of four rows 1594.
     a.box = std::min(kv->page_size & -kv->page_size, pf_keys(kv->head_dim));
     const int64_t d = kv->head_dim, group = n_head / kv->n_head_kv;
     const int64_t page_dims[4] = {d, kv->page_size, kv->n_head_kv, kv->n_pages};
-    if (a.box < 4 || !encode_view(&a.map_k, kv->k, page_dims, {kv->k_row, kv->k_head, kv->k_page}, a.box, 1) ||
+    if (a.box < 8 || !encode_view(&a.map_k, kv->k, page_dims, {kv->k_row, kv->k_head, kv->k_page}, a.box, 1) ||
         !encode_view(&a.map_v, kv->v, page_dims, {kv->v_row, kv->v_head, kv->v_page}, a.box, 1))
         a.box = 0;
     a.q_box = kPfRows % group == 0 ? (int)(kPfRows / group) : 0;
