@@ -602,9 +602,11 @@ def token_logprobs(logits, tokens=None, k: int = 0) -> TokenLogprobs:
     int32 and top_logprobs f32 [n_rows, k] in descending order, ties by the
     lower id (None for k = 0; k at most LOGPROBS_MAX_K and n_vocab)."""
     torch = _torch()
-    types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
-    if logits.dtype not in types:
-        raise B200Unsupported(EUNSUPPORTED, f"token_logprobs of {logits.dtype}")
+    dtype, f32 = logits.dtype, torch.float32
+    kind = (TYPE_F32 if dtype is f32 else TYPE_F16 if dtype is torch.float16
+            else TYPE_BF16 if dtype is torch.bfloat16 else None)
+    if kind is None:
+        raise B200Unsupported(EUNSUPPORTED, f"token_logprobs of {dtype}")
     dev, shape = logits.device, logits.shape
     if dev.type != "cuda" or len(shape) != 2 or shape[1] == 0 or (logits.stride(1) != 1 and shape[1] > 1):
         _bad("token_logprobs", "logits must be [n_rows, n_vocab] with contiguous rows on a CUDA device")
@@ -615,15 +617,15 @@ def token_logprobs(logits, tokens=None, k: int = 0) -> TokenLogprobs:
         logits = logits.contiguous()  # rows that overlap, as an expanded one
     i32 = torch.int32
     logprob = top_ids = top_logprobs = None
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    entropy = torch.empty(rows, dtype=f32, device=dev)
     if tokens is not None:
         if tokens.dtype != i32 or tokens.device != dev or tokens.shape != shape[:1] or not tokens.is_contiguous():
             _bad("token_logprobs", "tokens must be a contiguous int32 [n_rows] on the logits' device")
-        logprob = torch.empty_like(entropy)
+        logprob = torch.empty(rows, dtype=f32, device=dev)
     if k:
         top_ids = torch.empty((rows, k), dtype=i32, device=dev)
-        top_logprobs = torch.empty((rows, k), dtype=torch.float32, device=dev)
-    _launch("token_logprobs", dev, lib().b200_token_logprobs, logits.data_ptr(), types[logits.dtype], logits.stride(0),
+        top_logprobs = torch.empty((rows, k), dtype=f32, device=dev)
+    _launch("token_logprobs", dev, lib().b200_token_logprobs, logits.data_ptr(), kind, logits.stride(0),
             rows, vocab, None if tokens is None else tokens.data_ptr(), k,
             *(None if t is None else t.data_ptr() for t in (logprob, entropy, top_ids, top_logprobs)))
     return TokenLogprobs(logprob, entropy, top_ids, top_logprobs)
@@ -1027,13 +1029,18 @@ def paged_fork(src, keep, seq_lens, block_table, free_pages, n_free, page_size: 
     table_out = block_table if table_out is None else table_out
     seq_lens_out = seq_lens if seq_lens_out is None else seq_lens_out
     n_free_out = n_free if n_free_out is None else n_free_out
-    for t in (block_table, table_out):
-        if (t.dtype != i32 or t.device != dev or len(t.shape) != 2 or t.shape != table or t.shape[0] != n
-                or t.shape[1] == 0 or t.stride(1) != 1):
-            _bad("paged_fork", "block_table and table_out must be int32 [n_seq, max_blocks] with contiguous rows")
-    for t in (src, keep, seq_lens, seq_lens_out, free_pages, n_free, n_free_out):
-        if t.dtype != i32 or t.device != dev or not t.is_contiguous() or t.dim() != 1:
-            _bad("paged_fork", "src, keep, seq_lens, free_pages and n_free must be contiguous int32 vectors on one device")
+    if (block_table.dtype != i32 or block_table.device != dev or len(table) != 2 or table[0] != n or table[1] == 0
+            or block_table.stride(1) != 1):
+        _bad("paged_fork", "block_table must be int32 [n_seq, max_blocks] with contiguous rows")
+    if table_out is not block_table and (table_out.dtype != i32 or table_out.device != dev or table_out.shape != table
+                                         or table_out.stride(1) != 1):
+        _bad("paged_fork", "table_out must be int32 [n_seq, max_blocks] with contiguous rows, as block_table")
+    if (src.dtype != i32 or keep.dtype != i32 or seq_lens.dtype != i32 or seq_lens_out.dtype != i32
+            or free_pages.dtype != i32 or n_free.dtype != i32 or n_free_out.dtype != i32 or src.device != dev
+            or keep.device != dev or seq_lens_out.device != dev or free_pages.device != dev or n_free.device != dev
+            or n_free_out.device != dev or free_pages.dim() != 1 or not src.is_contiguous() or not keep.is_contiguous()
+            or not seq_lens.is_contiguous() or not seq_lens_out.is_contiguous() or not free_pages.is_contiguous()):
+        _bad("paged_fork", "src, keep, seq_lens, free_pages and n_free must be contiguous int32 vectors on one device")
     if seq_lens_out.shape != shape or n_free.numel() != 1 or n_free_out.numel() != 1 or free_pages.numel() == 0:
         _bad("paged_fork", "seq_lens_out must be [n_seq], n_free and n_free_out [1], free_pages [n_pages]")
     if workspace is None:

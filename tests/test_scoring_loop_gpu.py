@@ -3,6 +3,10 @@ store, chunk attention, log probabilities, fork and copy, drafts that are taken
 back, and requests that end.  Each attention output is checked against 64 bits over
 the cache as it is, and after every step the cache against what the tokens of each
 beam stored, bit for bit."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -119,3 +123,80 @@ def test_beam_search(dtype, ps, hq, hkv, d):
     branch([-1] * n, [0] * n)
     check()
     assert int(n_free) == n_pages and B().device_status(reset=True) == 0
+
+
+def calls(seed):
+    """One call of every operator on seeded inputs, as a function, and the tensors that it leaves."""
+    bw = B()
+    r = np.random.default_rng(seed)
+    c = R.make_cache(r, [300, 77, 0], 16, 2, 128, "f16")
+    dk, dv = R.to_device(c, "f16")
+    cache = bw.PagedKV(dk, dv)
+    i32 = lambda v: torch.from_numpy(np.asarray(v, np.int32)).cuda()  # noqa: E731
+    q = torch.from_numpy(r.standard_normal((210, 8, 128)).astype(np.float32)).cuda().half()
+    table, lens, cu = i32(c["table"]), i32(c["lens"]), i32([0, 200, 205, 210])
+    logits = torch.from_numpy(r.standard_normal((40, 5000)).astype(np.float32)).cuda()
+    free, n_free = i32(r.permutation(60)), i32([40])
+    out = torch.zeros_like(q)
+    ws = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in
+          (bw.paged_prefill_workspace_size(128, 210, 3, 8, 2), bw.paged_fork_workspace_size(3, table.shape[1], 60))]
+    new = torch.zeros_like(table)
+    src, keep, tokens = i32([0, 0, 1]), i32([290, 33, 70]), i32(r.integers(0, 5000, 40))
+    left = torch.empty_like(lens), torch.empty_like(n_free)
+
+    def run():
+        bw.paged_prefill(cache, q, table, lens, cu, 0.1, out=out, workspace=ws[0])
+        f = bw.paged_fork(src, keep, lens, table, free, n_free, 16, table_out=new, seq_lens_out=left[0],
+                          n_free_out=left[1], workspace=ws[1])
+        p = bw.token_logprobs(logits, tokens, 7)
+        return [out, new, left[0], left[1], f.copy_src, f.copy_dst, f.copy_rows, p.logprob, p.entropy, p.top_ids,
+                p.top_logprobs]
+
+    return run
+
+
+def test_two_streams_at_once():
+    """Two programs' calls beside one another, each with workspaces of its own."""
+    runs = [calls(1), calls(2)]
+    alone = []
+    for run in runs:
+        alone.append([x.clone() for x in run()])
+    streams = [torch.cuda.Stream() for _ in runs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for stream, run in zip(streams, runs):
+            with torch.cuda.stream(stream):
+                for _ in range(3):
+                    last = run()
+                got.append(last)
+        torch.cuda.synchronize()
+        for a, b in zip(alone, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert B().device_status(reset=True) == 0
+
+
+FIRST = """
+import sys
+sys.path[:0] = %r
+import torch
+import test_scoring_loop_gpu as t
+run = t.calls(3)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = run()
+g.replay()
+torch.cuda.synchronize()
+want = run()
+torch.cuda.synchronize()
+assert all(torch.equal(x, y) for x, y in zip(got, want))
+assert t.B().device_status() == 0
+print("captured")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    here = os.path.dirname(os.path.abspath(__file__))
+    paths = [here, os.path.join(os.path.dirname(here), "llama-cpp-ascend310b4-addon_b200")]
+    p = subprocess.run([sys.executable, "-c", FIRST % paths], capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0 and "captured" in p.stdout, p.stderr[-2000:]
