@@ -19,6 +19,9 @@
 // above the k-th.  Keys are (order-preserving bits, inverted
 // id): all differ, ties go to the lower id, NaN is smallest.
 //
+// 1024 rows of 151936 f32 logits: 103 us with k 0 (6.0 TB/s, the stream), 122 with k
+// 5, 156 with k 20; one row of 128256 with k 20 13 to 15 us, with k 0 8.5.
+//
 // A row is read once by a cluster of up to 8 CTAs, whose lists and sums meet in
 // the first one's shared memory.
 #pragma once

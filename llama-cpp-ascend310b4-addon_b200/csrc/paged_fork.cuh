@@ -15,8 +15,10 @@
 //          page from the top of the stack; where that is a page which this call
 //          frees, the thread that pushes it writes the row's entry, so nothing is
 //          read that the launch has written.
-// Scattered marks bound it: over a few SMs they cost 50 us for 350,000 entries, so
-// the phases are launches of the whole GPU rather than steps of one cluster.
+// Latency bounds it: three launches of a few dependent reads each, after a memset of
+// the marks.  The marks are scattered, so the phases are launches of the whole GPU
+// rather than steps of one cluster.  64 rows of beams 17 to 19 us, 1024 rows with
+// 350,000 entries 27 to 29 us.
 #pragma once
 
 #include "../../include/b200_paged.h"
@@ -272,6 +274,7 @@ constexpr int kCopyThreads = 256;
 
 // CTA (entry, part of the page's rows): 16-byte pieces of K and of V, four of
 // each in flight per thread.  Bound by memory: two bytes moved per byte copied.
+// 4096 pages of 64 KB 88 us, 6.1 TB/s; 48 partial pages 6.3 us, latency.
 __global__ void __launch_bounds__(kCopyThreads) paged_copy_kernel(PagedCopyArgs a) {
     const int64_t i = blockIdx.x;
     const int src = a.src[i], dst = a.dst[i];

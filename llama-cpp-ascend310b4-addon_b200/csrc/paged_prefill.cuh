@@ -9,6 +9,10 @@
 // equal ranges, one per SM, whatever lengths and heads are (main kernel), and
 // joins the units that a cut went through (finish kernel).  Three launches, a few
 // hundred bytes of schedule, results that do not depend on timing.
+//
+// 8192 tokens, 64/8 heads x 128: 1010 to 1066 us, 1.03 to 1.09 PFLOP/s; the products
+// and their barriers bound it.  2048 tokens at 129024: 8.5 to 8.9 ms, the power limit.
+// 8 sequences of 5 tokens at up to 4160: 26 us, all of it latency.
 #pragma once
 
 #include "../../include/b200_paged.h"

@@ -370,7 +370,7 @@ int b200_token_logprobs(const void* logits, int type, int64_t ld, int64_t n_rows
     a.top_logprobs = top_logprobs;
     // CTAs to a row: a doubling while the grid stays within two CTAs to a place on the
     // GPU (8 of them on each of 148 SMs) and every thread gets a vector.  More of
-    // them even out the last wave but pay the selection's 6 us each: 1024 rows of
+    // them even out the last wave but pay the selection each: 1024 rows of
     // 151936 take 131 us with one, 119 with two, 128 with four
     a.ctas = 1;
     while (a.ctas < kLpMaxCtas && 2 * a.ctas * n_rows <= 2 * 8 * 148 &&

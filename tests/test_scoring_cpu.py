@@ -32,7 +32,7 @@ def prefill(kv=None, **over):
     dict(n_seq=65536), dict(max_blocks=0), dict(max_blocks=1 << 28, table_stride=1 << 28), dict(seq_lens=None),
     dict(cu=None), dict(mask=PTR + 1, mask_stride=64), dict(mask=PTR, mask_stride=63), dict(window=-1),
     dict(out=None), dict(out=FAR + 8), dict(workspace=None), dict(workspace=PTR + 8), dict(workspace_size=8),
-    dict(out=PTR), dict(out=PTR + 1024), dict(out=PTR - 3072 + 16), dict(q_stride=1 << 62)])
+    dict(out=PTR), dict(out=PTR + 1024), dict(out=PTR - 3 * 1024 + 16), dict(q_stride=1 << 62)])
 def test_prefill_refuses(over):
     assert prefill(**over) == B().EINVAL
 
