@@ -183,3 +183,26 @@ def test_captured_and_replayed():
         g.replay()
         want = logprobs_ref(x.double(), t, 20)
         assert torch.equal(got.top_ids, want[2]) and (got.logprob.double() - want[0]).abs().max() < 1e-4
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("k", [1, 4, 20, 32])
+@pytest.mark.parametrize("rows", [1, 700])
+def test_alternatives_that_share_threads(rows, k, dtype):
+    """The largest logits in one vector, in one thread's vectors, in neighbours, and
+    mixes of these with ties, at every rank where one kind gives way to another."""
+    r = rng(7 * k + rows)
+    vocab, vec = 128 * 256, 16 // (4 if dtype == "f32" else 2)
+    x, tokens = logits(r, rows, vocab, dtype, 1.0)
+    stride = 256 * vec  # of a thread's vectors
+    for i in range(rows):
+        near = int(r.integers(0, 256)) * vec
+        n = int(r.integers(1, k + 1))
+        places = [near + np.arange(vec),  # one vector
+                  near + stride * np.arange(min(k, vocab // stride)),  # one thread
+                  near + vec * np.arange(k),  # a thread each
+                  np.concatenate([near + stride * np.arange(min(n, vocab // stride)), near + vec * np.arange(1, k - n + 1)])]
+        at = places[i % 4] % vocab
+        high = np.full(len(at), 8.0) if i % 3 == 0 else 8.0 + np.arange(len(at)) * 0.125 * (-1) ** (i % 2)
+        x[i, torch.from_numpy(at).cuda()] = torch.from_numpy(high.astype(np.float32)).cuda().to(x.dtype)
+    check(x, tokens, k)
