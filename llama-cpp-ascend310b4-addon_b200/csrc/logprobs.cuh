@@ -22,7 +22,9 @@
 // id): all differ, ties go to the lower id, NaN is smallest.
 //
 // 1024 rows of 151936 f32 logits: 103 us with k 0 (6.0 TB/s, the stream), 111 with k
-// 5, 117 with k 20; one row of 128256 with k 20 11 us, with k 0 8.5.
+// 5, 117 with k 20; one row of 128256 with k 20 11 to 12.5 us, with k 0 8.5.  16-bit
+// logits are bound by the instructions instead: 1024 rows of f16 82 us with k 0 (3.8
+// TB/s), 91 with k 5.
 //
 // A row is read once by a cluster of up to 8 CTAs, whose lists and sums meet in
 // the first one's shared memory.
@@ -51,6 +53,10 @@ constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpBatch = 4;       // vectors of 16 bytes in flight per thread
 constexpr int kLpMaxCtas = 8;
+// CTAs on an SM at once.  f32 takes 40 registers where nothing is asked (0); asked for
+// six CTAs it spills (1% slower), for one it takes 56 (6% slower).  16-bit types are
+// held to 48 instead of 56 (1024 rows of bf16 97 -> 94 us).
+constexpr int kLpPerSmF32 = 6, kLpPerSm16 = 5;
 // kept by the thread of rank r: k - r at most or a vector's eight, besides the row's
 // unaligned ends
 constexpr int kLpFound = B200_LOGPROBS_MAX_K * (B200_LOGPROBS_MAX_K + 1) / 2 + B200_LOGPROBS_MAX_K * 8 + 16;
@@ -185,7 +191,8 @@ struct LpShared {
 };
 
 template <int TYPE>
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const __grid_constant__ LogprobsArgs a) {
+__global__ void __launch_bounds__(kLpThreads, TYPE == B200_TYPE_F32 ? 0 : kLpPerSm16)
+logprobs_kernel(const __grid_constant__ LogprobsArgs a) {
     using T = LpType<TYPE>;
     constexpr int VEC = T::kVec;
     __shared__ LpShared sh;

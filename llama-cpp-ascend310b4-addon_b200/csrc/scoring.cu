@@ -368,14 +368,17 @@ int b200_token_logprobs(const void* logits, int type, int64_t ld, int64_t n_rows
     a.entropy = entropy;
     a.top_ids = top_ids;
     a.top_logprobs = top_logprobs;
-    // CTAs to a row: a doubling while the grid stays within two CTAs to a place on the
-    // GPU (8 of them on each of 148 SMs) and every thread gets a vector.  More of
-    // them even out the last wave but pay the selection each: 1024 rows of
-    // 151936 take 131 us with one, 119 with two, 128 with four
-    a.ctas = 1;
-    while (a.ctas < kLpMaxCtas && 2 * a.ctas * n_rows <= 2 * 8 * 148 &&
-           n_vocab * size / 16 / (2 * a.ctas) >= kLpThreads)
-        a.ctas *= 2;
+    // CTAs to a row: as many as make waves of CTAs x (logits to a thread + what the
+    // selection costs, about 100 logits) least, while every thread gets a vector.  Rows of
+    // 151936 f32 logits: 200 take 31 us with four, 39 with eight; 600 70 with one, 73 with
+    // two; 1024 124 with one, 111 with two, 123 with four; in bf16 89, 97, 124
+    const int64_t places = 148 * (type == B200_TYPE_F32 ? kLpPerSmF32 : kLpPerSm16);
+    int64_t least = INT64_MAX;
+    for (int ctas = 1; ctas <= kLpMaxCtas; ctas *= 2) {
+        if (ctas > 1 && n_vocab * size / 16 / ctas < kLpThreads) break;
+        const int64_t cost = (n_rows * ctas + places - 1) / places * (n_vocab / (ctas * kLpThreads) + 100);
+        if (cost < least) least = cost, a.ctas = ctas;
+    }
     if (n_rows * a.ctas > INT32_MAX) return B200_EUNSUPPORTED;
     const cudaStream_t st = (cudaStream_t)stream;
     return type == B200_TYPE_F32   ? launch_logprobs<B200_TYPE_F32>(a, st)
