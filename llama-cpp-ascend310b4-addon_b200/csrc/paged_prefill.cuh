@@ -10,8 +10,8 @@
 // joins the units that a cut went through (finish kernel).  Three launches, a few
 // hundred bytes of schedule, results that do not depend on timing.
 //
-// 8192 tokens, 64/8 heads x 128: 1010 to 1066 us, 1.03 to 1.09 PFLOP/s; the products
-// and their barriers bound it.  2048 tokens at 129024: 8.5 to 8.9 ms, the power limit.
+// 8192 tokens, 64/8 heads x 128: 1010 to 1066 us, 1.03 to 1.09 PFLOP/s, in short runs,
+// 1176 us in long ones (power limit, 1.67 GHz); the products and their barriers bound it.  2048 tokens at 129024: 8.5 to 8.9 ms, the power limit.
 // 8 sequences of 5 tokens at up to 4160: 26 us, all of it latency.
 #pragma once
 
