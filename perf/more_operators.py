@@ -407,13 +407,13 @@ def _plain_fork(s):
 
 
 def _plain_copy(s):
-    ps = s["page_size"]
+    ps, last = s["page_size"], s["k"].shape[0] - 1
     src, dst = s["src"].long(), s["dst"].long()
+    on = src >= 0
+    # (an entry of nothing writes what another place already holds)
+    src, dst = torch.where(on, src, last), torch.where(on, dst, last)
     rows = torch.full_like(src, ps) if s["rows"] is None else s["rows"].long()
-    # (an entry of nothing repeats the first one that is something)
-    on, some = src >= 0, (src >= 0).int().argmax()
-    src, dst, rows = (torch.where(on, x, x[some]) for x in (src, dst, rows))
-    takes = torch.arange(ps, device=src.device) < rows[:, None]
+    takes = (torch.arange(ps, device=src.device) < rows[:, None]) & on[:, None]
     for x in ("k", "v"):
         s[x][dst] = torch.where(takes[..., None, None], s[x][src], s[x][dst])
     if s["lo"] is not None:
