@@ -189,8 +189,9 @@ int b200_paged_attn(const b200_paged_kv *kv, const float *q, int64_t q_stride, i
  * length: its rows come out as if its last n tokens were the new ones.
  * Scores, weights' sums and outputs are kept in 32 bits; the weights enter the
  * product with V rounded to the cache's type, as the output is.  Infinities and
- * NaN as in b200_paged_attn, a weight counting as 0 below 2^-149 of the largest:
- * a row that meets any (in positions it does not see too) is computed again in
+ * NaN as in b200_paged_attn, a weight counting as 0 below 2^-149 of the largest;
+ * positions on pages out of range are left out: a row that meets any of these
+ * (in positions it does not see too) is computed again in
  * f32, a warp to a row, which takes up to 60 times as long and leaves no trace of
  * what it does not see.  n_tokens * n_head and max_blocks * page_size stay 128
  * below 2^31 (B200_EUNSUPPORTED); a scale that is NaN is refused (B200_EINVAL).

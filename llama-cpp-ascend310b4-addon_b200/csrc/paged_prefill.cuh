@@ -382,6 +382,12 @@ __device__ __forceinline__ float pf_exp2(float x) {
     return y;
 }
 
+// Rows of a tile that are not copied: no query sees them (zeros), or their page is out
+// of range.  A value there is NaN, which no weight hides, so every row of the unit is
+// computed again, and that leaves such positions out.
+constexpr uint32_t kPfNone = ~0u, kPfLost = ~1u;
+__device__ const uint4 kPfNan = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};  // of f16 and of bf16
+
 constexpr int kPfThreads = 384;     // two softmax warpgroups; two warps of copies, tensor-core issue
 constexpr int kPfCopyThreads = 64;
 constexpr int kPfIssueWarp = 10;
@@ -563,13 +569,14 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         expects(&sh.full[stage], 0, 32);
                     }
                 };
-                // by cp.async, a lane's rows of a tile: their places in 16-byte steps, or ~0 for none
+                // by cp.async, a lane's rows of a tile: their places in 16-byte steps (K and V span
+                // less than 2^36 bytes), or kPfNone, or for values kPfLost
                 uint32_t k_off[RPL], v_off[RPL], v_next[RPL];
                 auto find_rows = [&](int t) {
 #pragma unroll
                     for (int e = 0; e < RPL; ++e) {
                         const int p = x.tile(t) * KT + pw * RPW + 32 * e + lane;
-                        k_off[e] = v_next[e] = ~0u;
+                        k_off[e] = v_next[e] = kPfNone;
                         if (p > at1) continue;
                         const int b = (int)((unsigned)p / (unsigned)ps), page = __ldg(table + b);
                         if ((unsigned)page < (unsigned)a.kv.n_pages) {
@@ -577,6 +584,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                             k_off[e] = (uint32_t)((unsigned)page * kpage + r * krow);
                             v_next[e] = (uint32_t)((unsigned)page * vpage + r * vrow);
                         } else {
+                            v_next[e] = kPfLost;
                             record_status(B200_DEVSTATUS_BOUNDS);
                         }
                     }
@@ -590,7 +598,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                             const int rl = j + lane / CH, c = lane % CH, r = pw * RPW + 32 * e + rl;
                             const uint32_t o = __shfl_sync(0xffffffffu, off[e], rl);
                             pf_cp16(dst + (c >> 3) * KHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4),
-                                    o == ~0u ? base : base + ((uint64_t)o << 4) + c * 16, o != ~0u);
+                                    o == kPfLost ? reinterpret_cast<const uint8_t*>(&kPfNan)
+                                    : o == kPfNone ? base : base + ((uint64_t)o << 4) + c * 16, o != kPfNone);
                         }
                     issued(&sh.full[stage]);
                 };
