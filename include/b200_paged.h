@@ -193,8 +193,8 @@ int b200_paged_attn(const b200_paged_kv *kv, const float *q, int64_t q_stride, i
  * positions on pages out of range are left out: a row that meets any of these
  * (in positions it does not see too) is computed again in
  * f32, a warp to a row, which takes up to 60 times as long and leaves no trace of
- * what it does not see.  n_tokens * n_head and max_blocks * page_size stay 128
- * below 2^31 (B200_EUNSUPPORTED); a scale that is NaN is refused (B200_EINVAL).
+ * what it does not see.  n_tokens * n_head stays 256 and max_blocks * page_size
+ * 128 below 2^31 (B200_EUNSUPPORTED); a scale that is NaN is refused (B200_EINVAL).
  * Fastest for pages of a multiple of 8 rows.
  * workspace: 16-byte aligned, no initial contents needed, not shared by calls
  * that overlap on the GPU. */

@@ -194,8 +194,9 @@ int b200_paged_prefill(const b200_paged_kv* kv, const void* q, int64_t q_stride,
     if ((reinterpret_cast<uintptr_t>(mask) & 1) ||
         (mask && n_seq > 1 && mask_stride != 0 && mask_stride < (int64_t)max_blocks * kv->page_size))
         return B200_EINVAL;
-    // rows and positions are counted in int, a tile past the last
-    if (n_tokens > INT32_MAX / n_head || (int64_t)max_blocks * kv->page_size > INT32_MAX - kPfRows)
+    // rows and positions are counted in int: a unit's two tiles of rows from the last row
+    // on, and a tile of positions past the last
+    if (n_tokens > (INT32_MAX - 2 * kPfRows) / n_head || (int64_t)max_blocks * kv->page_size > INT32_MAX - kPfRows)
         return B200_EUNSUPPORTED;
     if (workspace_size < b200_paged_prefill_workspace_size(kv->head_dim, n_tokens, n_seq, n_head, kv->n_head_kv))
         return B200_EINVAL;

@@ -43,6 +43,13 @@ def test_prefill_refuses_more_rows_than_it_counts():
     assert prefill(scale=float("nan")) == B().EINVAL
 
 
+def test_prefill_refuses_rows_that_its_last_tiles_would_count_past():
+    """Rows are counted in int up to two tiles of 128 from the last one on."""
+    far = PTR + (1 << 45)
+    for n_tokens, n_head in [((1 << 31) // 4 - 1, 4), ((1 << 31) // 4 - 64, 4), ((1 << 31) // 2 - 100, 2)]:
+        assert prefill(n_tokens=n_tokens, n_head=n_head, out=far) == B().EUNSUPPORTED
+
+
 @pytest.mark.parametrize("over", BAD_KV)
 def test_bad_cache_is_refused(over):
     kv = kv_struct(**over)
