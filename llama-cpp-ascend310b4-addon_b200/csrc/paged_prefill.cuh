@@ -382,10 +382,6 @@ __device__ __forceinline__ float pf_exp2(float x) {
     return y;
 }
 
-// Rows of a tile that are not copied: no query sees them (zeros), or their page is out
-// of range.  A value there is NaN, which no weight hides, so every row of the unit is
-// computed again, and that leaves such positions out.
-constexpr uint32_t kPfNone = ~0u, kPfLost = ~1u;
 __device__ const uint4 kPfNan = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};  // of f16 and of bf16
 
 constexpr int kPfThreads = 384;     // two softmax warpgroups; two warps of copies, tensor-core issue
@@ -569,14 +565,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         expects(&sh.full[stage], 0, 32);
                     }
                 };
-                // by cp.async, a lane's rows of a tile: their places in 16-byte steps (K and V span
-                // less than 2^36 bytes), or kPfNone, or for values kPfLost
-                uint32_t k_off[RPL], v_off[RPL], v_next[RPL];
+                // by cp.async, a lane's rows of a tile: their places in 16-byte steps, or ~0 for
+                // none; a bit each for those on a page out of range
+                uint32_t k_off[RPL], v_off[RPL], v_next[RPL], v_lost = 0, lost_next = 0;
                 auto find_rows = [&](int t) {
+                    lost_next = 0;
 #pragma unroll
                     for (int e = 0; e < RPL; ++e) {
                         const int p = x.tile(t) * KT + pw * RPW + 32 * e + lane;
-                        k_off[e] = v_next[e] = kPfNone;
+                        k_off[e] = v_next[e] = ~0u;
                         if (p > at1) continue;
                         const int b = (int)((unsigned)p / (unsigned)ps), page = __ldg(table + b);
                         if ((unsigned)page < (unsigned)a.kv.n_pages) {
@@ -584,7 +581,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                             k_off[e] = (uint32_t)((unsigned)page * kpage + r * krow);
                             v_next[e] = (uint32_t)((unsigned)page * vpage + r * vrow);
                         } else {
-                            v_next[e] = kPfLost;
+                            lost_next |= 1u << e;
                             record_status(B200_DEVSTATUS_BOUNDS);
                         }
                     }
@@ -598,10 +595,22 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                             const int rl = j + lane / CH, c = lane % CH, r = pw * RPW + 32 * e + rl;
                             const uint32_t o = __shfl_sync(0xffffffffu, off[e], rl);
                             pf_cp16(dst + (c >> 3) * KHALF + r * 128 + (((c & 7) ^ (r & 7)) << 4),
-                                    o == kPfLost ? reinterpret_cast<const uint8_t*>(&kPfNan)
-                                    : o == kPfNone ? base : base + ((uint64_t)o << 4) + c * 16, o != kPfNone);
+                                    o == ~0u ? base : base + ((uint64_t)o << 4) + c * 16, o != ~0u);
                         }
-                    issued(&sh.full[stage]);
+                };
+                // Values on a page out of range are NaN, which no weight hides: every row of
+                // the unit is computed again, and that leaves such positions out
+                auto lose_rows = [&] {
+                    if (!__any_sync(0xffffffffu, v_lost != 0)) return;
+                    asm volatile("cp.async.wait_all;" ::: "memory");  // the zeros are written
+                    __syncwarp();
+#pragma unroll 1
+                    for (int e = 0; e < RPL; ++e)
+                        if (v_lost >> e & 1u) {
+                            const uint32_t dst = ring + stage * STAGE + (pw * RPW + 32 * e + lane) * 128;
+#pragma unroll 1
+                            for (int c = 0; c < CH; ++c) pf_cp16(dst + (c >> 3) * KHALF + (c & 7) * 16, &kPfNan);
+                        }
                 };
                 // the mask entries of a lane's rows
                 uint16_t bias[RPL], bias_next[RPL];
@@ -636,7 +645,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                     if (t < n) {
                         if (!(ok = pf_wait(&sh.empty[stage], lap ^ 1u))) break;
                         if (now.on) copy_boxes(now, false);
-                        else copy_rows(kb, k_off);
+                        else copy_rows(kb, k_off), issued(&sh.full[stage]);
                         advance();
                     }
                     const Boxes later = t + 2 < n ? find_boxes(t + 2) : next;
@@ -644,11 +653,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         if (!(ok = pf_wait(&sh.empty[stage], lap ^ 1u))) break;
                         if (MASK) put_mask();
                         if (before.on) copy_boxes(before, true);
-                        else copy_rows(vb, v_off);
+                        else copy_rows(vb, v_off), lose_rows(), issued(&sh.full[stage]);
                         if (!ok) break;
                         advance();
                     }
-                    before = now, now = next, next = later;
+                    before = now, now = next, next = later, v_lost = lost_next;
 #pragma unroll
                     for (int e = 0; e < RPL; ++e) v_off[e] = v_next[e], bias[e] = bias_next[e];
                 }
