@@ -19,6 +19,7 @@
 #include "args.h"
 #include "common.cuh"
 #include "f32_pairs.cuh"
+#include "paged_ring.h"
 #include "paged_store.cuh"
 #include "tcgen05.cuh"
 
@@ -316,7 +317,8 @@ struct PfShared {
     static constexpr int ST = pf_stages(D);
     uint64_t q_full, q_empty, full[ST], empty[ST], s_full[2], p_ready[2], o_done[2], fix, done;
     uint32_t tmem;
-    int aborted;
+    int aborted;                         // a wait ran out
+    uint32_t filled[2], asked[2], fixed[2];  // phases of full, q_full and fix that each copying warp entered
     float tmax[4][2];  // the largest of each copying warp's rows
     // mask entries of the last tiles.  Those of V's tile i are written when its stage is
     // free: then the tile before i - 2 (i - 3 with 8 stages) has been through the softmax
@@ -349,14 +351,15 @@ __device__ __forceinline__ uint32_t pf_bits(int lo, int hi) {
     const int l = max(lo, 0), h = min(hi, 31);
     return h < l ? 0u : (0xffffffffu >> (31 - h + l)) << l;
 }
-// Waits of this kernel: the clock and the limit are read once in 4096 tries that found
-// nothing, by as few instructions as can be: there are twenty such places, and what
-// they take of the instruction cache costs the others (8192 tokens 1231 -> 1115 us).
+// Waits of this kernel: the clock and the limit are read once in 256 tries that found
+// nothing (a wait may last that much longer than the limit), by as few instructions as
+// can be: there are twenty such places, and what they take of the instruction cache
+// costs the others (8192 tokens 1231 -> 1115 us).
 __device__ __forceinline__ bool pf_wait_one(uint64_t* bar, uint32_t parity) {
     unsigned long long began = 0;
 #pragma unroll 1
     for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i)
-        if ((i & 4095u) == 0) {
+        if ((i & 255u) == 0) {
             const unsigned long long now = globaltimer();
             if (began == 0) began = now;
             if (now - began > g_wait_timeout_ns) {
@@ -369,6 +372,16 @@ __device__ __forceinline__ bool pf_wait_one(uint64_t* bar, uint32_t parity) {
 // A warp's wait: the same answer for every lane.
 __device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, pf_wait_one(bar, parity));
+}
+// pf_land_phases on the barriers from bars on; a warp has `share` arrivals in a phase.
+__device__ __forceinline__ void pf_land(uint64_t* bars, PfPhases p, uint32_t share) {
+    pf_land_phases(
+        p,
+        [&](uint32_t stage) {
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bars + stage)), "r"(share)
+                         : "memory");
+        },
+        [&](uint32_t stage, uint32_t parity) { mbar_wait_drain(bars + stage, parity); });
 }
 __device__ __forceinline__ void pf_cp16(uint32_t dst, const void* src, bool on) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
@@ -467,7 +480,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
             };
             constexpr int HALVES = D / 64, MINE = HALVES / 2;  // blocks of 64 channels; of each warp
             int stage = 0, unit = 0, tiles = 0;
-            uint32_t lap = 0, fix = 0;  // parities of the ring's lap and of sh.fix
+            uint32_t lap = 0, fix = 0;  // laps of the ring, phases of sh.fix
             bool ok = true;
             const int ps = a.kv.page_size, box_log = __ffs(a.box) - 1;
             const uint64_t krow = a.kv.k_row >> 4, vrow = a.kv.v_row >> 4, kpage = a.kv.k_page >> 4, vpage = a.kv.v_page >> 4;
@@ -481,6 +494,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                 const int n = x.te - x.tb, rows = min(NT * kPfRows, x.n * a.group - x.row0);
                 const int at1 = x.len - x.n + (x.row0 + rows - 1) / a.group;  // the last position that a row sees
                 if (unit && !(ok = pf_wait(&sh.q_empty, (unit - 1) & 1))) break;
+                ++unit;
                 if (a.q_box) {
                     // 128 rows of 64 channels to a copy; rows past the sequence's are not used
                     const int tiles = (rows + kPfRows - 1) / kPfRows;
@@ -541,7 +555,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         __syncwarp();
                         if (lane == 0) pf_arrive(&sh.full[stage]);  // the mask entries are written
                     }
-                    if (++stage == ST) stage = 0, lap ^= 1u;
+                    if (++stage == ST) stage = 0, ++lap;
                 };
                 auto copy_boxes = [&](const Boxes& b, bool value) {
                     const bool part = value && b.rows < KT;
@@ -549,8 +563,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                     send_boxes(value ? &a.map_v : &a.map_k, b, part ? &sh.fix : &sh.full[stage], part ? 1 : 32);
                     if (part) {
                         // a weight of 0 meets every value: rows that no query sees become 0
-                        if (!(ok = pf_wait(&sh.fix, fix))) return;
-                        fix ^= 1u;
+                        if (!(ok = pf_wait(&sh.fix, fix++ & 1u))) return;
                         const int per = (KT - b.rows) * 8;  // 16-byte pieces of a block of 64 channels
 #pragma unroll 1
                         for (int hf = 0; hf < HALVES; ++hf)
@@ -643,14 +656,14 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                         find_mask(t);
                     }
                     if (t < n) {
-                        if (!(ok = pf_wait(&sh.empty[stage], lap ^ 1u))) break;
+                        if (!(ok = pf_wait(&sh.empty[stage], ~lap & 1u))) break;
                         if (now.on) copy_boxes(now, false);
                         else copy_rows(kb, k_off), issued(&sh.full[stage]);
                         advance();
                     }
                     const Boxes later = t + 2 < n ? find_boxes(t + 2) : next;
                     if (t > 0) {
-                        if (!(ok = pf_wait(&sh.empty[stage], lap ^ 1u))) break;
+                        if (!(ok = pf_wait(&sh.empty[stage], ~lap & 1u))) break;
                         if (MASK) put_mask();
                         if (before.on) copy_boxes(before, true);
                         else copy_rows(vb, v_off), lose_rows(), issued(&sh.full[stage]);
@@ -661,10 +674,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
 #pragma unroll
                     for (int e = 0; e < RPL; ++e) v_off[e] = v_next[e], bias[e] = bias_next[e];
                 }
-                ++unit;
             }
             if (tid == 256) a.cut[2 * blockIdx.x] = cut, a.cut[2 * blockIdx.x + 1] = cut_seq;
             asm volatile("cp.async.wait_all;" ::: "memory");
+            if (lane == 0) sh.filled[pw] = lap * ST + stage, sh.asked[pw] = unit, sh.fixed[pw] = fix;
             if (!ok) sh.aborted = 1;
         } else if (warp == kPfIssueWarp && lane == 0) {
             // ---- tensor-core issue
@@ -987,7 +1000,14 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
         if (!ok && j < NT) sh.aborted = 1;
     }
     tc_fence_before();
-    __syncthreads();
+    __syncthreads();  // every loop is over
+    if (tid == 256 && sh.aborted) {
+        // A wait ran out (recorded; the outputs are not what they should be): TMA copies
+        // that nobody waited for must land before the CTA's shared memory is another's.
+        pf_land(sh.full, {{sh.filled[0], sh.filled[1]}, (uint32_t)ST}, 32 + (MASK ? 1 : 0));
+        pf_land(&sh.q_full, {{sh.asked[0], sh.asked[1]}, 1u}, 32);
+        pf_land(&sh.fix, {{sh.fixed[0], sh.fixed[1]}, 1u}, 1);
+    }
     if (tid == kPfIssueWarp * 32) tc_commit(&sh.done);  // every product issued has ended
     if (warp == kPfIssueWarp) {
         mbar_wait_drain(&sh.done, 0);

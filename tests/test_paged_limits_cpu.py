@@ -209,3 +209,73 @@ def test_attn_refuses_an_output_that_meets_the_queries(n_seq, q_stride, out, mee
     rc = bw.lib().b200_paged_attn(C.byref(kv), at, q_stride, n_seq, 4, PTR, 4, 4, PTR, None, 0, None, 0, 1.0, at + out, PTR,
                                   1 << 30, None)
     assert (rc == bw.EINVAL) == meets
+
+
+LAND_TEST = r'''
+// pf_land_phases (csrc/paged_ring.h) on a model of a ring of barriers: two warps copy
+// into its stages, a third frees them, and any of the three may stop anywhere.
+#include <cstdio>
+#include <cstdlib>
+#include <random>
+#include <vector>
+
+#include "paged_ring.h"
+
+int main(int argc, char** argv) {
+    const unsigned stages = (unsigned)atoi(argv[1]);
+    std::mt19937 g(stages);
+    long stopped_apart = 0, in_flight = 0;
+    for (int trial = 0; trial < 20000; ++trial) {
+        unsigned entered[2] = {0, 0}, freed = 0, end[3];
+        for (unsigned& e : end) e = g() % 20;
+        std::vector<unsigned> arrivals(64, 0);  // of a phase
+        std::vector<bool> landed(64, false);
+        for (;;) {  // as far as each comes: a warp needs its stage freed, the third both warps' arrivals
+            std::vector<int> can;
+            for (int w = 0; w < 2; ++w)
+                if (entered[w] < end[w] && (entered[w] < stages || freed > entered[w] - stages)) can.push_back(w);
+            if (freed < end[2] && arrivals[freed] == 2) can.push_back(2);
+            if (can.empty() || g() % 50 == 0) break;
+            const int who = can[g() % can.size()];
+            if (who == 2) landed[freed++] = true;  // it waited for the copies
+            else ++arrivals[entered[who]++];
+        }
+        const b200::PfPhases p = {{entered[0], entered[1]}, stages};
+        stopped_apart += entered[0] != entered[1];
+        // a barrier is in the phase of its first one without both arrivals
+        auto current = [&](unsigned stage) {
+            unsigned f = stage;
+            while (f < 64 && arrivals[f] == 2) f += stages;
+            return f;
+        };
+        b200::pf_land_phases(
+            p, [&](unsigned stage) { ++arrivals[current(stage)]; },
+            [&](unsigned stage, unsigned parity) {
+                const unsigned now = current(stage);
+                if (((now / stages) & 1u) == parity) printf("trial %d: stage %u is waited for in vain\n", trial, stage), exit(1);
+                for (unsigned f = stage; f < now; f += stages) in_flight += !landed[f], landed[f] = true;
+            });
+        for (unsigned f = 0; f < 64; ++f) {
+            const bool any = f < entered[0] || f < entered[1];
+            if (any != landed[f] || (any && arrivals[f] != 2) || (!any && arrivals[f]))
+                printf("trial %d: phase %u\n", trial, f), exit(1);
+        }
+    }
+    printf("%d\n", stopped_apart > 1000 && in_flight > 1000);
+}
+'''
+
+
+@pytest.mark.parametrize("stages", [1, 5, 8])
+def test_copies_left_behind_are_waited_for(tmp_path, stages):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no g++")
+    src, exe = tmp_path / "land.cpp", tmp_path / "land"
+    src.write_text(LAND_TEST)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    csrc = os.path.join(root, "llama-cpp-ascend310b4-addon_b200", "csrc")
+    subprocess.run([gxx, "-O1", "-std=c++17", "-I" + csrc, "-I/usr/local/cuda/include", str(src), "-o",
+                    str(exe)], check=True)
+    out = subprocess.run([str(exe), str(stages)], capture_output=True, text=True)
+    assert out.returncode == 0 and out.stdout.strip() == "1", out.stdout
