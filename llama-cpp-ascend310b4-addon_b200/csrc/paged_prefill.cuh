@@ -96,23 +96,25 @@ __device__ __forceinline__ PfSeq pf_seq(const PagedPrefillArgs& a, int s, bool r
 }
 
 // One row of one head by a warp, in f32 products of whole values: what the formula
-// says whatever infinities and NaN meet.  Lane l owns channels l * D / 32 on.
+// says whatever infinities and NaN meet.  Values near bf16's largest add up past the
+// f32 range though their mean is in it: sums are kept in 64 bits.  Lane l owns channels
+// l * D / 32 on.
 template <bool BF16, int D>
 __device__ void pf_row(const PagedPrefillArgs& a, int s, const PfSeq& sq, int i, int head) {
     constexpr int E = D / 32;
     const int lane = threadIdx.x & 31, h = head / a.group, ps = a.kv.page_size;
     const int64_t t = sq.first + i;
     const uint16_t* qp = a.q + t * a.q_stride + head * D + lane * E;
-    float q[E], o[E];
+    float q[E];
+    double o[E];
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
         const float2 f = unpack16<BF16>(*reinterpret_cast<const uint32_t*>(qp + e));
-        q[e] = f.x, q[e + 1] = f.y, o[e] = o[e + 1] = 0.f;
+        q[e] = f.x, q[e + 1] = f.y, o[e] = o[e + 1] = 0.;
     }
     const int at = sq.len - sq.n + i;  // may be negative: sees nothing
     const int p0 = a.window > 0 ? max(0, at - a.window + 1) : 0;
-    double m = -INFINITY;
-    float sum = 0.f;
+    double m = -INFINITY, sum = 0.;
     for (int p = p0; p <= at; ++p) {
         float bias = 0.f;
         if (a.mask) {
@@ -148,14 +150,14 @@ __device__ void pf_row(const PagedPrefillArgs& a, int s, const PfSeq& sq, int i,
         const float w = y == -INFINITY ? 0.f : exp2f((float)((y - m) * 1.4426950408889634));
         sum += w;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(w, v[e], o[e]);
+        for (int e = 0; e < E; ++e) o[e] = fma((double)w, (double)v[e], o[e]);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const double inv = sum == 0. ? 0. : 1. / sum;
     uint16_t* op = a.out + (t * a.n_head + head) * D + lane * E;
 #pragma unroll
     for (int e = 0; e < E; e += 2)
         *reinterpret_cast<uint32_t*>(op + e) =
-            sum == 0.f ? 0u : pack16<BF16>(o[e] * inv, o[e + 1] * inv);
+            sum == 0. ? 0u : pack16<BF16>((float)(o[e] * inv), (float)(o[e + 1] * inv));
 }
 
 // ------------------------------------------------------------------- plan

@@ -67,3 +67,20 @@ def test_only_pages_out_of_range():
     out = run(c, q, cu, "f16", 0.1)
     assert B().device_status(reset=True) == BOUNDS
     assert (out[: int(cu[-1])] == 0).all()
+
+
+@pytest.mark.parametrize("past,new,ps,hq,hkv,d", [([64], [16], 16, 8, 2, 128), ([3000, 0], [5, 200], 16, 12, 2, 64),
+                                                  ([300], [140], 5, 4, 2, 256), ([0], [1], 16, 2, 2, 128)])
+def test_values_near_the_largest(past, new, ps, hq, hkv, d):
+    """bf16 values whose weighted sums pass the f32 range, but no mean does: all of one
+    sign in half of the channels, of both in the others."""
+    r, c, cu, q = make(past, new, ps, hq, hkv, d, "bf16")
+    most = float(torch.finfo(torch.bfloat16).max)
+    v = r.choice([most, most / 2, 0.75 * most], c["v"].shape) * r.choice([1, -1], c["v"].shape)
+    v[..., ::2] = np.abs(v[..., ::2])
+    c["v"] = np.where(np.isnan(c["v"]), np.nan, R.rounded(v, "bf16"))
+    out = run(c, q, cu, "bf16", d ** -0.5)
+    want, tol = chunk_ref(c, q, cu, ps, d ** -0.5)
+    rows = slice(0, int(cu[-1]))
+    assert torch.isfinite(out[rows].float()).all()
+    assert ((out.double() - want).abs()[rows] <= tol[rows]).all()
