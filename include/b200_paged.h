@@ -191,10 +191,13 @@ int b200_paged_attn(const b200_paged_kv *kv, const float *q, int64_t q_stride, i
  * product with V rounded to the cache's type, as the output is.  Infinities and
  * NaN as in b200_paged_attn, a weight counting as 0 below 2^-149 of the largest;
  * positions on pages out of range are left out: a row that meets any of these
- * (in positions it does not see too) is computed again in
- * f32, a warp to a row, which takes up to 60 times as long and leaves no trace of
- * what it does not see.  n_tokens * n_head stays 256 and max_blocks * page_size
- * 128 below 2^31 (B200_EUNSUPPORTED); a scale that is NaN is refused (B200_EINVAL).
+ * (in positions it does not see too) is computed again in f32 products, a block
+ * of threads to a row, and has no trace of what it does not see.  That takes 0.14
+ * us per 1000 positions of a row and head where every row is such, up to 320 times
+ * as long as the call without: 5 rows of 12 heads 0.17 ms over 4096 positions (4
+ * times) and 5.3 to 6.3 ms over 131072 (85), 512 of 64 heads over 16384 73 ms (260).
+ * n_tokens * n_head stays 256 and max_blocks * page_size 128 below 2^31
+ * (B200_EUNSUPPORTED); a scale that is NaN is refused (B200_EINVAL).
  * Fastest for pages of a multiple of 8 rows.
  * workspace: 16-byte aligned, no initial contents needed, not shared by calls
  * that overlap on the GPU. */

@@ -51,6 +51,7 @@ struct PagedPrefillArgs {
     int4* cut;          // [CTAs] two for the unit that begins in a CTA's range and goes on past it:
                         // {sequence, KV head, first flat row, pieces (0: no such unit)}, {first, n, len, -}
     int2* bad;          // rows to compute again: {flat (token, head), unit}
+    unsigned* claim;    // [CTAs][8] those of the unit that begins in a CTA's range and goes on past it: bits of its rows
     float4* piece_ml;   // [2 * CTAs][tiles][128] {reference, sum, mask reference, -} of cut units
     float4* piece_o;    // [2 * CTAs][tiles][D / 4][128] their sums of weighted values
 };
@@ -95,69 +96,134 @@ __device__ __forceinline__ PfSeq pf_seq(const PagedPrefillArgs& a, int s, bool r
     return q;
 }
 
-// One row of one head by a warp, in f32 products of whole values: what the formula
-// says whatever infinities and NaN meet.  Values near bf16's largest add up past the
-// f32 range though their mean is in it: sums are kept in 64 bits.  Lane l owns channels
-// l * D / 32 on.
-template <bool BF16, int D>
-__device__ void pf_row(const PagedPrefillArgs& a, int s, const PfSeq& sq, int i, int head) {
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31, h = head / a.group, ps = a.kv.page_size;
-    const int64_t t = sq.first + i;
-    const uint16_t* qp = a.q + t * a.q_stride + head * D + lane * E;
-    float q[E];
-    double o[E];
+// ------------------------------------------------- rows computed once more
+
+constexpr int kPfFinishThreads = 256;
+constexpr int kPfAgainWarps = kPfFinishThreads / 32;
+
+template <int D>
+struct PfAgain {
+    double m[kPfAgainWarps], sum[kPfAgainWarps], o[kPfAgainWarps][D];
+};
+
+// D / 32 channels of a row from their address on, as f32.
+template <bool BF16, int E>
+__device__ __forceinline__ void pf_channels(const void* at, float (&x)[E]) {
+    uint32_t w[E / 2];
+    if constexpr (E == 2) w[0] = __ldg(static_cast<const uint32_t*>(at));
+    else if constexpr (E == 4) {
+        const uint2 v = __ldg(static_cast<const uint2*>(at));
+        w[0] = v.x, w[1] = v.y;
+    } else {
+        const uint4 v = __ldg(static_cast<const uint4*>(at));
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    }
 #pragma unroll
     for (int e = 0; e < E; e += 2) {
-        const float2 f = unpack16<BF16>(*reinterpret_cast<const uint32_t*>(qp + e));
-        q[e] = f.x, q[e + 1] = f.y, o[e] = o[e + 1] = 0.;
+        const float2 f = unpack16<BF16>(w[e / 2]);
+        x[e] = f.x, x[e + 1] = f.y;
     }
-    const int at = sq.len - sq.n + i;  // may be negative: sees nothing
+}
+
+// One row of one head by a CTA, in f32 products of whole values: what the formula says
+// whatever infinities and NaN meet.  Values near bf16's largest add up past the f32
+// range though their mean is in it: sums are kept in 64 bits.  Every warp takes every
+// eighth run of 32 positions, looked up by a lane each and read four at a time; lane l
+// owns channels l * D / 32 on.  The warps' sums are joined in order.
+// Bound by 64-bit arithmetic and conversions: 7 x 10^9 positions of a row a second with
+// every SM at it.  5 rows of 12 heads over 131072 positions 5.3 to 6.3 ms (452 ms with a
+// warp to a row and a position at a time); 512 rows of 64 heads over 16384 73 ms (167).
+template <bool BF16, int D>
+__device__ __noinline__ void pf_row(const PagedPrefillArgs& a, PfAgain<D>& sh, int s, int n, int len, int64_t t, int i,
+                                    int head) {
+    constexpr int E = D / 32, AT_ONCE = 4;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = head / a.group, ps = a.kv.page_size;
+    float q[E];
+    pf_channels<BF16, E>(a.q + t * a.q_stride + head * D + lane * E, q);
+    double o[E], m = -INFINITY, sum = 0.;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.;
+    const int at = len - n + i;  // may be negative: sees nothing
     const int p0 = a.window > 0 ? max(0, at - a.window + 1) : 0;
-    double m = -INFINITY, sum = 0.;
-    for (int p = p0; p <= at; ++p) {
+    const uint8_t* kb = static_cast<const uint8_t*>(a.kv.k) + h * a.kv.k_head + lane * E * 2;
+    const uint8_t* vb = static_cast<const uint8_t*>(a.kv.v) + h * a.kv.v_head + lane * E * 2;
+    for (int64_t first = (int64_t)p0 + 32 * warp; first <= at; first += 32 * kPfAgainWarps) {
+        const int64_t p = first + lane;
         float bias = 0.f;
-        if (a.mask) {
+        int64_t ko = 0, vo = 0;
+        bool seen = p <= at;
+        if (seen && a.mask) {
             bias = h2f(a.mask[s * a.mask_stride + p]);
-            if (bias == -INFINITY) continue;
+            seen = bias != -INFINITY;
         }
-        const int page = a.table[s * a.table_stride + p / ps], r = p % ps;
-        if ((unsigned)page >= (unsigned)a.kv.n_pages) {
-            if (lane == 0) record_status(B200_DEVSTATUS_BOUNDS);
-            continue;
+        if (seen) {
+            const int page = a.table[s * a.table_stride + p / ps], r = (int)(p % ps);
+            seen = (unsigned)page < (unsigned)a.kv.n_pages;
+            if (!seen) record_status(B200_DEVSTATUS_BOUNDS);
+            ko = seen ? page * a.kv.k_page + r * a.kv.k_row : 0;
+            vo = seen ? page * a.kv.v_page + r * a.kv.v_row : 0;
         }
-        const uint8_t* kp = static_cast<const uint8_t*>(a.kv.k) + page * a.kv.k_page + r * a.kv.k_row + h * a.kv.k_head;
-        const uint8_t* vp = static_cast<const uint8_t*>(a.kv.v) + page * a.kv.v_page + r * a.kv.v_row + h * a.kv.v_head;
-        float x = 0.f, v[E];
+        for (unsigned left = __ballot_sync(0xffffffffu, seen); left;) {
+            float k[AT_ONCE][E], v[AT_ONCE][E], x[AT_ONCE], b[AT_ONCE];
+            int count = 0;
 #pragma unroll
-        for (int e = 0; e < E; e += 2) {
-            const float2 k = unpack16<BF16>(*reinterpret_cast<const uint32_t*>(kp + 2 * (lane * E + e)));
-            const float2 w = unpack16<BF16>(*reinterpret_cast<const uint32_t*>(vp + 2 * (lane * E + e)));
-            x = fmaf(q[e + 1], k.y, fmaf(q[e], k.x, x));
-            v[e] = w.x, v[e + 1] = w.y;
-        }
-        x = warp_sum(x);
-        const double y = (double)(x * a.scale) + (double)bias;  // a mask of the lowest value keeps the score's bits
-        if (y > m) {
-            const float f = exp2f((float)((m - y) * 1.4426950408889634));
-            if (m != -INFINITY) {
-                sum *= f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[e] *= f;
+            for (int j = 0; j < AT_ONCE; ++j) {  // (past the last one: what lane 0 names, not counted)
+                const int from = __ffs(left) - 1;
+                if (from >= 0) count = j + 1, left &= left - 1;
+                const int l = from >= 0 ? from : 0;
+                pf_channels<BF16, E>(kb + __shfl_sync(0xffffffffu, ko, l), k[j]);
+                pf_channels<BF16, E>(vb + __shfl_sync(0xffffffffu, vo, l), v[j]);
+                b[j] = __shfl_sync(0xffffffffu, bias, l);
             }
-            m = y;
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) {
+                x[j] = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[j] = fmaf(q[e], k[j][e], x[j]);
+                x[j] = warp_sum(x[j]);
+            }
+            double y[AT_ONCE], top = m;  // a mask of the lowest value keeps the score's bits
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) {
+                y[j] = (double)(x[j] * a.scale) + (double)b[j];
+                if (j < count && y[j] > top) top = y[j];
+            }
+            if (top > m) {
+                if (m != -INFINITY) {
+                    const double f = exp2f((float)((m - top) * 1.4426950408889634));
+                    sum *= f;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[e] *= f;
+                }
+                m = top;
+            }
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) {
+                if (j >= count) break;
+                const double w = y[j] == -INFINITY ? 0.f : exp2f((float)((y[j] - m) * 1.4426950408889634));
+                sum += w;
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = fma(w, (double)v[j][e], o[e]);
+            }
         }
-        const float w = y == -INFINITY ? 0.f : exp2f((float)((y - m) * 1.4426950408889634));
-        sum += w;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fma((double)w, (double)v[e], o[e]);
     }
-    const double inv = sum == 0. ? 0. : 1. / sum;
-    uint16_t* op = a.out + (t * a.n_head + head) * D + lane * E;
+    __syncthreads();  // the row before has been read
+    if (lane == 0) sh.m[warp] = m, sh.sum[warp] = sum;
 #pragma unroll
-    for (int e = 0; e < E; e += 2)
-        *reinterpret_cast<uint32_t*>(op + e) =
-            sum == 0. ? 0u : pack16<BF16>((float)(o[e] * inv), (float)(o[e + 1] * inv));
+    for (int e = 0; e < E; ++e) sh.o[warp][lane * E + e] = o[e];
+    __syncthreads();
+    const int c = 2 * threadIdx.x;
+    if (c >= D) return;
+    double most = -INFINITY, all = 0., y0 = 0., y1 = 0.;
+    for (int w = 0; w < kPfAgainWarps; ++w) most = fmax(most, sh.m[w]);
+    for (int w = 0; w < kPfAgainWarps; ++w) {
+        const double f = sh.m[w] == -INFINITY ? 0.f : exp2f((float)((sh.m[w] - most) * 1.4426950408889634));
+        all += f * sh.sum[w];
+        y0 += f * sh.o[w][c], y1 += f * sh.o[w][c + 1];
+    }
+    const double inv = all == 0. ? 0. : 1. / all;
+    *reinterpret_cast<uint32_t*>(a.out + (t * a.n_head + head) * D + c) =
+        all == 0. ? 0u : pack16<BF16>((float)(y0 * inv), (float)(y1 * inv));
 }
 
 // ------------------------------------------------------------------- plan
@@ -255,8 +321,11 @@ __global__ void __launch_bounds__(kPfPlanThreads) paged_prefill_plan_kernel(cons
         a.header->units = (int)units;
         a.header->n_bad = 0;
     }
-    // where every CTA starts (the loops above end with a barrier behind the last prefix)
-    if (whole) {
+    // where every CTA starts (the loops above end with a barrier behind the last prefix),
+    // and beside it no row is listed yet
+    if (tid >= kPfPlanThreads / 2) {
+        for (int i = tid - kPfPlanThreads / 2; i < kPfCtas * 8; i += kPfPlanThreads / 2) a.claim[i] = 0;
+    } else if (whole) {
         if (tid < units * a.kv.n_head_kv) a.start[tid] = make_int2((int)(tid % units), (int)(tid / units));
     } else if (tid < kPfCtas && tid * per < all) {
         const int64_t h = tid * per / tiles, x = tid * per - h * tiles;
@@ -937,11 +1006,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
             if (!(ok = pf_wait(&sh.o_done[j], (o_par + 1u) & 1u))) break;
             tc_fence_after();
             if (!any) continue;
+            const int64_t out_row = (int64_t)(x.first + i) * a.n_head + x.h * a.group + (flat - i * a.group);
+            bool again;
             if (n == x.cost) {
-                const float inv = l == 0.f ? 0.f : 1.f / l;
                 float odd = l * 0.f;  // NaN where anything is not finite
-                const int g = flat - i * a.group;
-                const int64_t out_row = (int64_t)(x.first + i) * a.n_head + x.h * a.group + g;
+                const float inv = l == 0.f ? 0.f : 1.f / l;
                 uint4* to = reinterpret_cast<uint4*>(a.out + out_row * D);
 #pragma unroll 1
                 for (int c = 0; c < D; c += 64) {
@@ -965,20 +1034,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                                 to[c / 8 + 4 * b + e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
                     }
                 }
-                const bool again = real && l != 0.f && odd != 0.f;
-                const unsigned votes = __ballot_sync(0xffffffffu, again);
-                if (votes) {
-                    int at_list = 0;
-                    if (lane == 0) at_list = atomicAdd(&a.header->n_bad, __popc(votes));
-                    at_list = __shfl_sync(0xffffffffu, at_list, 0) + __popc(votes & ((1u << lane) - 1u));
-                    if (again && at_list < a.n_tokens * a.n_head) a.bad[at_list] = make_int2((int)out_row, x.u);
-                }
+                again = real && l != 0.f && odd != 0.f;
             } else {
                 // at most one unit goes on from the CTA before, and one goes on in the next
                 const int slot = 2 * blockIdx.x + (x.tb > 0 ? 0 : 1);
                 float4* ml = a.piece_ml + ((int64_t)slot * NT + j) * kPfRows + row;
                 float4* po = a.piece_o + ((int64_t)slot * NT + j) * (D / 4) * kPfRows + row;
                 if (real) *ml = make_float4(ref, l, c_ref, 0.f);
+                const uint64_t none = f2_pair(0.f, 0.f);
+                uint64_t zero = none;  // NaN where anything is not finite
 #pragma unroll 1
                 for (int c = 0; c < D; c += 64) {
                     uint32_t o[2][32];
@@ -988,6 +1052,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
                         tc_loaded(o[b]);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2)
+                            zero = f2_fma(f2_pair(__uint_as_float(o[b][e]), __uint_as_float(o[b][e + 1])), none, zero);
                         if (real)
 #pragma unroll
                             for (int e = 0; e < 8; ++e)
@@ -996,6 +1063,21 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                                                 __uint_as_float(o[b][4 * e + 2]), __uint_as_float(o[b][4 * e + 3]));
                     }
                 }
+                const float2 odd = f2_unpair(zero);
+                again = real && l * 0.f + odd.x + odd.y != 0.f;
+            }
+            unsigned votes = __ballot_sync(0xffffffffu, again);
+            if (votes) {
+                int at_list = 0;
+                if (lane == 0) {
+                    // (the CTA where the unit's first key tile is: one of its pieces lists the row)
+                    if (n != x.cost)
+                        votes &= ~atomicOr(a.claim + (walk.w - x.cost) / per_cta * 8 + j * 4 + (warp & 3), votes);
+                    at_list = atomicAdd(&a.header->n_bad, __popc(votes));
+                }
+                votes = __shfl_sync(0xffffffffu, votes, 0);
+                at_list = __shfl_sync(0xffffffffu, at_list, 0) + __popc(votes & ((1u << lane) - 1u));
+                if ((votes >> lane & 1u) && at_list < a.n_tokens * a.n_head) a.bad[at_list] = make_int2((int)out_row, x.u);
             }
             tc_fence_before();
         }
@@ -1020,15 +1102,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
 
 // ----------------------------------------------------------------- finish
 
-constexpr int kPfFinishThreads = 256;
-
 // CTA (CTA of the main kernel, 32 rows): the pieces of the unit that begins in that
-// one's range and goes on past it, joined in order.  Then the rows that infinities or NaN met, and which
-// no product of whole tiles can tell apart from positions they do not see.
+// one's range and goes on past it, joined in order.  Then the rows that infinities or NaN
+// met, and which no product of whole tiles can tell apart from positions they do not see:
+// a CTA to a row.
 template <bool BF16, int D>
 __global__ void __launch_bounds__(kPfFinishThreads) paged_prefill_finish_kernel(const __grid_constant__ PagedPrefillArgs a) {
     constexpr int NT = pf_tiles(D), W = kPfFinishThreads / 32, CPW = D / 4 / W;  // float4 columns to a warp
     __shared__ int s_odd[W][32];
+    __shared__ PfAgain<D> s_again;
     griddep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int4 cut = a.cut[2 * blockIdx.y], d1 = a.cut[2 * blockIdx.y + 1];
@@ -1038,6 +1120,7 @@ __global__ void __launch_bounds__(kPfFinishThreads) paged_prefill_finish_kernel(
         const int r0 = blockIdx.x * 32, j = r0 / kPfRows, row = (r0 & (kPfRows - 1)) + lane;
         const int flat = cut.z + r0 + lane;
         const bool real = flat < d1.y * a.group;
+        const unsigned listed = a.claim[c0 * 8 + r0 / 32];  // rows that a piece has listed are not joined
         if (cut.z + r0 < d1.y * a.group) {
             // piece k: the last of CTA c0's range, then the first of each one's
             auto slot = [&](int k) { return (int64_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * NT + j; };
@@ -1091,34 +1174,30 @@ __global__ void __launch_bounds__(kPfFinishThreads) paged_prefill_finish_kernel(
                 w[2 * e] = l == 0.f ? 0u : pack16<BF16>(o[e].x * inv, o[e].y * inv);
                 w[2 * e + 1] = l == 0.f ? 0u : pack16<BF16>(o[e].z * inv, o[e].w * inv);
             }
-            if (real) {
+            const bool mine = real && !(listed >> lane & 1u);
+            if (mine) {
                 uint2* to = reinterpret_cast<uint2*>(a.out + out_row * D) + warp * CPW;
 #pragma unroll
                 for (int e = 0; e < CPW; ++e) to[e] = make_uint2(w[2 * e], w[2 * e + 1]);
             }
-            s_odd[warp][lane] = real && l != 0.f && odd != 0.f;
+            s_odd[warp][lane] = mine && l != 0.f && odd != 0.f;
             __syncthreads();
             bool again = false;
 #pragma unroll
             for (int v = 0; v < W; ++v) again |= s_odd[v][lane] != 0;
             unsigned votes = __ballot_sync(0xffffffffu, again);
-            PfSeq sq;
-            sq.first = d1.x, sq.n = d1.y, sq.len = d1.z;
-            for (int k = 0; votes; votes &= votes - 1, ++k)
-                if (k % W == warp) {
-                    const int r = cut.z + r0 + __ffs(votes) - 1, t = r / a.group;
-                    pf_row<BF16, D>(a, cut.x, sq, t, h * a.group + r - t * a.group);
-                }
+            for (; votes; votes &= votes - 1) {  // finite pieces whose sum is not
+                const int r = cut.z + r0 + __ffs(votes) - 1, i1 = r / a.group;
+                pf_row<BF16, D>(a, s_again, cut.x, d1.y, d1.z, d1.x + i1, i1, h * a.group + r - i1 * a.group);
+            }
         }
     }
     const int cta = blockIdx.y * gridDim.x + blockIdx.x, ctas = gridDim.x * gridDim.y;
-    for (int64_t b = (int64_t)cta * W + warp; b < n_bad; b += (int64_t)ctas * W) {
+    for (int64_t b = cta; b < n_bad; b += ctas) {
         const int2 e = a.bad[b];
-        const int4 d1 = a.desc[2 * (int64_t)e.y + 1];
-        PfSeq sq;
-        sq.first = d1.x, sq.n = d1.y, sq.len = d1.z;
+        const int4 d0 = a.desc[2 * (int64_t)e.y], d1 = a.desc[2 * (int64_t)e.y + 1];
         const int t = e.x / a.n_head;
-        pf_row<BF16, D>(a, a.desc[2 * (int64_t)e.y].x, sq, t - sq.first, e.x - t * a.n_head);
+        pf_row<BF16, D>(a, s_again, d0.x, d1.y, d1.z, t, t - d1.x, e.x - t * a.n_head);
     }
 }
 

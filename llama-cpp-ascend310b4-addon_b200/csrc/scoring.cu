@@ -106,7 +106,7 @@ bool encode_view(CUtensorMap* m, const void* base, const int64_t (&dims)[4], con
 
 struct PrefillLayout {
     int64_t units;  // at most
-    size_t start, cut, desc, prefix, bad, ml, o, total;
+    size_t start, cut, claim, desc, prefix, bad, ml, o, total;
 };
 
 PrefillLayout prefill_layout(int head_dim, int64_t n_tokens, int64_t n_seq, int64_t n_head, int64_t n_head_kv) {
@@ -115,7 +115,8 @@ PrefillLayout prefill_layout(int head_dim, int64_t n_tokens, int64_t n_seq, int6
     l.units = n_tokens * (n_head / n_head_kv) / rows + n_seq;
     l.start = 256;
     l.cut = l.start + align256(kPfCtas * sizeof(int2));
-    l.desc = l.cut + align256(2 * kPfCtas * sizeof(int4));
+    l.claim = l.cut + align256(2 * kPfCtas * sizeof(int4));
+    l.desc = l.claim + align256(8 * kPfCtas * sizeof(unsigned));
     l.prefix = l.desc + align256((size_t)l.units * 2 * sizeof(int4));
     l.bad = l.prefix + align256((size_t)(l.units + 1) * sizeof(int64_t));
     l.ml = l.bad + align256((size_t)(n_tokens * n_head) * sizeof(int2));
@@ -241,6 +242,7 @@ int b200_paged_prefill(const b200_paged_kv* kv, const void* q, int64_t q_stride,
     a.header = reinterpret_cast<PfHeader*>(ws);
     a.start = reinterpret_cast<int2*>(ws + l.start);
     a.cut = reinterpret_cast<int4*>(ws + l.cut);
+    a.claim = reinterpret_cast<unsigned*>(ws + l.claim);
     a.desc = reinterpret_cast<int4*>(ws + l.desc);
     a.prefix = reinterpret_cast<int64_t*>(ws + l.prefix);
     a.bad = reinterpret_cast<int2*>(ws + l.bad);

@@ -84,3 +84,81 @@ def test_values_near_the_largest(past, new, ps, hq, hkv, d):
     rows = slice(0, int(cu[-1]))
     assert torch.isfinite(out[rows].float()).all()
     assert ((out.double() - want).abs()[rows] <= tol[rows]).all()
+
+
+def nonfinite_want(c, q, cu, ps, scale, mask, window):
+    """The formula in 64 bits, infinities and NaN included: a position that is not seen
+    has no part in it."""
+    n_head, d = q.shape[1:]
+    group = n_head // c["k"].shape[2]
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    qs, k_all, v_all = q.double().cpu(), torch.from_numpy(c["k"]), torch.from_numpy(c["v"])
+    for s in range(len(cu) - 1):
+        n, length = int(cu[s + 1] - cu[s]), int(c["lens"][s])
+        for i in range(n):
+            at = length - n + i
+            pos = np.arange(max(0, at - window + 1) if window else 0, at + 1)
+            bias = np.zeros(pos.size)
+            if mask is not None:
+                pos = pos[mask[s, pos] != -np.inf]
+                bias = mask[s, pos].astype(np.float64)
+            if pos.size == 0:
+                continue
+            page = torch.from_numpy(c["table"][s, pos // ps].astype(np.int64))
+            for j in range(n_head):
+                k, v = k_all[page, pos % ps, j // group], v_all[page, pos % ps, j // group]
+                x = (qs[cu[s] + i, j] * k).sum(-1) * scale + torch.from_numpy(bias)
+                if (x == -np.inf).all():
+                    continue
+                w = (x - x.max()).exp()
+                out[cu[s] + i, j] = (w[:, None] * v).sum(0) / w.sum()
+    return out
+
+
+@pytest.mark.parametrize("also", ["", "mask", "window"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("past,new,ps,hq,hkv,d", [([2500, 0], [7, 40], 16, 12, 2, 128), ([1900], [5], 5, 24, 2, 64),
+                                                  ([700, 300, 600, 100], [40, 1, 60, 9], 24, 4, 4, 256)])
+def test_infinities_in_units_that_ranges_cut(past, new, ps, hq, hkv, d, dtype, also):
+    """Far from each other, so that several pieces of a unit meet one."""
+    r, c, cu, q = make(past, new, ps, hq, hkv, d, dtype)
+    for s, n in enumerate(past):
+        for p, what in ((n // 9, np.inf), (n // 2, -np.inf), (n - n // 8, np.nan), (n + new[s] // 2, np.inf)):
+            c["v"][c["table"][s, p // ps], p % ps, 0, int(r.integers(d))] = what
+        c["k"][c["table"][s, (n // 3) // ps], (n // 3) % ps, hkv - 1] = np.inf if s % 2 else np.nan
+    mask, window = None, 0
+    if also == "mask":
+        mask = r.standard_normal((len(past), c["table"].shape[1] * ps)).astype(np.float16)
+        mask[r.random(mask.shape) < 0.3] = -np.inf
+        mask[:, [n // 3 for n in past]] = -np.inf
+    elif also == "window":
+        window = 150
+    out = run(c, q, cu, dtype, 0.07, mask, window)[: int(cu[-1])].double().cpu()
+    want = nonfinite_want(c, q, cu, ps, 0.07, mask, window)[: int(cu[-1])]
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(torch.where(out.isinf(), out, 0.0), torch.where(want.isinf(), want, 0.0))
+    fine = want.isfinite()
+    assert fine.double().mean() > 0.2
+    # two roundings to 16 bits of sums of values below 6, and f32 sums far below
+    assert (out - want).abs()[fine].max() <= 2 * 6 * torch.finfo(q.dtype).eps / 2 * 1.1
+
+
+def test_an_infinity_far_back_does_not_take_forever():
+    """5 rows of 12 heads over 65536 positions: 3 ms with a CTA to a row (about 220 ms when
+    a warp took a row and one position at a time)."""
+    bw, n, new = B(), 65536, 5
+    k = torch.randn((n // 16 + 1, 16, 2, 128), device="cuda").half()
+    v = torch.randn_like(k)
+    v[0, 3, :, 7] = float("inf")
+    table = torch.arange(n // 16 + 1, device="cuda").int()[None]
+    q = torch.randn((new, 12, 128), device="cuda").half()
+    times = []
+    for _ in range(3):
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        out = bw.paged_prefill(bw.PagedKV(k, v), q, table, i32([n + new]), i32([0, new]), 0.1)
+        end.record()
+        end.synchronize()
+        times.append(start.elapsed_time(end))
+    assert (out[:, :, 7] == float("inf")).all() and torch.isfinite(out[:, :, 8:].float()).all()
+    assert min(times) < 20, times
