@@ -278,7 +278,12 @@ int b200_paged_fork(const int32_t* src, const int32_t* keep, const int32_t* seq_
     const bool in_place = table_out == block_table && (n_seq == 1 || table_out_stride == table_stride);
     if (n_seq > 1 && (table_stride > INT64_MAX / 8 / n_seq || table_out_stride > INT64_MAX / 8 / n_seq))
         return B200_EINVAL;
-    if (!in_place &&
+    // (rows of one stride may stand between each other's, as two halves of one tensor do)
+    const int64_t ahead = (reinterpret_cast<intptr_t>(table_out) - reinterpret_cast<intptr_t>(block_table)) / 4;
+    const int64_t place = table_stride > 0 ? (ahead % table_stride + table_stride) % table_stride : 0;
+    const bool between = n_seq > 1 && table_out_stride == table_stride && place >= max_blocks &&
+                         place <= table_stride - max_blocks;
+    if (!in_place && !between &&
         meets_rows(table_out, ((n_seq - 1) * (n_seq > 1 ? table_out_stride : 0) + max_blocks) * 4, block_table,
                    (n_seq > 1 ? table_stride : 0) * 4, (int64_t)max_blocks * 4, n_seq))
         return B200_EINVAL;

@@ -113,6 +113,21 @@ def test_random_forks_and_the_steps_after_them(n, ps, max_len, in_place):
         owners(table, lens, stack, top, ps, n_pages)
 
 
+@pytest.mark.parametrize("second", [False, True])
+def test_tables_in_two_halves_of_one_tensor(second):
+    r, n, ps, width = rng(8), 33, 16, 6
+    lens, table, stack, top = state(r, n, ps, width, 150, 90)
+    both = torch.full((n, 2 * width), 44, dtype=torch.int32, device="cuda")
+    old, new = (both[:, width:], both[:, :width]) if second else (both[:, :width], both[:, width:])
+    old.copy_(i32(table))
+    src, keep = r.integers(-1, n, n), r.integers(0, 90, n)
+    want = fork_ref(src, keep, lens, table, stack, top, ps)
+    f = B().paged_fork(i32(src), i32(keep), i32(lens), old, i32(stack), i32([top]), ps, table_out=new)
+    np.testing.assert_array_equal(f.block_table.cpu().numpy(), want[0])
+    np.testing.assert_array_equal(f.seq_lens.cpu().numpy(), want[1])
+    assert torch.equal(old, i32(table))
+
+
 def test_beams_share_all_but_their_last_page():
     lens = np.array([37, 0, 0, 0], np.int32)
     table = np.full((4, 5), -1, np.int32)

@@ -78,6 +78,20 @@ def test_fork_refuses(over):
     assert B().lib().b200_paged_fork(*{**FORK, **over}.values()) == B().EINVAL
 
 
+def test_fork_takes_tables_that_stand_between_each_others_rows():
+    """Two parts of one tensor: apart, whichever comes first, as long as no entry is in both
+    (no device here: a call that is not refused ends with a CUDA error)."""
+    def fork(at, stride, blocks=4):
+        over = dict(table_out=PTR + 4 * at, table_stride=stride, table_out_stride=stride, max_blocks=blocks)
+        return B().lib().b200_paged_fork(*{**FORK, **over}.values())
+
+    for at, stride in [(4, 8), (-4, 8), (5, 9), (4, 9), (-4, 9), (12, 8), (6, 10)]:
+        assert fork(at, stride) not in (B().OK, B().EINVAL), (at, stride)
+    for at, stride in [(3, 8), (5, 8), (-3, 8), (-5, 8), (3, 9), (6, 9), (4, 7), (2, 100), (-2, 100), (8, 8), (0, 8)]:
+        if at:
+            assert fork(at, stride) == B().EINVAL, (at, stride)
+
+
 def test_fork_refuses_more_entries_than_it_counts():
     a = {**FORK, "n_seq": 1 << 16, "max_blocks": 1 << 16, "table_stride": 1 << 16, "table_out_stride": 1 << 16}
     assert B().lib().b200_paged_fork(*a.values()) == B().EUNSUPPORTED
