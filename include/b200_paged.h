@@ -179,8 +179,9 @@ int b200_paged_attn(const b200_paged_kv *kv, const float *q, int64_t q_stride, i
  *         (elements, a multiple of 8), heads [n_head][head_dim] contiguous,
  *         16-byte aligned
  *   cu    int32 [n_seq + 1], ascending, within [0, n_tokens]; the rows before
- *         cu[0] and from cu[n_seq] on are neither read nor written.  Other
- *         values are clamped and recorded (B200_DEVSTATUS_BOUNDS).
+ *         cu[0] and from cu[n_seq] on are not written, and what they hold does
+ *         not matter.  Other values are clamped and recorded
+ *         (B200_DEVSTATUS_BOUNDS).
  *   mask  as in b200_paged_attn: one row per sequence
  *   out   16-bit values of the cache's type [n_tokens][n_head][head_dim],
  *         16-byte aligned, apart from q's rows (B200_EINVAL); a row that sees no

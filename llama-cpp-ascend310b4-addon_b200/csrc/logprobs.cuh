@@ -55,7 +55,7 @@ constexpr int kLpBatch = 4;       // vectors of 16 bytes in flight per thread
 constexpr int kLpMaxCtas = 8;
 // CTAs on an SM at once.  f32 takes 40 registers where nothing is asked (0); asked for
 // six CTAs it spills (1% slower), for one it takes 56 (6% slower).  16-bit types are
-// held to 48 instead of 56 (1024 rows of bf16 97 -> 94 us).
+// held to 48 instead of 56, with 12 bytes spilled (1024 rows of bf16 97 -> 94 us).
 constexpr int kLpPerSmF32 = 6, kLpPerSm16 = 5;
 // kept by the thread of rank r: k - r at most or a vector's eight, besides the row's
 // unaligned ends

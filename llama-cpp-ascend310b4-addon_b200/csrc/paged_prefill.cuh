@@ -7,12 +7,22 @@
 // one (sequence, KV head) with the tiles of keys that any of its rows sees; a
 // launch lays all units end to end (plan kernel), cuts the line of key tiles into
 // equal ranges, one per SM, whatever lengths and heads are (main kernel), and
-// joins the units that a cut went through (finish kernel).  Three launches, a few
-// hundred bytes of schedule, results that do not depend on timing.
+// joins the units that a cut went through (finish kernel).  Three launches, 40 bytes of
+// schedule a unit and 11 KB, results that do not depend on timing.
 //
 // 8192 tokens, 64/8 heads x 128: 1010 to 1066 us, 1.03 to 1.09 PFLOP/s, in short runs,
-// 1176 us in long ones (power limit, 1.67 GHz); the products and their barriers bound it.  2048 tokens at 129024: 8.5 to 8.9 ms, the power limit.
-// 8 sequences of 5 tokens at up to 4160: 26 us, all of it latency.
+// 1180 us in long ones (power limit, 1.67 GHz); the products and their barriers bound
+// it.  2048 tokens at 129024: 8.4 to 8.9 ms, the power limit.  8 sequences of 5 tokens
+// at up to 4160: 26 us, all of it latency.
+//
+// The weights are rounded once to 16 bits for their product with V: the tensor core
+// takes them in V's type, and sums of two or three 16-bit parts, as paged_attn has them,
+// would take as many products.  Against 64 bits f16 outputs are 2.6e-4 and bf16 2.3e-3 off
+// (RMS), 1.3 to 1.45 times an output that is only rounded.
+//
+// The main kernel spills: the compiler counts 112 to 124 bytes of stores and 160 to 200 of
+// loads at head dim 256, 256 to 268 and 316 to 324 at 128, 112 to 184 and 212 to 280 at 64.
+// A row's 128 scores leave 72 of the 200 registers to the rest.
 #pragma once
 
 #include "../../include/b200_paged.h"
@@ -66,12 +76,15 @@ struct PfHeader {
 constexpr int kPfCtas = 148;   // one per SM
 constexpr int kPfRows = 128;   // rows of a tile: the lanes of tensor memory
 // A unit counts as many steps as it has key tiles and these: its queries, the first
-// scores and the outputs, which nothing overlaps.  (8192 tokens: 1105 us with 2,
-// 1077 with 3, 1094 with 4; 33 ragged sequences 76, 76, 79.)
+// scores and the outputs, which nothing overlaps.  (8192 tokens, at a step where they
+// took 1077 us with 3: 1105 with 2, 1094 with 4; 33 ragged sequences 76, 76, 79.)
 constexpr int kPfUnitSteps = 3;
 // A unit stays whole on a CTA of its own where all find one and the largest has at most
 // this many steps more than an equal range: a second unit's start and the pieces'
-// join would cost as much.  (512 tokens, 64/8 heads x 128: 33.7 us cut, 29.0 whole.)
+// join would cost as much.  (us, always cut / 2 / 6 / 12: 512 tokens of 64/8 heads x 128
+// 30.8 / 26.7 / 26.7 / 26.7; 384 at 700 40.9 / 40.9 / 37.0 / 36.9; 256 at 1000 36.9 / 36.9 /
+// 36.9 / 39.0; 2 x 300 at 100, 32/8 29.3 / 29.3 / 26.7 / 26.7; 3 x 300 at 300, 16/4 x 256 36.9 /
+// 37.0 / 30.8 / 30.8; 16 x 5 at 600, 12/2 22.6 / 22.6 / 26.5 / 26.3; five others alike.)
 constexpr int kPfWholeSteps = 6;
 // Key tiles and row tiles of a unit by head dim: two row tiles take turns between
 // the tensor core and the exponentials; at head dim 256 the outputs of one fill

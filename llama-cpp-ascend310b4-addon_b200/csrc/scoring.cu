@@ -207,8 +207,9 @@ int b200_paged_prefill(const b200_paged_kv* kv, const void* q, int64_t q_stride,
     a.kv = *kv;
     // Rows of a page to a box: the largest power of two that divides the page, a tile
     // of keys at most, eight (a group of the swizzle) at least; other pages go row by
-    // row.  8192 tokens, 64/8 heads x 128: pages of 64 1090 us, of 24 1095, of 5 by
-    // rows 1476, of 100 in boxes of four rows 1594.
+    // row.  8192 tokens, 64/8 heads x 128: pages of 64 1010 to 1066 us, of 5 by rows 1455
+    // to 1480; at a step where these took 1090 and 1476, pages of 24 1095 and of 100 in
+    // boxes of four rows 1594.
     a.box = std::min(kv->page_size & -kv->page_size, pf_keys(kv->head_dim));
     const int64_t d = kv->head_dim, group = n_head / kv->n_head_kv;
     const int64_t page_dims[4] = {d, kv->page_size, kv->n_head_kv, kv->n_pages};
