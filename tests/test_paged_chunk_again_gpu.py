@@ -162,3 +162,42 @@ def test_an_infinity_far_back_does_not_take_forever():
         times.append(start.elapsed_time(end))
     assert (out[:, :, 7] == float("inf")).all() and torch.isfinite(out[:, :, 8:].float()).all()
     assert min(times) < 20, times
+
+
+def test_lists_start_empty_in_every_replay_and_streams_have_their_own():
+    """A captured call whose infinity comes and goes, and two calls at once: every one
+    gives the bits that it gives alone."""
+    bw = B()
+    _, c, cu, q = make([2500, 40], [9, 30], 16, 12, 2, 128, "f16", pad=0)
+    dk, dv = R.to_device(c, "f16")
+    cache = bw.PagedKV(dk, dv)
+    args = i32(c["table"]), i32(c["lens"]), i32(cu), 0.09
+    size = bw.paged_prefill_workspace_size(128, q.shape[0], 2, 12, 2)
+    ws = [torch.full((size,), 0xA5, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    outs = [torch.zeros_like(q) for _ in range(2)]
+    cells = [(int(c["table"][0, p // 16]), p % 16, h, 3) for p, h in ((7, 0), (1300, 1), (2400, 0))]
+    alone = []
+    for what in (1.0, float("inf")):
+        for cell in cells:
+            dv[cell] = what
+        alone.append(bw.paged_prefill(cache, q, *args, workspace=ws[0]).clone())
+    assert torch.isfinite(alone[0].float()).all() and (alone[1][: int(cu[1]), :, 3] == float("inf")).all()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        bw.paged_prefill(cache, q, *args, out=outs[0], workspace=ws[0])
+    for turn in (1, 0, 1, 1, 0):
+        for cell in cells:
+            dv[cell] = (1.0, float("inf"))[turn]
+        outs[0].zero_()
+        g.replay()
+        assert torch.equal(outs[0], alone[turn])
+    for cell in cells:
+        dv[cell] = float("inf")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for stream, w, out in zip(streams, ws, outs):
+            with torch.cuda.stream(stream):
+                bw.paged_prefill(cache, q, *args, out=out, workspace=w)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], alone[1]) and torch.equal(outs[1], alone[1])
