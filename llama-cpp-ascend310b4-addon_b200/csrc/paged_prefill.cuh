@@ -21,7 +21,7 @@
 // (RMS), 1.3 to 1.45 times an output that is only rounded.
 //
 // The main kernel spills: the compiler counts 112 to 124 bytes of stores and 160 to 200 of
-// loads at head dim 256, 256 to 268 and 316 to 324 at 128, 112 to 184 and 212 to 280 at 64.
+// loads at head dim 256, 256 to 268 and 316 to 328 at 128, 116 to 192 and 216 to 292 at 64.
 // A row's 128 scores leave 72 of the 200 registers to the rest.
 #pragma once
 
@@ -577,6 +577,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                 }
                 const int n = x.te - x.tb, rows = min(NT * kPfRows, x.n * a.group - x.row0);
                 const int at1 = x.len - x.n + (x.row0 + rows - 1) / a.group;  // the last position that a row sees
+                const int at0 = a.window > 0 ? x.len - x.n + x.row0 / a.group - a.window + 1 : 0;  // and the first
                 if (unit && !(ok = pf_wait(&sh.q_empty, (unit - 1) & 1))) break;
                 ++unit;
                 if (a.q_box) {
@@ -678,7 +679,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_kernel(const __gr
                             k_off[e] = (uint32_t)((unsigned)page * kpage + r * krow);
                             v_next[e] = (uint32_t)((unsigned)page * vpage + r * vrow);
                         } else {
-                            lost_next |= 1u << e;
+                            // (behind every row's window or masked, it has no part in any sum)
+                            if (p >= at0 && !(MASK && __ldg(mask + p) == 0xfc00)) lost_next |= 1u << e;
                             record_status(B200_DEVSTATUS_BOUNDS);
                         }
                     }

@@ -60,6 +60,27 @@ def test_positions_on_pages_out_of_range_are_left_out(past, new, ps, hq, hkv, d,
     assert (off <= 0).all(), f"{(~(off <= 0)).sum().item()} of {off.numel()} off"
 
 
+@pytest.mark.parametrize("ps", [16, 5])
+@pytest.mark.parametrize("hides", ["window", "mask"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_pages_out_of_range_that_no_row_sees_change_nothing(d, hides, ps):
+    """Behind the window or under -inf: recorded, but the tiles' sums stay as they are."""
+    _, c, cu, q = make([700], [30], ps, 8, 2, d, "f16")
+    mask, window = None, 0
+    if hides == "window":
+        window = 300
+        first = 700 - 300 + 1
+    else:
+        first = 333
+        mask = np.zeros((1, c["table"].shape[1] * ps), np.float16)
+        mask[0, :first] = -np.inf
+    good = run(c, q, cu, "f16", 0.1, mask, window)
+    c["table"][0, : first // ps] = -1
+    out = run(c, q, cu, "f16", 0.1, mask, window)
+    assert B().device_status(reset=True) == BOUNDS
+    assert torch.equal(out, good)
+
+
 def test_only_pages_out_of_range():
     """No position is left: zeros."""
     _, c, cu, q = make([0, 40], [30, 3], 16, 8, 2, 128, "f16")
